@@ -621,6 +621,54 @@ SLC_API int slc_hip_rope_decode_attention(
     int64_t kv_stride_s, int64_t kv_stride_h, int64_t mask_stride_b, int64_t mask_stride_s,
     int64_t out_stride_b, int64_t out_stride_h, float scale, int softmax_order, void* stream);
 
+/*
+ * 8-bit linears: rows as signed 8-bit codes with one fp32 scale each, and the
+ * product of two such matrices.  The reference has no 8-bit path.
+ *
+ * A row y of `hidden` values has scale = max|y| / 127 (fp32, rounded once) and
+ * codes = the nearest whole numbers, ties to even, to 127 y / max|y|, decided as
+ * 64-bit arithmetic does; code * scale is the value that a code stands for.  A
+ * row of zeros has scale 0 and codes 0; a row with a NaN or an infinity, or whose
+ * scale has no finite fp32 value, has scale NaN and codes 0.  rows <= 2^31 - 1,
+ * hidden <= SLC_Q8_MAX_K, any alignment that the element type allows; codes
+ * [rows, hidden] and scales [rows] are contiguous.  Outputs must not overlap the
+ * inputs.
+ *
+ *   quantize_q8 : y = input
+ *   rms_norm_q8 : h = input, or with a residual (and then `summed`, contiguous)
+ *                 h = summed = round(input + residual);
+ *                 y = h * rsqrt(mean(h^2) + epsilon) * weight, unrounded (the
+ *                 mean in fp64); one dtype for all
+ *   swiglu_q8   : y = gate / (1 + exp(-gate)) * up, unrounded
+ */
+#define SLC_Q8_MAX_K 131071
+SLC_API int slc_hip_quantize_q8(const void* input, int8_t* codes, float* scales, int dtype,
+                                int64_t rows, int64_t hidden, int64_t in_stride_row,
+                                void* stream);
+SLC_API int slc_hip_rms_norm_q8(const void* input, const void* residual, const void* weight,
+                                void* summed, int8_t* codes, float* scales, int dtype,
+                                int64_t rows, int64_t hidden, int64_t in_stride_row,
+                                int64_t residual_stride_row, float epsilon, void* stream);
+SLC_API int slc_hip_swiglu_q8(const void* gate, const void* up, int8_t* codes, float* scales,
+                              int dtype, int64_t rows, int64_t hidden, int64_t gate_stride_row,
+                              int64_t up_stride_row, void* stream);
+
+/*
+ * linear_q8: output[m, n] = round(float(sum_k input[m, k] * weight[n, k]) *
+ * in_scales[m] * weight_scales[n] (+ bias[n])): the sum exact in 32-bit integers
+ * (in_features <= SLC_Q8_MAX_K, codes -128 .. 127), the rest in fp32 in this
+ * order, one rounding to dtype (fp32, fp16 or bf16; the bias has it too).
+ *   input  : rows x in_features codes, row stride in_stride_row
+ *   weight : out_features x in_features codes, contiguous
+ *   output : rows x out_features, row stride out_stride_row
+ * 16-byte aligned rows of codes run the fast kernels; any other alignment and
+ * size is taken.
+ */
+SLC_API int slc_hip_linear_q8(const int8_t* input, const float* in_scales, const int8_t* weight,
+                              const float* weight_scales, const void* bias, void* output,
+                              int dtype, int64_t rows, int64_t out_features, int64_t in_features,
+                              int64_t in_stride_row, int64_t out_stride_row, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

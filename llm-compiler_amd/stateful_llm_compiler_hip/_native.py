@@ -138,6 +138,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I,
         [_P, _P, _P, _P, _I, _P, _I, _L, _L, _L, _L, _L, _I] + [_L] * 15 + [_F, _I, _P],
     ),
+    "slc_hip_quantize_q8": (_I, [_P, _P, _P, _I, _L, _L, _L, _P]),
+    "slc_hip_rms_norm_q8": (_I, [_P] * 6 + [_I, _L, _L, _L, _L, _F, _P]),
+    "slc_hip_swiglu_q8": (_I, [_P] * 4 + [_I, _L, _L, _L, _L, _P]),
+    "slc_hip_linear_q8": (_I, [_P] * 6 + [_I, _L, _L, _L, _L, _L, _P]),
     "slc_hip_rope": (
         _I,
         [_P] * 6 + [_I] + [_L] * 5 + [_L] * 16 + [_P],

@@ -23,6 +23,13 @@ from .hip_ops import (
     hip_swiglu,
 )
 from .hip_prefill_attention import hip_prefill_attention, hip_prefill_mask_tiles
+from .hip_q8 import (
+    hip_add_rms_norm_q8,
+    hip_linear_q8,
+    hip_quantize_q8,
+    hip_rms_norm_q8,
+    hip_swiglu_q8,
+)
 from .hip_rmsnorm import hip_rms_norm
 from .hip_rope import hip_rope
 
@@ -47,6 +54,11 @@ __all__ = [
     "hip_linear",
     "hip_prefill_attention",
     "hip_prefill_mask_tiles",
+    "hip_add_rms_norm_q8",
+    "hip_linear_q8",
+    "hip_quantize_q8",
+    "hip_rms_norm_q8",
+    "hip_swiglu_q8",
     "hip_rms_norm",
     "hip_rope",
 ]

@@ -1,0 +1,184 @@
+"""8-bit linears: rows as int8 codes with an fp32 scale each, and their product.
+
+A row ``y`` has ``scale = max|y| / 127`` and ``codes`` = the whole numbers nearest
+to ``127 y / max|y|`` (ties to even), decided as 64-bit arithmetic does;
+``code * scale`` is the value that a code stands for.  A row of zeros has scale 0; a
+row with a NaN or an infinity (or whose scale fp32 cannot hold) has scale NaN, so
+that whatever is computed from it is NaN too, and codes 0.
+
+A layer's linears run on them as ``hip_add_rms_norm_q8`` -> ``hip_linear_q8``
+(Q/K/V, or gate and up in one weight), ``hip_quantize_q8`` of the attention output
+-> ``hip_linear_q8`` (O), ``hip_swiglu_q8`` -> ``hip_linear_q8`` (down).
+``hip_quantize_q8`` of a weight ``[N, K]`` gives its codes and the scales of its
+output channels.  The reference has no 8-bit path; the operators take their
+arguments as ``hip_rms_norm``, ``hip_swiglu`` and ``hip_linear`` do.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _native
+
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+MAX_FEATURES = 131071  # SLC_Q8_MAX_K: sums of so many products of codes fit 32 bits
+
+
+def _check_rows(what: str, *tensors: torch.Tensor) -> None:
+    """Float GPU tensors of one shape, dtype and device with a last axis to code."""
+
+    first = tensors[0]
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError(f"{what}: all tensors must be on the GPU")
+        if t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
+            raise ValueError(f"{what}: tensors need one shape, dtype and device")
+    if first.dtype not in _FLOATS:
+        raise ValueError(f"{what}: unsupported dtype {first.dtype}")
+    if first.ndim < 1 or not 1 <= first.shape[-1] <= MAX_FEATURES:
+        raise ValueError(f"{what}: the last axis must hold 1 to {MAX_FEATURES} values")
+
+
+def _flat(tensor: torch.Tensor) -> torch.Tensor:
+    """``tensor`` as evenly strided rows; a copy only where no view is."""
+
+    if tensor.stride(-1) != 1 and tensor.shape[-1] != 1:
+        tensor = tensor.contiguous()
+    try:
+        return tensor.view(-1, tensor.shape[-1])
+    except RuntimeError:
+        return tensor.reshape(-1, tensor.shape[-1])
+
+
+def _outputs(tensor: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return (torch.empty(tensor.shape, device=tensor.device, dtype=torch.int8),
+            torch.empty(tensor.shape[:-1], device=tensor.device, dtype=torch.float32))
+
+
+def _call(name: str, device: torch.device, *arguments) -> None:
+    """The entry point on ``device``'s current stream, with that device current."""
+
+    function = getattr(_native.library(), name)
+    if device.index == torch.cuda.current_device():
+        status = function(*arguments, _native.current_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = function(*arguments, _native.current_stream(device))
+    _native.check(status, name)
+
+
+def hip_quantize_q8(tensor: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)`` of ``tensor`` [..., K] along its last axis."""
+
+    _check_rows("HIP quantize q8", tensor)
+    codes, scales = _outputs(tensor)
+    if tensor.numel():
+        flat = _flat(tensor)
+        _call("slc_hip_quantize_q8", tensor.device, flat.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+              _native.dtype_tag(tensor.dtype), flat.shape[0], flat.shape[1], flat.stride(0))
+    return codes, scales
+
+
+def _norm(what, tensor, residual, weight, epsilon):
+    tensors = (tensor,) if residual is None else (tensor, residual)
+    _check_rows(what, *tensors)
+    if not weight.is_cuda or weight.device != tensor.device or weight.dtype != tensor.dtype:
+        raise ValueError(f"{what}: the weight needs the input's dtype and device")
+    if weight.shape != tensor.shape[-1:]:
+        raise ValueError(f"{what}: weight must be [{tensor.shape[-1]}], got {tuple(weight.shape)}")
+    codes, scales = _outputs(tensor)
+    summed = None if residual is None else torch.empty(tensor.shape, device=tensor.device, dtype=tensor.dtype)
+    if tensor.numel():
+        flat = _flat(tensor)
+        other = None if residual is None else _flat(residual)
+        weight = weight.contiguous()
+        _call("slc_hip_rms_norm_q8", tensor.device, flat.data_ptr(), None if other is None else other.data_ptr(),
+              weight.data_ptr(), None if summed is None else summed.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+              _native.dtype_tag(tensor.dtype), flat.shape[0], flat.shape[1], flat.stride(0),
+              0 if other is None else other.stride(0), float(epsilon))
+    return summed, codes, scales
+
+
+def hip_rms_norm_q8(
+    tensor: torch.Tensor, weight: torch.Tensor, *, epsilon: float
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)`` of ``tensor * rsqrt(mean(tensor^2) + epsilon) * weight``
+    over the last axis; nothing is rounded before the codes are."""
+
+    return _norm("HIP RMSNorm q8", tensor, None, weight, epsilon)[1:]
+
+
+def hip_add_rms_norm_q8(
+    tensor: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, *, epsilon: float
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(summed, codes, scales)``: ``hip_add(tensor, residual)``, bit for bit, and
+    ``hip_rms_norm_q8`` of it, in one pass."""
+
+    return _norm("HIP add RMSNorm q8", tensor, residual, weight, epsilon)
+
+
+def hip_swiglu_q8(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)`` of ``silu(gate) * up``; nothing is rounded before the
+    codes are.  ``gate`` and ``up`` may be the halves of a fused projection."""
+
+    _check_rows("HIP swiglu q8", gate, up)
+    codes, scales = _outputs(gate)
+    if gate.numel():
+        a, b = _flat(gate), _flat(up)
+        _call("slc_hip_swiglu_q8", gate.device, a.data_ptr(), b.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+              _native.dtype_tag(gate.dtype), a.shape[0], a.shape[1], a.stride(0), b.stride(0))
+    return codes, scales
+
+
+def hip_linear_q8(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scales: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    output_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``codes`` [..., K] times ``weight`` [N, K]^T, each output times its token's
+    and its channel's scale (+ ``bias`` [N], of the output's dtype).
+
+    ``codes`` and ``weight`` are int8 (-128 included), ``scales`` [...] and
+    ``weight_scales`` [N] fp32.  The sum over K is exact; float(sum) * scale *
+    weight scale + bias runs in fp32 and is rounded once to ``output_dtype``.
+    """
+
+    what = "HIP linear q8"
+    tensors = [codes, scales, weight, weight_scales]
+    if bias is not None:
+        tensors.append(bias)
+    if not all(t.is_cuda for t in tensors):
+        raise ValueError(f"{what}: all tensors must be on the GPU")
+    device = codes.device
+    if any(t.device != device for t in tensors):
+        raise ValueError(f"{what}: tensors need one device")
+    if codes.dtype != torch.int8 or weight.dtype != torch.int8:
+        raise ValueError(f"{what}: codes and weight must be int8")
+    if scales.dtype != torch.float32 or weight_scales.dtype != torch.float32:
+        raise ValueError(f"{what}: scales must be fp32")
+    if output_dtype not in _FLOATS:
+        raise ValueError(f"{what}: unsupported output dtype {output_dtype}")
+    if codes.ndim < 1 or weight.ndim != 2:
+        raise ValueError(f"{what}: codes need at least one axis and the weight two")
+    features, width = weight.shape
+    if codes.shape[-1] != width:
+        raise ValueError(f"{what}: input K does not match weight K")
+    if not 1 <= width <= MAX_FEATURES or features < 1:
+        raise ValueError(f"{what}: K must be 1 to {MAX_FEATURES} and N at least 1")
+    if scales.shape != codes.shape[:-1] or weight_scales.shape != (features,):
+        raise ValueError(f"{what}: one scale per token and one per output channel are needed")
+    if bias is not None and (bias.shape != (features,) or bias.dtype != output_dtype):
+        raise ValueError(f"{what}: bias must be [{features}] of the output's dtype")
+    if not all(t.is_contiguous() for t in tensors):
+        raise ValueError(f"{what}: tensors must be contiguous")
+    output = torch.empty((*codes.shape[:-1], features), device=device, dtype=output_dtype)
+    if codes.numel():
+        _call("slc_hip_linear_q8", device, codes.data_ptr(), scales.data_ptr(), weight.data_ptr(),
+              weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), output.data_ptr(),
+              _native.dtype_tag(output_dtype), codes.numel() // width, features, width, width, features)
+    return output

@@ -1,0 +1,514 @@
+"""The 8-bit operators against plain implementations in 64 bits.
+
+Codes are whole numbers and have to be equal: a code is the number nearest to
+127 y / max|y|, ties to even, and products of 16-bit values are exact in fp64.
+Tolerances count half steps: 2^-24 for each fp32 operation, eps / 2 for the last
+rounding to the output's type.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from helpers import announce, assert_bitwise_equal, generator
+from stateful_llm_compiler_hip import backends
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+HALF32 = 2.0**-24
+
+
+def q8(y):
+    """Codes (float64) and scales of the rows of a float64 y."""
+
+    amax = y.abs().amax(-1, keepdim=True)
+    good = torch.isfinite(amax)
+    codes = torch.where((amax > 0) & good, torch.round(y * 127 / amax), 0.0)
+    return codes, torch.where(good, amax / 127, torch.nan).squeeze(-1)
+
+
+def check_rows(codes, scales, y, factor=1.0):
+    """Codes of y and scales of y * factor [..., 1]; the scale is rounded once,
+    after few fp64 operations."""
+
+    want, want_scales = q8(y)
+    want_scales = want_scales * (factor if isinstance(factor, float) else factor.squeeze(-1))
+    assert codes.dtype == torch.int8 and codes.shape == y.shape and codes.is_contiguous()
+    assert scales.dtype == torch.float32 and scales.shape == y.shape[:-1]
+    codes, scales = codes.cpu().double(), scales.cpu().double()
+    wrong = (codes != want).nonzero()
+    assert not len(wrong), f"{len(wrong)} codes differ, first at {wrong[0].tolist()}"
+    assert torch.equal(scales.isnan(), want_scales.isnan())
+    fine = ~want_scales.isnan()
+    # 2^-150 is half a step of the smallest fp32 numbers.
+    bound = want_scales * (HALF32 * 1.001) + 2.0**-150
+    assert ((scales - want_scales).abs() <= bound)[fine].all()
+
+
+def rows_of(rows, k, dtype, seed, scale=1.0):
+    g = generator(seed)
+    x = torch.randn(rows, k, generator=g) * (torch.rand(rows, 1, generator=g) * 3 + 0.1) * scale
+    x[:, :: max(1, k // 3)] *= 6
+    if rows > 2:
+        x[2] = 0.0
+    return x.to(dtype)
+
+
+def swiglu_exact(gate, up):
+    g = gate.double()
+    return g / (1 + torch.exp(-g)) * up.double()
+
+
+# A vector's tail, one wave's and several waves' registers, and rows read twice.
+WIDTHS = [1, 2, 7, 8, 9, 511, 512, 513, 896, 1001, 1024, 1030, 2048, 2055, 4096, 4864, 6144, 6150, 16384, 16390,
+          32768, 33001]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", WIDTHS)
+def test_quantize(gpu, dtype, k):
+    announce(f"quantize {dtype} {k}")
+    x = rows_of(5, k, dtype, k)
+    check_rows(*backends.hip_quantize_q8(x.to(gpu)), x.double())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("k", WIDTHS)
+def test_norm(gpu, dtype, residual, k):
+    announce(f"norm {dtype} {residual} {k}")
+    x, r = rows_of(5, k, dtype, k), rows_of(5, k, dtype, k + 1, 3.0)
+    w = (torch.randn(k, generator=generator(k + 2)) * 0.5 + 1).to(dtype)
+    eps = 1e-6
+    if residual:
+        summed, codes, scales = backends.hip_add_rms_norm_q8(x.to(gpu), r.to(gpu), w.to(gpu), epsilon=eps)
+        assert_bitwise_equal(summed, backends.hip_add(x.to(gpu), r.to(gpu)))
+        assert_bitwise_equal(summed, (x.float() + r.float()).to(dtype))
+        x = summed.cpu()
+    else:
+        codes, scales = backends.hip_rms_norm_q8(x.to(gpu), w.to(gpu), epsilon=eps)
+    h = x.double()
+    eps32 = float(torch.tensor(eps, dtype=torch.float32))
+    check_rows(codes, scales, h * w.double(), torch.rsqrt(h.square().mean(-1, keepdim=True) + eps32))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", WIDTHS)
+def test_swiglu(gpu, dtype, k):
+    announce(f"swiglu {dtype} {k}")
+    # The halves of one projection's output, whose rows are 2k apart.
+    both = rows_of(5, 2 * k, dtype, k, 2.0)
+    device = both.to(gpu)
+    codes, scales = backends.hip_swiglu_q8(device[:, :k], device[:, k:])
+    check_rows(codes, scales, swiglu_exact(both[:, :k], both[:, k:]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows(gpu, dtype):
+    announce(f"many rows {dtype}")
+    x = rows_of(4099, 896, dtype, 3)
+    check_rows(*backends.hip_quantize_q8(x.to(gpu)), x.double())
+    up = rows_of(4099, 896, dtype, 4)
+    check_rows(*backends.hip_swiglu_q8(x.to(gpu), up.to(gpu)), swiglu_exact(x, up))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ties_go_to_even(gpu, dtype):
+    # Largest value 127 * 2^e: every odd half step is a tie.
+    steps = torch.arange(-254, 255, dtype=torch.float64) / 2
+    x = torch.stack([steps * 2.0**e for e in (-6, 0, 1, 5)]).to(dtype)
+    assert torch.equal(x[1].double(), steps)  # no rounding in any of the types
+    announce(f"ties {dtype}")
+    codes, scales = backends.hip_quantize_q8(x.to(gpu))
+    check_rows(codes, scales, x.double())
+    assert torch.equal(codes[1].cpu().double(), torch.round(steps))
+    # The same of products: a weight of 2^-3 moves every value alike.
+    w = torch.full((steps.numel(),), 0.125, dtype=dtype)
+    codes, _ = backends.hip_rms_norm_q8(x.to(gpu), w.to(gpu), epsilon=0.0)
+    assert torch.equal(codes[1].cpu().double(), torch.round(steps))
+
+
+def test_products_next_to_a_border(gpu):
+    # amax 127 * 3 in 16-bit products: v * (127 / amax) rounds, ties do not.
+    g = generator(5)
+    odd = torch.randint(-127, 128, (64, 256), generator=g).double() * 1.5  # half steps of amax / 127 = 3
+    x = odd.clone()
+    x[:, 0] = 381.0
+    w = torch.ones(256)
+    announce("border products")
+    for dtype in (torch.float16, torch.float32):
+        codes, _ = backends.hip_rms_norm_q8(x.to(dtype).to(gpu), w.to(dtype).to(gpu), epsilon=1e-6)
+        assert torch.equal(codes.cpu().double(), torch.round(x / 3))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [40, 896, 4864, 33001])
+def test_rows_without_a_value_and_extreme_rows(gpu, dtype, k):
+    info = torch.finfo(dtype)
+    x = rows_of(12, k, dtype, 11)
+    x[0] = 0.0
+    x[1, k // 2] = torch.nan
+    x[3, k - 1] = torch.inf
+    x[4, 0] = -torch.inf
+    x[5] = 0.0
+    x[5, k - 1] = info.max
+    x[6] = info.tiny * 0.25  # below the normal numbers
+    x[7, 3] = info.max
+    x[8] *= info.tiny * 64
+    announce(f"extreme rows {dtype} {k}")
+    check_rows(*backends.hip_quantize_q8(x.to(gpu)), x.double())
+
+    w = torch.full((k,), 100.0, dtype=dtype)  # products past fp32 in bf16 and fp32
+    w[: k // 2] = 0.01
+    h = x.double()
+    rstd = torch.rsqrt(h.square().mean(-1, keepdim=True) + float(torch.tensor(1e-6, dtype=torch.float32)))
+    y = h * w.double()
+    y[~torch.isfinite(y).all(-1) | ~torch.isfinite(rstd).squeeze(-1)] = torch.nan
+    codes, scales = backends.hip_rms_norm_q8(x.to(gpu), w.to(gpu), epsilon=1e-6)
+    check_rows(codes, scales, y, rstd)
+    residual = torch.zeros_like(x)
+    summed, codes2, scales2 = backends.hip_add_rms_norm_q8(x.to(gpu), residual.to(gpu), w.to(gpu), epsilon=1e-6)
+    assert_bitwise_equal(codes2, codes)
+    assert torch.equal(summed.cpu().nan_to_num(7.0), x.nan_to_num(7.0))
+
+    up = rows_of(12, k, dtype, 12)
+    up[9] = info.max
+    gate = x.clone()
+    gate[10] = -100.0  # exp(100) is past fp32, silu(-100) is not 0
+    up[10] = min(info.max, 2.0**100)
+    gate[11] = -30.0
+    y = swiglu_exact(gate, up)
+    y[(y.abs().amax(-1) / 127) > torch.finfo(torch.float32).max] = torch.nan
+    y[~torch.isfinite(y).all(-1)] = torch.nan
+    check_rows(*backends.hip_swiglu_q8(gate.to(gpu), up.to(gpu)), y)
+
+
+def test_norm_of_zeros_without_epsilon_is_nan(gpu):
+    announce("zeros, eps 0")
+    codes, scales = backends.hip_rms_norm_q8(torch.zeros(3, 64, device=gpu), torch.ones(64, device=gpu), epsilon=0.0)
+    assert scales.isnan().all() and not codes.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layouts(gpu, dtype):
+    announce(f"layouts {dtype}")
+    base = rows_of(6 * 7, 104, dtype, 21)
+    device = base.to(gpu)
+    # A first element off the vectors' alignment, rows apart.
+    check_rows(*backends.hip_quantize_q8(device[:, 1:98]), base[:, 1:98].double())
+    w = torch.linspace(-1, 2, 98).to(dtype)
+    codes, _ = backends.hip_rms_norm_q8(device[:, 1:98], w.to(gpu)[1:], epsilon=1e-6)
+    check_codes = q8(base[:, 1:98].double() * w[1:].double())[0]
+    assert torch.equal(codes.cpu().double(), check_codes)
+    # Heads out of place (a copy), every other row, a column stride, one row twice.
+    heads, host = device.view(6, 7, 104).permute(1, 0, 2), base.view(6, 7, 104).permute(1, 0, 2)
+    check_rows(*backends.hip_quantize_q8(heads), host.double())
+    check_rows(*backends.hip_quantize_q8(device[::2]), base[::2].double())
+    check_rows(*backends.hip_quantize_q8(device[:, ::2]), base[:, ::2].double())
+    check_rows(*backends.hip_quantize_q8(device[:1].expand(5, 104)), base[:1].expand(5, 104).double())
+    check_rows(*backends.hip_quantize_q8(device[:, 5:6]), base[:, 5:6].double())
+    check_rows(*backends.hip_quantize_q8(device[3]), base[3].double())
+    check_rows(*backends.hip_swiglu_q8(device[:21], heads.reshape(42, 104)[21:]),
+               swiglu_exact(base[:21], host.reshape(42, 104)[21:]))
+    other = torch.randn(42, 104, generator=generator(1)).to(dtype)
+    padded = torch.zeros(42, 300, dtype=dtype)
+    padded[:, 3:107] = other
+    summed, codes, _ = backends.hip_add_rms_norm_q8(device, padded.to(gpu)[:, 3:107], torch.ones(104, dtype=dtype,
+                                                                                               device=gpu), epsilon=0.1)
+    assert_bitwise_equal(summed, (base.float() + other.float()).to(dtype))
+    assert torch.equal(codes.cpu().double(), q8(summed.cpu().double())[0])
+
+
+def test_empty_calls(gpu):
+    announce("empty")
+    x = torch.zeros(0, 3, 16, device=gpu)
+    codes, scales = backends.hip_quantize_q8(x)
+    assert codes.shape == (0, 3, 16) and scales.shape == (0, 3)
+    w = torch.zeros(5, 16, dtype=torch.int8, device=gpu)
+    y = backends.hip_linear_q8(codes, scales, w, torch.ones(5, device=gpu))
+    assert y.shape == (0, 3, 5) and y.dtype == torch.bfloat16
+    summed, codes, _ = backends.hip_add_rms_norm_q8(x, x, torch.ones(16, device=gpu), epsilon=1e-6)
+    assert summed.shape == x.shape and codes.shape == x.shape
+
+
+def test_refusals(gpu):
+    x, w = torch.zeros(2, 16, device=gpu), torch.ones(16, device=gpu)
+    codes, scales = torch.zeros(2, 16, dtype=torch.int8, device=gpu), torch.zeros(2, device=gpu)
+    weight, weight_scales = torch.zeros(5, 16, dtype=torch.int8, device=gpu), torch.zeros(5, device=gpu)
+    linear = backends.hip_linear_q8
+    for call in (
+        lambda: backends.hip_quantize_q8(codes),
+        lambda: backends.hip_quantize_q8(x.double()),
+        lambda: backends.hip_quantize_q8(x[0, 0]),
+        lambda: backends.hip_quantize_q8(x[:, :0]),
+        lambda: backends.hip_quantize_q8(torch.zeros(1, 131072, device=gpu)),
+        lambda: backends.hip_rms_norm_q8(x, w.bfloat16(), epsilon=1e-6),
+        lambda: backends.hip_rms_norm_q8(x, w[:15], epsilon=1e-6),
+        lambda: backends.hip_rms_norm_q8(x, w.view(1, 16), epsilon=1e-6),
+        lambda: backends.hip_add_rms_norm_q8(x, x[:1], w, epsilon=1e-6),
+        lambda: backends.hip_add_rms_norm_q8(x, x.bfloat16(), w, epsilon=1e-6),
+        lambda: backends.hip_add_rms_norm_q8(x, x.cpu(), w, epsilon=1e-6),
+        lambda: backends.hip_swiglu_q8(x, x[:, :8]),
+        lambda: backends.hip_swiglu_q8(x, x.half()),
+        lambda: linear(x, scales, weight, weight_scales),
+        lambda: linear(codes, scales.double(), weight, weight_scales),
+        lambda: linear(codes, scales, weight.float(), weight_scales),
+        lambda: linear(codes, scales, weight[:, :8], weight_scales),
+        lambda: linear(codes, scales[:1], weight, weight_scales),
+        lambda: linear(codes, scales, weight, weight_scales[:4]),
+        lambda: linear(codes, scales, weight, weight_scales, torch.zeros(5, device=gpu)),  # fp32 bias, bf16 output
+        lambda: linear(codes, scales, weight, weight_scales, torch.zeros(4, device=gpu, dtype=torch.bfloat16)),
+        lambda: linear(codes, scales, weight, weight_scales, output_dtype=torch.float64),
+        lambda: linear(codes, scales, weight.view(5, 4, 4), weight_scales),
+        lambda: linear(codes.t().contiguous().t(), scales, weight, weight_scales),
+        lambda: linear(codes.cpu(), scales, weight, weight_scales),
+        lambda: linear(codes[:, :0], scales, weight[:, :0], weight_scales),
+        lambda: linear(codes, scales, weight[:0], weight_scales[:0]),
+    ):
+        with pytest.raises(ValueError):
+            call()
+
+
+# ---- the product ---------------------------------------------------------------
+
+
+def product_exact(codes, scales, weight, weight_scales, bias):
+    """(result, magnitude of the product) in 64 bits."""
+
+    sums = codes.double() @ weight.double().t()
+    product = sums * scales.double().unsqueeze(-1) * weight_scales.double()
+    return (product if bias is None else product + bias.double()), product.abs()
+
+
+def check_product(y, codes, scales, weight, weight_scales, bias, dtype):
+    want, size = product_exact(codes, scales, weight, weight_scales, bias)
+    assert y.dtype == dtype and y.shape == want.shape
+    # The sum's conversion and the token's scale, then the channel's scale and the
+    # bias in one fma; then the output's type, whose subnormals' half step is last.
+    half, fine = torch.finfo(dtype).eps / 2, torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+    bound = 2 * HALF32 * size * 1.001 + want.abs() * (HALF32 + half) * 1.001 + fine
+    off = (y.cpu().double() - want).abs()
+    assert (off <= bound).all(), f"off by {(off / bound).max().item():.3g} of the bound"
+
+
+def operands(m, n, k, bias_dtype, seed, low=-128, high=128):
+    g = generator(seed)
+    codes = torch.randint(low, high, (m, k), generator=g, dtype=torch.int8)
+    weight = torch.randint(low, high, (n, k), generator=g, dtype=torch.int8)
+    scales, weight_scales = torch.rand(m, generator=g) * 0.02, torch.rand(n, generator=g) * 0.01
+    bias = None if bias_dtype is None else torch.randn(n, generator=g).to(bias_dtype)
+    return codes, scales, weight, weight_scales, bias
+
+
+def run_product(gpu, m, n, k, dtype, bias=True, seed=0, **kw):
+    announce(f"linear {m} x {n} x {k} {dtype}")
+    ops = operands(m, n, k, dtype if bias else None, seed, **kw)
+    y = backends.hip_linear_q8(*(None if t is None else t.to(gpu) for t in ops), output_dtype=dtype)
+    check_product(y, *ops, dtype)
+    return y
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 1), (1, 5, 16), (3, 7, 15), (2, 17, 17), (8, 1152, 896), (16, 896, 4864), (17, 100, 64), (31, 33, 1001),
+    (33, 64, 128), (48, 896, 144), (64, 4864, 896), (65, 66, 130), (100, 200, 112), (129, 257, 1040), (300, 1003, 1001),
+    (512, 896, 4864), (5, 20000, 80), (20, 18000, 896), (260, 4104, 272),
+])
+def test_linear(gpu, dtype, m, n, k):
+    run_product(gpu, m, n, k, dtype, bias=(m + n) % 2 == 0, seed=m + n + k)
+
+
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 1025])
+def test_linear_rows(gpu, m):
+    run_product(gpu, m, 192, 320, torch.bfloat16, seed=m)
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 15, 16, 31, 32, 48, 63, 64, 65, 127, 128, 129, 144, 255, 256, 384, 511, 512,
+                               528, 1024, 1040, 4096])
+def test_linear_depths(gpu, k):
+    for m in (4, 40, 200):
+        run_product(gpu, m, 136, k, torch.float32, seed=k)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 8, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 255, 257, 300])
+def test_linear_widths(gpu, n):
+    for m in (4, 40, 200):
+        run_product(gpu, m, n, 256, torch.float16, seed=n)
+
+
+@pytest.mark.parametrize("m", [1, 100])
+@pytest.mark.parametrize("sign", [-128, 127])
+def test_linear_longest_sums(gpu, m, sign):
+    # K = 131071 products of (-128)^2 are 2^31 - 2^14, the largest sum of 32 bits.
+    announce(f"longest sums {m} {sign}")
+    k, n = 131071, 40
+    codes = torch.full((m, k), -128, dtype=torch.int8, device=gpu)
+    weight = torch.full((n, k), sign, dtype=torch.int8, device=gpu)
+    one = torch.ones(max(m, n), device=gpu)
+    y = backends.hip_linear_q8(codes, one[:m], weight, one[:n], output_dtype=torch.float32)
+    assert (y.double() == float(torch.tensor(-128.0 * sign * k, dtype=torch.float32))).all()
+
+
+def test_linear_is_the_same_on_every_path(gpu):
+    # The sums are exact, so a row's result does not depend on the rows beside it.
+    announce("rows alone")
+    codes, scales, weight, weight_scales, bias = (t.to(gpu) for t in operands(600, 904, 896, torch.bfloat16, 3))
+    whole = backends.hip_linear_q8(codes, scales, weight, weight_scales, bias)
+    for rows in (1, 8, 17, 40, 64, 100, 300):
+        part = backends.hip_linear_q8(codes[:rows], scales[:rows], weight, weight_scales, bias)
+        assert_bitwise_equal(part, whole[:rows])
+    # Off the vectors' alignment.
+    odd = torch.zeros(600 * 896 + 1, dtype=torch.int8, device=gpu)[1:].view(600, 896)
+    odd.copy_(codes)
+    assert_bitwise_equal(backends.hip_linear_q8(odd, scales, weight, weight_scales, bias), whole)
+    odd_w = torch.zeros(904 * 896 + 3, dtype=torch.int8, device=gpu)[3:].view(904, 896)
+    odd_w.copy_(weight)
+    for rows in (5, 50, 600):
+        y = backends.hip_linear_q8(codes[:rows], scales[:rows], odd_w, weight_scales, bias)
+        assert_bitwise_equal(y, whole[:rows])
+
+
+def test_linear_leading_axes_and_nan_rows(gpu):
+    announce("leading axes")
+    codes, scales, weight, weight_scales, _ = operands(12, 64, 128, None, 9)
+    scales[5] = torch.nan
+    y = backends.hip_linear_q8(codes.view(3, 4, 128).to(gpu), scales.view(3, 4).to(gpu), weight.to(gpu),
+                               weight_scales.to(gpu)).cpu()
+    assert y.shape == (3, 4, 64)
+    flat = y.view(12, 64)
+    assert flat[5].isnan().all() and not flat[torch.arange(12) != 5].isnan().any()
+    one = backends.hip_linear_q8(codes[0].to(gpu), scales[0].to(gpu), weight.to(gpu), weight_scales.to(gpu))
+    assert one.shape == (64,)
+    assert_bitwise_equal(one, flat[0])
+
+
+def test_weight_rows_past_32_bits(gpu):
+    # A weight of 2^31 bytes and more: its last rows are past 32-bit offsets.
+    announce("weight past 2^31 bytes")
+    n, k = 2**18 + 40, 8208
+    g = torch.Generator(device=gpu).manual_seed(1)
+    weight = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8, device=gpu)
+    for m in (3, 70):
+        codes = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device=gpu)
+        scales = torch.rand(m, generator=g, device=gpu)
+        weight_scales = torch.rand(n, generator=g, device=gpu)
+        y = backends.hip_linear_q8(codes, scales, weight, weight_scales, output_dtype=torch.float32)
+        for part in (slice(0, 40), slice(2**17, 2**17 + 40), slice(n - 40, n)):
+            check_product(y[:, part], codes.cpu(), scales.cpu(), weight[part].cpu(), weight_scales[part].cpu(), None,
+                          torch.float32)
+
+
+def test_rows_past_32_bits(gpu):
+    announce("rows past 2^31 values")
+    rows, k = 65540, 32770
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=gpu)
+    x[:: rows - 1, ::7] = 3.0
+    x[rows - 1, k - 1] = -4.0
+    codes, scales = backends.hip_quantize_q8(x)
+    last = x[rows - 1].cpu()
+    check_rows(codes[rows - 1], scales[rows - 1], last.double())
+    check_rows(codes[0], scales[0], x[0].cpu().double())
+    assert not scales[1 : rows - 1].any()
+
+
+# ---- as they are used ------------------------------------------------------------
+
+
+def weights(n, k, seed):
+    return torch.randn(n, k, generator=generator(seed)) * 0.05
+
+
+def layer(x, residual, params):
+    """Norm, gate/up, SwiGLU, down: an MLP block on 8-bit linears."""
+
+    summed, codes, scales = backends.hip_add_rms_norm_q8(x, residual, params["norm"], epsilon=1e-6)
+    both = backends.hip_linear_q8(codes, scales, *params["gate_up"])
+    codes, scales = backends.hip_swiglu_q8(*both.chunk(2, dim=-1))
+    return summed, backends.hip_linear_q8(codes, scales, *params["down"])
+
+
+def layer_params(gpu):
+    k, n = 896, 1216
+    return {"norm": (torch.rand(k, generator=generator(1)) + 0.5).bfloat16().to(gpu),
+            "gate_up": backends.hip_quantize_q8(weights(2 * n, k, 2).to(gpu)),
+            "down": backends.hip_quantize_q8(weights(k, n, 3).to(gpu))}
+
+
+@pytest.mark.parametrize("rows", [1, 30, 70, 300])
+def test_mlp_block(gpu, rows):
+    announce(f"mlp {rows}")
+    params = layer_params(gpu)
+    x, residual = rows_of(rows, 896, torch.bfloat16, 4), rows_of(rows, 896, torch.bfloat16, 5)
+    summed, y = layer(x.to(gpu), residual.to(gpu), params)
+
+    def plain(name):
+        codes, scales = params[name]
+        return codes.cpu().double() * scales.cpu().double().unsqueeze(-1)
+
+    h = (x.float() + residual.float()).bfloat16().double()
+    assert torch.equal(summed.cpu().double(), h)
+    eps32 = float(torch.tensor(1e-6, dtype=torch.float32))
+    codes, scales = q8(h * params["norm"].cpu().double())
+    scales = scales * torch.rsqrt(h.square().mean(-1) + eps32)
+    both = codes * scales.unsqueeze(-1) @ plain("gate_up").t()
+    # The projection is stored in bf16; from the kernels' own values of it on, so
+    # that a rounding's flip does not move the codes that follow.
+    got = backends.hip_linear_q8(codes.to(torch.int8).to(gpu), scales.float().to(gpu), *params["gate_up"]).cpu().double()
+    assert ((got - both).abs() <= both.abs() * 2.0**-8 + 1e-6 * both.abs().amax()).all()
+    codes, scales = q8(swiglu_exact(*got.chunk(2, dim=-1)))
+    want = codes * scales.unsqueeze(-1) @ plain("down").t()
+    # Half a step of bf16, and the fp32 operations on the sums.
+    assert ((y.cpu().double() - want).abs() <= want.abs() * 2.0**-8 * 1.001 + want.abs().amax() * 2.0**-20).all()
+
+
+def test_side_stream_and_graph(gpu):
+    announce("stream and graph")
+    params = layer_params(gpu)
+    inputs = [(rows_of(24, 896, torch.bfloat16, s).to(gpu), rows_of(24, 896, torch.bfloat16, s + 50).to(gpu))
+              for s in range(4)]
+    wants = [layer(x, r, params) for x, r in inputs]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        side = [layer(x, r, params) for x, r in inputs]
+    stream.synchronize()
+    for got, want in zip(side, wants):
+        for a, b in zip(got, want):
+            assert_bitwise_equal(a, b)
+    x, r = inputs[0][0].clone(), inputs[0][1].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(x, r, params)
+    for turn in range(3):
+        for (new_x, new_r), want in zip(inputs, wants):
+            x.copy_(new_x)
+            r.copy_(new_r)
+            graph.replay()
+            eager = layer(new_x, new_r, params)
+            torch.cuda.synchronize()
+            for a, b, c in zip(out, want, eager):
+                assert_bitwise_equal(a, b)
+                assert_bitwise_equal(c, b)
+
+
+def test_two_streams_at_once(gpu):
+    announce("two streams")
+    params = layer_params(gpu)
+    inputs = [(rows_of(200, 896, torch.bfloat16, s).to(gpu), rows_of(200, 896, torch.bfloat16, s + 9).to(gpu))
+              for s in (1, 2)]
+    wants = [layer(x, r, params) for x, r in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(layer(*inputs[i], params))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for result in got[i]:
+            for a, b in zip(result, wants[i]):
+                assert_bitwise_equal(a, b)
