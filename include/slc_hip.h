@@ -629,7 +629,7 @@ SLC_API int slc_hip_rope_decode_attention(
  * codes = the nearest whole numbers, ties to even, to 127 y / max|y|, decided as
  * 64-bit arithmetic does; code * scale is the value that a code stands for.  A
  * row of zeros has scale 0 and codes 0; a row with a NaN or an infinity, or whose
- * scale has no finite fp32 value, has scale NaN and codes 0.  rows <= 2^31 - 1,
+ * scale has no finite fp32 value, has scale NaN (and codes without a meaning).  rows <= 2^31 - 1,
  * hidden <= SLC_Q8_MAX_K, any alignment that the element type allows; codes
  * [rows, hidden] and scales [rows] are contiguous.  Outputs must not overlap the
  * inputs.
@@ -637,8 +637,8 @@ SLC_API int slc_hip_rope_decode_attention(
  *   quantize_q8 : y = input
  *   rms_norm_q8 : h = input, or with a residual (and then `summed`, contiguous)
  *                 h = summed = round(input + residual);
- *                 y = h * rsqrt(mean(h^2) + epsilon) * weight, unrounded (the
- *                 mean in fp64); one dtype for all
+ *                 y = h * rsqrt(mean(h^2) + epsilon) * weight, unrounded;
+ *                 epsilon finite and not negative, one dtype for all
  *   swiglu_q8   : y = gate / (1 + exp(-gate)) * up, unrounded
  */
 #define SLC_Q8_MAX_K 131071

@@ -4,7 +4,7 @@ A row ``y`` has ``scale = max|y| / 127`` and ``codes`` = the whole numbers neare
 to ``127 y / max|y|`` (ties to even), decided as 64-bit arithmetic does;
 ``code * scale`` is the value that a code stands for.  A row of zeros has scale 0; a
 row with a NaN or an infinity (or whose scale fp32 cannot hold) has scale NaN, so
-that whatever is computed from it is NaN too, and codes 0.
+that whatever is computed from it is NaN too.
 
 A layer's linears run on them as ``hip_add_rms_norm_q8`` -> ``hip_linear_q8``
 (Q/K/V, or gate and up in one weight), ``hip_quantize_q8`` of the attention output

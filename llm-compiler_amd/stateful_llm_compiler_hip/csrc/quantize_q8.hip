@@ -1,29 +1,27 @@
 // Rows to 8-bit codes with one scale per row: of a tensor, of its RMSNorm (with
 // the residual's addition), or of a SwiGLU product.
 //
-// With y the row that is coded (float for the tensor itself, h * w * rstd for
-// the norm, silu(g) * u for SwiGLU) and a = max |y|:
+// With y the row that is coded (the tensor itself, h * w * rstd for the norm,
+// silu(g) * u for SwiGLU) and a = max |y|:
 //   scale = a / 127,   code = nearest whole number, ties to even, of 127 y / a.
 // rstd divides every y of a row alike, so the norm's codes are those of h * w
 // and do not wait for the statistic.
 //
 // Every code is the formula's, not that of a rounded y: a code is decided in
 // fp32 from v ~ y and 1 / a (one fma rounds v * 127 / a to a whole number, a
-// second gives the exact distance r to it), and where |r| comes within the
+// second gives its distance from it), and where the distance comes within the
 // error of the fp32 form of 1/2 it is decided again in fp64 from the inputs,
-// with a itself in fp64.  The fp32 form's error: products of two 16-bit values
-// are exact in fp32, so 127 / a and nothing else rounds, 127 * 2^-23; products
-// of fp32 values add 2 * 127 * 2^-24; SwiGLU's exp, sum, quotient and product
-// add at most 8 * 127 * 2^-24.  kBorder covers each; about one element in 5000
+// with a itself in fp64.  In units of 127 * 2^-24: a and 127 / a round by 1 each,
+// v by 0 where both factors have 16 bits, by 1 in the norm of fp32 values, by 8
+// in SwiGLU (silu_f32); kBorder covers the sum.  About one element in 4000
 // (SwiGLU) is decided twice.  Rows whose a is 0, not finite, or so small or
 // large that fp32 products round or overflow run in fp64 as a whole.
 //
-// One workgroup of W waves holds a row (a wave each of four rows for W = 1) in
-// registers, NV 16-byte vectors per lane, so every input is read once and every
-// output written once: HBM-bound from about a thousand rows, bound by the launch
-// and two dependent reductions below.  Rows past 16 waves' registers are read
-// twice (LOOP).  The sum of squares is held in fp64: it costs a conversion and
-// an fma per element, and no square overflows.
+// One workgroup holds a row in registers, NV 16-byte vectors per lane, so every
+// input is read once and every output written once: HBM-bound from about a
+// thousand rows, bound by the launch and two dependent reductions below.  Rows
+// past 16 waves' registers are read twice (LOOP).  All loads are issued before
+// the first use, without branches: buffer loads whose range ends with the row.
 #include <float.h>
 
 #include "common.hpp"
@@ -39,15 +37,22 @@ struct Args {
   void* summed;        // a + b
   int8_t* codes;
   float* scales;
-  int64_t rows, a_rs, b_rs;
+  int64_t row0, a_rs, b_rs;
+  double per_hidden;   // 1 / hidden
   int hidden;
   float eps;
 };
 
+constexpr int kMaxWaves = 16;
 constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to a whole number
-constexpr float kLow = 0x1p-60f, kHigh = 0x1p100f;  // a in fp32: products neither lost nor infinite
-// SwiGLU: where exp(-g) overflows fp32, |silu(g)| < 2^-121 counts as 0; with
-// |u| up to this the product is under 2^-31 of the least a.
+// a in fp32 between these: no product is lost or infinite, nor is a scale (a norm's
+// mean square within the next range makes rstd at most 2^49).
+constexpr float kLow = 0x1p-60f, kHigh = 0x1p60f;
+// Squares of eight values are summed in fp32 before they join the row's fp64
+// sum; one whose total is between these has lost nothing to the ends of fp32.
+constexpr double kLowSquares = 0x1p-80, kHighSquares = 0x1p100;
+// SwiGLU: where 1 + exp(-g) has no normal fp32 reciprocal, |silu(g)| < 2^-119
+// counts as 0; with |u| up to this the product is under 2^-29 of the least a.
 constexpr float kMostUp = 0x1p30f;
 
 template <typename T, int SRC>
@@ -57,349 +62,471 @@ struct Traits {
   static constexpr bool kHasW = SRC == kNorm || SRC == kAddNorm;
   // Whether the fp32 v may differ from y (then a is taken again in fp64).
   static constexpr bool kInexact = SRC == kSwiglu || (kHasW && sizeof(T) == 4);
-  static constexpr float kBorder = 0.5f - (SRC == kSwiglu ? 0x1.8p-14f : 0x1p-14f);
+  static constexpr float kBorder = 0.5f - (SRC == kSwiglu ? 0x1p-13f : 0x1p-15f);
   // v within this factor below the largest v may be the largest y.
   static constexpr float kNear = 1.0f - 0x1p-19f;
 };
 
-template <typename T>
-struct Raw {
-  uint4 a, b, w;
-};
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// 16 bytes from an address of any alignment that T allows, zeros past `left`
-// elements.
-template <typename T>
-__device__ __forceinline__ uint4 load_vec(const T* p, int left) {
-  constexpr int VEC = 16 / sizeof(T);
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (left >= VEC) {
-    __builtin_memcpy(&v, p, 16);
-  } else {
-    T e[VEC] = {};
-#pragma unroll
-    for (int k = 0; k < VEC; ++k)
-      if (k < left) e[k] = p[k];
-    __builtin_memcpy(&v, e, 16);
-  }
-  return v;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* row, int bytes) {
+  const uint64_t address = reinterpret_cast<uint64_t>(row);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(address));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(address >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<void*>(static_cast<uint64_t>(hi) << 32 | lo), 0,
+      __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
+// One row of an operand: 16-byte vectors, zeros past its end.  The range holds
+// whole 4-byte words; an odd 16-bit element at the end is loaded by itself.
 template <typename T>
-__device__ __forceinline__ float elem(const uint4& v, int k) {
-  T e[16 / sizeof(T)];
-  __builtin_memcpy(e, &v, 16);
-  return slc::to_f32(e[k]);
+struct Row {
+  const T* base;
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ Row(const void* p, int64_t offset, int hidden)
+      : base(static_cast<const T*>(p) + offset),
+        rsrc(row_rsrc(base, hidden * static_cast<int>(sizeof(T)) & ~3)) {}
+  __device__ __forceinline__ u32x4 load(int vec) const {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, vec * 16, 0, 0));
+  }
+  // The odd element into the vector that it belongs to.
+  __device__ __forceinline__ void patch(u32x4& v, int vec, int hidden) const {
+    if constexpr (sizeof(T) == 2) {
+      const int last = hidden - 1;
+      if (last / 8 != vec) return;
+      const uint32_t bits = __builtin_bit_cast(uint16_t, base[last]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (last % 8 == 2 * k) v[k] = bits;
+    }
+  }
+};
+
+// Element k of a vector as fp32.
+template <typename T>
+__device__ __forceinline__ float elem(const u32x4& v, int k) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(v[k]);
+  } else {
+    T e;
+    e.bits = static_cast<uint16_t>(v[k / 2] >> (16 * (k % 2)));
+    return slc::to_f32(e);
+  }
 }
 
 // round(a + b) in T, element by element.
 template <typename T>
-__device__ __forceinline__ uint4 add_vec(const uint4& a, const uint4& b) {
-  constexpr int VEC = 16 / sizeof(T);
-  T o[VEC];
+__device__ __forceinline__ u32x4 add_vec(const u32x4& a, const u32x4& b) {
+  u32x4 v;
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) o[k] = slc::from_f32<T>(elem<T>(a, k) + elem<T>(b, k));
-  uint4 v;
-  __builtin_memcpy(&v, o, 16);
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      v[k] = __float_as_uint(elem<T>(a, k) + elem<T>(b, k));
+    } else {
+      const T lo = slc::from_f32<T>(elem<T>(a, 2 * k) + elem<T>(b, 2 * k));
+      const T hi = slc::from_f32<T>(elem<T>(a, 2 * k + 1) + elem<T>(b, 2 * k + 1));
+      v[k] = lo.bits | static_cast<uint32_t>(hi.bits) << 16;
+    }
+  }
   return v;
 }
 
-__device__ __forceinline__ float swiglu_f32(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-
-// v of element k of a vector (after the residual's addition).
-template <typename T, int SRC>
-__device__ __forceinline__ float value(const Raw<T>& r, int k) {
-  if constexpr (SRC == kPlain) return elem<T>(r.a, k);
-  if constexpr (SRC == kSwiglu) return swiglu_f32(elem<T>(r.a, k), elem<T>(r.b, k));
-  return elem<T>(r.a, k) * elem<T>(r.w, k);
+// silu(g) to 7 * 2^-24 of itself: exp(-g) = 2^t (1 + d), t = -g log2(e) rounded
+// and d the rest of that product times ln 2 (rounding 2^t by 2 * 2^-24, which the
+// division's result keeps at most), the sum by 1, the reciprocal by 2, the product
+// by 1, d by under 1.
+__device__ __forceinline__ float silu_f32(float g) {
+  constexpr float kLog2e = 0x1.715476p+0f, kLog2eLow = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;
+  const float t = -g * kLog2e;
+  const float rest = fmaf(-g, kLog2eLow, fmaf(-g, kLog2e, -t));
+  const float p = __builtin_amdgcn_exp2f(t);
+  // Past the range p is infinite (and rest may be too): the sum stays so.
+  const float e = t < 128.0f ? fmaf(p, rest * kLn2, p) : p;
+  return g * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-// y of element i of a row in fp64, without the norm's rstd, from memory.
+// h (the input, or its rounded sum with the residual) and y, without the norm's
+// rstd, of element i of a row in fp64, from memory.
+template <typename T, int SRC>
+__device__ __forceinline__ double summed_value(const Args& p, int64_t row, int i) {
+  const float a = slc::to_f32(static_cast<const T*>(p.a)[row * p.a_rs + i]);
+  if constexpr (SRC != kAddNorm) return a;
+  return slc::round_to<T>(a + slc::to_f32(static_cast<const T*>(p.b)[row * p.b_rs + i]));
+}
 template <typename T, int SRC>
 __device__ __forceinline__ double value64(const Args& p, int64_t row, int i) {
-  const float a = slc::to_f32(static_cast<const T*>(p.a)[row * p.a_rs + i]);
-  if constexpr (SRC == kPlain) return a;
-  if constexpr (SRC == kNorm)
-    return static_cast<double>(a) * slc::to_f32(static_cast<const T*>(p.w)[i]);
-  const float b = slc::to_f32(static_cast<const T*>(p.b)[row * p.b_rs + i]);
-  if constexpr (SRC == kAddNorm)
-    return static_cast<double>(slc::round_to<T>(a + b)) * slc::to_f32(static_cast<const T*>(p.w)[i]);
-  return a / (1.0 + exp(-static_cast<double>(a))) * b;
+  const double h = summed_value<T, SRC>(p, row, i);
+  if constexpr (Traits<T, SRC>::kHasW) return h * slc::to_f32(static_cast<const T*>(p.w)[i]);
+  if constexpr (SRC == kSwiglu)
+    return h / (1.0 + exp(-h)) * slc::to_f32(static_cast<const T*>(p.b)[row * p.b_rs + i]);
+  return h;
 }
 
-__device__ __forceinline__ double shfl_xor64(double v, int offset) {
-  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(bits), offset, 64);
-  const uint32_t hi = __shfl_xor(static_cast<uint32_t>(bits >> 32), offset, 64);
-  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+// 1 / sqrt(x) to a few units of 2^-52: the instruction's 2^-24 or better, squared
+// by a Newton step.  (NaN for 0 and infinity, whose rows have no scale.)
+__device__ __forceinline__ double rsqrt64(double x) {
+  double r = __builtin_amdgcn_rsq(x);
+  r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
+  return fma(r * 0.5, fma(-x * r, r, 1.0), r);
 }
 
-// The row's sums and maxima over its W waves.  Each use of an array of `slots`
-// is followed by a barrier before its next.
+// ---- reductions over a wave in the VALU --------------------------------------------
+// Lane pairs one apart, two apart, mirrored in eight, mirrored in sixteen (DPP),
+// then rows of 16 and halves of 32 (lane swaps): every lane ends with the total.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
+}
+constexpr int kPairs = 0xB1, kQuads = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {
+  x = max(x, dpp<kPairs>(x));
+  x = max(x, dpp<kQuads>(x));
+  x = max(x, dpp<kHalfMirror>(x));
+  x = max(x, dpp<kMirror>(x));
+  auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(r[0], r[1]);
+}
+
+template <typename OP>
+__device__ __forceinline__ double wave_reduce64(double v, OP op) {
+  auto both = [](uint32_t lo, uint32_t hi) {
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+  };
+  auto split = [](double x, uint32_t& lo, uint32_t& hi) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    lo = static_cast<uint32_t>(bits);
+    hi = static_cast<uint32_t>(bits >> 32);
+  };
+  uint32_t lo, hi;
+  split(v, lo, hi);
+  v = op(v, both(dpp<kPairs>(lo), dpp<kPairs>(hi)));
+  split(v, lo, hi);
+  v = op(v, both(dpp<kQuads>(lo), dpp<kQuads>(hi)));
+  split(v, lo, hi);
+  v = op(v, both(dpp<kHalfMirror>(lo), dpp<kHalfMirror>(hi)));
+  split(v, lo, hi);
+  v = op(v, both(dpp<kMirror>(lo), dpp<kMirror>(hi)));
+  split(v, lo, hi);
+  auto l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+  auto h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+  v = op(both(l[0], h[0]), both(l[1], h[1]));
+  split(v, lo, hi);
+  l = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+  h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+  return op(both(l[0], h[0]), both(l[1], h[1]));
+}
+
 struct Shared {
-  double sum[16];
-  double max64[16];
-  uint32_t max32[16];
-  uint32_t max_up[16];
+  double sum[kMaxWaves];
+  double max64[kMaxWaves];
+  double sum64[kMaxWaves];
+  uint32_t max32[kMaxWaves];
+  uint32_t max_up[kMaxWaves];
 };
 
-template <typename T, int SRC, int W, int NV, bool LOOP>
-__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void quantize_kernel(Args p) {
+// Low bytes of eight (four) words, first lowest.
+__device__ __forceinline__ uint32_t pack4(const uint32_t* b) {
+  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+  return lo | hi;
+}
+
+// One workgroup of whole waves per row.
+template <typename T, int SRC, int NV, bool LOOP>
+__global__ __launch_bounds__(kMaxWaves * 64) void quantize_kernel(Args p) {
   using TR = Traits<T, SRC>;
   constexpr int VEC = TR::VEC;
-  constexpr int kLanes = W * 64;
   __shared__ Shared shared;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : blockIdx.x;
-  if (row >= p.rows) return;  // whole waves, and whole workgroups for W > 1
-  const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const int lanes = blockDim.x, waves = lanes >> 6;
+  const int t = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int64_t row = p.row0 + blockIdx.x;
   const int hidden = p.hidden;
-  const int rounds = LOOP ? (hidden + kLanes * VEC - 1) / (kLanes * VEC) : NV;
-  const T* a = static_cast<const T*>(p.a) + row * p.a_rs;
-  const T* b = static_cast<const T*>(p.b) + row * p.b_rs;
-  const T* w = static_cast<const T*>(p.w);
+  const int rounds = LOOP ? (hidden + lanes * VEC - 1) / (lanes * VEC) : NV;
+  const bool odd = sizeof(T) == 2 && (hidden & 1) != 0;
+  const Row<T> ra(p.a, row * p.a_rs, hidden);
+  const Row<T> rb(TR::kHasB ? p.b : p.a, TR::kHasB ? row * p.b_rs : 0, TR::kHasB ? hidden : 0);
+  const Row<T> rw(TR::kHasW ? p.w : p.a, 0, TR::kHasW ? hidden : 0);
   T* summed = static_cast<T*>(p.summed) + row * hidden;
   int8_t* codes = p.codes + row * hidden;
 
-  auto load = [&](int i, Raw<T>& r) {
-    const int e = (t + kLanes * i) * VEC;
-    const int left = hidden - e;
-    r.a = load_vec<T>(a + e, left);
-    if constexpr (TR::kHasW) r.w = load_vec<T>(w + e, left);
-    if constexpr (TR::kHasB) r.b = load_vec<T>(b + e, left);
+  u32x4 a[LOOP ? 1 : NV], b[TR::kHasB && !LOOP ? NV : 1], w[TR::kHasW && !LOOP ? NV : 1];
+  float v[LOOP ? 1 : NV][VEC];
+  auto load = [&](int i, int slot) {
+    const int vec = t + lanes * i;
+    a[slot] = ra.load(vec);
+    if constexpr (TR::kHasW) w[slot] = rw.load(vec);
+    if constexpr (TR::kHasB) b[slot] = rb.load(vec);
   };
-
-  // ---- the row's largest |v|, its sum of squares, the sum h ------------------
-  Raw<T> raw[LOOP ? 1 : NV];
-  float v[(LOOP || SRC != kSwiglu) ? 1 : NV][VEC];
-  double sq = 0.0;
-  uint32_t top = 0, top_up = 0;
-  if constexpr (!LOOP) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) load(i, raw[i]);
-  }
-  auto gather = [&](int i, Raw<T>& r, float (&keep)[VEC]) {
-    const int e = (t + kLanes * i) * VEC;
-    const int left = hidden - e;
-    if (left <= 0) return;
-    if constexpr (SRC == kAddNorm) {
-      r.a = add_vec<T>(r.a, r.b);
-      if (left >= VEC) {
-        __builtin_memcpy(summed + e, &r.a, 16);
-      } else {
-        T o[VEC];
-        __builtin_memcpy(o, &r.a, 16);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k)
-          if (k < left) summed[e + k] = o[k];
-      }
-    }
+  auto patch = [&](int i, int slot) {
+    const int vec = t + lanes * i;
+    ra.patch(a[slot], vec, hidden);
+    if constexpr (TR::kHasW) rw.patch(w[slot], vec, hidden);
+    if constexpr (TR::kHasB) rb.patch(b[slot], vec, hidden);
+  };
+  // The slot's v (and h, in a) from its vectors; zeros past the row stay zeros.
+  auto evaluate = [&](int slot) {
+    if constexpr (SRC == kAddNorm) a[slot] = add_vec<T>(a[slot], b[slot]);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      const float x = value<T, SRC>(r, k);
-      if constexpr (SRC == kSwiglu) {
-        keep[k] = x;
-        top_up = max(top_up, __float_as_uint(fabsf(elem<T>(r.b, k))));
-      }
-      // As bits: a NaN is above infinity and stays.
-      top = max(top, __float_as_uint(fabsf(x)));
+      const float x = elem<T>(a[slot], k);
+      if constexpr (SRC == kPlain) v[slot][k] = x;
+      if constexpr (TR::kHasW) v[slot][k] = x * elem<T>(w[slot], k);
+      if constexpr (SRC == kSwiglu) v[slot][k] = silu_f32(x) * elem<T>(b[slot], k);
+    }
+  };
+
+  // ---- the largest |v|, the sum of squares, the sum h --------------------------
+  // As bits, in two halves: the largest positive (and positive NaNs above) by
+  // signed order, the largest negative by unsigned order.
+  int most = 0;
+  uint32_t least = 0, most_up = 0;
+  double sq = 0.0;
+  auto gather = [&](int i, int slot) {
+    evaluate(slot);
+    float squares = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const uint32_t bits = __float_as_uint(v[slot][k]);
+      most = max(most, static_cast<int>(bits));
+      least = max(least, bits);
+      if constexpr (SRC == kSwiglu)
+        most_up = max(most_up, __float_as_uint(fabsf(elem<T>(b[slot], k))));
       if constexpr (TR::kHasW) {
-        const double h = elem<T>(r.a, k);
-        sq = fma(h, h, sq);
+        const float h = elem<T>(a[slot], k);
+        squares = fmaf(h, h, squares);
+      }
+    }
+    if constexpr (TR::kHasW) sq += squares;
+    if constexpr (SRC == kAddNorm) {
+      const int e = (t + lanes * i) * VEC;
+      if (e + VEC <= hidden) {
+        __builtin_memcpy(summed + e, &a[slot], 16);
+      } else if (e < hidden) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (e + k < hidden) summed[e + k] = slc::from_f32<T>(elem<T>(a[slot], k));
       }
     }
   };
   if constexpr (LOOP) {
     for (int i = 0; i < rounds; ++i) {
-      load(i, raw[0]);
-      gather(i, raw[0], v[0]);
+      load(i, 0);
+      if (odd) patch(i, 0);
+      gather(i, 0);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) gather(i, raw[i], v[SRC == kSwiglu ? i : 0]);
-  }
+    for (int i = 0; i < NV; ++i) load(i, i);
+    if (odd) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    top = max(top, static_cast<uint32_t>(__shfl_xor(top, o, 64)));
-    if constexpr (SRC == kSwiglu) top_up = max(top_up, static_cast<uint32_t>(__shfl_xor(top_up, o, 64)));
-    if constexpr (TR::kHasW) sq += shfl_xor64(sq, o);
+      for (int i = 0; i < NV; ++i) patch(i, i);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) gather(i, i);
   }
-  if constexpr (W > 1) {
+  uint32_t top = max(static_cast<uint32_t>(most), (least >> 31) != 0 ? least & 0x7fffffffu : 0u);
+  const uint32_t own_top = top;  // this lane's largest
+  top = wave_max_u32(top);
+  if constexpr (SRC == kSwiglu) most_up = wave_max_u32(most_up);
+  auto add = [](double x, double y) { return x + y; };
+  if constexpr (TR::kHasW) sq = wave_reduce64(sq, add);
+  if (waves > 1) {
     if ((t & 63) == 0) {
       shared.max32[wave] = top;
-      shared.max_up[wave] = top_up;
-      shared.sum[wave] = sq;
+      if constexpr (SRC == kSwiglu) shared.max_up[wave] = most_up;
+      if constexpr (TR::kHasW) shared.sum[wave] = sq;
     }
     __syncthreads();
-    top = top_up = 0;
-    sq = 0.0;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
+    for (int i = 0; i < waves; ++i) {
       top = max(top, shared.max32[i]);
-      top_up = max(top_up, shared.max_up[i]);
-      sq += shared.sum[i];
+      if constexpr (SRC == kSwiglu) most_up = max(most_up, shared.max_up[i]);
     }
   }
-  // Every wave of the row holds the same values from here on.
+  // Every wave of the row holds the same top from here on.
   const float vmax = __uint_as_float(top);
   bool fast = vmax >= kLow && vmax <= kHigh;
-  if constexpr (SRC == kSwiglu) fast = fast && __uint_as_float(top_up) <= kMostUp;
+  if constexpr (SRC == kSwiglu) fast = fast && __uint_as_float(most_up) <= kMostUp;
 
-  // ---- a in fp64 ---------------------------------------------------------------
-  double a64 = vmax;
+  // ---- a in fp64: of the values near the largest, or of all that are not zero -----
+  double a64 = vmax, sq64 = 0.0;
   if (TR::kInexact || !fast) {
     a64 = 0.0;
-    bool bad = false;
-    auto take = [&](int e) {
-      const double y = fabs(value64<T, SRC>(p, row, e));
-      bad = bad || !(y <= DBL_MAX);
-      a64 = y > a64 ? y : a64;
-    };
-    if (fast) {
-      if constexpr (TR::kInexact) {
-        const float near = vmax * TR::kNear;
-        auto pick = [&](int i, const Raw<T>& r, const float (&kept)[VEC]) {
-          const int e = (t + kLanes * i) * VEC;
-          uint32_t mask = 0;
+    const float near = vmax * TR::kNear;
+    auto pick = [&](int i, int slot) {
+      uint32_t mask = 0;
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            const float x = SRC == kSwiglu && !LOOP ? kept[k] : value<T, SRC>(r, k);
-            mask |= fabsf(x) >= near ? 1u << k : 0u;
-          }
-          if (e >= hidden) mask = 0;
-          while (mask != 0) {  // elements past the row hold 0, under `near`
-            take(e + __builtin_ctz(mask));
-            mask &= mask - 1;
-          }
-        };
-        if constexpr (LOOP) {
-          for (int i = 0; i < rounds; ++i) {
-            load(i, raw[0]);
-            if constexpr (SRC == kAddNorm) raw[0].a = add_vec<T>(raw[0].a, raw[0].b);
-            pick(i, raw[0], v[0]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < NV; ++i) pick(i, raw[i], v[SRC == kSwiglu ? i : 0]);
+      for (int k = 0; k < VEC; ++k) {
+        // NaNs and infinities are not zero; 0 stays 0 whatever it is multiplied
+        // by, but an infinity (whose product is NaN in v too).
+        const bool live = fast ? fabsf(v[slot][k]) >= near
+                               : elem<T>(a[slot], k) != 0.0f || v[slot][k] != 0.0f;
+        mask |= live ? 1u << k : 0u;
+      }
+      while (mask != 0) {  // elements past the row hold 0
+        const int k = __builtin_ctz(mask), e = (t + lanes * i) * VEC + k;
+        mask &= mask - 1;
+        double y = fabs(value64<T, SRC>(p, row, e));
+        if (!(y <= DBL_MAX)) y = __builtin_inf();
+        a64 = y > a64 ? y : a64;
+        if (TR::kHasW && !fast) {
+          const double h = summed_value<T, SRC>(p, row, e);
+          sq64 = fma(h, h, sq64);
         }
       }
-    } else {
-      for (int e = t; e < hidden; e += kLanes) take(e);
-    }
-    if (bad) a64 = __builtin_inf();
+    };
+    if (!fast || __uint_as_float(own_top) >= near) {
+      if constexpr (LOOP) {
+        for (int i = 0; i < rounds; ++i) {
+          load(i, 0);
+          if (odd) patch(i, 0);
+          evaluate(0);
+          pick(i, 0);
+        }
+      } else {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const double other = shfl_xor64(a64, o);
-      a64 = other > a64 ? other : a64;
+        for (int i = 0; i < NV; ++i) pick(i, i);
+      }
     }
-    if constexpr (W > 1) {
-      if ((t & 63) == 0) shared.max64[wave] = a64;
+    a64 = wave_reduce64(a64, [](double x, double y) { return x > y ? x : y; });
+    if constexpr (TR::kHasW) sq64 = wave_reduce64(sq64, add);
+    if (waves > 1) {
+      if ((t & 63) == 0) {
+        shared.max64[wave] = a64;
+        if constexpr (TR::kHasW) shared.sum64[wave] = sq64;
+      }
       __syncthreads();
-      a64 = 0.0;
-#pragma unroll
-      for (int i = 0; i < W; ++i) a64 = shared.max64[i] > a64 ? shared.max64[i] : a64;
+      sq64 = 0.0;
+      for (int i = 0; i < waves; ++i) {
+        a64 = shared.max64[i] > a64 ? shared.max64[i] : a64;
+        if constexpr (TR::kHasW) sq64 += shared.sum64[i];
+      }
     }
   }
-
-  // ---- the scale ---------------------------------------------------------------
-  double scale = a64 / 127.0;
-  if constexpr (TR::kHasW) scale /= sqrt(sq / static_cast<double>(hidden) + static_cast<double>(p.eps));
-  const bool coded = scale <= static_cast<double>(FLT_MAX);  // false for NaN
-  if (t == 0) p.scales[row] = coded ? static_cast<float>(scale) : __builtin_nanf("");
+  // a / 127, times the norm's rstd; 1 / 127 rounds far below fp32.
+  auto scale_of = [&](double squares) {
+    double scale = a64 * (1.0 / 127.0);
+    if constexpr (TR::kHasW) scale *= rsqrt64(fma(squares, p.per_hidden, static_cast<double>(p.eps)));
+    return scale;
+  };
 
   // ---- the codes ---------------------------------------------------------------
   auto code64 = [&](int e) {
     return static_cast<int>(rint(value64<T, SRC>(p, row, e) * 127.0 / a64));
   };
   if (!fast) {
-    for (int e = t; e < hidden; e += kLanes)
-      codes[e] = static_cast<int8_t>(coded && a64 > 0.0 ? code64(e) : 0);
+    const double scale = scale_of(sq64);
+    const bool coded = scale <= static_cast<double>(FLT_MAX);  // false for NaN
+    if (t == 0) p.scales[row] = coded ? static_cast<float>(scale) : __builtin_nanf("");
+    const bool zero = !coded || a64 == 0.0;
+    for (int e = t; e < hidden; e += lanes) codes[e] = static_cast<int8_t>(zero ? 0 : code64(e));
     return;
   }
   const float inv = 127.0f / static_cast<float>(a64);
-  auto emit = [&](int i, const Raw<T>& r, const float (&kept)[VEC]) {
-    const int e = (t + kLanes * i) * VEC;
-    const int left = hidden - e;
-    if (left <= 0) return;
-    uint32_t bits[VEC];
-    float off[VEC], worst = 0.0f;
+  auto emit = [&](int i, int slot) {
+    const int e = (t + lanes * i) * VEC;
+    if (e >= hidden) return;
+    uint32_t bits[VEC], packed[VEC / 4];
+    float worst = 0.0f;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      const float x = SRC == kSwiglu && !LOOP ? kept[k] : value<T, SRC>(r, k);
-      const float whole = fmaf(x, inv, kMagic);
+      const float whole = fmaf(v[slot][k], inv, kMagic);
       bits[k] = __float_as_uint(whole);
-      off[k] = fabsf(fmaf(x, inv, kMagic - whole));
-      worst = fmaxf(worst, off[k]);
+      worst = fmaxf(worst, fabsf(fmaf(v[slot][k], inv, kMagic - whole)));
     }
-    uint64_t packed = 0;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) packed |= static_cast<uint64_t>(bits[k] & 0xff) << (8 * k);
+    for (int k = 0; k < VEC / 4; ++k) packed[k] = pack4(bits + 4 * k);
     if (worst > TR::kBorder) {
       uint32_t mask = 0;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) mask |= off[k] > TR::kBorder ? 1u << k : 0u;
+      for (int k = 0; k < VEC; ++k) {
+        const float whole = __uint_as_float(bits[k]);
+        mask |= fabsf(fmaf(v[slot][k], inv, kMagic - whole)) > TR::kBorder ? 1u << k : 0u;
+      }
       while (mask != 0) {  // elements past the row hold 0, at no border
-        const int k = __builtin_ctz(mask);
-        const uint64_t code = static_cast<uint64_t>(code64(e + k) & 0xff);
-        packed = (packed & ~(uint64_t{0xff} << (8 * k))) | code << (8 * k);
+        const int k = __builtin_ctz(mask), shift = 8 * (k & 3);
+        const uint32_t code = static_cast<uint32_t>(code64(e + k) & 0xff);
+#pragma unroll
+        for (int j = 0; j < VEC / 4; ++j)
+          if (j == k / 4) packed[j] = (packed[j] & ~(0xffu << shift)) | code << shift;
         mask &= mask - 1;
       }
     }
-    if (!coded) packed = 0;
-    if (left >= VEC) {
-      __builtin_memcpy(codes + e, &packed, VEC);
+    if (e + VEC <= hidden) {
+      __builtin_memcpy(codes + e, packed, VEC);
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
-        if (k < left) codes[e + k] = static_cast<int8_t>(packed >> (8 * k));
+        if (e + k < hidden) codes[e + k] = static_cast<int8_t>(packed[k / 4] >> (8 * (k % 4)));
     }
   };
   if constexpr (LOOP) {
     for (int i = 0; i < rounds; ++i) {
-      load(i, raw[0]);
-      if constexpr (SRC == kAddNorm) raw[0].a = add_vec<T>(raw[0].a, raw[0].b);
-      emit(i, raw[0], v[0]);
+      load(i, 0);
+      if (odd) patch(i, 0);
+      evaluate(0);
+      emit(i, 0);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) emit(i, raw[i], v[SRC == kSwiglu ? i : 0]);
+    for (int i = 0; i < NV; ++i) emit(i, i);
   }
+
+  // ---- the scale: not waited for by the codes ------------------------------------
+  if (wave != 0) return;
+  if constexpr (TR::kHasW) {
+    if (waves > 1) {
+      sq = 0.0;
+      for (int i = 0; i < waves; ++i) sq += shared.sum[i];
+    }
+    if (!(sq >= kLowSquares && sq <= kHighSquares)) {
+      sq = 0.0;
+      for (int e = t; e < hidden; e += 64) {
+        const double h = summed_value<T, SRC>(p, row, e);
+        sq = fma(h, h, sq);
+      }
+      sq = wave_reduce64(sq, add);
+    }
+  }
+  const double scale = scale_of(sq);
+  if (t == 0) p.scales[row] = scale <= static_cast<double>(FLT_MAX) ? static_cast<float>(scale) : __builtin_nanf("");
 }
 
+#ifndef SLC_Q8_NV
+#define SLC_Q8_NV 2
+#endif
 template <typename T, int SRC>
-int launch(const Args& p, const char* what, hipStream_t stream) {
+int launch(Args p, int64_t rows, const char* what, hipStream_t stream) {
   const int vecs = (p.hidden + Traits<T, SRC>::VEC - 1) / Traits<T, SRC>::VEC;
-#define SLC_Q8(W, NV, LOOP)                                                              \
-  hipLaunchKernelGGL((quantize_kernel<T, SRC, W, NV, LOOP>),                             \
-                     dim3(static_cast<unsigned>(W == 1 ? (p.rows + 3) / 4 : p.rows)),    \
-                     dim3(W == 1 ? 256 : W * 64), 0, stream, p)
-  if (vecs <= 64) {
-    SLC_Q8(1, 1, false);
-  } else if (vecs <= 128) {
-    SLC_Q8(1, 2, false);
-  } else if (vecs <= 256) {
-    SLC_Q8(4, 1, false);
-  } else if (vecs <= 512) {
-    SLC_Q8(4, 2, false);
-  } else if (vecs <= 768) {
-    SLC_Q8(4, 3, false);
-  } else if (vecs <= 2048) {
-    SLC_Q8(16, 2, false);
-  } else if (vecs <= 4096) {
-    SLC_Q8(16, 4, false);
-  } else {
-    SLC_Q8(16, 1, true);
-  }
-#undef SLC_Q8
-  return slc_host::check_launch(what);
+  auto waves = [&](int nv) { return (vecs + 64 * nv - 1) / (64 * nv); };
+  // A grid holds fewer than 2^32 threads.
+  auto go = [&](auto kernel, int w) {
+    const int64_t most = ((int64_t{1} << 32) - 1) / (64 * w);
+    for (p.row0 = 0; p.row0 < rows; p.row0 += most) {
+      const int64_t part = rows - p.row0 < most ? rows - p.row0 : most;
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(part)), dim3(static_cast<unsigned>(w) * 64), 0,
+                         stream, p);
+      const int rc = slc_host::check_launch(what);
+      if (rc != SLC_OK) return rc;
+    }
+    return static_cast<int>(SLC_OK);
+  };
+  if (SLC_Q8_NV == 1 && waves(1) <= kMaxWaves) return go(quantize_kernel<T, SRC, 1, false>, waves(1));
+  if (waves(2) <= kMaxWaves) return go(quantize_kernel<T, SRC, 2, false>, waves(2));
+  if (waves(4) <= kMaxWaves) return go(quantize_kernel<T, SRC, 4, false>, waves(4));
+  return go(quantize_kernel<T, SRC, 1, true>, kMaxWaves);
 }
 
 template <int SRC>
-int dispatch(const Args& p, int dtype, const char* what, void* stream) {
+int dispatch(const Args& p, int64_t rows, int dtype, const char* what, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == SLC_BF16) return launch<slc::bf16_t, SRC>(p, what, s);
-  if (dtype == SLC_F16) return launch<slc::f16_t, SRC>(p, what, s);
-  return launch<float, SRC>(p, what, s);
+  if (dtype == SLC_BF16) return launch<slc::bf16_t, SRC>(p, rows, what, s);
+  if (dtype == SLC_F16) return launch<slc::f16_t, SRC>(p, rows, what, s);
+  return launch<float, SRC>(p, rows, what, s);
 }
 
 int check(const char* what, int dtype, int64_t rows, int64_t hidden) {
@@ -427,10 +554,9 @@ extern "C" int slc_hip_quantize_q8(const void* input, int8_t* codes, float* scal
   p.a = input;
   p.codes = codes;
   p.scales = scales;
-  p.rows = rows;
   p.a_rs = in_stride_row;
   p.hidden = static_cast<int>(hidden);
-  return dispatch<kPlain>(p, dtype, what, stream);
+  return dispatch<kPlain>(p, rows, dtype, what, stream);
 }
 
 extern "C" int slc_hip_rms_norm_q8(const void* input, const void* residual, const void* weight,
@@ -441,6 +567,7 @@ extern "C" int slc_hip_rms_norm_q8(const void* input, const void* residual, cons
   const int rc = check(what, dtype, rows, hidden);
   if (rc != SLC_OK || rows == 0) return rc;
   SLC_REQUIRE(input && weight && codes && scales, "%s: null pointer", what);
+  SLC_REQUIRE(epsilon >= 0.0f && epsilon <= FLT_MAX, "%s: epsilon must be finite and not negative", what);
   SLC_REQUIRE((residual == nullptr) == (summed == nullptr),
               "%s: a residual comes with a place for the sum, and the other way round", what);
   SLC_REQUIRE(aligned(input, dtype) && aligned(residual, dtype) && aligned(weight, dtype) &&
@@ -453,13 +580,13 @@ extern "C" int slc_hip_rms_norm_q8(const void* input, const void* residual, cons
   p.summed = summed;
   p.codes = codes;
   p.scales = scales;
-  p.rows = rows;
   p.a_rs = in_stride_row;
   p.b_rs = residual_stride_row;
   p.hidden = static_cast<int>(hidden);
+  p.per_hidden = 1.0 / static_cast<double>(hidden);
   p.eps = epsilon;
-  if (residual == nullptr) return dispatch<kNorm>(p, dtype, what, stream);
-  return dispatch<kAddNorm>(p, dtype, what, stream);
+  if (residual == nullptr) return dispatch<kNorm>(p, rows, dtype, what, stream);
+  return dispatch<kAddNorm>(p, rows, dtype, what, stream);
 }
 
 extern "C" int slc_hip_swiglu_q8(const void* gate, const void* up, int8_t* codes, float* scales,
@@ -476,9 +603,8 @@ extern "C" int slc_hip_swiglu_q8(const void* gate, const void* up, int8_t* codes
   p.b = up;
   p.codes = codes;
   p.scales = scales;
-  p.rows = rows;
   p.a_rs = gate_stride_row;
   p.b_rs = up_stride_row;
   p.hidden = static_cast<int>(hidden);
-  return dispatch<kSwiglu>(p, dtype, what, stream);
+  return dispatch<kSwiglu>(p, rows, dtype, what, stream);
 }

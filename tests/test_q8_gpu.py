@@ -20,6 +20,12 @@ DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 HALF32 = 2.0**-24
 
 
+# Squares are summed in fp32 in chains of at most eight, each step off by at most
+# half a step of a growing sum: 8 * 2^-24 of the mean, half of that of its root;
+# one more for the scale's own rounding.
+NORM = 5
+
+
 def q8(y):
     """Codes (float64) and scales of the rows of a float64 y."""
 
@@ -29,9 +35,9 @@ def q8(y):
     return codes, torch.where(good, amax / 127, torch.nan).squeeze(-1)
 
 
-def check_rows(codes, scales, y, factor=1.0):
+def check_rows(codes, scales, y, factor=1.0, half_steps=1):
     """Codes of y and scales of y * factor [..., 1]; the scale is rounded once,
-    after few fp64 operations."""
+    after few fp64 operations, and a norm's by the five half steps of NORM."""
 
     want, want_scales = q8(y)
     want_scales = want_scales * (factor if isinstance(factor, float) else factor.squeeze(-1))
@@ -43,7 +49,7 @@ def check_rows(codes, scales, y, factor=1.0):
     assert torch.equal(scales.isnan(), want_scales.isnan())
     fine = ~want_scales.isnan()
     # 2^-150 is half a step of the smallest fp32 numbers.
-    bound = want_scales * (HALF32 * 1.001) + 2.0**-150
+    bound = want_scales * (half_steps * HALF32 * 1.001) + 2.0**-150
     assert ((scales - want_scales).abs() <= bound)[fine].all()
 
 
@@ -91,7 +97,7 @@ def test_norm(gpu, dtype, residual, k):
         codes, scales = backends.hip_rms_norm_q8(x.to(gpu), w.to(gpu), epsilon=eps)
     h = x.double()
     eps32 = float(torch.tensor(eps, dtype=torch.float32))
-    check_rows(codes, scales, h * w.double(), torch.rsqrt(h.square().mean(-1, keepdim=True) + eps32))
+    check_rows(codes, scales, h * w.double(), torch.rsqrt(h.square().mean(-1, keepdim=True) + eps32), NORM)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -167,7 +173,7 @@ def test_rows_without_a_value_and_extreme_rows(gpu, dtype, k):
     y = h * w.double()
     y[~torch.isfinite(y).all(-1) | ~torch.isfinite(rstd).squeeze(-1)] = torch.nan
     codes, scales = backends.hip_rms_norm_q8(x.to(gpu), w.to(gpu), epsilon=1e-6)
-    check_rows(codes, scales, y, rstd)
+    check_rows(codes, scales, y, rstd, NORM)
     residual = torch.zeros_like(x)
     summed, codes2, scales2 = backends.hip_add_rms_norm_q8(x.to(gpu), residual.to(gpu), w.to(gpu), epsilon=1e-6)
     assert_bitwise_equal(codes2, codes)
@@ -398,6 +404,18 @@ def test_weight_rows_past_32_bits(gpu):
         for part in (slice(0, 40), slice(2**17, 2**17 + 40), slice(n - 40, n)):
             check_product(y[:, part], codes.cpu(), scales.cpu(), weight[part].cpu(), weight_scales[part].cpu(), None,
                           torch.float32)
+
+
+def test_more_rows_than_one_grid(gpu):
+    # 64 threads a row: 2^26 rows are 2^32 threads, one more than a grid holds.
+    announce("2^26 + 5 rows")
+    rows = 2**26 + 5
+    x = torch.ones(rows, 1, dtype=torch.bfloat16, device=gpu)
+    x[-1] = -2.0
+    codes, scales = backends.hip_quantize_q8(x)
+    assert int(codes[:-1].amin()) == 127 and int(codes[-1]) == -127
+    one = torch.tensor(1.0, dtype=torch.float64) / 127
+    assert (scales[:-1] == float(one.float())).all() and float(scales[-1]) == float((2 * one).float())
 
 
 def test_rows_past_32_bits(gpu):
