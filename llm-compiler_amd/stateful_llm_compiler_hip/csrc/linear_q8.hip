@@ -137,11 +137,309 @@ __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
   }
 }
 
+// ---- prefill: tiles streamed through an LDS ring -----------------------------------
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, int64_t bytes) {
+  const uint64_t address = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(address));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(address >> 32));
+  const int clamped = bytes > 0x7fffffff ? 0x7fffffff : static_cast<int>(bytes);
+  return __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<void*>(static_cast<uint64_t>(hi) << 32 | lo), 0,
+      __builtin_amdgcn_readfirstlane(clamped), 0x00020000);
+}
+
+__device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds,
+                                          int voffset, int soffset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      rsrc, (__attribute__((address_space(3))) void*)lds, 16, voffset, soffset, 0, 0);
+}
+
+// Tile id -> (m_blk, n_blk): workgroup ids go round-robin to the 8 XCDs, each with
+// its own L2, so ids are gathered per XCD, then run in groups of kGroupM M-tiles,
+// N-tile-major inside a group.
+template <int kGroupM>
+__device__ __forceinline__ void xcd_tile_of(int id, int n_tiles, int m_tiles, int& m_blk,
+                                            int& n_blk) {
+  constexpr int kXcds = 8;
+  const int per = n_tiles * m_tiles / kXcds;
+  const int t = id < per * kXcds ? (id % kXcds) * per + id / kXcds : id;
+  const int span = kGroupM * n_tiles;
+  const int first_m = (t / span) * kGroupM;
+  const int gm = m_tiles - first_m < kGroupM ? m_tiles - first_m : kGroupM;
+  m_blk = first_m + (t % span) % gm;
+  n_blk = (t % span) / gm;
+}
+
+// Swizzle of the W tile: the 16 rows of a fragment are four runs of four, eight
+// apart, so the key takes row bits 0, 1 and 3.
+__device__ __forceinline__ int w_key(int row) { return (row & 3) | ((row >> 1) & 4); }
+
+// Element n of the bias; 0 past its range (of 0 bytes without a bias).
+template <typename T>
+__device__ __forceinline__ float load_bias(const __amdgpu_buffer_rsrc_t& rbias, int n) {
+  if constexpr (sizeof(T) == 4) {
+    return __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rbias, n * 4, 0, 0));
+  } else {
+    T v;
+    v.bits = static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rbias, n * 2, 0, 0));
+    return slc::to_f32(v);
+  }
+}
+
+// A lane's eight (16-bit) consecutive outputs, or two times four (fp32).
+template <typename T>
+__device__ __forceinline__ void store_run(const __amdgpu_buffer_rsrc_t& ry, const float (&v)[8],
+                                          int offset, int left, bool vectors) {
+  if constexpr (sizeof(T) == 4) {
+    if (vectors) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        i32x4_t o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __float_as_int(v[4 * h + e]);
+        if (4 * h < left) __builtin_amdgcn_raw_buffer_store_b128(o, ry, offset + 16 * h, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v[e]), ry, offset + 4 * e, 0, 0);
+    }
+  } else {
+    uint32_t o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = slc::from_f32<T>(v[e]).bits;
+    if (vectors) {
+      i32x4_t packed;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) packed[d] = static_cast<int>(o[2 * d] | (o[2 * d + 1] << 16));
+      if (left > 0) __builtin_amdgcn_raw_buffer_store_b128(packed, ry, offset, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left)
+          __builtin_amdgcn_raw_buffer_store_b16(static_cast<short>(o[e]), ry, offset + 2 * e, 0, 0);
+    }
+  }
+}
+
+// An offset past every range (kLimit) that stays below 2^31 with K added.
+constexpr int kPastRange = 0x7fffffff - (1 << 18);
+
+// 16-byte aligned rows of codes.  PW producer waves stream X and W k-tiles of
+// 128 codes straight into an S-stage LDS ring (buffer_load ... lds), without a
+// break at tile boundaries; CWM x CWN consumer waves read LDS and issue MFMAs.
+// Workgroups walk the output tiles id, id + grid, ....  One barrier per k-tile:
+// before it the producers wait until their loads of tile q have landed, after it
+// they refill the stage that every consumer has finished reading.  The consumers
+// multiply with W rows as the A operand, the W rows of two fragments interleaved
+// in runs of four, so that a lane holds eight consecutive outputs of one row and
+// stores them from registers.  Past K the X chunks are loaded as zeros (an offset
+// past the range), whatever the W chunks beside them hold.
+template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM>
+__global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p, int n_tiles,
+                                                                       int m_tiles, bool vectors) {
+  constexpr int CW = CWM * CWN;
+  constexpr int TM = BM / CWM, TN = BN / CWN;
+  constexpr int FM = TM / 16, FN = TN / 16;
+  constexpr int XB = BM * kBK;
+  constexpr int kStage = (BM + BN) * kBK;
+  constexpr int XO = BM / 8 / PW, WO = BN / 8 / PW, kOps = XO + WO;
+  static_assert(XO * PW * 8 == BM && WO * PW * 8 == BN, "operands split evenly over the producers");
+  static_assert((S - 2) * kOps <= 63, "the wait count fits vmcnt");
+  static_assert(TM % 16 == 0 && TN % 32 == 0, "whole fragments, in pairs over N");
+  __shared__ __attribute__((aligned(16))) unsigned char ring[S * kStage];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int total = n_tiles * m_tiles;
+  const int ktiles = (p.K + kBK - 1) / kBK;
+  const int first = blockIdx.x, step = gridDim.x;
+
+  if (wave >= CW) {
+    const int pw = wave - CW;
+    int voff[kOps];
+#pragma unroll
+    for (int i = 0; i < kOps; ++i) {
+      const int local = i < XO ? i : i - XO;
+      const int row = 8 * (pw + PW * local) + lane / 8;
+      const int chunk = (lane % 8) ^ (i < XO ? row & 7 : w_key(row));
+      voff[i] = (i < XO ? static_cast<int>(row * p.x_rs) : row * p.K) + chunk * 16;
+    }
+    // Whether this lane's X chunk of the last k-tile is past K: the chunk index
+    // depends on the lane alone (rows step by 8 over the instructions).
+    const int last_chunk = (lane % 8) ^ ((lane / 8) & 7);
+    const bool past = (ktiles - 1) * kBK + last_chunk * 16 >= p.K;
+    // The tile's ranges as base + bytes, rebuilt into scalars at every issue.
+    const int8_t* xb = p.x;
+    const int8_t* wb = p.w;
+    int64_t x_bytes = 0, w_bytes = 0;
+    int load_id = first, load_k = 0, slot = 0;
+    auto set_tile = [&](int id) {
+      x_bytes = w_bytes = 0;
+      if (id >= total) return;
+      int m_blk, n_blk;
+      xcd_tile_of<GM>(id, n_tiles, m_tiles, m_blk, n_blk);
+      const int64_t m0 = static_cast<int64_t>(m_blk) * BM, n0 = static_cast<int64_t>(n_blk) * BN;
+      const int64_t x_rows = p.M - m0 < BM ? p.M - m0 : BM;
+      const int64_t w_rows = p.N - n0 < BN ? p.N - n0 : BN;
+      xb = p.x + m0 * p.x_rs;
+      x_bytes = (x_rows - 1) * p.x_rs + p.K;
+      wb = p.w + n0 * p.K;
+      w_bytes = w_rows * p.K;
+    };
+    set_tile(load_id);
+    auto issue = [&]() {
+      unsigned char* dst = ring + __builtin_amdgcn_readfirstlane(slot) * kStage;
+      const int kb = __builtin_amdgcn_readfirstlane(load_id < total ? load_k * kBK : 0);
+      const __amdgpu_buffer_rsrc_t rx = make_rsrc(xb, x_bytes);
+      const __amdgpu_buffer_rsrc_t rw = make_rsrc(wb, w_bytes);
+      const bool cut = load_k == ktiles - 1 && past;
+#pragma unroll
+      for (int i = 0; i < kOps; ++i) {
+        if (i < XO)
+          lds_dma16(rx, dst + (pw + PW * i) * 1024, cut ? kPastRange : voff[i], kb);
+        else
+          lds_dma16(rw, dst + XB + (pw + PW * (i - XO)) * 1024, voff[i], kb);
+      }
+      slot = slot == S - 1 ? 0 : slot + 1;
+      if (++load_k == ktiles) {
+        load_k = 0;
+        load_id += step;
+        set_tile(load_id);
+      }
+    };
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t) issue();
+    const int64_t steps = static_cast<int64_t>((total - 1 - first) / step + 1) * ktiles;
+    for (int64_t q = 0; q < steps; ++q) {
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((S - 2) * kOps) : "memory");
+      issue();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    return;
+  }
+
+  const int c = lane & 15, g = lane >> 4;
+  const int wm = wave / CWN, wn = wave % CWN;
+  int slot = 0;
+  for (int id = first; id < total; id += step) {
+    int m_blk, n_blk;
+    xcd_tile_of<GM>(id, n_tiles, m_tiles, m_blk, n_blk);
+    const int64_t m0 = static_cast<int64_t>(m_blk) * BM, n0 = static_cast<int64_t>(n_blk) * BN;
+    const int rows = p.M - m0 < BM ? static_cast<int>(p.M - m0) : BM;
+    const int cols = p.N - n0 < BN ? static_cast<int>(p.N - n0) : BN;
+    // Scales and bias of this lane's outputs, requested before the k loop.
+    const __amdgpu_buffer_rsrc_t rsx = make_rsrc(p.sx + m0, rows * 4);
+    const __amdgpu_buffer_rsrc_t rsw = make_rsrc(p.sw + n0, cols * 4);
+    const __amdgpu_buffer_rsrc_t rbias =
+        make_rsrc(p.bias != nullptr ? static_cast<const T*>(p.bias) + n0 : nullptr,
+                  p.bias != nullptr ? cols * static_cast<int>(sizeof(T)) : 0);
+    float sx[FM], sw[FN][4], bias[FN][4];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      sx[i] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsx, (wm * TM + i * 16 + c) * 4, 0, 0));
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int n = wn * TN + (j >> 1) * 32 + 8 * g + (j & 1) * 4;
+      const auto four = __builtin_amdgcn_raw_buffer_load_b128(rsw, n * 4, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sw[j][r] = __int_as_float(static_cast<int>(four[r]));
+        bias[j][r] = load_bias<T>(rbias, n + r);
+      }
+    }
+    i32x4_t acc[FN][FM];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[j][i] = i32x4_t{0, 0, 0, 0};
+    for (int kt = 0; kt < ktiles; ++kt) {
+      // Tile kt is in its stage; the stage read before may be refilled.  No wait
+      // on stores: the previous tile's output may still be in flight.
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const unsigned char* xs = ring + slot * kStage;
+      const unsigned char* ws = xs + XB;
+      slot = slot == S - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int kk = 0; kk < kBK / 64; ++kk) {
+        i32x4_t a[FM], b[FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+          a[i] = *reinterpret_cast<const i32x4_t*>(xs + lds_offset(wm * TM + i * 16 + c, kk * 4 + g));
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int wrow = wn * TN + (j >> 1) * 32 + 8 * (c >> 2) + (j & 1) * 4 + (c & 3);
+          b[j] = *reinterpret_cast<const i32x4_t*>(ws + wrow * kBK + (((kk * 4 + g) ^ w_key(wrow)) << 4));
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int i = 0; i < FM; ++i) acc[j][i] = mfma(b[j], a[i], acc[j][i]);
+      }
+    }
+    constexpr int kSize = static_cast<int>(sizeof(T));
+    const __amdgpu_buffer_rsrc_t ry =
+        make_rsrc(static_cast<T*>(p.y) + m0 * p.y_rs + n0, (static_cast<int64_t>(rows) - 1) * p.y_rs * kSize + cols * kSize);
+#pragma unroll
+    for (int q = 0; q < FN / 2; ++q) {
+      const int n = wn * TN + q * 32 + 8 * g;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = wm * TM + i * 16 + c;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = 2 * q + (e >> 2), r = e & 3;
+          v[e] = finish(acc[j][i][r], sx[i], sw[j][r], bias[j][r]);
+        }
+        store_run<T>(ry, v, static_cast<int>(m * p.y_rs + n) * kSize, m < rows ? cols - n : 0, vectors);
+      }
+    }
+  }
+}
+
+constexpr int kNoPath = -2;
+
+// kNoPath (nothing launched) where 32-bit offsets do not reach over a tile's rows.
+template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM>
+int launch_stream(const Problem& p, hipStream_t stream) {
+  constexpr int64_t kLimit = (int64_t{1} << 31) - (1 << 20);
+  const int64_t m_tiles = (static_cast<int64_t>(p.M) + BM - 1) / BM;
+  const int64_t n_tiles = (static_cast<int64_t>(p.N) + BN - 1) / BN;
+  if (BM * p.x_rs >= kLimit || BM * p.y_rs * static_cast<int64_t>(sizeof(T)) >= kLimit ||
+      m_tiles * n_tiles >= (int64_t{1} << 30))
+    return kNoPath;
+  const int64_t total = m_tiles * n_tiles;
+  const int cus = slc_host::device_cu_count() / 8 * 8;
+  const int grid = static_cast<int>(total < cus || cus <= 0 ? total : cus);
+  const int64_t unit = 16 / static_cast<int64_t>(sizeof(T));
+  const bool vectors = p.N % unit == 0 && p.y_rs % unit == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+  hipLaunchKernelGGL((stream_kernel<T, BM, BN, CWM, CWN, PW, S, GM>), dim3(static_cast<unsigned>(grid)),
+                     dim3((CWM * CWN + PW) * 64), 0, stream, p, static_cast<int>(n_tiles),
+                     static_cast<int>(m_tiles), vectors);
+  return slc_host::check_launch("slc_hip_linear_q8(stream)");
+}
+
 template <typename T>
 int launch(const Problem& p, hipStream_t stream) {
+  const bool vec = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) == 0 &&
+                   p.K % 16 == 0 && p.x_rs % 16 == 0;
+#ifndef SLC_Q8_TILE
+#define SLC_Q8_TILE 1
+#endif
+  if (vec && p.M > 64) {
+    int rc = kNoPath;
+    if (SLC_Q8_TILE == 1) rc = launch_stream<T, 256, 128, 4, 2, 4, 3, 4>(p, stream);
+    if (SLC_Q8_TILE == 2) rc = launch_stream<T, 128, 128, 2, 4, 2, 4, 8>(p, stream);
+    if (SLC_Q8_TILE == 3) rc = launch_stream<T, 128, 64, 2, 2, 2, 4, 8>(p, stream);
+    if (SLC_Q8_TILE == 4) rc = launch_stream<T, 64, 64, 2, 2, 2, 6, 8>(p, stream);
+    if (rc != kNoPath) return rc;
+  }
   const int64_t m_tiles = (static_cast<int64_t>(p.M) + 63) / 64;
   const int64_t n_tiles = (static_cast<int64_t>(p.N) + 63) / 64;
-  SLC_REQUIRE(m_tiles <= 65535, "slc_hip_linear_q8: %d rows exceed one launch's grid", p.M);
+  SLC_REQUIRE(m_tiles <= 65535 && n_tiles < (1 << 24),
+              "slc_hip_linear_q8: %d x %d outputs exceed one launch's grid", p.M, p.N);
   hipLaunchKernelGGL((tile_kernel<T, 64, 64>),
                      dim3(static_cast<unsigned>(n_tiles), static_cast<unsigned>(m_tiles)), dim3(256),
                      0, stream, p);
@@ -160,6 +458,7 @@ extern "C" int slc_hip_linear_q8(const int8_t* input, const float* in_scales, co
               (long long)out_features, (long long)in_features);
   SLC_REQUIRE(rows < (1LL << 31) && out_features < (1LL << 31),
               "slc_hip_linear_q8: sizes exceed 2^31");
+  SLC_REQUIRE(in_stride_row >= 0 && out_stride_row >= 0, "slc_hip_linear_q8: negative stride");
   if (rows == 0) return SLC_OK;
   SLC_REQUIRE(input && in_scales && weight && weight_scales && output,
               "slc_hip_linear_q8: null pointer");
