@@ -174,56 +174,64 @@ __device__ __forceinline__ void xcd_tile_of(int id, int n_tiles, int m_tiles, in
 // apart, so the key takes row bits 0, 1 and 3.
 __device__ __forceinline__ int w_key(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-// Element n of the bias; 0 past its range (of 0 bytes without a bias).
+// Element n of the bias as it is stored (0 past its range, of 0 bytes without a
+// bias), and its value: converted at its use, so that the load is not waited for
+// where it is issued.
 template <typename T>
-__device__ __forceinline__ float load_bias(const __amdgpu_buffer_rsrc_t& rbias, int n) {
+__device__ __forceinline__ uint32_t load_bias(const __amdgpu_buffer_rsrc_t& rbias, int n) {
+  if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rbias, n * 4, 0, 0);
+  return static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rbias, n * 2, 0, 0));
+}
+template <typename T>
+__device__ __forceinline__ float bias_value(uint32_t bits) {
   if constexpr (sizeof(T) == 4) {
-    return __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rbias, n * 4, 0, 0));
+    return __uint_as_float(bits);
   } else {
     T v;
-    v.bits = static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rbias, n * 2, 0, 0));
+    v.bits = static_cast<uint16_t>(bits);
     return slc::to_f32(v);
-  }
-}
-
-// A lane's eight (16-bit) consecutive outputs, or two times four (fp32).
-template <typename T>
-__device__ __forceinline__ void store_run(const __amdgpu_buffer_rsrc_t& ry, const float (&v)[8],
-                                          int offset, int left, bool vectors) {
-  if constexpr (sizeof(T) == 4) {
-    if (vectors) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        i32x4_t o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __float_as_int(v[4 * h + e]);
-        if (4 * h < left) __builtin_amdgcn_raw_buffer_store_b128(o, ry, offset + 16 * h, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v[e]), ry, offset + 4 * e, 0, 0);
-    }
-  } else {
-    uint32_t o[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = slc::from_f32<T>(v[e]).bits;
-    if (vectors) {
-      i32x4_t packed;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) packed[d] = static_cast<int>(o[2 * d] | (o[2 * d + 1] << 16));
-      if (left > 0) __builtin_amdgcn_raw_buffer_store_b128(packed, ry, offset, 0, 0);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left)
-          __builtin_amdgcn_raw_buffer_store_b16(static_cast<short>(o[e]), ry, offset + 2 * e, 0, 0);
-    }
   }
 }
 
 // An offset past every range (kLimit) that stays below 2^31 with K added.
 constexpr int kPastRange = 0x7fffffff - (1 << 18);
+
+// A lane's run of eight consecutive outputs at a byte offset from the tile's first.
+// VST, 16-byte stores: what is outside the tile has an offset past the range (a run is
+// inside its row as a whole or not at all; 4 x 2 fp32 of it at `half`).  Else `left` of
+// the run are inside.
+template <typename T, bool VST>
+__device__ __forceinline__ void store_run(const __amdgpu_buffer_rsrc_t& ry, const float (&v)[8],
+                                          uint32_t offset, uint32_t half, int left) {
+  constexpr int kSize = static_cast<int>(sizeof(T));
+  uint32_t o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (kSize == 4)
+      o[e] = __float_as_uint(v[e]);
+    else
+      o[e] = slc::from_f32<T>(v[e]).bits;
+  }
+  if constexpr (VST) {
+#pragma unroll
+    for (int h = 0; h < kSize / 2; ++h) {
+      i32x4_t packed;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        packed[d] = static_cast<int>(kSize == 4 ? o[4 * h + d] : o[2 * d] | (o[2 * d + 1] << 16));
+      __builtin_amdgcn_raw_buffer_store_b128(packed, ry, static_cast<int>(h == 0 ? offset : half), 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e >= left) continue;
+      if constexpr (kSize == 4)
+        __builtin_amdgcn_raw_buffer_store_b32(static_cast<int>(o[e]), ry, static_cast<int>(offset + 4 * e), 0, 0);
+      else
+        __builtin_amdgcn_raw_buffer_store_b16(static_cast<short>(o[e]), ry, static_cast<int>(offset + 2 * e), 0, 0);
+    }
+  }
+}
 
 // 16-byte aligned rows of codes.  PW producer waves stream X and W k-tiles of
 // 128 codes straight into an S-stage LDS ring (buffer_load ... lds), without a
@@ -235,9 +243,9 @@ constexpr int kPastRange = 0x7fffffff - (1 << 18);
 // in runs of four, so that a lane holds eight consecutive outputs of one row and
 // stores them from registers.  Past K the X chunks are loaded as zeros (an offset
 // past the range), whatever the W chunks beside them hold.
-template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM>
+template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM, bool VST>
 __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p, int n_tiles,
-                                                                       int m_tiles, bool vectors) {
+                                                                       int m_tiles) {
   constexpr int CW = CWM * CWN;
   constexpr int TM = BM / CWM, TN = BN / CWN;
   constexpr int FM = TM / 16, FN = TN / 16;
@@ -335,7 +343,8 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
     const __amdgpu_buffer_rsrc_t rbias =
         make_rsrc(p.bias != nullptr ? static_cast<const T*>(p.bias) + n0 : nullptr,
                   p.bias != nullptr ? cols * static_cast<int>(sizeof(T)) : 0);
-    float sx[FM], sw[FN][4], bias[FN][4];
+    float sx[FM], sw[FN][4];
+    uint32_t bias[FN][4];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
       sx[i] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsx, (wm * TM + i * 16 + c) * 4, 0, 0));
@@ -378,12 +387,23 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
           for (int i = 0; i < FM; ++i) acc[j][i] = mfma(b[j], a[i], acc[j][i]);
       }
     }
+    // The scales have arrived while the tile was multiplied: waited for here, as a
+    // later wait would count this tile's stores too.
+#pragma unroll
+    for (int i = 0; i < FM; ++i) asm volatile("" : "+v"(sx[i]));
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) asm volatile("" : "+v"(sw[j][r]), "+v"(bias[j][r]));
     constexpr int kSize = static_cast<int>(sizeof(T));
     const __amdgpu_buffer_rsrc_t ry =
         make_rsrc(static_cast<T*>(p.y) + m0 * p.y_rs + n0, (static_cast<int64_t>(rows) - 1) * p.y_rs * kSize + cols * kSize);
+    const uint32_t rows16 = static_cast<uint32_t>(16 * p.y_rs) * kSize;  // 16 rows further down
 #pragma unroll
     for (int q = 0; q < FN / 2; ++q) {
       const int n = wn * TN + q * 32 + 8 * g;
+      const uint32_t at = static_cast<uint32_t>((wm * TM + c) * p.y_rs + n) * kSize;
+      const uint32_t whole = !VST || n < cols ? at : kPastRange, half = n + 4 < cols ? at + 16 : kPastRange;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int m = wm * TM + i * 16 + c;
@@ -391,15 +411,322 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = 2 * q + (e >> 2), r = e & 3;
-          v[e] = finish(acc[j][i][r], sx[i], sw[j][r], bias[j][r]);
+          v[e] = finish(acc[j][i][r], sx[i], sw[j][r], bias_value<T>(bias[j][r]));
         }
-        store_run<T>(ry, v, static_cast<int>(m * p.y_rs + n) * kSize, m < rows ? cols - n : 0, vectors);
+        store_run<T, VST>(ry, v, whole + i * rows16, half + i * rows16, m < rows ? cols - n : 0);
       }
     }
   }
 }
 
+// N loads of 1 KB into LDS, 8 KB apart from `lds` on, as one statement without results:
+// the compiler, which would wait for open loads into LDS before every read of it, does
+// not see them, and the kernel counts them itself.  (Five wait states between a vector
+// instruction's scalar result and its use here, one after each write of m0.)
+template <int N>
+__device__ __forceinline__ void lds_dma_batch(i32x4_t rsrc, uint32_t lds, const int (&voff)[N], int soffset) {
+  static_assert(N == 2 || N == 4, "the forms below");
+  uint32_t m0;  // put back: the compiler may not be told of its change
+  if constexpr (N == 4) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %6, %7 offen lds\n\t"
+        "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %6, %7 offen lds\n\t"
+        "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %6, %7 offen lds\n\t"
+        "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %6, %7 offen lds\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(m0)
+        : "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(rsrc), "s"(soffset)
+        : "memory", "scc");
+  } else {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %4, %5 offen lds\n\t"
+        "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, %5 offen lds\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(m0)
+        : "s"(lds), "v"(voff[0]), "v"(voff[1]), "s"(rsrc), "s"(soffset)
+        : "memory", "scc");
+  }
+}
+__device__ __forceinline__ i32x4_t descriptor(const void* base, int64_t bytes) {
+  const uint64_t address = reinterpret_cast<uint64_t>(base);
+  i32x4_t r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(address));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>((address >> 32) & 0xffff));
+  r[2] = __builtin_amdgcn_readfirstlane(bytes > 0x7fffffff ? 0x7fffffff : static_cast<int>(bytes));
+  r[3] = 0x00020000;
+  return r;
+}
+
+// 16-byte aligned rows of codes, several k-tiles.  Eight waves, two on each SIMD, in
+// two groups of four that take turns: while one group's waves multiply a k-step from
+// registers, the other's read their next k-step from LDS and issue the loads of a
+// tile ahead (global -> LDS, no registers); a barrier ends each turn.  Group 0 holds
+// the upper half of the BM rows of the output tile, group 1 the lower.
+//
+// Turns (one barrier after each), k-tile q, k-step s of it: group 0 reads (q, s) in
+// turn 4q + 2s and multiplies it in the next, group 1 one turn later.  So what tile
+// q - 1 occupied is free from turn 4q on.  X has three slots and W has WS: with (q, 0)
+// a wave issues its part of W tile q + WS - 1, with (q, 1) of X tile q + 2, each into
+// the slot of tile q - 1.  Every wave waits for its part of tile q + 1 before the
+// barrier that ends turn 4q + 3 (group 0 after multiplying (q, 1), group 1 after
+// reading it).  Memory operations complete in order, so the wait leaves open what was
+// issued later: X tile q + 2 and, with three W slots, W tile q + 2.  At the end of an
+// output tile the next W tile is issued before the stores, so that the first such wait
+// leaves the stores open too.
+//
+// Workgroups walk the output tiles id, id + grid, ...; the loads run on across tile
+// boundaries.  The MFMA's A operand is W, the rows of two fragments interleaved in runs
+// of four, so that a lane holds eight consecutive outputs of one row and stores them
+// from registers.  Past K the X chunks are loaded as zeros (an offset past the range),
+// whatever the W chunks beside them hold.
+template <typename T, int BM, int BN, int WS, int GM, bool VST>
+__global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, int m_tiles) {
+  constexpr int CW = 8, CWN = 4, XS = 3;
+  constexpr int TM = BM / 2, TN = BN / CWN;
+  constexpr int FM = TM / 16, FN = TN / 16;
+  constexpr int XB = BM * kBK, WB = BN * kBK;
+  constexpr int XO = BM / 8 / CW, WO = BN / 8 / CW;
+  constexpr int kSize = static_cast<int>(sizeof(T));
+  constexpr int kStores = VST ? FM * FN / 2 * (kSize / 2) : 0;
+  constexpr int kOpen = (WS - 2) * WO + XO;
+  static_assert(XO * CW * 8 == BM && WO * CW * 8 == BN, "operands split evenly over the waves");
+  static_assert(TM % 64 == 0 && TN % 32 == 0 && TN <= 64, "whole fragments, in pairs over N; scales by lane");
+  static_assert(kOpen + kStores <= 63, "the wait count fits vmcnt");
+  static_assert(XS * XB + WS * WB <= 160 * 1024, "the slots fit the LDS");
+  __shared__ __attribute__((aligned(16))) unsigned char ring[XS * XB + WS * WB];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int c = lane & 15, g = lane >> 4;
+  const int wm = wave / CWN, wn = wave % CWN;
+  const bool late = wm != 0;
+  const int total = n_tiles * m_tiles;
+  const int ktiles = (p.K + kBK - 1) / kBK;
+  const int first = blockIdx.x, step = gridDim.x;
+  const uint32_t base = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)ring));
+
+  // ---- loads: each operand walks the tiles and k-tiles by itself --------------------
+  int xoff[XO], woff[WO];
+#pragma unroll
+  for (int i = 0; i < XO; ++i) {
+    const int row = 8 * (wave + CW * i) + lane / 8;
+    xoff[i] = static_cast<int>(row * p.x_rs) + ((lane % 8) ^ (row & 7)) * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < WO; ++i) {
+    const int row = 8 * (wave + CW * i) + lane / 8;
+    woff[i] = row * p.K + ((lane % 8) ^ w_key(row)) * 16;
+  }
+  // Whether this lane's X chunk of the last k-tile is past K: the chunk index
+  // depends on the lane alone (rows step by 8 over the instructions).
+  const bool past = (ktiles - 1) * kBK + ((lane % 8) ^ ((lane / 8) & 7)) * 16 >= p.K;
+  struct Walk {
+    const int8_t* from;
+    int64_t bytes;
+    int id, k, slot;
+  };
+  Walk wx{p.x, 0, first, 0, 0}, ww{p.w, 0, first, 0, 0};
+  auto aim_x = [&]() {
+    wx.bytes = 0;
+    if (wx.id >= total) return;
+    int m_blk, n_blk;
+    xcd_tile_of<GM>(wx.id, n_tiles, m_tiles, m_blk, n_blk);
+    const int64_t m0 = static_cast<int64_t>(m_blk) * BM;
+    wx.from = p.x + m0 * p.x_rs;
+    wx.bytes = ((p.M - m0 < BM ? p.M - m0 : BM) - 1) * p.x_rs + p.K;
+  };
+  auto aim_w = [&]() {
+    ww.bytes = 0;
+    if (ww.id >= total) return;
+    int m_blk, n_blk;
+    xcd_tile_of<GM>(ww.id, n_tiles, m_tiles, m_blk, n_blk);
+    const int64_t n0 = static_cast<int64_t>(n_blk) * BN;
+    ww.from = p.w + n0 * p.K;
+    ww.bytes = (p.N - n0 < BN ? p.N - n0 : BN) * p.K;
+  };
+  auto advance = [&](Walk& w, int slots, auto aim) {
+    w.slot = w.slot == slots - 1 ? 0 : w.slot + 1;
+    if (++w.k == ktiles) {
+      w.k = 0;
+      w.id += step;
+      aim();
+    }
+  };
+  auto issue_x = [&]() {
+    int off[XO];
+    const bool cut = wx.k == ktiles - 1 && past;
+#pragma unroll
+    for (int i = 0; i < XO; ++i) off[i] = cut ? kPastRange : xoff[i];
+    lds_dma_batch<XO>(descriptor(wx.from, wx.bytes),
+                      __builtin_amdgcn_readfirstlane(base + wx.slot * XB + wave * 1024), off,
+                      __builtin_amdgcn_readfirstlane(wx.id < total ? wx.k * kBK : 0));
+    advance(wx, XS, aim_x);
+  };
+  auto issue_w = [&]() {
+    lds_dma_batch<WO>(descriptor(ww.from, ww.bytes),
+                      __builtin_amdgcn_readfirstlane(base + XS * XB + ww.slot * WB + wave * 1024), woff,
+                      __builtin_amdgcn_readfirstlane(ww.id < total ? ww.k * kBK : 0));
+    advance(ww, WS, aim_w);
+  };
+  auto barrier = []() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // This wave's part of the next tile; `stores`: its stores may be open too.
+  auto landed = [&](bool stores) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (stores)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kOpen + kStores) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kOpen) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  aim_x();
+  aim_w();
+  issue_x();
+  issue_w();
+  issue_x();
+#pragma unroll
+  for (int i = 2; i < WS; ++i) issue_w();
+  landed(false);
+  barrier();
+  if (late) barrier();
+  int x_slot = 0, w_slot = 0;
+  const int x_read = lds_offset(wm * TM + c, g);
+  const int w_row = wn * TN + 8 * (c >> 2) + (c & 3);
+  const int w_read = XS * XB + w_row * kBK + ((g ^ w_key(w_row)) << 4);
+  for (int id = first; id < total; id += step) {
+    int m_blk, n_blk;
+    xcd_tile_of<GM>(id, n_tiles, m_tiles, m_blk, n_blk);
+    const int64_t m0 = static_cast<int64_t>(m_blk) * BM, n0 = static_cast<int64_t>(n_blk) * BN;
+    const int rows = p.M - m0 < BM ? static_cast<int>(p.M - m0) : BM;
+    const int cols = p.N - n0 < BN ? static_cast<int>(p.N - n0) : BN;
+    i32x4_t acc[FN][FM];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[j][i] = i32x4_t{0, 0, 0, 0};
+    uint32_t own_x[TM / 64], own_w = 0, own_bias = 0;
+#pragma clang loop unroll(disable)
+    for (int kt = 0; kt < ktiles; ++kt) {
+      const int x_at = x_read + x_slot * XB, w_at = w_read + w_slot * WB;
+      x_slot = x_slot == XS - 1 ? 0 : x_slot + 1;
+      w_slot = w_slot == WS - 1 ? 0 : w_slot + 1;
+#pragma unroll
+      for (int kk = 0; kk < kBK / 64; ++kk) {
+        // Fragments are constant distances apart; the second k-step is 64 bytes across
+        // (bit 2 of the swizzled chunk).
+        i32x4_t a[FM], b[FN];
+        const unsigned char* ws = ring + (w_at ^ (kk * 64));
+        const unsigned char* xs = ring + (x_at ^ (kk * 64));
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          b[j] = *reinterpret_cast<const i32x4_t*>(ws + ((j >> 1) * 32 + (j & 1) * 4) * kBK);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) a[i] = *reinterpret_cast<const i32x4_t*>(xs + i * 16 * kBK);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kk == 0) {
+          if (kt > 0 || id == first) issue_w();
+          if (kt == 0) {
+            // Lane l of a load holds the scale of row l, or of column l, of the wave's.
+            const __amdgpu_buffer_rsrc_t rsx = make_rsrc(p.sx + m0, rows * 4);
+            const __amdgpu_buffer_rsrc_t rsw = make_rsrc(p.sw + n0, cols * 4);
+            const __amdgpu_buffer_rsrc_t rbias =
+                make_rsrc(p.bias != nullptr ? static_cast<const T*>(p.bias) + n0 : nullptr,
+                          p.bias != nullptr ? cols * kSize : 0);
+#pragma unroll
+            for (int r = 0; r < TM / 64; ++r)
+              own_x[r] = __builtin_amdgcn_raw_buffer_load_b32(rsx, (wm * TM + 64 * r + lane) * 4, 0, 0);
+            own_w = __builtin_amdgcn_raw_buffer_load_b32(rsw, (wn * TN + lane) * 4, 0, 0);
+            own_bias = load_bias<T>(rbias, wn * TN + lane);
+          }
+        } else {
+          issue_x();
+          // Nobody may still read the tile when its slots are refilled.
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (late) landed(kt == 0 && id != first);
+        }
+        barrier();
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[j][i] = mfma(b[j], a[i], acc[j][i]);
+        __builtin_amdgcn_s_setprio(0);
+        if (kk == 1 && !late) landed(kt == 0 && id != first);
+        if (kk == 0 || kt + 1 < ktiles || !late) barrier();
+      }
+    }
+    // The scales, waited for before the next loads are issued.
+#pragma unroll
+    for (int r = 0; r < TM / 64; ++r) asm volatile("" : "+v"(own_x[r]));
+    asm volatile("" : "+v"(own_w), "+v"(own_bias));
+    issue_w();
+    const __amdgpu_buffer_rsrc_t ry =
+        make_rsrc(static_cast<T*>(p.y) + m0 * p.y_rs + n0,
+                  (static_cast<int64_t>(rows) - 1) * p.y_rs * kSize + cols * kSize);
+    float sx[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      sx[i] = __uint_as_float(__shfl(own_x[i / 4], (i % 4) * 16 + c, 64));
+    const uint32_t rows16 = static_cast<uint32_t>(16 * p.y_rs) * kSize;  // 16 rows further down
+#pragma unroll
+    for (int q = 0; q < FN / 2; ++q) {
+      const int n = wn * TN + q * 32 + 8 * g;
+      float sw[8], bs[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sw[e] = __uint_as_float(__shfl(own_w, q * 32 + 8 * g + e, 64));
+        bs[e] = bias_value<T>(__shfl(own_bias, q * 32 + 8 * g + e, 64));
+      }
+      const uint32_t at = static_cast<uint32_t>((wm * TM + c) * p.y_rs + n) * kSize;
+      const uint32_t whole = !VST || n < cols ? at : kPastRange, half = n + 4 < cols ? at + 16 : kPastRange;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = wm * TM + i * 16 + c;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = finish(acc[2 * q + (e >> 2)][i][e & 3], sx[i], sw[e], bs[e]);
+        store_run<T, VST>(ry, v, whole + i * rows16, half + i * rows16, m < rows ? cols - n : 0);
+      }
+    }
+    if (late) barrier();
+  }
+  if (!late) barrier();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
 constexpr int kNoPath = -2;
+
+template <typename T, int BM, int BN, int WS, int GM>
+int launch_turns(const Problem& p, hipStream_t stream) {
+  constexpr int64_t kLimit = (int64_t{1} << 31) - (1 << 20);
+  const int64_t m_tiles = (static_cast<int64_t>(p.M) + BM - 1) / BM;
+  const int64_t n_tiles = (static_cast<int64_t>(p.N) + BN - 1) / BN;
+  if (BM * p.x_rs >= kLimit || BM * p.y_rs * static_cast<int64_t>(sizeof(T)) >= kLimit ||
+      m_tiles * n_tiles >= (int64_t{1} << 30))
+    return kNoPath;
+  const int64_t total = m_tiles * n_tiles;
+  const int cus = slc_host::device_cu_count() / 8 * 8;
+  const int grid = static_cast<int>(total < cus || cus <= 0 ? total : cus);
+  const int64_t unit = 16 / static_cast<int64_t>(sizeof(T));
+  const bool vectors = p.N % unit == 0 && p.y_rs % unit == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+#define SLC_TURNS(VST)                                                                             \
+  hipLaunchKernelGGL((turns_kernel<T, BM, BN, WS, GM, VST>), dim3(static_cast<unsigned>(grid)), \
+                     dim3(512), 0, stream, p, static_cast<int>(n_tiles), static_cast<int>(m_tiles))
+  if (vectors) {
+    SLC_TURNS(true);
+  } else {
+    SLC_TURNS(false);
+  }
+#undef SLC_TURNS
+  return slc_host::check_launch("slc_hip_linear_q8(turns)");
+}
+
 
 // kNoPath (nothing launched) where 32-bit offsets do not reach over a tile's rows.
 template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM>
@@ -415,9 +742,16 @@ int launch_stream(const Problem& p, hipStream_t stream) {
   const int grid = static_cast<int>(total < cus || cus <= 0 ? total : cus);
   const int64_t unit = 16 / static_cast<int64_t>(sizeof(T));
   const bool vectors = p.N % unit == 0 && p.y_rs % unit == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
-  hipLaunchKernelGGL((stream_kernel<T, BM, BN, CWM, CWN, PW, S, GM>), dim3(static_cast<unsigned>(grid)),
-                     dim3((CWM * CWN + PW) * 64), 0, stream, p, static_cast<int>(n_tiles),
-                     static_cast<int>(m_tiles), vectors);
+#define SLC_STREAM(VST)                                                                       \
+  hipLaunchKernelGGL((stream_kernel<T, BM, BN, CWM, CWN, PW, S, GM, VST>),                    \
+                     dim3(static_cast<unsigned>(grid)), dim3((CWM * CWN + PW) * 64), 0, stream, p, \
+                     static_cast<int>(n_tiles), static_cast<int>(m_tiles))
+  if (vectors) {
+    SLC_STREAM(true);
+  } else {
+    SLC_STREAM(false);
+  }
+#undef SLC_STREAM
   return slc_host::check_launch("slc_hip_linear_q8(stream)");
 }
 
@@ -433,6 +767,9 @@ int launch(const Problem& p, hipStream_t stream) {
     if (SLC_Q8_TILE == 1) rc = launch_stream<T, 256, 128, 4, 2, 4, 3, 4>(p, stream);
     if (SLC_Q8_TILE == 2) rc = launch_stream<T, 128, 128, 2, 4, 2, 4, 8>(p, stream);
     if (SLC_Q8_TILE == 3) rc = launch_stream<T, 128, 64, 2, 2, 2, 4, 8>(p, stream);
+    if (SLC_Q8_TILE == 5) rc = launch_turns<T, 256, 256, 2, 4>(p, stream);
+    if (SLC_Q8_TILE == 6) rc = launch_turns<T, 256, 128, 3, 4>(p, stream);
+    if (SLC_Q8_TILE == 7) rc = launch_turns<T, 128, 256, 3, 4>(p, stream);
     if (SLC_Q8_TILE == 4) rc = launch_stream<T, 64, 64, 2, 2, 2, 6, 8>(p, stream);
     if (rc != kNoPath) return rc;
   }
@@ -458,7 +795,8 @@ extern "C" int slc_hip_linear_q8(const int8_t* input, const float* in_scales, co
               (long long)out_features, (long long)in_features);
   SLC_REQUIRE(rows < (1LL << 31) && out_features < (1LL << 31),
               "slc_hip_linear_q8: sizes exceed 2^31");
-  SLC_REQUIRE(in_stride_row >= 0 && out_stride_row >= 0, "slc_hip_linear_q8: negative stride");
+  SLC_REQUIRE(in_stride_row >= 0 && (rows <= 1 || out_stride_row >= out_features),
+              "slc_hip_linear_q8: rows of %lld outputs overlap, or a stride is negative", (long long)out_features);
   if (rows == 0) return SLC_OK;
   SLC_REQUIRE(input && in_scales && weight && weight_scales && output,
               "slc_hip_linear_q8: null pointer");
