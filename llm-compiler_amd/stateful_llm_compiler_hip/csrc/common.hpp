@@ -52,6 +52,19 @@ __device__ __forceinline__ f16_t from_f32<f16_t>(float f) {
   return f16_t{__builtin_bit_cast(uint16_t, h)};
 }
 
+// Two floats rounded to the 16-bit type T, a in the low half (one instruction in
+// bf16).
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return from_f32<T>(a).bits | static_cast<uint32_t>(from_f32<T>(b).bits) << 16;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16_t>(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
 // Round a float to the precision of T and return it as float again.  This is
 // the "materialise in dtype" step PyTorch performs between two bf16 ops.
 template <typename T>

@@ -193,7 +193,10 @@ __device__ __forceinline__ float bias_value(uint32_t bits) {
   }
 }
 
-// An offset past every range (kLimit) that stays below 2^31 with K added.
+// Rows whose span is under this are reached by 32-bit offsets.
+constexpr int64_t kRangeLimit = (int64_t{1} << 31) - (1 << 20);
+constexpr int kNoPath = -2;
+// An offset past every such range that stays below 2^31 with K added.
 constexpr int kPastRange = 0x7fffffff - (1 << 18);
 
 // A lane's run of eight consecutive outputs at a byte offset from the tile's first.
@@ -204,21 +207,17 @@ template <typename T, bool VST>
 __device__ __forceinline__ void store_run(const __amdgpu_buffer_rsrc_t& ry, const float (&v)[8],
                                           uint32_t offset, uint32_t half, int left) {
   constexpr int kSize = static_cast<int>(sizeof(T));
-  uint32_t o[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (kSize == 4)
-      o[e] = __float_as_uint(v[e]);
-    else
-      o[e] = slc::from_f32<T>(v[e]).bits;
-  }
   if constexpr (VST) {
 #pragma unroll
     for (int h = 0; h < kSize / 2; ++h) {
       i32x4_t packed;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-        packed[d] = static_cast<int>(kSize == 4 ? o[4 * h + d] : o[2 * d] | (o[2 * d + 1] << 16));
+      for (int d = 0; d < 4; ++d) {
+        if constexpr (kSize == 4)
+          packed[d] = __float_as_int(v[4 * h + d]);
+        else
+          packed[d] = static_cast<int>(slc::pack2<T>(v[2 * d], v[2 * d + 1]));
+      }
       __builtin_amdgcn_raw_buffer_store_b128(packed, ry, static_cast<int>(h == 0 ? offset : half), 0, 0);
     }
   } else {
@@ -226,9 +225,9 @@ __device__ __forceinline__ void store_run(const __amdgpu_buffer_rsrc_t& ry, cons
     for (int e = 0; e < 8; ++e) {
       if (e >= left) continue;
       if constexpr (kSize == 4)
-        __builtin_amdgcn_raw_buffer_store_b32(static_cast<int>(o[e]), ry, static_cast<int>(offset + 4 * e), 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v[e]), ry, static_cast<int>(offset + 4 * e), 0, 0);
       else
-        __builtin_amdgcn_raw_buffer_store_b16(static_cast<short>(o[e]), ry, static_cast<int>(offset + 2 * e), 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b16(static_cast<short>(slc::from_f32<T>(v[e]).bits), ry, static_cast<int>(offset + 2 * e), 0, 0);
     }
   }
 }
@@ -700,14 +699,11 @@ __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, i
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-constexpr int kNoPath = -2;
-
 template <typename T, int BM, int BN, int WS, int GM>
 int launch_turns(const Problem& p, hipStream_t stream) {
-  constexpr int64_t kLimit = (int64_t{1} << 31) - (1 << 20);
   const int64_t m_tiles = (static_cast<int64_t>(p.M) + BM - 1) / BM;
   const int64_t n_tiles = (static_cast<int64_t>(p.N) + BN - 1) / BN;
-  if (BM * p.x_rs >= kLimit || BM * p.y_rs * static_cast<int64_t>(sizeof(T)) >= kLimit ||
+  if (BM * p.x_rs >= kRangeLimit || BM * p.y_rs * static_cast<int64_t>(sizeof(T)) >= kRangeLimit ||
       m_tiles * n_tiles >= (int64_t{1} << 30))
     return kNoPath;
   const int64_t total = m_tiles * n_tiles;
@@ -731,10 +727,9 @@ int launch_turns(const Problem& p, hipStream_t stream) {
 // kNoPath (nothing launched) where 32-bit offsets do not reach over a tile's rows.
 template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM>
 int launch_stream(const Problem& p, hipStream_t stream) {
-  constexpr int64_t kLimit = (int64_t{1} << 31) - (1 << 20);
   const int64_t m_tiles = (static_cast<int64_t>(p.M) + BM - 1) / BM;
   const int64_t n_tiles = (static_cast<int64_t>(p.N) + BN - 1) / BN;
-  if (BM * p.x_rs >= kLimit || BM * p.y_rs * static_cast<int64_t>(sizeof(T)) >= kLimit ||
+  if (BM * p.x_rs >= kRangeLimit || BM * p.y_rs * static_cast<int64_t>(sizeof(T)) >= kRangeLimit ||
       m_tiles * n_tiles >= (int64_t{1} << 30))
     return kNoPath;
   const int64_t total = m_tiles * n_tiles;
@@ -755,22 +750,208 @@ int launch_stream(const Problem& p, hipStream_t stream) {
   return slc_host::check_launch("slc_hip_linear_q8(stream)");
 }
 
+// ---- decode: few rows, the weight streamed once -----------------------------------
+// A workgroup owns `feat` consecutive features (up to 16 * TILES; MFMA rows past them
+// are masked off by the buffer range) and splits K over its waves; the waves' sums meet
+// in LDS by integer adds, whose order does not matter.  Each wave keeps U k-steps of 64
+// codes in flight while it multiplies the U before.  Bound by the weight's bytes where
+// it is wide, by latency where it is narrow.
+template <typename T, int MB, int TILES, int U>
+__global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
+  __shared__ int sums[TILES * MB * 256];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int waves = blockDim.x >> 6;
+  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * feat;
+  const int cols = p.N - n0 < feat ? static_cast<int>(p.N - n0) : feat;
+  const int steps = (p.K + 63) / 64, per = (steps + waves - 1) / waves;
+  const int begin = wave * per, end = begin + per < steps ? begin + per : steps;
+
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (p.M - 1) * p.x_rs + p.K);
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + n0 * p.K, static_cast<int64_t>(cols) * p.K);
+  int x_off[MB], w_off[TILES];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) x_off[i] = static_cast<int>((i * 16 + c) * p.x_rs) + g * 16;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) w_off[t] = (t * 16 + c) * p.K + g * 16;
+  i32x4_t acc[TILES][MB];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t)
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[t][i] = i32x4_t{0, 0, 0, 0};
+
+  // Zeros for X past K and past this wave's steps, whatever W holds there.
+  i32x4_t wa[U][TILES], wb[U][TILES], xa[U][MB], xb[U][MB];
+  auto load16 = [](const __amdgpu_buffer_rsrc_t& r, int at) {
+    return __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+  };
+  auto fetch = [&](int s0, i32x4_t (&w)[U][TILES], i32x4_t (&x)[U][MB]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u;
+      const bool live = s < end;
+      const bool in = live && s * 64 + g * 16 < p.K;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) w[u][t] = load16(rw, live ? w_off[t] + s * 64 : kPastRange);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) x[u][i] = load16(rx, in ? x_off[i] + s * 64 : kPastRange);
+    }
+  };
+  auto multiply = [&](const i32x4_t (&w)[U][TILES], const i32x4_t (&x)[U][MB]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[t][i] = mfma(x[u][i], w[u][t], acc[t][i]);
+  };
+  int s0 = begin;
+  fetch(s0, wa, xa);
+  // This thread's first output's scales, behind the first loads: element e of the
+  // fragments is row 4 * (l / 16) + r of block i, column l % 16 of tile t.
+  auto place = [&](int e, int& m, int& n) {
+    const int l = (e / 4) & 63;
+    m = (e / 256 % MB) * 16 + 4 * (l >> 4) + e % 4;
+    n = e / (256 * MB) * 16 + (l & 15);
+  };
+  int m, n;
+  place(tid, m, n);
+  float sx = 0.0f, sw = 0.0f;
+  uint32_t bias = 0;
+  auto scales = [&]() {
+    sx = p.sx[m];
+    sw = p.sw[n0 + n];
+    if (p.bias != nullptr) {
+      if constexpr (sizeof(T) == 4)
+        bias = static_cast<const uint32_t*>(p.bias)[n0 + n];
+      else
+        bias = static_cast<const uint16_t*>(p.bias)[n0 + n];
+    }
+  };
+  const bool mine = tid < TILES * MB * 256 && m < p.M && n < cols;
+  if (mine) scales();
+  for (int e = tid; e < TILES * MB * 256; e += blockDim.x) sums[e] = 0;
+  __syncthreads();
+  while (s0 < end) {
+    fetch(s0 + U, wb, xb);
+    multiply(wa, xa);
+    s0 += U;
+    if (s0 >= end) break;
+    fetch(s0 + U, wa, xa);
+    multiply(wb, xb);
+    s0 += U;
+  }
+  if (begin < end) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) atomicAdd(&sums[((t * MB + i) * 64 + lane) * 4 + r], acc[t][i][r]);
+  }
+  __syncthreads();
+  for (int e = tid; e < TILES * MB * 256; e += blockDim.x) {
+    if (e != tid) place(e, m, n);
+    if (m >= p.M || n >= cols) continue;
+    if (e != tid) scales();
+    static_cast<T*>(p.y)[m * p.y_rs + n0 + n] =
+        slc::from_f32<T>(finish(sums[e], sx, sw, bias_value<T>(bias)));
+  }
+}
+
+// About 256 workgroups of equal shares of the features, 32 at most; eight waves, fewer
+// where K has fewer steps (16 waves: 1 x 896 x 896 3.9 us for 3.4, 8 x 896 x 4864 6.4 for
+// 5.5; four: 3.4 and 5.7).
+template <typename T>
+int launch_rows(const Problem& p, hipStream_t stream) {
+  if (p.M > 32 || 32 * p.x_rs >= kRangeLimit) return kNoPath;
+  const int64_t share = (static_cast<int64_t>(p.N) + 255) / 256;
+  const int feat = static_cast<int>(share > 32 ? 32 : share);
+  const int steps = (p.K + 63) / 64, waves = steps < 8 ? steps : 8;
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.N) + feat - 1) / feat));
+#define SLC_ROWS(MB, TILES, U) \
+  hipLaunchKernelGGL((rows_kernel<T, MB, TILES, U>), grid, dim3(waves * 64), 0, stream, p, feat)
+  if (feat <= 16) {
+    if (p.M <= 16) SLC_ROWS(1, 1, 4);
+    else SLC_ROWS(2, 1, 2);
+  } else {
+    if (p.M <= 16) SLC_ROWS(1, 2, 2);
+    else SLC_ROWS(2, 2, 2);
+  }
+#undef SLC_ROWS
+  return slc_host::check_launch("slc_hip_linear_q8(rows)");
+}
+
+// Which kernel takes a shape of aligned rows, all giving the same bits.
+//
+// Up to 32 rows and 8192 features, rows_kernel: a tile would leave most CUs idle (us,
+// rows | 64 x 64 tiles: 8 x 1152 x 896 3.6 | 4.8, 32 x 896 x 4864 8.4 | 10.5, 32 x 4096 x
+// 4096 8.8 | 9.8; but 48 x 896 x 4864 10.7 | 10.6, 8 x 9728 x 896 5.6 | 5.1, 8 x 11008 x
+// 4096 14.6 | 10.5), and up to 8 rows from 16384 features, where it reads the weight a
+// little faster (1 x 151936 x 896 24.1 | 26.9, 8 x 50257 x 896 11.1 | 13.1, 8 x 151936 x
+// 896 29.1 | 28.2).
+//
+// Else the tile whose rounds over the CUs cost least: a round takes fixed + per_k * k-tiles
+// us, measured with every CU busy (K 896 and 4096).  Rounds, not tiles: 8192 x 896 x 896
+// 13.0 us as one round of 256 x 128, 13.4 as two of 128 x 128; 4096 x 9728 x 896 44.8 as
+// five rounds of 256 x 128, 53 as three of 256 x 256; 32768 x 896 x 4864 127 as two of 256 x
+// 256, 147 as four of 256 x 128; 65 x 896 x 896 5.0 as 64 x 64, 8.7 as 256 x 128.
+enum Kernel { kRows, k64x64, k128x64, k128x128, k256x128, k256x256 };
+inline Kernel choose(int64_t M, int64_t N, int64_t K) {
+  if ((M <= 32 && N <= 8192) || (M <= 8 && N >= 16384)) return kRows;
+  struct Cost {
+    Kernel kernel;
+    int bm, bn;
+    double fixed, per_k;
+  };
+  constexpr Cost costs[] = {{k64x64, 64, 64, 0.67, 0.20},
+                            {k128x64, 128, 64, 0.70, 0.33},
+                            {k128x128, 128, 128, 1.28, 0.51},
+                            {k256x128, 256, 128, 2.6, 0.89},
+                            {k256x256, 256, 256, 6.3, 1.59}};
+  const int64_t cus = slc_host::device_cu_count(), k_tiles = (K + kBK - 1) / kBK;
+  Kernel best = k64x64;
+  double least = 0.0;
+  for (const Cost& c : costs) {
+    const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    const double cost = static_cast<double>((tiles + cus - 1) / cus) * (c.fixed + c.per_k * static_cast<double>(k_tiles));
+    if (c.kernel == k64x64 || cost < least) {
+      best = c.kernel;
+      least = cost;
+    }
+  }
+  return best;
+}
+
+#ifndef SLC_Q8_CHOICE
+#define SLC_Q8_CHOICE(M, N, K) choose(M, N, K)
+#endif
 template <typename T>
 int launch(const Problem& p, hipStream_t stream) {
-  const bool vec = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) == 0 &&
-                   p.K % 16 == 0 && p.x_rs % 16 == 0;
-#ifndef SLC_Q8_TILE
-#define SLC_Q8_TILE 1
-#endif
-  if (vec && p.M > 64) {
+  const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) == 0 &&
+                       p.K % 16 == 0 && p.x_rs % 16 == 0;
+  if (aligned) {
     int rc = kNoPath;
-    if (SLC_Q8_TILE == 1) rc = launch_stream<T, 256, 128, 4, 2, 4, 3, 4>(p, stream);
-    if (SLC_Q8_TILE == 2) rc = launch_stream<T, 128, 128, 2, 4, 2, 4, 8>(p, stream);
-    if (SLC_Q8_TILE == 3) rc = launch_stream<T, 128, 64, 2, 2, 2, 4, 8>(p, stream);
-    if (SLC_Q8_TILE == 5) rc = launch_turns<T, 256, 256, 2, 4>(p, stream);
-    if (SLC_Q8_TILE == 6) rc = launch_turns<T, 256, 128, 3, 4>(p, stream);
-    if (SLC_Q8_TILE == 7) rc = launch_turns<T, 128, 256, 3, 4>(p, stream);
-    if (SLC_Q8_TILE == 4) rc = launch_stream<T, 64, 64, 2, 2, 2, 6, 8>(p, stream);
+    switch (SLC_Q8_CHOICE(p.M, p.N, p.K)) {
+      case kRows:
+        rc = launch_rows<T>(p, stream);
+        break;
+      case k64x64:
+        rc = launch_stream<T, 64, 64, 2, 2, 2, 6, 8>(p, stream);
+        break;
+      case k128x64:
+        rc = launch_stream<T, 128, 64, 2, 2, 2, 4, 8>(p, stream);
+        break;
+      case k128x128:
+        rc = launch_stream<T, 128, 128, 2, 4, 2, 4, 8>(p, stream);
+        break;
+      case k256x128:
+        rc = launch_stream<T, 256, 128, 4, 2, 4, 3, 4>(p, stream);
+        break;
+      default:
+        rc = launch_turns<T, 256, 256, 2, 4>(p, stream);
+    }
     if (rc != kNoPath) return rc;
   }
   const int64_t m_tiles = (static_cast<int64_t>(p.M) + 63) / 64;

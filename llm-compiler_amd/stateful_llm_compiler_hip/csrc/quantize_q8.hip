@@ -124,9 +124,7 @@ __device__ __forceinline__ u32x4 add_vec(const u32x4& a, const u32x4& b) {
     if constexpr (sizeof(T) == 4) {
       v[k] = __float_as_uint(elem<T>(a, k) + elem<T>(b, k));
     } else {
-      const T lo = slc::from_f32<T>(elem<T>(a, 2 * k) + elem<T>(b, 2 * k));
-      const T hi = slc::from_f32<T>(elem<T>(a, 2 * k + 1) + elem<T>(b, 2 * k + 1));
-      v[k] = lo.bits | static_cast<uint32_t>(hi.bits) << 16;
+      v[k] = slc::pack2<T>(elem<T>(a, 2 * k) + elem<T>(b, 2 * k), elem<T>(a, 2 * k + 1) + elem<T>(b, 2 * k + 1));
     }
   }
   return v;
