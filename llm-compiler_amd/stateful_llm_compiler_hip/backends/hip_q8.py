@@ -21,46 +21,54 @@ import torch
 from .. import _native
 
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+_MOST_EPSILON = torch.finfo(torch.float32).max
 
 MAX_FEATURES = 131071  # SLC_Q8_MAX_K: sums of so many products of codes fit 32 bits
 
 
-def _check_rows(what: str, *tensors: torch.Tensor) -> None:
+_CONTIGUOUS = torch.contiguous_format
+
+
+def _check_rows(what: str, first: torch.Tensor, second: torch.Tensor | None = None) -> None:
     """Float GPU tensors of one shape, dtype and device with a last axis to code."""
 
-    first = tensors[0]
-    for t in tensors:
-        if not t.is_cuda:
-            raise ValueError(f"{what}: all tensors must be on the GPU")
-        if t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
-            raise ValueError(f"{what}: tensors need one shape, dtype and device")
+    if not first.is_cuda or (second is not None and not second.is_cuda):
+        raise ValueError(f"{what}: all tensors must be on the GPU")
+    if second is not None and (
+        second.shape != first.shape or second.dtype != first.dtype or second.device != first.device
+    ):
+        raise ValueError(f"{what}: tensors need one shape, dtype and device")
     if first.dtype not in _FLOATS:
         raise ValueError(f"{what}: unsupported dtype {first.dtype}")
     if first.ndim < 1 or not 1 <= first.shape[-1] <= MAX_FEATURES:
         raise ValueError(f"{what}: the last axis must hold 1 to {MAX_FEATURES} values")
 
 
-def _flat(tensor: torch.Tensor) -> torch.Tensor:
-    """``tensor`` as evenly strided rows; a copy only where no view is."""
+def _rows(tensor: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``tensor``, or a copy of it where its rows are no view of evenly strided
+    ones, and their stride."""
 
-    if tensor.stride(-1) != 1 and tensor.shape[-1] != 1:
-        tensor = tensor.contiguous()
-    try:
-        return tensor.view(-1, tensor.shape[-1])
-    except RuntimeError:
-        return tensor.reshape(-1, tensor.shape[-1])
+    hidden = tensor.shape[-1]
+    if tensor.is_contiguous():
+        return tensor, hidden
+    if tensor.stride(-1) == 1 or hidden == 1:
+        try:
+            return tensor, tensor.view(-1, hidden).stride(0)
+        except RuntimeError:
+            pass
+    return tensor.contiguous(), hidden
 
 
-def _outputs(tensor: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return (torch.empty(tensor.shape, device=tensor.device, dtype=torch.int8),
-            torch.empty(tensor.shape[:-1], device=tensor.device, dtype=torch.float32))
+def _codes_and_scales(tensor: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return (torch.empty_like(tensor, dtype=torch.int8, memory_format=_CONTIGUOUS),
+            tensor.new_empty(tensor.shape[:-1], dtype=torch.float32))
 
 
 def _call(name: str, device: torch.device, *arguments) -> None:
     """The entry point on ``device``'s current stream, with that device current."""
 
     function = getattr(_native.library(), name)
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         status = function(*arguments, _native.current_stream(device))
     else:
         with torch.cuda.device(device):
@@ -72,31 +80,36 @@ def hip_quantize_q8(tensor: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of ``tensor`` [..., K] along its last axis."""
 
     _check_rows("HIP quantize q8", tensor)
-    codes, scales = _outputs(tensor)
-    if tensor.numel():
-        flat = _flat(tensor)
-        _call("slc_hip_quantize_q8", tensor.device, flat.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-              _native.dtype_tag(tensor.dtype), flat.shape[0], flat.shape[1], flat.stride(0))
+    codes, scales = _codes_and_scales(tensor)
+    count = tensor.numel()
+    if count:
+        rows, stride = _rows(tensor)
+        hidden = tensor.shape[-1]
+        _call("slc_hip_quantize_q8", tensor.device, rows.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+              _native.dtype_tag(tensor.dtype), count // hidden, hidden, stride)
     return codes, scales
 
 
 def _norm(what, tensor, residual, weight, epsilon):
-    tensors = (tensor,) if residual is None else (tensor, residual)
-    _check_rows(what, *tensors)
-    if not weight.is_cuda or weight.device != tensor.device or weight.dtype != tensor.dtype:
+    _check_rows(what, tensor, residual)
+    hidden = tensor.shape[-1]
+    if not weight.is_cuda or weight.dtype != tensor.dtype or weight.device != tensor.device:
         raise ValueError(f"{what}: the weight needs the input's dtype and device")
-    if weight.shape != tensor.shape[-1:]:
-        raise ValueError(f"{what}: weight must be [{tensor.shape[-1]}], got {tuple(weight.shape)}")
-    codes, scales = _outputs(tensor)
-    summed = None if residual is None else torch.empty(tensor.shape, device=tensor.device, dtype=tensor.dtype)
-    if tensor.numel():
-        flat = _flat(tensor)
-        other = None if residual is None else _flat(residual)
+    if weight.ndim != 1 or weight.shape[0] != hidden:
+        raise ValueError(f"{what}: weight must be [{hidden}], got {tuple(weight.shape)}")
+    epsilon = float(epsilon)
+    if not 0.0 <= epsilon <= _MOST_EPSILON:
+        raise ValueError(f"{what}: epsilon must be finite and not negative, got {epsilon}")
+    codes, scales = _codes_and_scales(tensor)
+    summed = None if residual is None else torch.empty_like(tensor, memory_format=_CONTIGUOUS)
+    count = tensor.numel()
+    if count:
+        rows, stride = _rows(tensor)
+        other, other_stride = (None, 0) if residual is None else _rows(residual)
         weight = weight.contiguous()
-        _call("slc_hip_rms_norm_q8", tensor.device, flat.data_ptr(), None if other is None else other.data_ptr(),
+        _call("slc_hip_rms_norm_q8", tensor.device, rows.data_ptr(), None if other is None else other.data_ptr(),
               weight.data_ptr(), None if summed is None else summed.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-              _native.dtype_tag(tensor.dtype), flat.shape[0], flat.shape[1], flat.stride(0),
-              0 if other is None else other.stride(0), float(epsilon))
+              _native.dtype_tag(tensor.dtype), count // hidden, hidden, stride, other_stride, epsilon)
     return summed, codes, scales
 
 
@@ -123,11 +136,14 @@ def hip_swiglu_q8(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, t
     codes are.  ``gate`` and ``up`` may be the halves of a fused projection."""
 
     _check_rows("HIP swiglu q8", gate, up)
-    codes, scales = _outputs(gate)
-    if gate.numel():
-        a, b = _flat(gate), _flat(up)
+    codes, scales = _codes_and_scales(gate)
+    count = gate.numel()
+    if count:
+        a, a_stride = _rows(gate)
+        b, b_stride = _rows(up)
+        hidden = gate.shape[-1]
         _call("slc_hip_swiglu_q8", gate.device, a.data_ptr(), b.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-              _native.dtype_tag(gate.dtype), a.shape[0], a.shape[1], a.stride(0), b.stride(0))
+              _native.dtype_tag(gate.dtype), count // hidden, hidden, a_stride, b_stride)
     return codes, scales
 
 
@@ -149,13 +165,14 @@ def hip_linear_q8(
     """
 
     what = "HIP linear q8"
-    tensors = [codes, scales, weight, weight_scales]
-    if bias is not None:
-        tensors.append(bias)
-    if not all(t.is_cuda for t in tensors):
+    if not (codes.is_cuda and scales.is_cuda and weight.is_cuda and weight_scales.is_cuda) or (
+        bias is not None and not bias.is_cuda
+    ):
         raise ValueError(f"{what}: all tensors must be on the GPU")
     device = codes.device
-    if any(t.device != device for t in tensors):
+    if scales.device != device or weight.device != device or weight_scales.device != device or (
+        bias is not None and bias.device != device
+    ):
         raise ValueError(f"{what}: tensors need one device")
     if codes.dtype != torch.int8 or weight.dtype != torch.int8:
         raise ValueError(f"{what}: codes and weight must be int8")
@@ -174,11 +191,13 @@ def hip_linear_q8(
         raise ValueError(f"{what}: one scale per token and one per output channel are needed")
     if bias is not None and (bias.shape != (features,) or bias.dtype != output_dtype):
         raise ValueError(f"{what}: bias must be [{features}] of the output's dtype")
-    if not all(t.is_contiguous() for t in tensors):
+    if not (codes.is_contiguous() and scales.is_contiguous() and weight.is_contiguous()
+            and weight_scales.is_contiguous()) or (bias is not None and not bias.is_contiguous()):
         raise ValueError(f"{what}: tensors must be contiguous")
-    output = torch.empty((*codes.shape[:-1], features), device=device, dtype=output_dtype)
-    if codes.numel():
+    output = codes.new_empty((*codes.shape[:-1], features), dtype=output_dtype)
+    count = codes.numel()
+    if count:
         _call("slc_hip_linear_q8", device, codes.data_ptr(), scales.data_ptr(), weight.data_ptr(),
               weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), output.data_ptr(),
-              _native.dtype_tag(output_dtype), codes.numel() // width, features, width, width, features)
+              _native.dtype_tag(output_dtype), count // width, features, width, width, features)
     return output

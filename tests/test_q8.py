@@ -30,17 +30,17 @@ def quantize(x=P, codes=P, scales=P, dtype=BF16, rows=2, hidden=8, rs=8):
     return _native.library().slc_hip_quantize_q8(x, codes, scales, dtype, rows, hidden, rs, None)
 
 
-def norm(x=P, residual=P, w=P, summed=P, codes=P, scales=P, dtype=BF16, rows=2, hidden=8):
+def norm(x=P, residual=P, w=P, summed=P, codes=P, scales=P, dtype=BF16, rows=2, hidden=8, eps=1e-6):
     return _native.library().slc_hip_rms_norm_q8(x, residual, w, summed, codes, scales, dtype, rows, hidden,
-                                                 hidden, hidden, 1e-6, None)
+                                                 hidden, hidden, eps, None)
 
 
 def swiglu(gate=P, up=P, codes=P, scales=P, dtype=BF16, rows=2, hidden=8):
     return _native.library().slc_hip_swiglu_q8(gate, up, codes, scales, dtype, rows, hidden, hidden, hidden, None)
 
 
-def linear(x=P, sx=P, w=P, sw=P, bias=None, y=P, dtype=BF16, rows=2, n=16, k=64):
-    return _native.library().slc_hip_linear_q8(x, sx, w, sw, bias, y, dtype, rows, n, k, k, n, None)
+def linear(x=P, sx=P, w=P, sw=P, bias=None, y=P, dtype=BF16, rows=2, n=16, k=64, x_rs=64, y_rs=16):
+    return _native.library().slc_hip_linear_q8(x, sx, w, sw, bias, y, dtype, rows, n, k, x_rs, y_rs, None)
 
 
 @pytest.mark.parametrize("call", [quantize, norm, swiglu])
@@ -56,6 +56,7 @@ def test_row_entry_points_refuse_their_own_operands():
     assert quantize(x=None) == -1 and quantize(x=P + 1) == -1 and quantize(x=P + 2, dtype=F32) == -1
     assert norm(x=None) == -1 and norm(w=None) == -1 and norm(w=P + 1) == -1
     assert norm(residual=None) == -1 and norm(summed=None) == -1  # one without the other
+    assert all(norm(eps=eps) == -1 for eps in (-1e-6, float("nan"), float("inf")))
     assert norm(residual=P + 1) == -1 and norm(summed=P + 1) == -1
     assert swiglu(gate=None) == -1 and swiglu(up=None) == -1 and swiglu(up=P + 1) == -1
     assert b"slc_hip_swiglu_q8" in _native.library().slc_hip_last_error()
@@ -64,6 +65,6 @@ def test_row_entry_points_refuse_their_own_operands():
 def test_linear_entry_point_refuses():
     for bad in ({"dtype": I32}, {"rows": -1}, {"rows": 2**31}, {"n": 0}, {"n": 2**31}, {"k": 0}, {"k": 131072},
                 {"x": None}, {"sx": None}, {"w": None}, {"sw": None}, {"y": None}, {"sx": P + 2}, {"sw": P + 1},
-                {"y": P + 1}, {"bias": P + 1}, {"y": P + 2, "dtype": F32}):
+                {"y": P + 1}, {"bias": P + 1}, {"y": P + 2, "dtype": F32}, {"x_rs": -64}, {"y_rs": 15}, {"y_rs": -16}):
         assert linear(**bad) == -1, bad
     assert linear(rows=0) == 0

@@ -253,6 +253,9 @@ def test_refusals(gpu):
         lambda: backends.hip_rms_norm_q8(x, w.bfloat16(), epsilon=1e-6),
         lambda: backends.hip_rms_norm_q8(x, w[:15], epsilon=1e-6),
         lambda: backends.hip_rms_norm_q8(x, w.view(1, 16), epsilon=1e-6),
+        lambda: backends.hip_rms_norm_q8(x, w, epsilon=-1e-6),
+        lambda: backends.hip_rms_norm_q8(x, w, epsilon=float("nan")),
+        lambda: backends.hip_rms_norm_q8(x, w, epsilon=float("inf")),
         lambda: backends.hip_add_rms_norm_q8(x, x[:1], w, epsilon=1e-6),
         lambda: backends.hip_add_rms_norm_q8(x, x.bfloat16(), w, epsilon=1e-6),
         lambda: backends.hip_add_rms_norm_q8(x, x.cpu(), w, epsilon=1e-6),
