@@ -7,15 +7,15 @@
 // rstd divides every y of a row alike, so the norm's codes are those of h * w
 // and do not wait for the statistic.
 //
-// Every code is the formula's, not that of a rounded y: a code is decided in
-// fp32 from v ~ y and 1 / a (one fma rounds v * 127 / a to a whole number, a
-// second gives its distance from it), and where the distance comes within the
-// error of the fp32 form of 1/2 it is decided again in fp64 from the inputs,
-// with a itself in fp64.  In units of 127 * 2^-24: a and 127 / a round by 1 each,
-// v by 0 where both factors have 16 bits, by 1 in the norm of fp32 values, by 8
-// in SwiGLU (silu_f32); kBorder covers the sum.  About one element in 4000
-// (SwiGLU) is decided twice.  Rows whose a is 0, not finite, or so small or
-// large that fp32 products round or overflow run in fp64 as a whole.
+// Every code is the formula's, not that of a rounded y: with v ~ y in fp32, v * 127 / a
+// is rounded to a whole number (one fma) with the factor just below and just above 127 /
+// a, far enough apart to cover every error of the fp32 form, and where the two differ
+// the code is decided again in fp64 from the inputs, with a itself in fp64.  In units of
+// 2^-24: a and 127 / a round by 1 each, the factor's distance by 1, v by 0 where both
+// factors have 16 bits, by 1 in the norm of fp32 values, by 8 in SwiGLU (silu_f32);
+// kApart covers the sum.  About one element in 30000 (SwiGLU) is decided twice.  Rows
+// whose a is 0, not finite, or so small or large that fp32 products round or overflow
+// run in fp64 as a whole.
 //
 // One workgroup holds a row in registers, NV 16-byte vectors per lane, so every
 // input is read once and every output written once: HBM-bound from about a
@@ -23,6 +23,9 @@
 // past 16 waves' registers are read twice (LOOP).  All loads are issued before
 // the first use, without branches: buffer loads whose range ends with the row.
 #include <float.h>
+
+#include <initializer_list>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -52,8 +55,8 @@ constexpr float kLow = 0x1p-60f, kHigh = 0x1p60f;
 // sum; one whose total is between these has lost nothing to the ends of fp32.
 constexpr double kLowSquares = 0x1p-80, kHighSquares = 0x1p100;
 // SwiGLU: where 1 + exp(-g) has no normal fp32 reciprocal, |silu(g)| < 2^-119
-// counts as 0; with |u| up to this the product is under 2^-29 of the least a.
-constexpr float kMostUp = 0x1p30f;
+// counts as 0; with |u| up to this the product is under 2^-31 of the least a.
+constexpr float kMostUp = 0x1p28f;
 
 template <typename T, int SRC>
 struct Traits {
@@ -62,7 +65,7 @@ struct Traits {
   static constexpr bool kHasW = SRC == kNorm || SRC == kAddNorm;
   // Whether the fp32 v may differ from y (then a is taken again in fp64).
   static constexpr bool kInexact = SRC == kSwiglu || (kHasW && sizeof(T) == 4);
-  static constexpr float kBorder = 0.5f - (SRC == kSwiglu ? 0x1p-13f : 0x1p-15f);
+  static constexpr float kApart = (SRC == kSwiglu ? 14 : kInexact ? 6 : 4) * 0x1p-24f;
   // v within this factor below the largest v may be the largest y.
   static constexpr float kNear = 1.0f - 0x1p-19f;
 };
@@ -130,17 +133,27 @@ __device__ __forceinline__ u32x4 add_vec(const u32x4& a, const u32x4& b) {
   return v;
 }
 
-// silu(g) to 7 * 2^-24 of itself: exp(-g) = 2^t (1 + d), t = -g log2(e) rounded
-// and d the rest of that product times ln 2 (rounding 2^t by 2 * 2^-24, which the
-// division's result keeps at most), the sum by 1, the reciprocal by 2, the product
-// by 1, d by under 1.
+// silu(g) to 7 * 2^-24 of itself: exp(-g) = 2^t (1 + d), where t is -g log2(e) in fp32
+// and d the rest of it times ln 2.  (2^t is off by 2 * 2^-24, which the quotient keeps at
+// most, its product with 1 + d by 1, the sum by 1, the reciprocal by 2, the product by 1.)
+// A bf16 g times the first 15 bits of log2(e) is exact, so the rest is one product; d^2 / 2
+// is left out, under 2^-24 down to g = -66, where |silu| is under 2^-89 and, with |u| up to
+// kMostUp, the product below the least a that comes here.  Where 2^t is infinite the
+// quotient is 0 (d is positive there in bf16; else it is not looked at).
+template <typename T>
 __device__ __forceinline__ float silu_f32(float g) {
-  constexpr float kLog2e = 0x1.715476p+0f, kLog2eLow = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;
-  const float t = -g * kLog2e;
-  const float rest = fmaf(-g, kLog2eLow, fmaf(-g, kLog2e, -t));
-  const float p = __builtin_amdgcn_exp2f(t);
-  // Past the range p is infinite (and rest may be too): the sum stays so.
-  const float e = t < 128.0f ? fmaf(p, rest * kLn2, p) : p;
+  constexpr float kLn2 = 0x1.62e430p-1f;
+  float e;
+  if constexpr (std::is_same<T, slc::bf16_t>::value) {
+    constexpr float kLog2e = 0x1.7154p+0f, kRestLn2 = 0x1.d94ae1p-18f * kLn2;
+    const float p = __builtin_amdgcn_exp2f(-g * kLog2e);
+    e = fmaf(p, -g * kRestLn2, p);
+  } else {
+    constexpr float kLog2e = 0x1.715476p+0f, kLog2eLow = 0x1.4ae0c0p-26f;
+    const float t = -g * kLog2e;
+    const float p = __builtin_amdgcn_exp2f(t);
+    e = t < 128.0f ? fmaf(p, fmaf(-g, kLog2eLow, fmaf(-g, kLog2e, -t)) * kLn2, p) : p;
+  }
   return g * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
@@ -169,12 +182,35 @@ __device__ __forceinline__ double rsqrt64(double x) {
   return fma(r * 0.5, fma(-x * r, r, 1.0), r);
 }
 
+// The largest magnitude so far (as its bits, a pair of them for 16-bit types) and one
+// more word of the operand; and that magnitude as fp32 bits in the end.
+template <typename T>
+__device__ __forceinline__ void up_max(uint32_t& most, uint32_t word) {
+  if constexpr (sizeof(T) == 4) {
+    most = max(most, word & 0x7fffffffu);
+  } else {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                  __builtin_bit_cast(u16x2, word & 0x7fff7fffu)));
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t up_bits(uint32_t most) {
+  if constexpr (sizeof(T) == 4) {
+    return most;
+  } else {
+    T e;
+    e.bits = static_cast<uint16_t>(max(most & 0xffffu, most >> 16));
+    return __float_as_uint(slc::to_f32(e));
+  }
+}
+
 // ---- reductions over a wave in the VALU --------------------------------------------
 // Lane pairs one apart, two apart, mirrored in eight, mirrored in sixteen (DPP),
 // then rows of 16 and halves of 32 (lane swaps): every lane ends with the total.
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t x) {
-  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true);
 }
 constexpr int kPairs = 0xB1, kQuads = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
 
@@ -233,9 +269,12 @@ __device__ __forceinline__ uint32_t pack4(const uint32_t* b) {
   return lo | hi;
 }
 
+// Three vectors a lane with up to eight waves, whose registers then suffice.
+__host__ __device__ constexpr int max_waves(int nv) { return nv == 3 ? 8 : kMaxWaves; }
+
 // One workgroup of whole waves per row.
 template <typename T, int SRC, int NV, bool LOOP>
-__global__ __launch_bounds__(kMaxWaves * 64) void quantize_kernel(Args p) {
+__global__ __launch_bounds__(max_waves(NV) * 64) void quantize_kernel(Args p) {
   using TR = Traits<T, SRC>;
   constexpr int VEC = TR::VEC;
   __shared__ Shared shared;
@@ -274,7 +313,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void quantize_kernel(Args p) {
       const float x = elem<T>(a[slot], k);
       if constexpr (SRC == kPlain) v[slot][k] = x;
       if constexpr (TR::kHasW) v[slot][k] = x * elem<T>(w[slot], k);
-      if constexpr (SRC == kSwiglu) v[slot][k] = silu_f32(x) * elem<T>(b[slot], k);
+      if constexpr (SRC == kSwiglu) v[slot][k] = silu_f32<T>(x) * elem<T>(b[slot], k);
     }
   };
 
@@ -292,14 +331,16 @@ __global__ __launch_bounds__(kMaxWaves * 64) void quantize_kernel(Args p) {
       const uint32_t bits = __float_as_uint(v[slot][k]);
       most = max(most, static_cast<int>(bits));
       least = max(least, bits);
-      if constexpr (SRC == kSwiglu)
-        most_up = max(most_up, __float_as_uint(fabsf(elem<T>(b[slot], k))));
       if constexpr (TR::kHasW) {
         const float h = elem<T>(a[slot], k);
         squares = fmaf(h, h, squares);
       }
     }
     if constexpr (TR::kHasW) sq += squares;
+    if constexpr (SRC == kSwiglu) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) up_max<T>(most_up, b[slot][k]);
+    }
     if constexpr (SRC == kAddNorm) {
       const int e = (t + lanes * i) * VEC;
       if (e + VEC <= hidden) {
@@ -330,7 +371,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void quantize_kernel(Args p) {
   uint32_t top = max(static_cast<uint32_t>(most), (least >> 31) != 0 ? least & 0x7fffffffu : 0u);
   const uint32_t own_top = top;  // this lane's largest
   top = wave_max_u32(top);
-  if constexpr (SRC == kSwiglu) most_up = wave_max_u32(most_up);
+  if constexpr (SRC == kSwiglu) most_up = wave_max_u32(up_bits<T>(most_up));
   auto add = [](double x, double y) { return x + y; };
   if constexpr (TR::kHasW) sq = wave_reduce64(sq, add);
   if (waves > 1) {
@@ -425,33 +466,32 @@ __global__ __launch_bounds__(kMaxWaves * 64) void quantize_kernel(Args p) {
     return;
   }
   const float inv = 127.0f / static_cast<float>(a64);
+  const float below = inv * (1.0f - TR::kApart), above = inv * (1.0f + TR::kApart);
   auto emit = [&](int i, int slot) {
     const int e = (t + lanes * i) * VEC;
     if (e >= hidden) return;
-    uint32_t bits[VEC], packed[VEC / 4];
-    float worst = 0.0f;
+    uint32_t lo[VEC], hi[VEC], packed[VEC / 4], differ = 0, apart[VEC / 4];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      const float whole = fmaf(v[slot][k], inv, kMagic);
-      bits[k] = __float_as_uint(whole);
-      worst = fmaxf(worst, fabsf(fmaf(v[slot][k], inv, kMagic - whole)));
+      lo[k] = __float_as_uint(fmaf(v[slot][k], below, kMagic));
+      hi[k] = __float_as_uint(fmaf(v[slot][k], above, kMagic));
     }
 #pragma unroll
-    for (int k = 0; k < VEC / 4; ++k) packed[k] = pack4(bits + 4 * k);
-    if (worst > TR::kBorder) {
-      uint32_t mask = 0;
+    for (int j = 0; j < VEC / 4; ++j) {
+      packed[j] = pack4(lo + 4 * j);
+      apart[j] = packed[j] ^ pack4(hi + 4 * j);
+      differ |= apart[j];
+    }
+    if (differ != 0) {  // elements past the row hold 0, at no border
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float whole = __uint_as_float(bits[k]);
-        mask |= fabsf(fmaf(v[slot][k], inv, kMagic - whole)) > TR::kBorder ? 1u << k : 0u;
-      }
-      while (mask != 0) {  // elements past the row hold 0, at no border
-        const int k = __builtin_ctz(mask), shift = 8 * (k & 3);
-        const uint32_t code = static_cast<uint32_t>(code64(e + k) & 0xff);
-#pragma unroll
-        for (int j = 0; j < VEC / 4; ++j)
-          if (j == k / 4) packed[j] = (packed[j] & ~(0xffu << shift)) | code << shift;
-        mask &= mask - 1;
+      for (int j = 0; j < VEC / 4; ++j) {
+        uint32_t rest = apart[j];
+        while (rest != 0) {
+          const int k = __builtin_ctz(rest) / 8;
+          const uint32_t byte = 0xffu << (8 * k);
+          packed[j] = (packed[j] & ~byte) | static_cast<uint32_t>(code64(e + 4 * j + k) & 0xff) << (8 * k);
+          rest &= ~byte;
+        }
       }
     }
     if (e + VEC <= hidden) {
@@ -494,9 +534,22 @@ __global__ __launch_bounds__(kMaxWaves * 64) void quantize_kernel(Args p) {
   if (t == 0) p.scales[row] = scale <= static_cast<double>(FLT_MAX) ? static_cast<float>(scale) : __builtin_nanf("");
 }
 
-#ifndef SLC_Q8_NV
-#define SLC_Q8_NV 2
-#endif
+// Vectors per lane for rows of `vecs` vectors, or 0 for rows that no registers hold.  Few
+// rows leave CUs idle, so as many waves as the row fills share it (us, one | two vectors a
+// lane: SwiGLU 32 x 4864 bf16 4.7 | 5.0, norm 128 x 1001 3.8 | 4.4).  Many rows: a wave's
+// reductions cost about as much as a vector does, so more vectors share them, while the
+// row's waves still suffice to hide its loads (one | two | three | four: SwiGLU 4096 x 4864
+// bf16 35.8 | 24.7 | 23.3 | 24.6, codes 19.3 | 13.0 | 12.6 | 12.6, norm 4096 x 896 8.0 | 8.1
+// | 8.7 | 9.2, SwiGLU 4096 x 4864 fp32 two 40.7, three 34.0, four 33.0).
+inline int vectors_per_lane(int vecs, int64_t rows) {
+  auto waves = [&](int nv) { return (vecs + 64 * nv - 1) / (64 * nv); };
+  for (int nv : {1, 2, 4})
+    if (waves(nv) <= max_waves(nv) && rows * waves(nv) <= 2048) return nv;
+  if (vecs <= 256) return 2;
+  if (waves(3) <= max_waves(3)) return 3;
+  return waves(4) <= max_waves(4) ? 4 : 0;
+}
+
 template <typename T, int SRC>
 int launch(Args p, int64_t rows, const char* what, hipStream_t stream) {
   const int vecs = (p.hidden + Traits<T, SRC>::VEC - 1) / Traits<T, SRC>::VEC;
@@ -513,10 +566,18 @@ int launch(Args p, int64_t rows, const char* what, hipStream_t stream) {
     }
     return static_cast<int>(SLC_OK);
   };
-  if (SLC_Q8_NV == 1 && waves(1) <= kMaxWaves) return go(quantize_kernel<T, SRC, 1, false>, waves(1));
-  if (waves(2) <= kMaxWaves) return go(quantize_kernel<T, SRC, 2, false>, waves(2));
-  if (waves(4) <= kMaxWaves) return go(quantize_kernel<T, SRC, 4, false>, waves(4));
-  return go(quantize_kernel<T, SRC, 1, true>, kMaxWaves);
+  switch (vectors_per_lane(vecs, rows)) {
+    case 1:
+      return go(quantize_kernel<T, SRC, 1, false>, waves(1));
+    case 2:
+      return go(quantize_kernel<T, SRC, 2, false>, waves(2));
+    case 3:
+      return go(quantize_kernel<T, SRC, 3, false>, waves(3));
+    case 4:
+      return go(quantize_kernel<T, SRC, 4, false>, waves(4));
+    default:
+      return go(quantize_kernel<T, SRC, 1, true>, kMaxWaves);
+  }
 }
 
 template <int SRC>
