@@ -28,21 +28,6 @@ __device__ __forceinline__ i32x4_t mfma(i32x4_t a, i32x4_t b, i32x4_t c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-// 16 codes from any address, zeros past `left` of them.
-__device__ __forceinline__ uint4 load_codes(const int8_t* p, int left) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (left >= 16) {
-    __builtin_memcpy(&v, p, 16);
-  } else if (left > 0) {
-    uint32_t word[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 15; ++i)
-      if (i < left) word[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(p[i])) << (8 * (i % 4));
-    v = make_uint4(word[0], word[1], word[2], word[3]);
-  }
-  return v;
-}
-
 // float(sum) * sx * sw + bias; the last two in one fma (and one rounding) in
 // every kernel, so that all give the same bits.
 __device__ __forceinline__ float finish(int sum, float sx, float sw, float bias) {
@@ -60,12 +45,46 @@ struct Problem {
   int64_t x_rs, y_rs;
 };
 
-// Any sizes, strides and alignment: BM x BN tiles staged through registers into
-// one LDS tile pair, four waves of 2 x 2.
+// ---- any sizes, strides and alignment -----------------------------------------------
+// 16 codes of a row of K from code k on, zeros past K: all but the last chunk as they lie
+// (at any address), the last as the 16 codes that end the row, moved down by `shift`.  No
+// load leaves the row, and none waits for a branch.
+struct Chunk {
+  int at, shift;
+  __device__ __forceinline__ Chunk(int k, int K) : at(k < K - 16 ? k : K - 16), shift(k - at < 16 ? k - at : 16) {}
+};
+__device__ __forceinline__ uint4 moved_down(const uint4& v, int shift) {
+  uint64_t lo = static_cast<uint64_t>(v.y) << 32 | v.x, hi = static_cast<uint64_t>(v.w) << 32 | v.z;
+  const int bits = 8 * (shift & 7);
+  if (shift >= 8) {
+    lo = hi;
+    hi = 0;
+  }
+  if (shift >= 16) lo = 0;
+  if (bits > 0) {
+    lo = lo >> bits | hi << (64 - bits);
+    hi >>= bits;
+  }
+  return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+                    static_cast<uint32_t>(hi >> 32));
+}
+// A row of fewer than 16 codes.
+__device__ __forceinline__ uint4 short_row(const int8_t* p, int K) {
+  uint32_t word[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 15; ++i)
+    if (i < K) word[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(p[i])) << (8 * (i % 4));
+  return make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+// BM x BN tiles staged through registers into one LDS tile pair, the next k-tile on its
+// way while this one is multiplied; four waves of 2 x 2.  Rows past M and N repeat the
+// last one (their outputs are not stored).
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
   constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 16, FN = TN / 16;
   constexpr int XPT = BM * kChunks / 256, WPT = BN * kChunks / 256;
+  constexpr int kStep = 256 / kChunks;  // rows between a thread's chunks
   __shared__ __attribute__((aligned(16))) unsigned char xs[BM * kBK];
   __shared__ __attribute__((aligned(16))) unsigned char ws[BN * kBK];
   const int tid = threadIdx.x;
@@ -73,37 +92,50 @@ __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
   const int lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wm = wave >> 1, wn = wave & 1;
   const int64_t m0 = static_cast<int64_t>(blockIdx.y) * BM, n0 = static_cast<int64_t>(blockIdx.x) * BN;
+  const int row = tid / kChunks, chunk = tid % kChunks;
+
+  const int8_t* xp[XPT];
+  const int8_t* wp[WPT];
+#pragma unroll
+  for (int i = 0; i < XPT; ++i) {
+    const int64_t m = m0 + row + kStep * i;
+    xp[i] = p.x + (m < p.M ? m : p.M - 1) * p.x_rs;
+  }
+#pragma unroll
+  for (int i = 0; i < WPT; ++i) {
+    const int64_t n = n0 + row + kStep * i;
+    wp[i] = p.w + (n < p.N ? n : p.N - 1) * p.K;
+  }
+  uint4 xr[XPT], wr[WPT];
+  auto fetch = [&](int k0) {
+    const Chunk ch(k0 + chunk * 16, p.K);
+#pragma unroll
+    for (int i = 0; i < XPT; ++i) __builtin_memcpy(&xr[i], xp[i] + ch.at, 16);
+#pragma unroll
+    for (int i = 0; i < WPT; ++i) __builtin_memcpy(&wr[i], wp[i] + ch.at, 16);
+  };
+  auto stash = [&](int k0) {
+    if (p.K - k0 < kBK) {  // the last k-tile, and K is no multiple of it
+      const Chunk ch(k0 + chunk * 16, p.K);
+#pragma unroll
+      for (int i = 0; i < XPT; ++i) xr[i] = moved_down(xr[i], ch.shift);
+#pragma unroll
+      for (int i = 0; i < WPT; ++i) wr[i] = moved_down(wr[i], ch.shift);
+    }
+#pragma unroll
+    for (int i = 0; i < XPT; ++i)
+      *reinterpret_cast<uint4*>(xs + lds_offset(row + kStep * i, chunk)) = xr[i];
+#pragma unroll
+    for (int i = 0; i < WPT; ++i)
+      *reinterpret_cast<uint4*>(ws + lds_offset(row + kStep * i, chunk)) = wr[i];
+  };
 
   i32x4_t acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
-
-  for (int k0 = 0; k0 < p.K; k0 += kBK) {
-    uint4 xr[XPT], wr[WPT];
-#pragma unroll
-    for (int i = 0; i < XPT; ++i) {
-      const int id = tid + 256 * i, row = id / kChunks, k = k0 + (id % kChunks) * 16;
-      xr[i] = load_codes(p.x + (m0 + row) * p.x_rs + k, m0 + row < p.M ? p.K - k : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < WPT; ++i) {
-      const int id = tid + 256 * i, row = id / kChunks, k = k0 + (id % kChunks) * 16;
-      wr[i] = load_codes(p.w + (n0 + row) * p.K + k, n0 + row < p.N ? p.K - k : 0);
-    }
-    __syncthreads();  // the tiles before are read
-#pragma unroll
-    for (int i = 0; i < XPT; ++i) {
-      const int id = tid + 256 * i;
-      *reinterpret_cast<uint4*>(xs + lds_offset(id / kChunks, id % kChunks)) = xr[i];
-    }
-#pragma unroll
-    for (int i = 0; i < WPT; ++i) {
-      const int id = tid + 256 * i;
-      *reinterpret_cast<uint4*>(ws + lds_offset(id / kChunks, id % kChunks)) = wr[i];
-    }
-    __syncthreads();
+  auto multiply = [&]() {
 #pragma unroll
     for (int kk = 0; kk < kBK / 64; ++kk) {
       i32x4_t a[FM], b[FN];
@@ -117,6 +149,27 @@ __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
+    }
+  };
+
+  if (p.K < 16) {
+    const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < XPT; ++i)
+      *reinterpret_cast<uint4*>(xs + lds_offset(row + kStep * i, chunk)) = chunk == 0 ? short_row(xp[i], p.K) : none;
+#pragma unroll
+    for (int i = 0; i < WPT; ++i)
+      *reinterpret_cast<uint4*>(ws + lds_offset(row + kStep * i, chunk)) = chunk == 0 ? short_row(wp[i], p.K) : none;
+    __syncthreads();
+    multiply();
+  } else {
+    fetch(0);
+    for (int k0 = 0; k0 < p.K; k0 += kBK) {
+      stash(k0);
+      __syncthreads();
+      if (k0 + kBK < p.K) fetch(k0 + kBK);
+      multiply();
+      __syncthreads();  // every wave's reads of the tiles are done
     }
   }
   // Lane (c, g) of a 16 x 16 fragment: column c, rows 4g .. 4g + 3.
@@ -954,14 +1007,24 @@ int launch(const Problem& p, hipStream_t stream) {
     }
     if (rc != kNoPath) return rc;
   }
-  const int64_t m_tiles = (static_cast<int64_t>(p.M) + 63) / 64;
-  const int64_t n_tiles = (static_cast<int64_t>(p.N) + 63) / 64;
-  SLC_REQUIRE(m_tiles <= 65535 && n_tiles < (1 << 24),
-              "slc_hip_linear_q8: %d x %d outputs exceed one launch's grid", p.M, p.N);
-  hipLaunchKernelGGL((tile_kernel<T, 64, 64>),
-                     dim3(static_cast<unsigned>(n_tiles), static_cast<unsigned>(m_tiles)), dim3(256),
-                     0, stream, p);
-  return slc_host::check_launch("slc_hip_linear_q8");
+#ifndef SLC_Q8_ANY
+#define SLC_Q8_ANY 0
+#endif
+  // Other rows: 128 x 128 tiles from four rounds of them over the CUs, else 64 x 64, of which
+  // several share a CU (us, 64 x 64 | 128 x 128: 301 x 1003 x 1001 9.0 | 20, 4096 x 1003 x 1001
+  // 21.9 | 24.1, 500 x 9727 x 1001 25 | 30, 4096 x 9727 x 1001 150 | 119, 32768 x 897 x 3001
+  // 330 | 221).
+  auto any = [&](auto kernel, int64_t tile) -> int {
+    const int64_t m_tiles = (p.M + tile - 1) / tile, n_tiles = (p.N + tile - 1) / tile;
+    SLC_REQUIRE(m_tiles <= 65535 && n_tiles < (1 << 24), "slc_hip_linear_q8: %d x %d outputs exceed one launch's grid",
+                p.M, p.N);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_tiles), static_cast<unsigned>(m_tiles)), dim3(256), 0,
+                       stream, p);
+    return slc_host::check_launch("slc_hip_linear_q8(any)");
+  };
+  const int64_t large = ((static_cast<int64_t>(p.M) + 127) / 128) * ((static_cast<int64_t>(p.N) + 127) / 128);
+  if (SLC_Q8_ANY == 0 ? large >= 4 * slc_host::device_cu_count() : SLC_Q8_ANY == 128) return any(tile_kernel<T, 128, 128>, 128);
+  return any(tile_kernel<T, 64, 64>, 64);
 }
 
 }  // namespace
