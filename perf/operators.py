@@ -163,12 +163,20 @@ def _linear(codes, scales, w, ws, bias, dtype):
     return (y if bias is None else y + bias.float()).to(dtype)
 
 
-def _run_own(state):
+def _import_backends():
+    """The framework's kernels, imported once as a program does, not in every pass."""
+
     package = str(Path("llm-compiler_amd").resolve())
     if package not in sys.path:
         sys.path.insert(0, package)
     from stateful_llm_compiler_hip import backends
 
+    _run_own.backends = backends
+    return backends
+
+
+def _run_own(state):
+    backends = getattr(_run_own, "backends", None) or _import_backends()
     op = state["op"]
     if op == "linear":
         return backends.hip_linear_q8(state["codes"], state["scales"], state["w"], state["ws"], state["bias"],
