@@ -9,6 +9,8 @@
 //
 // X and W rows are K-contiguous, the operand layout of v_mfma_i32_16x16x64_i8
 // (16 consecutive k per lane), so neither operand is transposed.
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace {
@@ -208,19 +210,26 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned 
 }
 
 // Tile id -> (m_blk, n_blk): workgroup ids go round-robin to the 8 XCDs, each with
-// its own L2, so ids are gathered per XCD, then run in groups of kGroupM M-tiles,
-// N-tile-major inside a group.
+// its own L2, so ids are gathered per XCD, then run in groups of kGroupM M-tiles (a power
+// of two), N-tile-major inside a group.  One division, but in a last, smaller group.
 template <int kGroupM>
 __device__ __forceinline__ void xcd_tile_of(int id, int n_tiles, int m_tiles, int& m_blk,
                                             int& n_blk) {
-  constexpr int kXcds = 8;
-  const int per = n_tiles * m_tiles / kXcds;
-  const int t = id < per * kXcds ? (id % kXcds) * per + id / kXcds : id;
-  const int span = kGroupM * n_tiles;
-  const int first_m = (t / span) * kGroupM;
-  const int gm = m_tiles - first_m < kGroupM ? m_tiles - first_m : kGroupM;
-  m_blk = first_m + (t % span) % gm;
-  n_blk = (t % span) / gm;
+  static_assert((kGroupM & (kGroupM - 1)) == 0, "a power of two");
+  constexpr uint32_t kXcds = 8;
+  const uint32_t u = static_cast<uint32_t>(id), per = static_cast<uint32_t>(n_tiles * m_tiles) / kXcds;
+  const uint32_t t = u < per * kXcds ? (u % kXcds) * per + u / kXcds : u;
+  const uint32_t span = static_cast<uint32_t>(kGroupM * n_tiles);
+  const uint32_t group = t / span, rest = t - group * span;
+  const int first_m = static_cast<int>(group) * kGroupM;
+  if (first_m + kGroupM <= m_tiles) {
+    m_blk = first_m + static_cast<int>(rest % kGroupM);
+    n_blk = static_cast<int>(rest / kGroupM);
+  } else {
+    const uint32_t gm = static_cast<uint32_t>(m_tiles - first_m);
+    n_blk = static_cast<int>(rest / gm);
+    m_blk = first_m + static_cast<int>(rest % gm);
+  }
 }
 
 // Swizzle of the W tile: the 16 rows of a fragment are four runs of four, eight
@@ -251,6 +260,31 @@ constexpr int64_t kRangeLimit = (int64_t{1} << 31) - (1 << 20);
 constexpr int kNoPath = -2;
 // An offset past every such range that stays below 2^31 with K added.
 constexpr int kPastRange = 0x7fffffff - (1 << 18);
+
+// Four consecutive elements of the bias (0 without one), in words of two where the
+// outputs are whole runs of eight.
+template <typename T, bool PAIRS>
+struct BiasRun {
+  static constexpr int kWords = PAIRS && sizeof(T) == 2 ? 2 : 4;
+  uint32_t raw[kWords] = {};
+  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t& rbias, int n) {
+    if constexpr (kWords == 2) {
+      const auto two = __builtin_amdgcn_raw_buffer_load_b64(rbias, n * 2, 0, 0);
+      raw[0] = two[0];
+      raw[1] = two[1];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) raw[r] = load_bias<T>(rbias, n + r);
+    }
+  }
+  __device__ __forceinline__ void wait() {
+#pragma unroll
+    for (int r = 0; r < kWords; ++r) asm volatile("" : "+v"(raw[r]));
+  }
+  __device__ __forceinline__ float value(int r) const {
+    return bias_value<T>(kWords == 2 ? raw[r / 2] >> (16 * (r % 2)) & 0xffffu : raw[r]);
+  }
+};
 
 // A lane's run of eight consecutive outputs at a byte offset from the tile's first.
 // VST, 16-byte stores: what is outside the tile has an offset past the range (a run is
@@ -392,11 +426,8 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
     // Scales and bias of this lane's outputs, requested before the k loop.
     const __amdgpu_buffer_rsrc_t rsx = make_rsrc(p.sx + m0, rows * 4);
     const __amdgpu_buffer_rsrc_t rsw = make_rsrc(p.sw + n0, cols * 4);
-    const __amdgpu_buffer_rsrc_t rbias =
-        make_rsrc(p.bias != nullptr ? static_cast<const T*>(p.bias) + n0 : nullptr,
-                  p.bias != nullptr ? cols * static_cast<int>(sizeof(T)) : 0);
     float sx[FM], sw[FN][4];
-    uint32_t bias[FN][4];
+    BiasRun<T, VST> bias[FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
       sx[i] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsx, (wm * TM + i * 16 + c) * 4, 0, 0));
@@ -405,17 +436,17 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
       const int n = wn * TN + (j >> 1) * 32 + 8 * g + (j & 1) * 4;
       const auto four = __builtin_amdgcn_raw_buffer_load_b128(rsw, n * 4, 0, 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        sw[j][r] = __int_as_float(static_cast<int>(four[r]));
-        bias[j][r] = load_bias<T>(rbias, n + r);
-      }
+      for (int r = 0; r < 4; ++r) sw[j][r] = __int_as_float(static_cast<int>(four[r]));
+    }
+    if (p.bias != nullptr) {
+      const __amdgpu_buffer_rsrc_t rbias =
+          make_rsrc(static_cast<const T*>(p.bias) + n0, cols * static_cast<int>(sizeof(T)));
+#pragma unroll
+      for (int j = 0; j < FN; ++j) bias[j].load(rbias, wn * TN + (j >> 1) * 32 + 8 * g + (j & 1) * 4);
     }
     i32x4_t acc[FN][FM];
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int i = 0; i < FM; ++i) acc[j][i] = i32x4_t{0, 0, 0, 0};
-    for (int kt = 0; kt < ktiles; ++kt) {
+    auto k_tile = [&](auto is_first) {
+      constexpr bool FIRST = decltype(is_first)::value;
       // Tile kt is in its stage; the stage read before may be refilled.  No wait
       // on stores: the previous tile's output may still be in flight.
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -436,9 +467,12 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
-          for (int i = 0; i < FM; ++i) acc[j][i] = mfma(b[j], a[i], acc[j][i]);
+          for (int i = 0; i < FM; ++i) acc[j][i] = mfma(b[j], a[i], FIRST && kk == 0 ? i32x4_t{0, 0, 0, 0} : acc[j][i]);
       }
-    }
+    };
+    k_tile(std::true_type{});
+#pragma clang loop unroll(disable)
+    for (int kt = 1; kt < ktiles; ++kt) k_tile(std::false_type{});
     // The scales have arrived while the tile was multiplied: waited for here, as a
     // later wait would count this tile's stores too.
 #pragma unroll
@@ -446,7 +480,9 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) asm volatile("" : "+v"(sw[j][r]), "+v"(bias[j][r]));
+      for (int r = 0; r < 4; ++r) asm volatile("" : "+v"(sw[j][r]));
+#pragma unroll
+    for (int j = 0; j < FN; ++j) bias[j].wait();
     constexpr int kSize = static_cast<int>(sizeof(T));
     const __amdgpu_buffer_rsrc_t ry =
         make_rsrc(static_cast<T*>(p.y) + m0 * p.y_rs + n0, (static_cast<int64_t>(rows) - 1) * p.y_rs * kSize + cols * kSize);
@@ -463,7 +499,7 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = 2 * q + (e >> 2), r = e & 3;
-          v[e] = finish(acc[j][i][r], sx[i], sw[j][r], bias_value<T>(bias[j][r]));
+          v[e] = finish(acc[j][i][r], sx[i], sw[j][r], bias[j].value(r));
         }
         store_run<T, VST>(ry, v, whole + i * rows16, half + i * rows16, m < rows ? cols - n : 0);
       }
@@ -658,13 +694,9 @@ __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, i
     const int rows = p.M - m0 < BM ? static_cast<int>(p.M - m0) : BM;
     const int cols = p.N - n0 < BN ? static_cast<int>(p.N - n0) : BN;
     i32x4_t acc[FN][FM];
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int i = 0; i < FM; ++i) acc[j][i] = i32x4_t{0, 0, 0, 0};
     uint32_t own_x[TM / 64], own_w = 0, own_bias = 0;
-#pragma clang loop unroll(disable)
-    for (int kt = 0; kt < ktiles; ++kt) {
+    auto k_tile = [&](int kt, auto is_first) {
+      constexpr bool FIRST = decltype(is_first)::value;
       const int x_at = x_read + x_slot * XB, w_at = w_read + w_slot * WB;
       x_slot = x_slot == XS - 1 ? 0 : x_slot + 1;
       w_slot = w_slot == WS - 1 ? 0 : w_slot + 1;
@@ -682,8 +714,8 @@ __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, i
         for (int i = 0; i < FM; ++i) a[i] = *reinterpret_cast<const i32x4_t*>(xs + i * 16 * kBK);
         __builtin_amdgcn_sched_barrier(0);
         if (kk == 0) {
-          if (kt > 0 || id == first) issue_w();
-          if (kt == 0) {
+          if (!FIRST || id == first) issue_w();
+          if constexpr (FIRST) {
             // Lane l of a load holds the scale of row l, or of column l, of the wave's.
             const __amdgpu_buffer_rsrc_t rsx = make_rsrc(p.sx + m0, rows * 4);
             const __amdgpu_buffer_rsrc_t rsw = make_rsrc(p.sw + n0, cols * 4);
@@ -700,19 +732,22 @@ __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, i
           issue_x();
           // Nobody may still read the tile when its slots are refilled.
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (late) landed(kt == 0 && id != first);
+          if (late) landed(FIRST && id != first);
         }
         barrier();
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-          for (int j = 0; j < FN; ++j) acc[j][i] = mfma(b[j], a[i], acc[j][i]);
+          for (int j = 0; j < FN; ++j) acc[j][i] = mfma(b[j], a[i], FIRST && kk == 0 ? i32x4_t{0, 0, 0, 0} : acc[j][i]);
         __builtin_amdgcn_s_setprio(0);
-        if (kk == 1 && !late) landed(kt == 0 && id != first);
+        if (kk == 1 && !late) landed(FIRST && id != first);
         if (kk == 0 || kt + 1 < ktiles || !late) barrier();
       }
-    }
+    };
+    k_tile(0, std::true_type{});
+#pragma clang loop unroll(disable)
+    for (int kt = 1; kt < ktiles; ++kt) k_tile(kt, std::false_type{});
     // The scales, waited for before the next loads are issued.
 #pragma unroll
     for (int r = 0; r < TM / 64; ++r) asm volatile("" : "+v"(own_x[r]));
@@ -958,11 +993,11 @@ inline Kernel choose(int64_t M, int64_t N, int64_t K) {
     int bm, bn;
     double fixed, per_k;
   };
-  constexpr Cost costs[] = {{k64x64, 64, 64, 0.67, 0.20},
-                            {k128x64, 128, 64, 0.70, 0.33},
-                            {k128x128, 128, 128, 1.28, 0.51},
-                            {k256x128, 256, 128, 2.6, 0.89},
-                            {k256x256, 256, 256, 6.3, 1.59}};
+  constexpr Cost costs[] = {{k64x64, 64, 64, 0.46, 0.20},
+                            {k128x64, 128, 64, 0.53, 0.33},
+                            {k128x128, 128, 128, 1.16, 0.51},
+                            {k256x128, 256, 128, 2.25, 0.89},
+                            {k256x256, 256, 256, 5.8, 1.48}};
   const int64_t cus = slc_host::device_cu_count(), k_tiles = (K + kBK - 1) / kBK;
   Kernel best = k64x64;
   double least = 0.0;
