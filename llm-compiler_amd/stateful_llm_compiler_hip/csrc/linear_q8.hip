@@ -553,30 +553,31 @@ __device__ __forceinline__ i32x4_t descriptor(const void* base, int64_t bytes) {
 //
 // Turns (one barrier after each), k-tile q, k-step s of it: group 0 reads (q, s) in
 // turn 4q + 2s and multiplies it in the next, group 1 one turn later.  So what tile
-// q - 1 occupied is free from turn 4q on.  X has three slots and W has WS: with (q, 0)
-// a wave issues its part of W tile q + WS - 1, with (q, 1) of X tile q + 2, each into
-// the slot of tile q - 1.  Every wave waits for its part of tile q + 1 before the
-// barrier that ends turn 4q + 3 (group 0 after multiplying (q, 1), group 1 after
+// q - 1 occupied is free from turn 4q on.  X has three slots and W two, which fill the
+// LDS: with (q, 0) a wave issues its part of W tile q + 1, with (q, 1) of X tile q + 2,
+// each into the slot of tile q - 1.  Every wave waits for its part of tile q + 1 before
+// the barrier that ends turn 4q + 3 (group 0 after multiplying (q, 1), group 1 after
 // reading it).  Memory operations complete in order, so the wait leaves open what was
-// issued later: X tile q + 2 and, with three W slots, W tile q + 2.  At the end of an
-// output tile the next W tile is issued before the stores, so that the first such wait
-// leaves the stores open too.
+// issued later: X tile q + 2.  At the end of an output tile the next W tile is issued
+// before the stores, so that the first such wait leaves the stores open too.
 //
 // Workgroups walk the output tiles id, id + grid, ...; the loads run on across tile
 // boundaries.  The MFMA's A operand is W, the rows of two fragments interleaved in runs
 // of four, so that a lane holds eight consecutive outputs of one row and stores them
 // from registers.  Past K the X chunks are loaded as zeros (an offset past the range),
 // whatever the W chunks beside them hold.
-template <typename T, int BM, int BN, int WS, int GM, bool VST>
+constexpr int kTurnsTile = 256, kTurnsGroup = 4;
+template <typename T, bool VST>
 __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, int m_tiles) {
-  constexpr int CW = 8, CWN = 4, XS = 3;
+  constexpr int BM = kTurnsTile, BN = kTurnsTile, GM = kTurnsGroup;
+  constexpr int CW = 8, CWN = 4, XS = 3, WS = 2;
   constexpr int TM = BM / 2, TN = BN / CWN;
   constexpr int FM = TM / 16, FN = TN / 16;
   constexpr int XB = BM * kBK, WB = BN * kBK;
   constexpr int XO = BM / 8 / CW, WO = BN / 8 / CW;
   constexpr int kSize = static_cast<int>(sizeof(T));
   constexpr int kStores = VST ? FM * FN / 2 * (kSize / 2) : 0;
-  constexpr int kOpen = (WS - 2) * WO + XO;
+  constexpr int kOpen = XO;
   static_assert(XO * CW * 8 == BM && WO * CW * 8 == BN, "operands split evenly over the waves");
   static_assert(TM % 64 == 0 && TN % 32 == 0 && TN <= 64, "whole fragments, in pairs over N; scales by lane");
   static_assert(kOpen + kStores <= 63, "the wait count fits vmcnt");
@@ -678,8 +679,6 @@ __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, i
   issue_x();
   issue_w();
   issue_x();
-#pragma unroll
-  for (int i = 2; i < WS; ++i) issue_w();
   landed(false);
   barrier();
   if (late) barrier();
@@ -787,8 +786,9 @@ __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, i
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <typename T, int BM, int BN, int WS, int GM>
+template <typename T>
 int launch_turns(const Problem& p, hipStream_t stream) {
+  constexpr int BM = kTurnsTile, BN = kTurnsTile;
   const int64_t m_tiles = (static_cast<int64_t>(p.M) + BM - 1) / BM;
   const int64_t n_tiles = (static_cast<int64_t>(p.N) + BN - 1) / BN;
   if (BM * p.x_rs >= kRangeLimit || BM * p.y_rs * static_cast<int64_t>(sizeof(T)) >= kRangeLimit ||
@@ -800,7 +800,7 @@ int launch_turns(const Problem& p, hipStream_t stream) {
   const int64_t unit = 16 / static_cast<int64_t>(sizeof(T));
   const bool vectors = p.N % unit == 0 && p.y_rs % unit == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
 #define SLC_TURNS(VST)                                                                             \
-  hipLaunchKernelGGL((turns_kernel<T, BM, BN, WS, GM, VST>), dim3(static_cast<unsigned>(grid)), \
+  hipLaunchKernelGGL((turns_kernel<T, VST>), dim3(static_cast<unsigned>(grid)), \
                      dim3(512), 0, stream, p, static_cast<int>(n_tiles), static_cast<int>(m_tiles))
   if (vectors) {
     SLC_TURNS(true);
@@ -810,7 +810,6 @@ int launch_turns(const Problem& p, hipStream_t stream) {
 #undef SLC_TURNS
   return slc_host::check_launch("slc_hip_linear_q8(turns)");
 }
-
 
 // kNoPath (nothing launched) where 32-bit offsets do not reach over a tile's rows.
 template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM>
@@ -957,7 +956,9 @@ int launch_rows(const Problem& p, hipStream_t stream) {
   const int64_t share = (static_cast<int64_t>(p.N) + 255) / 256;
   const int feat = static_cast<int>(share > 32 ? 32 : share);
   const int steps = (p.K + 63) / 64, waves = steps < 8 ? steps : 8;
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.N) + feat - 1) / feat));
+  const int64_t groups = (static_cast<int64_t>(p.N) + feat - 1) / feat;
+  if (groups * waves * 64 >= (int64_t{1} << 32)) return kNoPath;  // threads of one launch
+  const dim3 grid(static_cast<unsigned>(groups));
 #define SLC_ROWS(MB, TILES, U) \
   hipLaunchKernelGGL((rows_kernel<T, MB, TILES, U>), grid, dim3(waves * 64), 0, stream, p, feat)
   if (feat <= 16) {
@@ -974,17 +975,17 @@ int launch_rows(const Problem& p, hipStream_t stream) {
 // Which kernel takes a shape of aligned rows, all giving the same bits.
 //
 // Up to 32 rows and 8192 features, rows_kernel: a tile would leave most CUs idle (us,
-// rows | 64 x 64 tiles: 8 x 1152 x 896 3.6 | 4.8, 32 x 896 x 4864 8.4 | 10.5, 32 x 4096 x
-// 4096 8.8 | 9.8; but 48 x 896 x 4864 10.7 | 10.6, 8 x 9728 x 896 5.6 | 5.1, 8 x 11008 x
-// 4096 14.6 | 10.5), and up to 8 rows from 16384 features, where it reads the weight a
-// little faster (1 x 151936 x 896 24.1 | 26.9, 8 x 50257 x 896 11.1 | 13.1, 8 x 151936 x
-// 896 29.1 | 28.2).
+// rows | 64 x 64 tiles: 8 x 1152 x 896 3.6 | 4.7, 32 x 896 x 4864 8.4 | 10.3, 32 x 4096 x
+// 4096 8.9 | 9.5; but 8 x 9728 x 896 5.6 | 5.0, 8 x 11008 x 4096 14.8 | 10.4), and up to 8
+// rows from 16384 features, where it reads the weight about as fast or faster (1 x 151936
+// x 896 24.4 | 26.6, 8 x 50257 x 896 11.1 | 12.4, 8 x 151936 x 896 29.2 | 28.2; 16 x 151936
+// x 896 32.8 | 28.5).
 //
 // Else the tile whose rounds over the CUs cost least: a round takes fixed + per_k * k-tiles
 // us, measured with every CU busy (K 896 and 4096).  Rounds, not tiles: 8192 x 896 x 896
-// 13.0 us as one round of 256 x 128, 13.4 as two of 128 x 128; 4096 x 9728 x 896 44.8 as
-// five rounds of 256 x 128, 53 as three of 256 x 256; 32768 x 896 x 4864 127 as two of 256 x
-// 256, 147 as four of 256 x 128; 65 x 896 x 896 5.0 as 64 x 64, 8.7 as 256 x 128.
+// 12.6 us as one round of 256 x 128, 13.1 as two of 128 x 128; 4096 x 9728 x 896 41.5 as
+// five rounds of 256 x 128, 51 as three of 256 x 256; 32768 x 896 x 4864 128 as two of 256 x
+// 256, 138 as four of 256 x 128; 65 x 896 x 896 4.9 as 64 x 64, 8.2 as 256 x 128.
 enum Kernel { kRows, k64x64, k128x64, k128x128, k256x128, k256x256 };
 inline Kernel choose(int64_t M, int64_t N, int64_t K) {
   if ((M <= 32 && N <= 8192) || (M <= 8 && N >= 16384)) return kRows;
@@ -1012,16 +1013,13 @@ inline Kernel choose(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-#ifndef SLC_Q8_CHOICE
-#define SLC_Q8_CHOICE(M, N, K) choose(M, N, K)
-#endif
 template <typename T>
 int launch(const Problem& p, hipStream_t stream) {
   const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) == 0 &&
                        p.K % 16 == 0 && p.x_rs % 16 == 0;
   if (aligned) {
     int rc = kNoPath;
-    switch (SLC_Q8_CHOICE(p.M, p.N, p.K)) {
+    switch (choose(p.M, p.N, p.K)) {
       case kRows:
         rc = launch_rows<T>(p, stream);
         break;
@@ -1038,27 +1036,32 @@ int launch(const Problem& p, hipStream_t stream) {
         rc = launch_stream<T, 256, 128, 4, 2, 4, 3, 4>(p, stream);
         break;
       default:
-        rc = launch_turns<T, 256, 256, 2, 4>(p, stream);
+        rc = launch_turns<T>(p, stream);
     }
     if (rc != kNoPath) return rc;
   }
-#ifndef SLC_Q8_ANY
-#define SLC_Q8_ANY 0
-#endif
   // Other rows: 128 x 128 tiles from four rounds of them over the CUs, else 64 x 64, of which
   // several share a CU (us, 64 x 64 | 128 x 128: 301 x 1003 x 1001 9.0 | 20, 4096 x 1003 x 1001
   // 21.9 | 24.1, 500 x 9727 x 1001 25 | 30, 4096 x 9727 x 1001 150 | 119, 32768 x 897 x 3001
   // 330 | 221).
   auto any = [&](auto kernel, int64_t tile) -> int {
-    const int64_t m_tiles = (p.M + tile - 1) / tile, n_tiles = (p.N + tile - 1) / tile;
-    SLC_REQUIRE(m_tiles <= 65535 && n_tiles < (1 << 24), "slc_hip_linear_q8: %d x %d outputs exceed one launch's grid",
-                p.M, p.N);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_tiles), static_cast<unsigned>(m_tiles)), dim3(256), 0,
-                       stream, p);
-    return slc_host::check_launch("slc_hip_linear_q8(any)");
+    const int64_t n_tiles = (p.N + tile - 1) / tile, most = 65535 * tile;  // rows of one grid
+    SLC_REQUIRE(n_tiles < (1 << 24), "slc_hip_linear_q8: %d features exceed one launch's grid", p.N);
+    Problem part = p;
+    for (int64_t done = 0; done < p.M; done += most) {
+      part.x = p.x + done * p.x_rs;
+      part.sx = p.sx + done;
+      part.y = static_cast<T*>(p.y) + done * p.y_rs;
+      part.M = static_cast<int>(p.M - done < most ? p.M - done : most);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_tiles), static_cast<unsigned>((part.M + tile - 1) / tile)),
+                         dim3(256), 0, stream, part);
+      const int rc = slc_host::check_launch("slc_hip_linear_q8(any)");
+      if (rc != SLC_OK) return rc;
+    }
+    return SLC_OK;
   };
   const int64_t large = ((static_cast<int64_t>(p.M) + 127) / 128) * ((static_cast<int64_t>(p.N) + 127) / 128);
-  if (SLC_Q8_ANY == 0 ? large >= 4 * slc_host::device_cu_count() : SLC_Q8_ANY == 128) return any(tile_kernel<T, 128, 128>, 128);
+  if (large >= 4 * slc_host::device_cu_count()) return any(tile_kernel<T, 128, 128>, 128);
   return any(tile_kernel<T, 64, 64>, 64);
 }
 
@@ -1074,7 +1077,7 @@ extern "C" int slc_hip_linear_q8(const int8_t* input, const float* in_scales, co
               (long long)out_features, (long long)in_features);
   SLC_REQUIRE(rows < (1LL << 31) && out_features < (1LL << 31),
               "slc_hip_linear_q8: sizes exceed 2^31");
-  SLC_REQUIRE(in_stride_row >= 0 && (rows <= 1 || out_stride_row >= out_features),
+  SLC_REQUIRE(rows <= 1 || (in_stride_row >= 0 && out_stride_row >= out_features),
               "slc_hip_linear_q8: rows of %lld outputs overlap, or a stride is negative", (long long)out_features);
   if (rows == 0) return SLC_OK;
   SLC_REQUIRE(input && in_scales && weight && weight_scales && output,
@@ -1083,9 +1086,10 @@ extern "C" int slc_hip_linear_q8(const int8_t* input, const float* in_scales, co
   SLC_REQUIRE((reinterpret_cast<uintptr_t>(in_scales) | reinterpret_cast<uintptr_t>(weight_scales)) % 4 == 0 &&
                   (reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(output)) % element == 0,
               "slc_hip_linear_q8: misaligned pointer");
+  // The kernels tell rows past the last by their offsets; one row's strides say nothing.
   const Problem p{input, in_scales, weight, weight_scales, bias, output, static_cast<int>(rows),
-                  static_cast<int>(out_features), static_cast<int>(in_features), in_stride_row,
-                  out_stride_row};
+                  static_cast<int>(out_features), static_cast<int>(in_features),
+                  rows == 1 ? in_features : in_stride_row, rows == 1 ? out_features : out_stride_row};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == SLC_BF16) return launch<slc::bf16_t>(p, s);
   if (dtype == SLC_F16) return launch<slc::f16_t>(p, s);

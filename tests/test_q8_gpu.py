@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from helpers import announce, assert_bitwise_equal, generator
-from stateful_llm_compiler_hip import backends
+from stateful_llm_compiler_hip import _native, backends
 
 pytestmark = pytest.mark.gpu
 
@@ -377,6 +377,110 @@ def test_linear_is_the_same_on_every_path(gpu):
     for rows in (5, 50, 600):
         y = backends.hip_linear_q8(codes[:rows], scales[:rows], odd_w, weight_scales, bias)
         assert_bitwise_equal(y, whole[:rows])
+
+
+# The row kernel, each tile (with 16-byte stores and without), unaligned rows.
+STRIDED = [(3, 200, 128), (30, 300, 144), (50, 96, 256), (200, 20000, 128), (500, 9728, 128), (1100, 9728, 128),
+           (2300, 9728, 896), (2300, 9731, 896), (4000, 4096, 2048), (4000, 4090, 2048), (70, 130, 77),
+           (1100, 9731, 33)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", STRIDED)
+def test_linear_writes_its_outputs_only(gpu, dtype, m, n, k):
+    announce(f"strided {m} x {n} x {k} {dtype}")
+    lib, tag = _native.library(), _native.dtype_tag(dtype)
+    codes, scales, weight, weight_scales, bias = (t.to(gpu) for t in operands(m, n, k, dtype, m + n))
+    x_rs, y_rs = k + 48, n + 24
+    padded = torch.full((m + 2, x_rs), 99, dtype=torch.int8, device=gpu)
+    padded[:m, :k] = codes
+    out = torch.full((m + 3, y_rs), 7.0, dtype=dtype, device=gpu)
+    want = backends.hip_linear_q8(codes, scales, weight, weight_scales, bias, output_dtype=dtype)
+    _native.check(lib.slc_hip_linear_q8(
+        padded.data_ptr(), scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), bias.data_ptr(),
+        out.data_ptr(), tag, m, n, k, x_rs, y_rs, _native.current_stream(gpu)), "slc_hip_linear_q8")
+    assert_bitwise_equal(out[:m, :n], want)
+    assert (out[m:] == 7).all() and (out[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("n", [40, 9728, 20000])
+def test_linear_of_one_row_takes_any_strides(gpu, n):
+    announce(f"one row {n}")
+    lib = _native.library()
+    codes, scales, weight, weight_scales, bias = (t.to(gpu) for t in operands(1, n, 256, torch.bfloat16, 4))
+    want = backends.hip_linear_q8(codes, scales, weight, weight_scales, bias)
+    for x_rs, y_rs in ((0, 0), (7, 1), (-5, -5)):
+        out = torch.full((70, n), 7.0, dtype=torch.bfloat16, device=gpu)
+        _native.check(lib.slc_hip_linear_q8(
+            codes.data_ptr(), scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), bias.data_ptr(),
+            out.data_ptr(), _native.SLC_BF16, 1, n, 256, x_rs, y_rs, _native.current_stream(gpu)), "slc_hip_linear_q8")
+        assert_bitwise_equal(out[:1], want)
+        assert (out[1:] == 7).all()
+
+
+def test_linear_of_a_repeated_row(gpu):
+    # A row stride of 0: every row of X is the same one.
+    announce("repeated row")
+    lib = _native.library()
+    codes, scales, weight, weight_scales, _ = operands(1, 512, 256, None, 6)
+    for m in (20, 100, 600):
+        tokens = torch.rand(m, generator=generator(m)).to(gpu)
+        out = torch.empty(m, 512, device=gpu)
+        row, w, ws = codes.to(gpu), weight.to(gpu), weight_scales.to(gpu)
+        _native.check(lib.slc_hip_linear_q8(
+            row.data_ptr(), tokens.data_ptr(), w.data_ptr(), ws.data_ptr(), None, out.data_ptr(), _native.SLC_F32, m,
+            512, 256, 0, 512, _native.current_stream(gpu)), "slc_hip_linear_q8")
+        assert_bitwise_equal(out, backends.hip_linear_q8(row.expand(m, 256).contiguous(), tokens, w, ws,
+                                                         output_dtype=torch.float32))
+
+
+def test_more_unaligned_rows_than_one_grid(gpu):
+    # 65535 tiles of 128 rows, and five rows more.
+    announce("8388485 rows")
+    m = 65535 * 128 + 5
+    codes = torch.ones(m, 3, dtype=torch.int8, device=gpu)
+    codes[-1] = 5
+    scales = torch.ones(m, device=gpu)
+    weight = torch.tensor([[1, 2, 3], [-1, 0, 1]], dtype=torch.int8, device=gpu)
+    y = backends.hip_linear_q8(codes, scales, weight, torch.ones(2, device=gpu), output_dtype=torch.float32)
+    assert (y[:-1] == torch.tensor([6.0, 0.0], device=gpu)).all() and y[-1].tolist() == [30.0, 0.0]
+
+
+def test_more_features_than_one_launch_has_threads(gpu):
+    # 2^23 groups of 32 features and one more.
+    n = (1 << 28) + 16
+    announce(f"{n} features")
+    weight = torch.empty(n, 16, dtype=torch.int8, device=gpu).random_(-128, 128)
+    codes, scales, _, _, _ = (t.to(gpu) if t is not None else None for t in operands(2, 16, 16, None, 8))
+    weight_scales = torch.full((n,), 0.5, device=gpu)
+    y = backends.hip_linear_q8(codes, scales, weight, weight_scales)
+    for at in (0, (1 << 27) - 64, n - 128):
+        part = slice(at, at + 128)
+        assert_bitwise_equal(y[:, part], backends.hip_linear_q8(codes, scales, weight[part], weight_scales[part]))
+
+
+@pytest.mark.parametrize("at", [1, 2, 8])
+def test_linear_of_operands_at_any_address(gpu, at):
+    announce(f"address {at}")
+    for m, n, k in ((5, 200, 128), (70, 130, 256), (70, 130, 37)):
+        codes, scales, weight, weight_scales, _ = (t.to(gpu) if t is not None else None for t in operands(m, n, k, None, at))
+        want = backends.hip_linear_q8(codes, scales, weight, weight_scales)
+        moved = [torch.full((t.numel() + 16,), 99, dtype=torch.int8, device=gpu) for t in (codes, weight)]
+        views = [b[at:at + t.numel()].view(t.shape) for b, t in zip(moved, (codes, weight))]
+        for view, t in zip(views, (codes, weight)):
+            view.copy_(t)
+        for x, w in ((views[0], weight), (codes, views[1]), views):
+            assert_bitwise_equal(backends.hip_linear_q8(x, scales, w, weight_scales), want)
+
+
+def test_outputs_past_32_bits(gpu):
+    m, n = 20000, 110000
+    announce(f"{m} x {n} outputs")
+    codes, scales, _, _, _ = (t.to(gpu) if t is not None else None for t in operands(m, 16, 64, None, 12))
+    _, _, weight, weight_scales, _ = (t.to(gpu) if t is not None else None for t in operands(1, n, 64, None, 13))
+    y = backends.hip_linear_q8(codes, scales, weight, weight_scales)
+    for part in (slice(0, 300), slice(9700, 10000), slice(m - 300, m)):
+        assert_bitwise_equal(y[part], backends.hip_linear_q8(codes[part], scales[part], weight, weight_scales))
 
 
 def test_linear_leading_axes_and_nan_rows(gpu):
