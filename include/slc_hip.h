@@ -31,6 +31,8 @@
  *                              (cost_model.py:125-245, lowering_selection.py:12-72)
  *   slc_hip_prefill_attention  backends/triton_prefill_attention.py:152-232
  *                              (semantics of execution.py:707-739)
+ *   slc_hip_quantize_q8, slc_hip_rms_norm_q8, slc_hip_swiglu_q8,
+ *   slc_hip_linear_q8: 8-bit linears, which the reference does not have
  */
 #ifndef SLC_HIP_H_
 #define SLC_HIP_H_
@@ -661,8 +663,8 @@ SLC_API int slc_hip_swiglu_q8(const void* gate, const void* up, int8_t* codes, f
  *   input  : rows x in_features codes, row stride in_stride_row
  *   weight : out_features x in_features codes, contiguous
  *   output : rows x out_features, row stride out_stride_row
- * 16-byte aligned rows of codes run the fast kernels; any other alignment and
- * size is taken.
+ * A single row's strides are not looked at.  16-byte aligned rows of codes run the
+ * fast kernels; any other alignment and size is taken.
  */
 SLC_API int slc_hip_linear_q8(const int8_t* input, const float* in_scales, const int8_t* weight,
                               const float* weight_scales, const void* bias, void* output,
