@@ -154,6 +154,16 @@ __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
     }
   };
 
+  // The wave's scales and bias, requested behind the first loads: lane l holds row l's and
+  // column l's.  (Asked for in the epilogue they cost 1 us of 301 x 1003 x 1001's 9.)
+  static_assert(TM <= 64 && TN <= 64, "a lane for each row and column");
+  float own_x = 0.0f, own_w = 0.0f, own_bias = 0.0f;
+  auto scales = [&]() {
+    const int64_t m = m0 + wm * TM + lane % TM, n = n0 + wn * TN + lane % TN;
+    own_x = p.sx[m < p.M ? m : p.M - 1];
+    own_w = p.sw[n < p.N ? n : p.N - 1];
+    if (p.bias != nullptr) own_bias = slc::to_f32(static_cast<const T*>(p.bias)[n < p.N ? n : p.N - 1]);
+  };
   if (p.K < 16) {
     const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -162,10 +172,12 @@ __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
 #pragma unroll
     for (int i = 0; i < WPT; ++i)
       *reinterpret_cast<uint4*>(ws + lds_offset(row + kStep * i, chunk)) = chunk == 0 ? short_row(wp[i], p.K) : none;
+    scales();
     __syncthreads();
     multiply();
   } else {
     fetch(0);
+    scales();
     for (int k0 = 0; k0 < p.K; k0 += kBK) {
       stash(k0);
       __syncthreads();
@@ -175,19 +187,23 @@ __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
     }
   }
   // Lane (c, g) of a 16 x 16 fragment: column c, rows 4g .. 4g + 3.
+  float sx[FM][4];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sx[i][r] = __shfl(own_x, i * 16 + 4 * g + r, 64);
 #pragma unroll
   for (int j = 0; j < FN; ++j) {
+    const float sw = __shfl(own_w, j * 16 + c, 64), bias = __shfl(own_bias, j * 16 + c, 64);
     const int64_t n = n0 + wn * TN + j * 16 + c;
     if (n >= p.N) continue;
-    const float sw = p.sw[n];
-    const float bias = p.bias != nullptr ? slc::to_f32(static_cast<const T*>(p.bias)[n]) : 0.0f;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int64_t m = m0 + wm * TM + i * 16 + 4 * g + r;
         if (m >= p.M) continue;
-        static_cast<T*>(p.y)[m * p.y_rs + n] = slc::from_f32<T>(finish(acc[i][j][r], p.sx[m], sw, bias));
+        static_cast<T*>(p.y)[m * p.y_rs + n] = slc::from_f32<T>(finish(acc[i][j][r], sx[i][r], sw, bias));
       }
   }
 }
@@ -1040,10 +1056,11 @@ int launch(const Problem& p, hipStream_t stream) {
     }
     if (rc != kNoPath) return rc;
   }
-  // Other rows: 128 x 128 tiles from four rounds of them over the CUs, else 64 x 64, of which
-  // several share a CU (us, 64 x 64 | 128 x 128: 301 x 1003 x 1001 9.0 | 20, 4096 x 1003 x 1001
-  // 21.9 | 24.1, 500 x 9727 x 1001 25 | 30, 4096 x 9727 x 1001 150 | 119, 32768 x 897 x 3001
-  // 330 | 221).
+  // Other rows: 128 x 128 tiles from a round of them over the CUs on, where they are not half
+  // empty; else 64 x 64, of which several share a CU (us, 64 x 64 | 128 x 128: 301 x 1003 x 1001
+  // 7.7 | 14.2, 2000 x 1003 x 1001 11.4 | 16.0, 500 x 9727 x 1001 22.0 | 23.0, 5 x 151937 x 897 40
+  // | 44; 4096 x 1003 x 1001 20.0 | 17.9, 4096 x 9727 x 1001 138 | 91, 32768 x 897 x 3001 323 |
+  // 204).
   auto any = [&](auto kernel, int64_t tile) -> int {
     const int64_t n_tiles = (p.N + tile - 1) / tile, most = 65535 * tile;  // rows of one grid
     SLC_REQUIRE(n_tiles < (1 << 24), "slc_hip_linear_q8: %d features exceed one launch's grid", p.N);
@@ -1061,7 +1078,7 @@ int launch(const Problem& p, hipStream_t stream) {
     return SLC_OK;
   };
   const int64_t large = ((static_cast<int64_t>(p.M) + 127) / 128) * ((static_cast<int64_t>(p.N) + 127) / 128);
-  if (large >= 4 * slc_host::device_cu_count()) return any(tile_kernel<T, 128, 128>, 128);
+  if (p.M > 64 && p.N > 64 && large >= slc_host::device_cu_count()) return any(tile_kernel<T, 128, 128>, 128);
   return any(tile_kernel<T, 64, 64>, 64);
 }
 

@@ -382,7 +382,7 @@ def test_linear_is_the_same_on_every_path(gpu):
 # The row kernel, each tile (with 16-byte stores and without), unaligned rows.
 STRIDED = [(3, 200, 128), (30, 300, 144), (50, 96, 256), (200, 20000, 128), (500, 9728, 128), (1100, 9728, 128),
            (2300, 9728, 896), (2300, 9731, 896), (4000, 4096, 2048), (4000, 4090, 2048), (70, 130, 77),
-           (1100, 9731, 33)]
+           (1100, 9731, 33), (4100, 1030, 7)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -435,7 +435,7 @@ def test_linear_of_a_repeated_row(gpu):
 
 
 def test_more_unaligned_rows_than_one_grid(gpu):
-    # 65535 tiles of 128 rows, and five rows more.
+    # More than 65535 tiles of 128 rows.
     announce("8388485 rows")
     m = 65535 * 128 + 5
     codes = torch.ones(m, 3, dtype=torch.int8, device=gpu)
