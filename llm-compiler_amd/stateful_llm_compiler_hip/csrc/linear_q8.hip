@@ -854,11 +854,12 @@ int launch_stream(const Problem& p, hipStream_t stream) {
 }
 
 // ---- decode: few rows, the weight streamed once -----------------------------------
-// A workgroup owns `feat` consecutive features (up to 16 * TILES; MFMA rows past them
-// are masked off by the buffer range) and splits K over its waves; the waves' sums meet
+// A workgroup owns a block of rows and `feat` consecutive features (up to 16 * TILES; MFMA
+// rows past them are masked off by the buffer range) and splits K over its waves; the waves' sums meet
 // in LDS by integer adds, whose order does not matter.  Each wave keeps U k-steps of 64
 // codes in flight while it multiplies the U before.  Bound by the weight's bytes where
 // it is wide, by latency where it is narrow.
+constexpr int kRowBlock = 32;
 template <typename T, int MB, int TILES, int U>
 __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
   __shared__ int sums[TILES * MB * 256];
@@ -871,7 +872,9 @@ __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
   const int steps = (p.K + 63) / 64, per = (steps + waves - 1) / waves;
   const int begin = wave * per, end = begin + per < steps ? begin + per : steps;
 
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (p.M - 1) * p.x_rs + p.K);
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kRowBlock;
+  const int rows = p.M - m0 < kRowBlock ? static_cast<int>(p.M - m0) : kRowBlock;
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + m0 * p.x_rs, (rows - 1) * p.x_rs + p.K);
   const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + n0 * p.K, static_cast<int64_t>(cols) * p.K);
   int x_off[MB], w_off[TILES];
 #pragma unroll
@@ -923,7 +926,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
   float sx = 0.0f, sw = 0.0f;
   uint32_t bias = 0;
   auto scales = [&]() {
-    sx = p.sx[m];
+    sx = p.sx[m0 + m];
     sw = p.sw[n0 + n];
     if (p.bias != nullptr) {
       if constexpr (sizeof(T) == 4)
@@ -932,7 +935,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
         bias = static_cast<const uint16_t*>(p.bias)[n0 + n];
     }
   };
-  const bool mine = tid < TILES * MB * 256 && m < p.M && n < cols;
+  const bool mine = tid < TILES * MB * 256 && m < rows && n < cols;
   if (mine) scales();
   for (int e = tid; e < TILES * MB * 256; e += blockDim.x) sums[e] = 0;
   __syncthreads();
@@ -956,25 +959,26 @@ __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
   __syncthreads();
   for (int e = tid; e < TILES * MB * 256; e += blockDim.x) {
     if (e != tid) place(e, m, n);
-    if (m >= p.M || n >= cols) continue;
+    if (m >= rows || n >= cols) continue;
     if (e != tid) scales();
-    static_cast<T*>(p.y)[m * p.y_rs + n0 + n] =
+    static_cast<T*>(p.y)[(m0 + m) * p.y_rs + n0 + n] =
         slc::from_f32<T>(finish(sums[e], sx, sw, bias_value<T>(bias)));
   }
 }
 
-// About 256 workgroups of equal shares of the features, 32 at most; eight waves, fewer
+// About 256 workgroups, of equal shares of the features, 32 at most; eight waves, fewer
 // where K has fewer steps (16 waves: 1 x 896 x 896 3.9 us for 3.4, 8 x 896 x 4864 6.4 for
 // 5.5; four: 3.4 and 5.7).
 template <typename T>
 int launch_rows(const Problem& p, hipStream_t stream) {
-  if (p.M > 32 || 32 * p.x_rs >= kRangeLimit) return kNoPath;
-  const int64_t share = (static_cast<int64_t>(p.N) + 255) / 256;
+  if (kRowBlock * p.x_rs >= kRangeLimit) return kNoPath;
+  const int64_t blocks = (static_cast<int64_t>(p.M) + kRowBlock - 1) / kRowBlock;
+  const int64_t share = (p.N * blocks + 255) / 256;
   const int feat = static_cast<int>(share > 32 ? 32 : share);
   const int steps = (p.K + 63) / 64, waves = steps < 8 ? steps : 8;
   const int64_t groups = (static_cast<int64_t>(p.N) + feat - 1) / feat;
   if (groups * waves * 64 >= (int64_t{1} << 32)) return kNoPath;  // threads of one launch
-  const dim3 grid(static_cast<unsigned>(groups));
+  const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(blocks));
 #define SLC_ROWS(MB, TILES, U) \
   hipLaunchKernelGGL((rows_kernel<T, MB, TILES, U>), grid, dim3(waves * 64), 0, stream, p, feat)
   if (feat <= 16) {
@@ -995,7 +999,9 @@ int launch_rows(const Problem& p, hipStream_t stream) {
 // 4096 8.9 | 9.5; but 8 x 9728 x 896 5.6 | 5.0, 8 x 11008 x 4096 14.8 | 10.4), and up to 8
 // rows from 16384 features, where it reads the weight about as fast or faster (1 x 151936
 // x 896 24.4 | 26.6, 8 x 50257 x 896 11.1 | 12.4, 8 x 151936 x 896 29.2 | 28.2; 16 x 151936
-// x 896 32.8 | 28.5).
+// x 896 32.8 | 28.5).  More rows too where one round of its workgroups, 32 rows by up to 16
+// features, covers them (48 x 896 x 896 4.3 | 4.8, 48 x 896 x 4864 9.1 | 10.3, 128 x 896 x 4864
+// 10.0 | 10.6; not for few features, whose tiles are as many: 1000 x 128 x 4864 11.2 | 10.5).
 //
 // Else the tile whose rounds over the CUs cost least: a round takes fixed + per_k * k-tiles
 // us, measured with every CU busy (K 896 and 4096).  Rounds, not tiles: 8192 x 896 x 896
@@ -1005,6 +1011,8 @@ int launch_rows(const Problem& p, hipStream_t stream) {
 enum Kernel { kRows, k64x64, k128x64, k128x128, k256x128, k256x256 };
 inline Kernel choose(int64_t M, int64_t N, int64_t K) {
   if ((M <= 32 && N <= 8192) || (M <= 8 && N >= 16384)) return kRows;
+  const int64_t cus = slc_host::device_cu_count();
+  if (N > 128 && (M + kRowBlock - 1) / kRowBlock * ((N + 15) / 16) <= cus) return kRows;
   struct Cost {
     Kernel kernel;
     int bm, bn;
@@ -1015,7 +1023,7 @@ inline Kernel choose(int64_t M, int64_t N, int64_t K) {
                             {k128x128, 128, 128, 1.16, 0.51},
                             {k256x128, 256, 128, 2.25, 0.89},
                             {k256x256, 256, 256, 5.8, 1.48}};
-  const int64_t cus = slc_host::device_cu_count(), k_tiles = (K + kBK - 1) / kBK;
+  const int64_t k_tiles = (K + kBK - 1) / kBK;
   Kernel best = k64x64;
   double least = 0.0;
   for (const Cost& c : costs) {
