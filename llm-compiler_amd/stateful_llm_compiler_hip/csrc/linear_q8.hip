@@ -419,9 +419,10 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
         set_tile(load_id);
       }
     };
-#pragma unroll
+#pragma clang loop unroll(disable)
     for (int t = 0; t < S - 1; ++t) issue();
     const int64_t steps = static_cast<int64_t>((total - 1 - first) / step + 1) * ktiles;
+#pragma clang loop unroll(disable)
     for (int64_t q = 0; q < steps; ++q) {
       asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((S - 2) * kOps) : "memory");
       issue();
@@ -1003,11 +1004,13 @@ int launch_rows(const Problem& p, hipStream_t stream) {
 // features, covers them (48 x 896 x 896 4.3 | 4.8, 48 x 896 x 4864 9.1 | 10.3, 128 x 896 x 4864
 // 10.0 | 10.6; not for few features, whose tiles are as many: 1000 x 128 x 4864 11.2 | 10.5).
 //
-// Else the tile whose rounds over the CUs cost least: a round takes fixed + per_k * k-tiles
-// us, measured with every CU busy (K 896 and 4096).  Rounds, not tiles: 8192 x 896 x 896
-// 12.6 us as one round of 256 x 128, 13.1 as two of 128 x 128; 4096 x 9728 x 896 41.5 as
-// five rounds of 256 x 128, 51 as three of 256 x 256; 32768 x 896 x 4864 128 as two of 256 x
-// 256, 138 as four of 256 x 128; 65 x 896 x 896 4.9 as 64 x 64, 8.2 as 256 x 128.
+// Else the tile that costs least: a start, and rounds over the CUs of a fixed part and one per
+// k-tile (us; fitted to every tile's time at 123 shapes of 9 to 32768 rows, 896 to 151936
+// features and K 896 to 11008, where the choice is the fastest tile or within 5 %, 0.2 % off on
+// average).  Rounds, not tiles: 8192 x 896 x 896 12.3 us as one round of 256 x 128, 12.6 as two
+// of 128 x 128; 4096 x 9728 x 896 43.5 as five rounds of 256 x 128, 50 as three of 256 x 256;
+// 32768 x 896 x 4864 127 as two of 256 x 256, 138 as four of 256 x 128; 65 x 896 x 896 4.7 as 64
+// x 64, 8.2 as 256 x 128.
 enum Kernel { kRows, k64x64, k128x64, k128x128, k256x128, k256x256 };
 inline Kernel choose(int64_t M, int64_t N, int64_t K) {
   if ((M <= 32 && N <= 8192) || (M <= 8 && N >= 16384)) return kRows;
@@ -1016,19 +1019,20 @@ inline Kernel choose(int64_t M, int64_t N, int64_t K) {
   struct Cost {
     Kernel kernel;
     int bm, bn;
-    double fixed, per_k;
+    double start, fixed, per_k;
   };
-  constexpr Cost costs[] = {{k64x64, 64, 64, 0.46, 0.20},
-                            {k128x64, 128, 64, 0.53, 0.33},
-                            {k128x128, 128, 128, 1.16, 0.51},
-                            {k256x128, 256, 128, 2.25, 0.89},
-                            {k256x256, 256, 256, 5.8, 1.48}};
+  constexpr Cost costs[] = {{k64x64, 64, 64, 2.7, 0.74, 0.20},
+                            {k128x64, 128, 64, 2.4, 0.88, 0.31},
+                            {k128x128, 128, 128, 2.7, 0.69, 0.50},
+                            {k256x128, 256, 128, 4.5, 1.24, 0.74},
+                            {k256x256, 256, 256, 2.9, 4.9, 1.36}};
   const int64_t k_tiles = (K + kBK - 1) / kBK;
   Kernel best = k64x64;
   double least = 0.0;
   for (const Cost& c : costs) {
     const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
-    const double cost = static_cast<double>((tiles + cus - 1) / cus) * (c.fixed + c.per_k * static_cast<double>(k_tiles));
+    const double rounds = static_cast<double>((tiles + cus - 1) / cus);
+    const double cost = c.start + rounds * (c.fixed + c.per_k * static_cast<double>(k_tiles));
     if (c.kernel == k64x64 || cost < least) {
       best = c.kernel;
       least = cost;
@@ -1048,13 +1052,13 @@ int launch(const Problem& p, hipStream_t stream) {
         rc = launch_rows<T>(p, stream);
         break;
       case k64x64:
-        rc = launch_stream<T, 64, 64, 2, 2, 2, 6, 8>(p, stream);
+        rc = launch_stream<T, 64, 64, 2, 2, 4, 5, 8>(p, stream);
         break;
       case k128x64:
-        rc = launch_stream<T, 128, 64, 2, 2, 2, 4, 8>(p, stream);
+        rc = launch_stream<T, 128, 64, 2, 2, 4, 4, 8>(p, stream);
         break;
       case k128x128:
-        rc = launch_stream<T, 128, 128, 2, 4, 2, 4, 8>(p, stream);
+        rc = launch_stream<T, 128, 128, 2, 4, 4, 3, 8>(p, stream);
         break;
       case k256x128:
         rc = launch_stream<T, 256, 128, 4, 2, 4, 3, 4>(p, stream);
