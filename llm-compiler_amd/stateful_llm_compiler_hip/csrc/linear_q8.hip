@@ -967,14 +967,14 @@ __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
   }
 }
 
-// About 256 workgroups, of equal shares of the features, 32 at most; eight waves, fewer
+// About a workgroup per CU, of equal shares of the features, 32 at most; eight waves, fewer
 // where K has fewer steps (16 waves: 1 x 896 x 896 3.9 us for 3.4, 8 x 896 x 4864 6.4 for
 // 5.5; four: 3.4 and 5.7).
 template <typename T>
 int launch_rows(const Problem& p, hipStream_t stream) {
   if (kRowBlock * p.x_rs >= kRangeLimit) return kNoPath;
   const int64_t blocks = (static_cast<int64_t>(p.M) + kRowBlock - 1) / kRowBlock;
-  const int64_t share = (p.N * blocks + 255) / 256;
+  const int64_t cus = slc_host::device_cu_count(), share = (p.N * blocks + cus - 1) / cus;
   const int feat = static_cast<int>(share > 32 ? 32 : share);
   const int steps = (p.K + 63) / 64, waves = steps < 8 ? steps : 8;
   const int64_t groups = (static_cast<int64_t>(p.N) + feat - 1) / feat;
@@ -986,8 +986,7 @@ int launch_rows(const Problem& p, hipStream_t stream) {
     if (p.M <= 16) SLC_ROWS(1, 1, 4);
     else SLC_ROWS(2, 1, 2);
   } else {
-    if (p.M <= 16) SLC_ROWS(1, 2, 2);
-    else SLC_ROWS(2, 2, 2);
+    SLC_ROWS(1, 2, 2);  // a vocabulary: choose() sends 4 rows at most here
   }
 #undef SLC_ROWS
   return slc_host::check_launch("slc_hip_linear_q8(rows)");
@@ -995,14 +994,15 @@ int launch_rows(const Problem& p, hipStream_t stream) {
 
 // Which kernel takes a shape of aligned rows, all giving the same bits.
 //
-// Up to 32 rows and 8192 features, rows_kernel: a tile would leave most CUs idle (us,
-// rows | 64 x 64 tiles: 8 x 1152 x 896 3.6 | 4.7, 32 x 896 x 4864 8.4 | 10.3, 32 x 4096 x
-// 4096 8.9 | 9.5; but 8 x 9728 x 896 5.6 | 5.0, 8 x 11008 x 4096 14.8 | 10.4), and up to 8
-// rows from 16384 features, where it reads the weight about as fast or faster (1 x 151936
-// x 896 24.4 | 26.6, 8 x 50257 x 896 11.1 | 12.4, 8 x 151936 x 896 29.2 | 28.2; 16 x 151936
-// x 896 32.8 | 28.5).  More rows too where one round of its workgroups, 32 rows by up to 16
-// features, covers them (48 x 896 x 896 4.3 | 4.8, 48 x 896 x 4864 9.1 | 10.3, 128 x 896 x 4864
-// 10.0 | 10.6; not for few features, whose tiles are as many: 1000 x 128 x 4864 11.2 | 10.5).
+// rows_kernel where 16 x 16 fragments of the outputs are no more than CUs: tiles would leave
+// most CUs idle (us, rows | 64 x 64 tiles: 8 x 1152 x 896 3.7 | 4.4, 16 x 896 x 4864 6.3 | 9.1,
+// 16 x 4096 x 4096 7.0 | 8.4, 48 x 896 x 896 4.3 | 4.5, 250 x 256 x 4864 9.5 | 9.8; past that 16 x
+// 6000 x 2048 6.4 | 6.1, 32 x 4096 x 4096 9.4 | 8.5), but for many rows of few features, whose
+// tiles are as many (1900 x 32 x 896 5.0 | 4.4).  And for up to 4 rows of a vocabulary, whose
+// weight it reads a little faster (1 x 50257 x 896 10.8 | 11.8, 1 x 151936 x 896 25.3 | 26.3; 2 x
+// 32768 x 896 7.8 | 7.2, 8 x 151936 x 896 29.4 | 27.4).  Else up to 32 rows 64 x 64 tiles, which
+// the others' empty rows make no faster (64 x 64 | 128 x 128: 8 x 151936 x 896 27.4 | 28.7, 16 x
+// 151936 x 896 28.3 | 28.9).
 //
 // Else the tile that costs least: a start, and rounds over the CUs of a fixed part and one per
 // k-tile (us; fitted to every tile's time at 123 shapes of 9 to 32768 rows, 896 to 151936
@@ -1013,9 +1013,9 @@ int launch_rows(const Problem& p, hipStream_t stream) {
 // x 64, 8.2 as 256 x 128.
 enum Kernel { kRows, k64x64, k128x64, k128x128, k256x128, k256x256 };
 inline Kernel choose(int64_t M, int64_t N, int64_t K) {
-  if ((M <= 32 && N <= 8192) || (M <= 8 && N >= 16384)) return kRows;
   const int64_t cus = slc_host::device_cu_count();
-  if (N > 128 && (M + kRowBlock - 1) / kRowBlock * ((N + 15) / 16) <= cus) return kRows;
+  if ((M + 15) / 16 * ((N + 15) / 16) <= cus && (M <= 32 || N >= 128)) return kRows;
+  if (M <= 32) return M <= 4 && N >= 50000 ? kRows : k64x64;
   struct Cost {
     Kernel kernel;
     int bm, bn;

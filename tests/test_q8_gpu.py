@@ -380,9 +380,10 @@ def test_linear_is_the_same_on_every_path(gpu):
 
 
 # The row kernel, each tile (with 16-byte stores and without), unaligned rows.
-STRIDED = [(3, 200, 128), (30, 300, 144), (50, 96, 256), (50, 200, 256), (125, 1000, 272), (200, 20000, 128),
-           (500, 9728, 128), (1100, 9728, 128), (2300, 9728, 896), (2300, 9731, 896), (4000, 4096, 2048),
-           (4000, 4090, 2048), (120, 9000, 272), (120, 9001, 272), (70, 130, 77), (1100, 9731, 33), (4100, 1030, 7)]
+STRIDED = [(3, 200, 128), (30, 300, 144), (50, 96, 256), (50, 200, 256), (120, 500, 272), (3, 50001, 128),
+           (200, 20000, 128), (500, 9728, 128), (1100, 9728, 128), (2300, 9728, 896), (2300, 9731, 896),
+           (4000, 4096, 2048), (4000, 4090, 2048), (120, 9000, 272), (120, 9001, 272), (70, 130, 77),
+           (1100, 9731, 33), (4100, 1030, 7)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
