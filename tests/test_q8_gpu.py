@@ -227,6 +227,20 @@ def test_layouts(gpu, dtype):
     assert torch.equal(codes.cpu().double(), q8(summed.cpu().double())[0])
 
 
+def test_halves_of_a_padded_batch(gpu):
+    # Gate and up as views of one projection [batch, tokens, 2 I]; the second sequence ends early.
+    announce("halves of a batch")
+    base = rows_of(3 * 5, 2 * 56, torch.bfloat16, 31).view(3, 5, 112)
+    base[1, 3:] = 0.0
+    gate, up = base.to(gpu).chunk(2, dim=-1)
+    codes, scales = backends.hip_swiglu_q8(gate, up)
+    check_rows(codes, scales, swiglu_exact(*base.chunk(2, dim=-1)))
+    assert not scales[1, 3:].any() and not codes[1, 3:].any()
+    # The first two sequences of it, and every second token: no view of evenly strided rows.
+    for part in ((slice(0, 2),), (slice(None), slice(0, 5, 2))):
+        check_rows(*backends.hip_swiglu_q8(gate[part], up[part]), swiglu_exact(*base[part].chunk(2, dim=-1)))
+
+
 def test_empty_calls(gpu):
     announce("empty")
     x = torch.zeros(0, 3, 16, device=gpu)
