@@ -22,6 +22,8 @@
 // thousand rows, bound by the launch and two dependent reductions below.  Rows
 // past 16 waves' registers are read twice (LOOP).  All loads are issued before
 // the first use, without branches: buffer loads whose range ends with the row.
+// 16384 x 896 fp16 9.5 us (4.6 TB/s), SwiGLU 4096 x 4864 bf16 23.6 (4.2 TB/s, with 14 us of
+// vector instructions), addition and norm of 4096 x 896 bf16 7.9, of one row 2.7.
 #include <float.h>
 
 #include <initializer_list>
