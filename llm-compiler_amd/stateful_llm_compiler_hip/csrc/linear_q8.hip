@@ -31,9 +31,14 @@ __device__ __forceinline__ i32x4_t mfma(i32x4_t a, i32x4_t b, i32x4_t c) {
 }
 
 // float(sum) * sx * sw + bias; the last two in one fma (and one rounding) in
-// every kernel, so that all give the same bits.
+// every kernel, so that all give the same bits.  The result is an fp32 value before
+// it is rounded to T: the compiler would else round fp16 outputs from the unrounded
+// fma, where it sees both.
+template <typename T>
 __device__ __forceinline__ float finish(int sum, float sx, float sw, float bias) {
-  return fmaf(static_cast<float>(sum) * sx, sw, bias);
+  float y = fmaf(static_cast<float>(sum) * sx, sw, bias);
+  if constexpr (std::is_same<T, slc::f16_t>::value) asm("" : "+v"(y));
+  return y;
 }
 
 struct Problem {
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(256) void tile_kernel(Problem p) {
       for (int r = 0; r < 4; ++r) {
         const int64_t m = m0 + wm * TM + i * 16 + 4 * g + r;
         if (m >= p.M) continue;
-        static_cast<T*>(p.y)[m * p.y_rs + n] = slc::from_f32<T>(finish(acc[i][j][r], sx[i][r], sw, bias));
+        static_cast<T*>(p.y)[m * p.y_rs + n] = slc::from_f32<T>(finish<T>(acc[i][j][r], sx[i][r], sw, bias));
       }
   }
 }
@@ -520,7 +525,7 @@ __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = 2 * q + (e >> 2), r = e & 3;
-          v[e] = finish(acc[j][i][r], sx[i], sw[j][r], bias[j].value(r));
+          v[e] = finish<T>(acc[j][i][r], sx[i], sw[j][r], bias[j].value(r));
         }
         store_run<T, VST>(ry, v, whole + i * rows16, half + i * rows16, m < rows ? cols - n : 0);
       }
@@ -800,7 +805,7 @@ __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, i
         const int m = wm * TM + i * 16 + c;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = finish(acc[2 * q + (e >> 2)][i][e & 3], sx[i], sw[e], bs[e]);
+        for (int e = 0; e < 8; ++e) v[e] = finish<T>(acc[2 * q + (e >> 2)][i][e & 3], sx[i], sw[e], bs[e]);
         store_run<T, VST>(ry, v, whole + i * rows16, half + i * rows16, m < rows ? cols - n : 0);
       }
     }
@@ -971,7 +976,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
     if (m >= rows || n >= cols) continue;
     if (e != tid) scales();
     static_cast<T*>(p.y)[(m0 + m) * p.y_rs + n0 + n] =
-        slc::from_f32<T>(finish(sums[e], sx, sw, bias_value<T>(bias)));
+        slc::from_f32<T>(finish<T>(sums[e], sx, sw, bias_value<T>(bias)));
   }
 }
 

@@ -418,6 +418,19 @@ def test_linear_writes_its_outputs_only(gpu, dtype, m, n, k):
     assert (out[m:] == 7).all() and (out[:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", STRIDED)
+def test_linear_rounds_where_it_says(gpu, dtype, m, n, k):
+    # Without a bias the bits follow: the sum is exact, float(sum) and its product with the
+    # token's scale are fp32 roundings, the product with the channel's scale is exact in fp64
+    # (24 x 24 bits), and then come one rounding to fp32 and one to the output's type.
+    announce(f"roundings {m} x {n} x {k} {dtype}")
+    codes, scales, weight, weight_scales, _ = (t.to(gpu) if t is not None else None for t in operands(m, n, k, None, 3))
+    sums = codes.double() @ weight.double().t()
+    want = ((sums.float() * scales.unsqueeze(-1)).double() * weight_scales.double()).float().to(dtype)
+    assert_bitwise_equal(backends.hip_linear_q8(codes, scales, weight, weight_scales, output_dtype=dtype), want)
+
+
 @pytest.mark.parametrize("n", [40, 9728, 20000])
 def test_linear_of_one_row_takes_any_strides(gpu, n):
     announce(f"one row {n}")
