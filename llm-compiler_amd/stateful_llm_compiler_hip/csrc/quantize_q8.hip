@@ -23,7 +23,8 @@
 // past 16 waves' registers are read twice (LOOP).  All loads are issued before
 // the first use, without branches: buffer loads whose range ends with the row.
 // 16384 x 896 fp16 9.5 us (4.6 TB/s), SwiGLU 4096 x 4864 bf16 23.6 (4.2 TB/s, with 14 us of
-// vector instructions), addition and norm of 4096 x 896 bf16 7.9, of one row 2.7.
+// vector instructions), norm of 9001 x 1001 fp32 11.8 (3.8 TB/s), addition and norm of 4096
+// x 896 bf16 7.9, of one row 2.7.
 #include <float.h>
 
 #include <initializer_list>
@@ -65,8 +66,12 @@ struct Traits {
   static constexpr int VEC = 16 / sizeof(T);
   static constexpr bool kHasB = SRC == kAddNorm || SRC == kSwiglu;
   static constexpr bool kHasW = SRC == kNorm || SRC == kAddNorm;
-  // Whether the fp32 v may differ from y (then a is taken again in fp64).
-  static constexpr bool kInexact = SRC == kSwiglu || (kHasW && sizeof(T) == 4);
+  // Whether the fp32 v may differ from y.  Then a is taken in fp64: of products of two fp32
+  // values, exact there, beside v (norm 9001 x 1001 10.9 us; in a second pass over the values
+  // near the largest, behind a second barrier, 13.1); of SwiGLU, whose fp64 values cost too
+  // much for that, in such a second pass.
+  static constexpr bool kWide = kHasW && sizeof(T) == 4;
+  static constexpr bool kInexact = SRC == kSwiglu || kWide;
   static constexpr float kApart = (SRC == kSwiglu ? 14 : kInexact ? 6 : 4) * 0x1p-24f;
   // v within this factor below the largest v may be the largest y.
   static constexpr float kNear = 1.0f - 0x1p-19f;
@@ -258,6 +263,7 @@ __device__ __forceinline__ double wave_reduce64(double v, OP op) {
 
 struct Shared {
   double sum[kMaxWaves];
+  double most64[kMaxWaves];
   double max64[kMaxWaves];
   double sum64[kMaxWaves];
   uint32_t max32[kMaxWaves];
@@ -324,7 +330,7 @@ __global__ __launch_bounds__(max_waves(NV) * 64) void quantize_kernel(Args p) {
   // signed order, the largest negative by unsigned order.
   int most = 0;
   uint32_t least = 0, most_up = 0;
-  double sq = 0.0;
+  double sq = 0.0, most64 = 0.0;
   auto gather = [&](int i, int slot) {
     evaluate(slot);
     float squares = 0.0f;
@@ -336,6 +342,7 @@ __global__ __launch_bounds__(max_waves(NV) * 64) void quantize_kernel(Args p) {
       if constexpr (TR::kHasW) {
         const float h = elem<T>(a[slot], k);
         squares = fmaf(h, h, squares);
+        if constexpr (TR::kWide) most64 = fmax(most64, fabs(static_cast<double>(h) * elem<T>(w[slot], k)));
       }
     }
     if constexpr (TR::kHasW) sq += squares;
@@ -375,17 +382,21 @@ __global__ __launch_bounds__(max_waves(NV) * 64) void quantize_kernel(Args p) {
   top = wave_max_u32(top);
   if constexpr (SRC == kSwiglu) most_up = wave_max_u32(up_bits<T>(most_up));
   auto add = [](double x, double y) { return x + y; };
+  auto larger = [](double x, double y) { return x > y ? x : y; };
   if constexpr (TR::kHasW) sq = wave_reduce64(sq, add);
+  if constexpr (TR::kWide) most64 = wave_reduce64(most64, larger);
   if (waves > 1) {
     if ((t & 63) == 0) {
       shared.max32[wave] = top;
       if constexpr (SRC == kSwiglu) shared.max_up[wave] = most_up;
       if constexpr (TR::kHasW) shared.sum[wave] = sq;
+      if constexpr (TR::kWide) shared.most64[wave] = most64;
     }
     __syncthreads();
     for (int i = 0; i < waves; ++i) {
       top = max(top, shared.max32[i]);
       if constexpr (SRC == kSwiglu) most_up = max(most_up, shared.max_up[i]);
+      if constexpr (TR::kWide) most64 = larger(most64, shared.most64[i]);
     }
   }
   // Every wave of the row holds the same top from here on.
@@ -393,9 +404,9 @@ __global__ __launch_bounds__(max_waves(NV) * 64) void quantize_kernel(Args p) {
   bool fast = vmax >= kLow && vmax <= kHigh;
   if constexpr (SRC == kSwiglu) fast = fast && __uint_as_float(most_up) <= kMostUp;
 
-  // ---- a in fp64: of the values near the largest, or of all that are not zero -----
-  double a64 = vmax, sq64 = 0.0;
-  if (TR::kInexact || !fast) {
+  // ---- a in fp64: of SwiGLU's values near the largest, or of all that are not zero -----
+  double a64 = TR::kWide ? most64 : vmax, sq64 = 0.0;
+  if (SRC == kSwiglu || !fast) {
     a64 = 0.0;
     const float near = vmax * TR::kNear;
     auto pick = [&](int i, int slot) {
@@ -433,7 +444,7 @@ __global__ __launch_bounds__(max_waves(NV) * 64) void quantize_kernel(Args p) {
         for (int i = 0; i < NV; ++i) pick(i, i);
       }
     }
-    a64 = wave_reduce64(a64, [](double x, double y) { return x > y ? x : y; });
+    a64 = wave_reduce64(a64, larger);
     if constexpr (TR::kHasW) sq64 = wave_reduce64(sq64, add);
     if (waves > 1) {
       if ((t & 63) == 0) {
