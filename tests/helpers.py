@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+import re
 import sys
 
 import torch
@@ -96,3 +98,39 @@ def attention_in_chains(query, key, value, bias, scale):
 
 def relative_error(actual: torch.Tensor, exact: torch.Tensor) -> float:
     return float((actual.double().cpu() - exact).norm() / exact.norm())
+
+
+class _Dim3(ctypes.Structure):
+    _fields_ = [(axis, ctypes.c_uint32) for axis in "xyz"]
+
+
+class _KernelNodeParams(ctypes.Structure):  # hipKernelNodeParams
+    _fields_ = [("block", _Dim3), ("extra", ctypes.c_void_p), ("function", ctypes.c_void_p), ("grid", _Dim3),
+                ("arguments", ctypes.c_void_p), ("shared_bytes", ctypes.c_uint)]
+
+
+def captured_kernels(call) -> list[tuple[str, tuple[int, ...], int]]:
+    """The kernels that ``call`` launches, read from a graph that captures it and is
+    never run: (name, its whole-number and truth-value template arguments,
+    workgroups) of each ``*_kernel``."""
+
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    with open("/proc/self/maps") as maps:
+        hip = ctypes.CDLL(next(line.split()[-1] for line in maps if "libamdhip64" in line))
+    hip.hipKernelNameRefByPtr.restype = ctypes.c_char_p
+    raw, count = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(0)
+    assert hip.hipGraphGetNodes(raw, None, ctypes.byref(count)) == 0
+    nodes = (ctypes.c_void_p * count.value)()
+    assert hip.hipGraphGetNodes(raw, nodes, ctypes.byref(count)) == 0
+    found = []
+    for node in nodes:
+        params = _KernelNodeParams()
+        assert hip.hipGraphKernelNodeGetParams(ctypes.c_void_p(node), ctypes.byref(params)) == 0
+        name = hip.hipKernelNameRefByPtr(ctypes.c_void_p(params.function), None).decode()
+        match = re.search(r"\d([a-z_]+)_kernelI(?:N3slc\d\w+?_tE|f)((?:L[ib]\d+E)*)E", name)
+        assert match, name
+        values = tuple(int(value) for value in re.findall(r"L[ib](\d+)E", match[2]))
+        found.append((match[1], values, params.grid.x * params.grid.y))
+    return found

@@ -11,7 +11,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from helpers import announce, assert_bitwise_equal, generator
+from helpers import announce, assert_bitwise_equal, captured_kernels, generator
 from stateful_llm_compiler_hip import _native, backends
 
 pytestmark = pytest.mark.gpu
@@ -665,3 +665,47 @@ def test_two_streams_at_once(gpu):
         for result in got[i]:
             for a, b in zip(result, wants[i]):
                 assert_bitwise_equal(a, b)
+
+
+# ---- every kernel, and past a workgroup's first tile ---------------------------------
+# Which kernel takes a shape is a matter of speed and may change; these tests name the
+# kernel that they mean, so that one which no longer runs it fails and its shape is moved.
+
+
+# Vectors a lane (0: rows read twice) of many rows, few values past them in a row or none,
+# the last row's end inside a vector.  SwiGLU of 2100 x 4864 is a prefill's.
+ROW_VARIANTS = [
+    (torch.bfloat16, 2100, 896, 2), (torch.bfloat16, 2100, 4864, 3), (torch.bfloat16, 2101, 4865, 3),
+    (torch.bfloat16, 1100, 2063, 3), (torch.bfloat16, 300, 8192, 4), (torch.bfloat16, 701, 16390, 4),
+    (torch.bfloat16, 300, 33001, 0), (torch.float16, 2101, 4864, 3), (torch.float16, 2100, 4867, 3),
+    (torch.float16, 700, 16391, 4), (torch.float32, 1100, 896, 4), (torch.float32, 2101, 896, 2),
+    (torch.float32, 2100, 4864, 3), (torch.float32, 2101, 4865, 3), (torch.float32, 701, 9001, 4),
+    (torch.float32, 300, 16390, 0),
+]
+
+
+@pytest.mark.parametrize("source", ["plain", "norm", "add norm", "swiglu"])
+@pytest.mark.parametrize("dtype,rows,k,vectors", ROW_VARIANTS)
+def test_row_kernels_of_many_rows(gpu, dtype, rows, k, vectors, source):
+    announce(f"{source} {rows} x {k} {dtype}")
+    x, other = rows_of(rows, 2 * k, dtype, k, 2.0), rows_of(rows, k, dtype, k + 1, 3.0)
+    w = (torch.randn(k, generator=generator(k + 2)) * 0.5 + 1).to(dtype)
+    both, other_gpu, w_gpu = x.to(gpu), other.to(gpu), w.to(gpu)
+    left, right = both[:, :k], both[:, k:]  # rows 2k apart
+    x, y = x[:, :k], x[:, k:]
+    call = {"plain": lambda: backends.hip_quantize_q8(left),
+            "norm": lambda: backends.hip_rms_norm_q8(left, w_gpu, epsilon=1e-6),
+            "add norm": lambda: backends.hip_add_rms_norm_q8(left, other_gpu, w_gpu, epsilon=1e-6),
+            "swiglu": lambda: backends.hip_swiglu_q8(left, right)}[source]
+    *summed, codes, scales = call()
+    if source in ("plain", "swiglu"):
+        check_rows(codes, scales, x.double() if source == "plain" else swiglu_exact(x, y))
+    else:
+        if summed:
+            x = (x.float() + other.float()).to(dtype)
+            assert_bitwise_equal(summed[0], x)
+        h = x.double()
+        eps32 = float(torch.tensor(1e-6, dtype=torch.float32))
+        check_rows(codes, scales, h * w.double(), torch.rsqrt(h.square().mean(-1, keepdim=True) + eps32), NORM)
+    (name, (_, nv, loop), _), = captured_kernels(call)
+    assert (name, 0 if loop else nv) == ("quantize", vectors)
