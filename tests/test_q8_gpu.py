@@ -709,3 +709,57 @@ def test_row_kernels_of_many_rows(gpu, dtype, rows, k, vectors, source):
         check_rows(codes, scales, h * w.double(), torch.rsqrt(h.square().mean(-1, keepdim=True) + eps32), NORM)
     (name, (_, nv, loop), _), = captured_kernels(call)
     assert (name, 0 if loop else nv) == ("quantize", vectors)
+
+
+# Kernel, tile (or row blocks, feature blocks and depth), 16-byte stores or not.  The rings and
+# the turns walk several output tiles a workgroup, of sizes that the tile divides and others;
+# the 256 x 256 ones two each, and two or three.
+LINEAR_VARIANTS = [
+    (8, 1152, 896, "rows", (1, 1, 4)), (30, 300, 144, "rows", (2, 1, 2)), (3, 50001, 128, "rows", (1, 2, 2)),
+    (20, 20000, 272, "stream", (64, 64, 1)), (20, 20001, 272, "stream", (64, 64, 0)),
+    (37692, 24, 2960, "stream", (128, 64, 1)), (34001, 23, 512, "stream", (128, 64, 0)),
+    (200, 20000, 128, "stream", (128, 128, 1)), (200, 20001, 128, "stream", (128, 128, 0)),
+    (500, 9731, 128, "stream", (128, 128, 0)), (2300, 9728, 896, "stream", (256, 128, 1)),
+    (2300, 9731, 896, "stream", (256, 128, 0)), (8192, 4096, 2048, "turns", (1,)), (8000, 4090, 2048, "turns", (0,)),
+    (8192, 5632, 4096, "turns", (1,)), (8100, 5626, 4096, "turns", (0,)), (300, 1003, 1001, "tile", (64, 64)),
+    (2200, 2051, 1001, "tile", (128, 128)), (4100, 1030, 263, "tile", (128, 128)),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,kernel,variant", LINEAR_VARIANTS)
+def test_linear_kernels_past_their_first_tile(gpu, dtype, m, n, k, kernel, variant):
+    announce(f"{kernel} {variant} {m} x {n} x {k} {dtype}")
+    g = torch.Generator(device=gpu).manual_seed(m + n + k)
+    # Rows of codes are 48 bytes, those of outputs 24 elements longer than their contents.
+    padded = torch.randint(-128, 128, (m, k + 48), generator=g, device=gpu, dtype=torch.int8)
+    codes = padded[:, :k].contiguous()
+    weight = torch.randint(-128, 128, (n, k), generator=g, device=gpu, dtype=torch.int8)
+    scales, weight_scales = torch.rand(m, generator=g, device=gpu) * 0.02, torch.rand(n, generator=g, device=gpu) * 0.01
+    bias = torch.randn(n, generator=g, device=gpu).to(dtype)
+    (name, values, workgroups), = captured_kernels(
+        lambda: backends.hip_linear_q8(codes, scales, weight, weight_scales, output_dtype=dtype))
+    shown = values[:2] + values[-1:] if name == "stream" else values
+    assert (name, shown) == (kernel, variant)
+    if name in ("stream", "turns"):
+        height, width = values[:2] if name == "stream" else (256, 256)
+        assert -(-m // height) * -(-n // width) > workgroups
+
+    # As in test_linear_rounds_where_it_says.
+    sums = codes.double() @ weight.double().t()
+    product = (sums.float() * scales.unsqueeze(-1)).double() * weight_scales.double()
+    del sums
+    y = backends.hip_linear_q8(codes, scales, weight, weight_scales, output_dtype=dtype)
+    assert torch.equal(y, product.float().to(dtype))  # no NaN, and -0 == 0
+
+    # With a bias: one rounding of the sum to fp32 and one to the output's type.
+    lib, tag = _native.library(), _native.dtype_tag(dtype)
+    out = torch.full((m + 3, n + 24), 7.0, dtype=dtype, device=gpu)
+    _native.check(lib.slc_hip_linear_q8(
+        padded.data_ptr(), scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), bias.data_ptr(),
+        out.data_ptr(), tag, m, n, k, k + 48, n + 24, _native.current_stream(gpu)), "slc_hip_linear_q8")
+    want = product.add_(bias.double())
+    info = torch.finfo(dtype)
+    bound = want.abs() * ((HALF32 + info.eps / 2) * 1.001) + info.tiny * info.eps / 2
+    assert ((out[:m, :n].double() - want).abs() <= bound).all()
+    assert (out[m:] == 7).all() and (out[:, n:] == 7).all()
