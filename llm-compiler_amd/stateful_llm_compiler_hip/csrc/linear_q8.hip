@@ -1091,18 +1091,24 @@ int launch(const Problem& p, hipStream_t stream) {
   // | 44; 4096 x 1003 x 1001 20.0 | 17.9, 4096 x 9727 x 1001 138 | 91, 32768 x 897 x 3001 323 |
   // 204).
   auto any = [&](auto kernel, int64_t tile) -> int {
-    const int64_t n_tiles = (p.N + tile - 1) / tile, most = 65535 * tile;  // rows of one grid
-    SLC_REQUIRE(n_tiles < (1 << 24), "slc_hip_linear_q8: %d features exceed one launch's grid", p.N);
+    // One grid holds 65535 tiles of rows, and fewer than 2^32 threads across the features.
+    const int64_t most_m = 65535 * tile, most_n = ((1 << 24) - 1) * tile;
     Problem part = p;
-    for (int64_t done = 0; done < p.M; done += most) {
-      part.x = p.x + done * p.x_rs;
-      part.sx = p.sx + done;
-      part.y = static_cast<T*>(p.y) + done * p.y_rs;
-      part.M = static_cast<int>(p.M - done < most ? p.M - done : most);
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_tiles), static_cast<unsigned>((part.M + tile - 1) / tile)),
-                         dim3(256), 0, stream, part);
-      const int rc = slc_host::check_launch("slc_hip_linear_q8(any)");
-      if (rc != SLC_OK) return rc;
+    for (int64_t n0 = 0; n0 < p.N; n0 += most_n) {
+      part.w = p.w + n0 * p.K;
+      part.sw = p.sw + n0;
+      part.bias = p.bias == nullptr ? nullptr : static_cast<const T*>(p.bias) + n0;
+      part.N = static_cast<int>(p.N - n0 < most_n ? p.N - n0 : most_n);
+      for (int64_t m0 = 0; m0 < p.M; m0 += most_m) {
+        part.x = p.x + m0 * p.x_rs;
+        part.sx = p.sx + m0;
+        part.y = static_cast<T*>(p.y) + m0 * p.y_rs + n0;
+        part.M = static_cast<int>(p.M - m0 < most_m ? p.M - m0 : most_m);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((part.N + tile - 1) / tile), static_cast<unsigned>((part.M + tile - 1) / tile)),
+                           dim3(256), 0, stream, part);
+        const int rc = slc_host::check_launch("slc_hip_linear_q8(any)");
+        if (rc != SLC_OK) return rc;
+      }
     }
     return SLC_OK;
   };

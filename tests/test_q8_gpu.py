@@ -763,3 +763,22 @@ def test_linear_kernels_past_their_first_tile(gpu, dtype, m, n, k, kernel, varia
     bound = want.abs() * ((HALF32 + info.eps / 2) * 1.001) + info.tiny * info.eps / 2
     assert ((out[:m, :n].double() - want).abs() <= bound).all()
     assert (out[m:] == 7).all() and (out[:, n:] == 7).all()
+
+
+def test_more_unaligned_features_than_one_grid(gpu):
+    # More than 2^24 - 1 tiles of 64 features.
+    n = (2**24 - 1) * 64 + 70
+    announce(f"{n} features of one code")
+    weight = torch.empty(n, 1, dtype=torch.int8, device=gpu).random_(-128, 128)
+    weight_scales = torch.full((n,), 0.5, device=gpu)
+    bias = torch.zeros(n, dtype=torch.float16, device=gpu)
+    bias[-70:] = 3.0
+    codes = torch.tensor([[7], [-3]], dtype=torch.int8, device=gpu)
+    scales = torch.tensor([1.0, 0.25], device=gpu)
+    call = lambda: backends.hip_linear_q8(codes, scales, weight, weight_scales, bias, output_dtype=torch.float16)  # noqa: E731
+    assert [(name, groups) for name, _, groups in captured_kernels(call)] == [("tile", 2**24 - 1), ("tile", 2)]
+    y = call()
+    for row, factor in enumerate((3.5, -0.375)):  # exact in fp16: 8 bits of a code times 3
+        for at in range(0, n, 2**28):
+            part = slice(at, min(n, at + 2**28))
+            assert torch.equal(y[row, part].float(), weight[part, 0] * factor + bias[part])
