@@ -20,9 +20,10 @@ DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 HALF32 = 2.0**-24
 
 
-# Squares are summed in fp32 in chains of at most eight, each step off by at most
-# half a step of a growing sum: 8 * 2^-24 of the mean, half of that of its root;
-# one more for the scale's own rounding.
+# What squares summed in fp32, in chains of at most eight, would need: each step off by
+# at most half a step of a growing sum, 8 * 2^-24 of the mean, half of that of its root;
+# one more for the scale's own rounding.  test_norm_scales_are_rounded_once asks for the
+# last alone.
 NORM = 5
 
 
@@ -782,3 +783,35 @@ def test_more_unaligned_features_than_one_grid(gpu):
         for at in range(0, n, 2**28):
             part = slice(at, min(n, at + 2**28))
             assert torch.equal(y[row, part].float(), weight[part, 0] * factor + bias[part])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("k", [896, 1001, 4864, 16390, 33001])
+def test_norm_scales_are_rounded_once(gpu, dtype, residual, k):
+    # Squares of 2^-24 beside those of 1: sums in 24 bits lose every one that follows a 1.
+    announce(f"norm scales {dtype} {residual} {k}")
+    x = torch.full((96, k), 2.0**-12)
+    x[:, :: 16 // dtype.itemsize] = 1.0
+    x[:32] *= torch.ldexp(torch.tensor(1.0), -torch.arange(32) // 4).unsqueeze(-1)
+    x[64:] = rows_of(32, k, torch.float32, k)
+    x = x.to(dtype)
+    # Every row has largest products of its own, and so a scale of its own.
+    x[torch.arange(96), torch.arange(96) * 7 % k] *= torch.linspace(1.5, 9.5, 96).to(dtype)
+    w = (torch.randn(k, generator=generator(k)) * 0.5 + 1).to(dtype)
+    if residual:
+        _, codes, scales = backends.hip_add_rms_norm_q8(x.to(gpu), torch.zeros_like(x, device=gpu), w.to(gpu),
+                                                        epsilon=1e-6)
+    else:
+        codes, scales = backends.hip_rms_norm_q8(x.to(gpu), w.to(gpu), epsilon=1e-6)
+    h = x.double()
+    eps32 = float(torch.tensor(1e-6, dtype=torch.float32))
+    want_codes, want = q8(h * w.double())
+    assert torch.equal(codes.cpu().double(), want_codes)
+    want = want * torch.rsqrt(h.square().mean(-1) + eps32)
+    # Half a step of fp32, and 2^-44 for what comes before it: chains of at most 150 fp64
+    # additions (2^-45.8 of a sum, half of it of its root) and a dozen operations more.
+    half = torch.ldexp(torch.ones_like(want), torch.frexp(want)[1] - 25)
+    live = want > 0
+    assert ((scales.cpu().double() - want).abs() <= half + want * 2.0**-44)[live].all()
+    assert not scales.cpu()[~live].any()
