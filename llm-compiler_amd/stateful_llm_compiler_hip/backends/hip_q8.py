@@ -133,8 +133,8 @@ def hip_rms_norm_q8(
 def hip_add_rms_norm_q8(
     tensor: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, *, epsilon: float
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(summed, codes, scales)``: ``hip_add(tensor, residual)``, bit for bit, and
-    ``hip_rms_norm_q8`` of it, in one pass."""
+    """``(summed, codes, scales)``: ``hip_add(tensor, residual)``, bit for bit (of two
+    NaNs either may be the sum's), and ``hip_rms_norm_q8`` of it, in one pass."""
 
     return _norm("HIP add RMSNorm q8", tensor, residual, weight, epsilon)
 

@@ -815,3 +815,26 @@ def test_norm_scales_are_rounded_once(gpu, dtype, residual, k):
     live = want > 0
     assert ((scales.cpu().double() - want).abs() <= half + want * 2.0**-44)[live].all()
     assert not scales.cpu()[~live].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [7, 1001, 33001])
+def test_sums_with_nans_are_those_of_hip_add(gpu, dtype, k):
+    # Any bits at all; NaNs in one operand, in the other, in both, and infinities that cancel.
+    announce(f"sums of any bits {dtype} {k}")
+    whole = {2: torch.int16, 4: torch.int32}[dtype.itemsize]
+    low, high = torch.iinfo(whole).min, torch.iinfo(whole).max
+    g = generator(k)
+    a, b = (torch.randint(low, high, (64, k), generator=g, dtype=whole).view(dtype) for _ in range(2))
+    kind = torch.rand(64, k, generator=g)
+    a[kind < 0.2] = torch.nan
+    b[(kind > 0.1) & (kind < 0.3)] = -torch.nan
+    a[(kind > 0.3) & (kind < 0.4)] = torch.inf
+    b[(kind > 0.35) & (kind < 0.4)] = -torch.inf
+    summed, _, scales = backends.hip_add_rms_norm_q8(a.to(gpu), b.to(gpu), torch.ones(k, dtype=dtype, device=gpu),
+                                                     epsilon=1e-6)
+    want = backends.hip_add(a.to(gpu), b.to(gpu))
+    both = (a.isnan() & b.isnan()).to(gpu)
+    assert torch.equal(summed.isnan(), want.isnan())
+    assert_bitwise_equal(summed[~both], want[~both])
+    assert scales[~want.isfinite().all(-1)].isnan().all()
