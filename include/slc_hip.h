@@ -659,7 +659,8 @@ SLC_API int slc_hip_swiglu_q8(const void* gate, const void* up, int8_t* codes, f
  * linear_q8: output[m, n] = round(float(sum_k input[m, k] * weight[n, k]) *
  * in_scales[m] * weight_scales[n] (+ bias[n])): the sum exact in 32-bit integers
  * (in_features <= SLC_Q8_MAX_K, codes -128 .. 127), the rest in fp32 in this
- * order, one rounding to dtype (fp32, fp16 or bf16; the bias has it too).
+ * order, each step rounded but the last product, which one fma adds to the bias;
+ * then one rounding to dtype (fp32, fp16 or bf16; the bias has it too).
  *   input  : rows x in_features codes, row stride in_stride_row
  *   weight : out_features x in_features codes, contiguous
  *   output : rows x out_features, row stride out_stride_row

@@ -169,7 +169,8 @@ def hip_linear_q8(
 
     ``codes`` and ``weight`` are int8 (-128 included), ``scales`` [...] and
     ``weight_scales`` [N] fp32.  The sum over K is exact; float(sum) * scale *
-    weight scale + bias runs in fp32 and is rounded once to ``output_dtype``.
+    weight scale + bias runs in fp32 in this order (the last product and the bias in
+    one fma) and is rounded once to ``output_dtype``.
     """
 
     what = "HIP linear q8"

@@ -838,3 +838,18 @@ def test_sums_with_nans_are_those_of_hip_add(gpu, dtype, k):
     assert torch.equal(summed.isnan(), want.isnan())
     assert_bitwise_equal(summed[~both], want[~both])
     assert scales[~want.isfinite().all(-1)].isnan().all()
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 1152, 896), (20, 20001, 272), (200, 20000, 128), (2300, 9731, 896),
+                                   (8000, 4090, 2048), (300, 1003, 1001), (2200, 2051, 1001)])
+def test_linear_adds_the_bias_before_it_rounds(gpu, m, n, k):
+    # Row 0's outputs are what the bias, its rounded products negated, leaves of them: 0 if the
+    # product were rounded before the addition.
+    announce(f"bias {m} x {n} x {k}")
+    codes, scales, weight, weight_scales, _ = (None if t is None else t.to(gpu) for t in operands(m, n, k, None, 17))
+    sums = (codes[:1].double() @ weight.double().t())[0]
+    product = (sums.float() * scales[0]).double() * weight_scales.double()  # exact: 24 x 24 bits
+    bias = -product.float()
+    y = backends.hip_linear_q8(codes, scales, weight, weight_scales, bias, output_dtype=torch.float32)
+    want = product + bias.double()  # exact, and of at most 24 bits: fp32 holds it
+    assert torch.equal(y[0].double(), want) and (want != 0).any()
