@@ -10,8 +10,14 @@ A layer's linears run on them as ``hip_add_rms_norm_q8`` -> ``hip_linear_q8``
 (Q/K/V, or gate and up in one weight), ``hip_quantize_q8`` of the attention output
 -> ``hip_linear_q8`` (O), ``hip_swiglu_q8`` -> ``hip_linear_q8`` (down).
 ``hip_quantize_q8`` of a weight ``[N, K]`` gives its codes and the scales of its
-output channels.  The reference has no 8-bit path; the operators take their
-arguments as ``hip_rms_norm``, ``hip_swiglu`` and ``hip_linear`` do.
+output channels.  The reference has no 8-bit path.
+
+The operators stand beside ``hip_rms_norm``, ``hip_swiglu`` and ``hip_linear`` and
+name their tensors alike, but compute other values than codes of those operators'
+results: nothing is rounded to a 16-bit type before the codes are.  So the norm has no
+``round_before_weight`` (the order of Qwen2's own norm, which rounds twice; a layer that
+needs it runs ``hip_rms_norm`` and ``hip_quantize_q8``), its weight has the input's
+dtype, and SwiGLU's silu is not rounded by itself.
 """
 
 from __future__ import annotations

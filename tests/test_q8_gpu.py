@@ -853,3 +853,16 @@ def test_linear_adds_the_bias_before_it_rounds(gpu, m, n, k):
     y = backends.hip_linear_q8(codes, scales, weight, weight_scales, bias, output_dtype=torch.float32)
     want = product + bias.double()  # exact, and of at most 24 bits: fp32 holds it
     assert torch.equal(y[0].double(), want) and (want != 0).any()
+
+
+def test_codes_of_the_norm_that_rounds_twice(gpu):
+    # As documented: hip_rms_norm in Qwen2's order, then its codes.
+    announce("norm in Qwen2's order")
+    x, w = rows_of(40, 896, torch.bfloat16, 1), (torch.rand(896, generator=generator(2)) + 0.5).bfloat16()
+    normed = backends.hip_rms_norm(x.to(gpu), w.to(gpu), epsilon=1e-6, round_before_weight=True)
+    h = x.float()
+    rstd = torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-6)
+    # Two roundings to bf16, and fp32's in front of them.
+    want = (h * rstd).bfloat16() * w
+    assert ((normed.cpu().double() - want.double()).abs() <= want.double().abs() * 2.0**-7 * 1.01).all()
+    check_rows(*backends.hip_quantize_q8(normed), normed.cpu().double())
