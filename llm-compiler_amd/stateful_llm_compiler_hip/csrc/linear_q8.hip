@@ -352,8 +352,11 @@ __device__ __forceinline__ void store_run(const __amdgpu_buffer_rsrc_t& ry, cons
 // stores them from registers.  Past K the X chunks are loaded as zeros (an offset
 // past the range), whatever the W chunks beside them hold.
 //
-// 4096 x 9728 x 896 42.8 us (1670 TOPS): loads and stores alone take 33, products and stores
-// 32.  8 x 151936 x 896 28 us, 5.0 TB/s of weight.
+// 4096 x 9728 x 896 43.5 us (1640 TOPS) where one buffer takes the outputs of call after call:
+// loads and stores alone take 33, products and stores 32; 56 us where outputs spread over 640
+// MB, past the caches.  fp32 outputs 62.  8 x 151936 x 896 28 us, 4.9 TB/s of weight.  Stores of
+// single elements (N that no 16 bytes divide) cost more than the products: 4096 x 9727 x 896
+// 112 us, in fp32 144.
 template <typename T, int BM, int BN, int CWM, int CWN, int PW, int S, int GM, bool VST>
 __global__ __launch_bounds__((CWM * CWN + PW) * 64) void stream_kernel(Problem p, int n_tiles,
                                                                        int m_tiles) {
@@ -593,8 +596,8 @@ __device__ __forceinline__ i32x4_t descriptor(const void* base, int64_t bytes) {
 // from registers.  Past K the X chunks are loaded as zeros (an offset past the range),
 // whatever the W chunks beside them hold.
 //
-// 8192 x 8192 x 8192 391 us (2810 TOPS), 32768 x 896 x 4864 125 (2280).  Bound by the clock that
-// the card's power leaves: codes of all zeros take 325 and 98.
+// 8192 x 8192 x 8192 404 us (2720 TOPS; on another card 391), 32768 x 896 x 4864 128 (2230).
+// Bound by the clock that the card's power leaves: codes of all zeros take 330 and 101.
 constexpr int kTurnsTile = 256, kTurnsGroup = 4;
 template <typename T, bool VST>
 __global__ __launch_bounds__(512, 2) void turns_kernel(Problem p, int n_tiles, int m_tiles) {
@@ -871,8 +874,8 @@ int launch_stream(const Problem& p, hipStream_t stream) {
 // rows past them are masked off by the buffer range) and splits K over its waves; the waves' sums meet
 // in LDS by integer adds, whose order does not matter.  Each wave keeps U k-steps of 64
 // codes in flight while it multiplies the U before.  Bound by the weight's bytes where
-// it is wide, by latency where it is narrow: 1 x 151936 x 896 25.3 us (5.4 TB/s), 8 x 1152 x
-// 896 3.3, 1 x 896 x 4864 4.9.
+// it is wide, by latency where it is narrow: 1 x 151936 x 896 25 us (5.4 TB/s), 8 x 1152 x
+// 896 3.3, 1 x 896 x 4864 4.6, 32 x 896 x 4864 8.5.
 constexpr int kRowBlock = 32;
 template <typename T, int MB, int TILES, int U>
 __global__ __launch_bounds__(1024) void rows_kernel(Problem p, int feat) {
@@ -1008,22 +1011,23 @@ int launch_rows(const Problem& p, hipStream_t stream) {
 // Which kernel takes a shape of aligned rows, all giving the same bits.
 //
 // rows_kernel where 16 x 16 fragments of the outputs are no more than CUs: tiles would leave
-// most CUs idle (us, rows | 64 x 64 tiles: 8 x 1152 x 896 3.7 | 4.4, 16 x 896 x 4864 6.3 | 9.1,
-// 16 x 4096 x 4096 7.0 | 8.4, 48 x 896 x 896 4.3 | 4.5, 250 x 256 x 4864 9.5 | 9.8; past that 16 x
-// 6000 x 2048 6.4 | 6.1, 32 x 4096 x 4096 9.4 | 8.5), but for many rows of few features, whose
-// tiles are as many (1900 x 32 x 896 5.0 | 4.4).  And for up to 4 rows of a vocabulary, whose
-// weight it reads a little faster (1 x 50257 x 896 10.8 | 11.8, 1 x 151936 x 896 25.3 | 26.3; 2 x
-// 32768 x 896 7.8 | 7.2, 8 x 151936 x 896 29.4 | 27.4).  Else up to 32 rows 64 x 64 tiles, which
-// the others' empty rows make no faster (64 x 64 | 128 x 128: 8 x 151936 x 896 27.4 | 28.7, 16 x
-// 151936 x 896 28.3 | 28.9).
+// most CUs idle (us, rows | 64 x 64 tiles: 8 x 1152 x 896 3.4 | 4.1, 16 x 896 x 4864 6.1 | 8.9,
+// 16 x 4096 x 4096 7.5 | 9.6, 48 x 896 x 896 4.0 | 4.2, 250 x 256 x 4864 9.0 | 9.4; past that 16 x
+// 6000 x 2048 6.4 | 5.9, 32 x 4096 x 4096 10.7 | 10.3), but for many rows of few features, whose
+// tiles are as many (1900 x 32 x 896 4.7 | 4.3).  And for up to 4 rows of a vocabulary, whose
+// weight it reads a little faster (1 x 50257 x 896 10.7 | 12.1, 1 x 151936 x 896 25.3 | 26.7; 2 x
+// 32768 x 896 8.0 | 7.8, 8 x 151936 x 896 29.7 | 28.2).  Else up to 32 rows 64 x 64 tiles, which
+// the others' empty rows make no faster (64 x 64 | 128 x 128: 8 x 151936 x 896 28.1 | 29.0, 16 x
+// 151936 x 896 29.5 | 30.1).  Operands and outputs of every call apart, 600 MB of them.
 //
 // Else the tile that costs least: a start, and rounds over the CUs of a fixed part and one per
 // k-tile (us; fitted to every tile's time at 123 shapes of 9 to 32768 rows, 896 to 151936
 // features and K 896 to 11008, where the choice is the fastest tile or within 5 %, 0.2 % off on
-// average).  Rounds, not tiles: 8192 x 896 x 896 12.3 us as one round of 256 x 128, 12.6 as two
-// of 128 x 128; 4096 x 9728 x 896 43.5 as five rounds of 256 x 128, 50 as three of 256 x 256;
-// 32768 x 896 x 4864 127 as two of 256 x 256, 138 as four of 256 x 128; 65 x 896 x 896 4.7 as 64
-// x 64, 8.2 as 256 x 128.
+// average, one buffer taking the outputs).  Rounds, not tiles: 8192 x 896 x 896 12.3 us as one
+// round of 256 x 128, 12.6 as two of 128 x 128 (outputs apart, as above: 13.4 and 14.3); 4096 x
+// 9728 x 896 43.5 as five rounds of 256 x 128, 50 as three of 256 x 256 (56 and 57); 32768 x 896 x
+// 4864 127 as two of 256 x 256, 137 as four of 256 x 128; 65 x 896 x 896 4.5 as 64 x 64, 7.9 as
+// 256 x 128.
 enum Kernel { kRows, k64x64, k128x64, k128x128, k256x128, k256x256 };
 inline Kernel choose(int64_t M, int64_t N, int64_t K) {
   const int64_t cus = slc_host::device_cu_count();

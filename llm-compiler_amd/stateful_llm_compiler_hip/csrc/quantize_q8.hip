@@ -22,9 +22,12 @@
 // thousand rows, bound by the launch and two dependent reductions below.  Rows
 // past 16 waves' registers are read twice (LOOP).  All loads are issued before
 // the first use, without branches: buffer loads whose range ends with the row.
-// 16384 x 896 fp16 9.5 us (4.6 TB/s), SwiGLU 4096 x 4864 bf16 23.6 (4.2 TB/s, with 14 us of
-// vector instructions), norm of 9001 x 1001 fp32 11.8 (3.8 TB/s), addition and norm of 4096
-// x 896 bf16 7.9, of one row 2.7.
+// Graphs over six sets of inputs: 16384 x 896 fp16 9.5 us (4.7 TB/s), SwiGLU 4096 x 4864 bf16
+// 23.8 (4.2 TB/s, with 14 us of vector instructions), norm of 9001 x 1001 fp32 11.2 (4.0
+// TB/s), addition and norm of 4096 x 896 bf16 8.0, of one row 2.4.  Where that fp32 norm's
+// time goes, over sixteen sets: 12.4, a plain copy of as many bytes 11.2; without the fp64
+// maximum 11.6, without the fp64 squares 12.1, without second decisions 11.8, without all
+// three 11.3.
 #include <float.h>
 
 #include <initializer_list>
@@ -63,9 +66,9 @@ struct Traits {
   static constexpr bool kHasB = SRC == kAddNorm || SRC == kSwiglu;
   static constexpr bool kHasW = SRC == kNorm || SRC == kAddNorm;
   // Whether the fp32 v may differ from y.  Then a is taken in fp64: of products of two fp32
-  // values, exact there, beside v (norm 9001 x 1001 10.9 us; in a second pass over the values
-  // near the largest, behind a second barrier, 13.1); of SwiGLU, whose fp64 values cost too
-  // much for that, in such a second pass.
+  // values, exact there, beside v (norm 9001 x 1001, one set of inputs | several: 10.9 us |
+  // 11.8; in a second pass over the values near the largest, behind a second barrier, 13.1 |
+  // 12.9); of SwiGLU, whose fp64 values cost too much for that, in such a second pass.
   static constexpr bool kWide = kHasW && sizeof(T) == 4;
   static constexpr bool kInexact = SRC == kSwiglu || kWide;
   static constexpr float kApart = (SRC == kSwiglu ? 14 : kInexact ? 6 : 4) * 0x1p-24f;
