@@ -866,3 +866,49 @@ def test_codes_of_the_norm_that_rounds_twice(gpu):
     want = (h * rstd).bfloat16() * w
     assert ((normed.cpu().double() - want.double()).abs() <= want.double().abs() * 2.0**-7 * 1.01).all()
     check_rows(*backends.hip_quantize_q8(normed), normed.cpu().double())
+
+
+@pytest.mark.parametrize("m,n,kernel", [(1, 40, "rows"), (100, 40, "stream"), (300, 9728, "stream"),
+                                        (4096, 4096, "turns")])
+def test_longest_aligned_sums(gpu, m, n, kernel):
+    # The largest K that 16 divides: 1024 k-tiles, the last of them cut.
+    k = 131056
+    announce(f"longest aligned sums {m} x {n}")
+    codes = torch.full((m, k), -128, dtype=torch.int8, device=gpu)
+    weight = torch.full((n, k), -128, dtype=torch.int8, device=gpu)
+    codes[-1], weight[-1, -16:] = 127, 1
+    one = torch.ones(max(m, n), device=gpu)
+    call = lambda: backends.hip_linear_q8(codes, one[:m], weight, one[:n], output_dtype=torch.float32)  # noqa: E731
+    assert [name for name, _, _ in captured_kernels(call)] == [kernel]
+    left = torch.full((m, 1), -128.0, dtype=torch.float64, device=gpu)
+    left[-1] = 127.0
+    right = torch.full((1, n), -128.0 * k, dtype=torch.float64, device=gpu)
+    right[0, -1] = -128.0 * (k - 16) + 16
+    assert torch.equal(call(), (left @ right).float())
+
+
+# Row strides of the codes and of the outputs (elements): at the end of what 32-bit offsets
+# within a 64-row tile reach, and past it.
+@pytest.mark.parametrize("dtype,m,x_rs,y_rs,kernel", [
+    (torch.bfloat16, 70, 2**25 - 2**15, 192, "stream"), (torch.bfloat16, 70, 2**25, 192, "tile"),
+    (torch.bfloat16, 70, 320, 2**24 - 2**14, "stream"), (torch.bfloat16, 70, 320, 2**24, "tile"),
+    (torch.float32, 70, 320, 2**23 - 2**13, "stream"), (torch.float32, 70, 320, 2**23, "tile"),
+    (torch.float32, 20, 2**26 - 2**16, 2**25, "rows"), (torch.float32, 20, 2**26, 192, "tile"),
+])
+def test_linear_of_rows_far_apart(gpu, dtype, m, x_rs, y_rs, kernel):
+    announce(f"rows {x_rs} and {y_rs} apart, {dtype}")
+    n, k = (100, 320) if m > 32 else (192, 320)
+    codes, scales, weight, weight_scales, bias = (t.to(gpu) for t in operands(m, n, k, dtype, 5))
+    want = backends.hip_linear_q8(codes, scales, weight, weight_scales, bias, output_dtype=dtype)
+    far = torch.empty((m - 1) * x_rs + k, dtype=torch.int8, device=gpu).as_strided((m, k), (x_rs, 1))
+    far.copy_(codes)
+    flat = torch.full((m * y_rs,), 7.0, dtype=dtype, device=gpu)
+    call = lambda: _native.check(_native.library().slc_hip_linear_q8(  # noqa: E731
+        far.data_ptr(), scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), bias.data_ptr(),
+        flat.data_ptr(), _native.dtype_tag(dtype), m, n, k, x_rs, y_rs, _native.current_stream(gpu)),
+        "slc_hip_linear_q8")
+    assert [name for name, _, _ in captured_kernels(call)] == [kernel]
+    call()
+    out = flat.view(m, y_rs)
+    assert_bitwise_equal(out[:, :n], want)
+    assert (out[:, n:] == 7).all()
