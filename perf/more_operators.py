@@ -208,7 +208,6 @@ def prepare(case, seed):
         state["keys"], state["values"] = (state["cache"][:LAYERS].unbind(0), state["cache"][LAYERS:].unbind(0))
         lengths = torch.randint(0, capacity - tokens + 1, (batch,), device=DEVICE, generator=g)
         state["lengths"] = lengths.repeat(LAYERS, 1)
-        state["slots"] = state["lengths"].unbind(0)
         # The tree's first branch lies in front of the others: an accepted path follows it for some nodes, then
         # goes on in a branch that lies behind.
         kept = case["kept"]
@@ -307,7 +306,7 @@ def _commit(state):
         page = state["cache"].shape[2]
         cache[layer, table[each, target // page].long(), target % page] = cache[
             layer, table[each, source // page].long(), source % page]
-    return cache, (lengths + counts).unbind(0)
+    return cache, lengths + counts
 
 
 def _import_backends():
@@ -329,13 +328,9 @@ def _run_own(state):
         return backends.hip_verify_tokens(state["tokens"], state["target"], state["uniforms"],
                                           parents=state["parents"], draft_probs=state["draft"])
     if op == "commit":
-        if state["table"] is None:
-            lengths = backends.hip_kv_commit(state["keys"], state["values"], state["slots"], state["path"],
-                                             state["counts"])
-        else:
-            lengths = backends.hip_paged_kv_commit(state["keys"], state["values"], state["table"], state["slots"],
-                                                   state["path"], state["counts"])
-        return state["cache"], lengths
+        if "layers" not in state:  # made once, with the cache, and kept as long
+            state["layers"] = backends.KVLayers(state["keys"], state["values"], block_table=state["table"])
+        return state["cache"], backends.hip_kv_commit(state["layers"], state["lengths"], state["path"], state["counts"])
     if state["table"] is None:
         return backends.hip_tree_attention(state["query"], state["key"], state["value"], state["lengths"],
                                            state["tree"], state["mask"], scale=state["scale"])
@@ -421,7 +416,7 @@ def _exact_verify(state):
                     rest[token] = 0.0
                     left -= chance
                 else:
-                    rest = torch.clamp(rest - draft[b, path[-1]].double(), min=0.0)
+                    rest = torch.clamp(rest - left * draft[b, path[-1]].double(), min=0.0)
                     left = float(rest.sum())
             if follows is None:
                 break
