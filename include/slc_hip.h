@@ -33,6 +33,8 @@
  *                              (semantics of execution.py:707-739)
  *   slc_hip_quantize_q8, slc_hip_rms_norm_q8, slc_hip_swiglu_q8,
  *   slc_hip_linear_q8: 8-bit linears, which the reference does not have
+ *   slc_hip_tree_attention, slc_hip_paged_tree_attention, slc_hip_verify_tokens,
+ *   slc_hip_kv_commit: a step on drafted tokens, which the reference does not have
  */
 #ifndef SLC_HIP_H_
 #define SLC_HIP_H_
@@ -671,6 +673,113 @@ SLC_API int slc_hip_linear_q8(const int8_t* input, const float* in_scales, const
                               const float* weight_scales, const void* bias, void* output,
                               int dtype, int64_t rows, int64_t out_features, int64_t in_features,
                               int64_t in_stride_row, int64_t out_stride_row, void* stream);
+
+/*
+ * A step on drafted tokens: several tokens per sequence, proposed by a cheaper
+ * model, go through the model at once.  A sequence's nodes form a tree: node 0, the
+ * last token that stands, is its root, every other node has an earlier one as its
+ * parent.  Their K and V rows are stored behind the sequence, node j at row
+ * lengths[b] + j (slc_hip_kv_store at the lengths, which are not advanced), attend
+ * as a tree, are verified by the target's probabilities and, where accepted,
+ * committed.  The reference has no such step.
+ *
+ * tree_attention:
+ *   output[b, h, i] = sum over the rows s that node i sees of softmax(t)[s] V[s],
+ *   t[s] = scale * query[b, h, i] . K[s] (+ mask[b, s]).
+ * Node i sees the sequence's rows s < lengths[b] and those of its nodes j with
+ * tree[b, i, j] != 0 (tree NULL: j <= i, a chain), all of them below the capacity
+ * and, with a mask, below mask_len; a row whose mask is -inf is not seen.  What K and
+ * V hold in rows that a node does not see, infinities and NaN among them, has no
+ * effect on it.  A node that sees no row has NaN.  Scores, the softmax and its sum
+ * are fp32; 16-bit types round the unnormalised weights to their type for the
+ * product with V.
+ *   query, output [B, q_heads, nodes, D], D 1 to 256 and contiguous; K and V rows
+ *   [B, capacity, kv_heads, D] (pages [num_pages, page_tokens, kv_heads, D]
+ *   and block_table int32 [B, pages_per_seq], unit stride) with one set of strides;
+ *   lengths int32 or int64; tree bytes; mask fp32, fp16 or bf16; scale > 0.
+ *   nodes <= SLC_TREE_MAX_NODES, capacity <= 2^30.
+ * The workspace (slc_hip_tree_attention_workspace_size bytes, 16-byte aligned; the
+ * paged form needs the same) holds the partial results of a split over the rows;
+ * calls that may overlap in time need their own.  Table entries that name no page of
+ * the pool are not followed; a node that sees rows of such a page has no meaning.
+ */
+#define SLC_TREE_MAX_NODES 4096
+SLC_API int64_t slc_hip_tree_attention_workspace_size(int64_t batch, int64_t q_heads,
+                                                      int64_t kv_heads, int64_t nodes,
+                                                      int64_t head_dim, int dtype);
+SLC_API int slc_hip_tree_attention(
+    const void* query, const void* key_buffer, const void* value_buffer, const void* lengths,
+    int lengths_dtype, const uint8_t* tree, const void* mask, int mask_dtype, void* output,
+    void* workspace, int64_t workspace_bytes, int dtype, int64_t batch, int64_t q_heads,
+    int64_t kv_heads, int64_t nodes, int64_t head_dim, int64_t capacity, int64_t mask_len,
+    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, int64_t kv_stride_b,
+    int64_t kv_stride_s, int64_t kv_stride_h, int64_t tree_stride_b, int64_t tree_stride_i,
+    int64_t tree_stride_j, int64_t mask_stride_b, int64_t mask_stride_s, int64_t out_stride_b,
+    int64_t out_stride_h, int64_t out_stride_t, float scale, void* stream);
+SLC_API int slc_hip_paged_tree_attention(
+    const void* query, const void* key_pool, const void* value_pool, const int32_t* block_table,
+    int64_t table_stride_b, int64_t pages_per_seq, int64_t page_tokens, int64_t num_pages,
+    int64_t page_stride, const void* lengths, int lengths_dtype, const uint8_t* tree,
+    const void* mask, int mask_dtype, void* output, void* workspace, int64_t workspace_bytes,
+    int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t head_dim,
+    int64_t mask_len, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+    int64_t kv_stride_s, int64_t kv_stride_h, int64_t tree_stride_b, int64_t tree_stride_i,
+    int64_t tree_stride_j, int64_t mask_stride_b, int64_t mask_stride_s, int64_t out_stride_b,
+    int64_t out_stride_h, int64_t out_stride_t, float scale, void* stream);
+
+/*
+ * verify_tokens: from node 0 down, which drafted tokens the target accepts, and the
+ * token that follows them.  At a node n with target row p = target[b, n] its
+ * children c (parents[b, c] == n; parents NULL: a chain, c - 1) are tried in
+ * ascending order, x = tokens[b, c], u = uniforms[b, c] in [0, 1), in fp64:
+ *   with draft rows (q = draft[b, n], from which the children were drawn
+ *   independently): w = max(p - M q, 0), M = 0 and m = 1 at first; accepted where
+ *   u m q(x) < w(x); refused: M += m, m = sum w of the new M;
+ *   without (draft NULL): w = p and m = 1 at first; accepted where u m < w(x) and
+ *   w(x) > 0; refused: m -= w(x), w(x) = 0.
+ * An accepted child is the next node.  Where none is, the token that follows is the
+ * first i with w(0) + .. + w(i) > uniforms[b, 0] * sum w, or, where no w is positive,
+ * the same of p (-1 where no p is).  A node whose parent is not an earlier node, and
+ * a token outside the vocabulary, is never accepted; a probability that is NaN or
+ * negative has no weight.  Probabilities sum to 1.
+ *   path[b, :]    : the accepted nodes in ascending order, 0 first, then -1
+ *   emitted[b, :] : their tokens without node 0's, the token that follows, then -1
+ *   counts[b]     : accepted nodes, node 0 among them, and so emitted tokens
+ * tokens, parents [B, nodes]; uniforms [B, nodes]; target [B, nodes, vocab] and draft
+ * [B, nodes - 1, vocab] of one dtype, rows contiguous; path and emitted [B, nodes]
+ * contiguous.  The workspace is slc_hip_verify_tokens_workspace_size bytes on 8 bytes,
+ * the counters `batch` ints, zero between calls; calls that may overlap need their own.
+ */
+#define SLC_VERIFY_MAX_NODES 1024
+SLC_API int64_t slc_hip_verify_tokens_workspace_size(int64_t batch, int64_t vocab);
+SLC_API int slc_hip_verify_tokens(
+    const int64_t* tokens, const int64_t* parents, const void* target, const void* draft,
+    const float* uniforms, int64_t* path, int64_t* emitted, int64_t* counts, void* workspace,
+    int64_t workspace_bytes, int* counters, int64_t num_counters, int dtype, int64_t batch,
+    int64_t nodes, int64_t vocab, int64_t tok_stride_b, int64_t parent_stride_b,
+    int64_t uniform_stride_b, int64_t target_stride_b, int64_t target_stride_t,
+    int64_t draft_stride_b, int64_t draft_stride_t, void* stream);
+
+/*
+ * kv_commit: in every layer l, K and V row lengths[l][b] + path[b, j] moves to row
+ * lengths[l][b] + j for j < counts[b], and lengths_out[l][b] = lengths[l][b] +
+ * counts[b] (in place allowed; *overflow set past the capacity).  path ascends
+ * within a count; entries outside [0, nodes) and rows past the capacity are not
+ * moved.  Rows behind the new lengths keep what they held.
+ *   key, value, lengths, lengths_out: host arrays of `layers` device pointers; the
+ *   caches all different; lengths_out[l] NULL (not written), lengths[l] itself or
+ *   memory that no other layer reads or writes; caches as in slc_hip_tree_attention
+ *   (block_table NULL: stride_b per sequence, else per page); path int64 [B, nodes]
+ *   contiguous, counts int64 [B].
+ */
+#define SLC_KV_COMMIT_MAX_LAYERS 96 /* of one launch; more take several */
+SLC_API int slc_hip_kv_commit(
+    void* const* key, void* const* value, const int64_t* const* lengths,
+    int64_t* const* lengths_out, const int32_t* block_table, int64_t table_stride_b,
+    int64_t pages_per_seq, int64_t page_tokens, int64_t num_pages, const int64_t* path,
+    const int64_t* counts, int* overflow, int dtype, int64_t layers, int64_t batch, int64_t nodes,
+    int64_t heads, int64_t head_dim, int64_t capacity, int64_t stride_b, int64_t stride_s,
+    int64_t stride_h, void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,13 @@ from .hip_attention import (
     hip_decode_attention_noalloc,
     hip_rope_decode_attention,
 )
+from .hip_draft import (
+    KVLayers,
+    hip_kv_commit,
+    hip_paged_tree_attention,
+    hip_tree_attention,
+    hip_verify_tokens,
+)
 from .hip_fused import (
     hip_linear_residual,
     hip_norm_linear_group,
@@ -61,4 +68,9 @@ __all__ = [
     "hip_swiglu_q8",
     "hip_rms_norm",
     "hip_rope",
+    "KVLayers",
+    "hip_kv_commit",
+    "hip_paged_tree_attention",
+    "hip_tree_attention",
+    "hip_verify_tokens",
 ]

@@ -20,18 +20,20 @@ from __future__ import annotations
 
 import re
 import weakref
-from dataclasses import dataclass, replace
+from dataclasses import dataclass, field, replace
 from typing import Any, Callable, Sequence
 
 import torch
 import torch.nn.functional as F
 
 from .backends import (
+    KVLayers,
     hip_add,
     hip_decode_attention,
     hip_rope_decode_attention,
     hip_embedding,
     hip_kv_advance,
+    hip_kv_commit,
     hip_kv_store,
     hip_linear,
     hip_linear_residual,
@@ -40,6 +42,7 @@ from .backends import (
     hip_paged_decode_attention,
     hip_paged_kv_store,
     hip_paged_rope_decode_attention,
+    hip_paged_tree_attention,
     hip_prefill_attention,
     hip_prefill_mask_tiles,
     hip_rms_norm,
@@ -47,6 +50,7 @@ from .backends import (
     hip_rope_kv_store,
     hip_rope_table,
     hip_swiglu,
+    hip_tree_attention,
 )
 from . import _native
 from .backends.hip_attention import exact_max_tokens
@@ -121,6 +125,9 @@ class PreallocatedKVCacheState:
     # one stream, and two states (two decoders) never share it.  None = the
     # current stream's workspace.
     workspace: _native.DeviceWorkspace | None = None
+    # The checked layers of commit(), made by the first one and passed on to later
+    # versions; made anew for other buffers.
+    layers: KVLayers | None = field(default=None, compare=False, repr=False)
 
     def __post_init__(self) -> None:
         if self.capacity <= 0:
@@ -387,6 +394,56 @@ class PreallocatedKVCacheState:
         zero = None if self.zero_slots is None else self.zero_slots - {slot}
         return replace(self, lengths=tuple(lengths), generation=self.generation + 1, zero_slots=zero)
 
+    def tree_attention(
+        self,
+        slot: int,
+        query: torch.Tensor,
+        tree_mask: torch.Tensor | None,
+        attention_mask: torch.Tensor | None = None,
+        *,
+        groups: int,
+        scale: float,
+    ) -> torch.Tensor:
+        """Attention of the nodes of a tree of drafted tokens, B x H x T x D, whose K
+        and V rows ``store`` or ``rope_store`` wrote at this slot's lengths (which
+        stay those before the nodes until ``commit``).  ``tree_mask`` and
+        ``attention_mask`` as in ``hip_tree_attention``."""
+
+        lengths = self._check_tree(slot, query, attention_mask, groups)
+        return hip_tree_attention(query, self.keys[slot], self.values[slot], lengths, tree_mask,
+                                  _kernel_mask(attention_mask, self.capacity), scale=scale,
+                                  workspace=self.workspace)
+
+    def _check_tree(self, slot, query, attention_mask, groups):
+        lengths = self.positions(slot)
+        heads, head_dim = self.keys[slot].shape[2:]
+        if query.ndim != 4 or query.shape[0] != lengths.shape[0] or query.shape[3] != head_dim:
+            raise ExecutionError("tree attention query must be B x H x T x D as the KV buffers")
+        if groups <= 0 or query.shape[1] != heads * groups:
+            raise ExecutionError("tree attention GQA groups do not match")
+        if attention_mask is not None and attention_mask.shape[-1] > self.capacity:
+            raise ExecutionError("tree attention mask is longer than the KV capacity")
+        return lengths
+
+    def commit(self, path: torch.Tensor, counts: torch.Tensor) -> "PreallocatedKVCacheState":
+        """The accepted nodes' rows (``path`` and ``counts`` of ``hip_verify_tokens``)
+        moved to their places in every layer, and every slot's lengths advanced by
+        ``counts``.  Older versions' visible prefixes are untouched."""
+
+        if path.ndim != 2 or path.shape[0] != self.lengths[0].shape[0] or counts.shape != (path.shape[0],):
+            raise ExecutionError("KV commit takes a B x T path and B counts")
+        layers = self.layers
+        if layers is None or layers.keys is not self.keys or layers.values is not self.values:
+            layers = KVLayers(self.keys, self.values, block_table=self._block_table())
+        out = hip_kv_commit(layers, self.lengths, path, counts, out=self.lengths if self.in_place_lengths else None,
+                            overflow=self.overflow)
+        object.__setattr__(self, "layers", layers)
+        zero = None if self.zero_slots is None else frozenset()
+        return replace(self, lengths=tuple(out), generation=self.generation + 1, zero_slots=zero)
+
+    def _block_table(self) -> torch.Tensor | None:
+        return None
+
     def check_capacity(self) -> None:
         """Synchronise and raise if any store or advance overflowed the capacity."""
 
@@ -587,6 +644,17 @@ class PagedKVCacheState(PreallocatedKVCacheState):
             query, self.keys[slot], self.values[slot], self.block_table, lengths,
             _kernel_mask(attention_mask, self.capacity),
             scale=scale, softmax_order=order, workspace=self.workspace, split_tokens=split_tokens)
+
+    def tree_attention(self, slot, query, tree_mask, attention_mask=None, *, groups, scale):
+        """The contiguous state's ``tree_attention`` through the block table."""
+
+        lengths = self._check_tree(slot, query, attention_mask, groups)
+        return hip_paged_tree_attention(query, self.keys[slot], self.values[slot], self.block_table, lengths,
+                                        tree_mask, _kernel_mask(attention_mask, self.capacity), scale=scale,
+                                        workspace=self.workspace)
+
+    def _block_table(self) -> torch.Tensor | None:
+        return self.block_table
 
     def _validate_store(self, slot, key, value, positions):
         try:

@@ -1,0 +1,123 @@
+"""Refusals of the operators on drafted tokens: by the wrappers on host tensors and by the C
+entry points on arguments that are checked before any device call."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from stateful_llm_compiler_hip import _native, backends
+from stateful_llm_compiler_hip.execution import ExecutionError, PreallocatedKVCacheState
+
+P = 0x1000  # 4 KiB-aligned, never dereferenced on these paths
+F32, F16, BF16, I32, I64 = 0, 1, 2, 3, 4
+
+
+def test_wrappers_refuse_host_tensors():
+    q, kv = torch.zeros(1, 2, 3, 64), torch.zeros(1, 16, 2, 64)
+    lengths, table = torch.zeros(1, dtype=torch.int64), torch.zeros(1, 1, dtype=torch.int32)
+    tokens, probs = torch.zeros(1, 3, dtype=torch.int64), torch.zeros(1, 3, 5)
+    for call in (
+        lambda: backends.hip_tree_attention(q, kv, kv, lengths, None, scale=1.0),
+        lambda: backends.hip_paged_tree_attention(q, kv, kv, table, lengths, None, scale=1.0),
+        lambda: backends.hip_verify_tokens(tokens, probs, torch.zeros(1, 3)),
+        lambda: backends.KVLayers([kv], [kv.clone()]),
+    ):
+        with pytest.raises(ValueError, match="on the GPU"):
+            call()
+
+
+def tree(paged=False, query=P, key=P, value=P, lengths=P, lengths_dtype=I64, mask=None, mask_dtype=F32, out=P,
+         workspace=P, nbytes=1 << 40, dtype=BF16, batch=2, q_heads=4, kv_heads=2, nodes=3, head_dim=64, rows=64,
+         mask_len=64, scale=0.125, table=P, page_tokens=16, num_pages=9, kv_ss=128):
+    lib = _native.library()
+    tail = (scale, None)
+    strides = (q_heads * nodes * head_dim, nodes * head_dim, head_dim)
+    if paged:
+        return lib.slc_hip_paged_tree_attention(
+            query, key, value, table, rows // 16, rows // 16, page_tokens, num_pages, 16 * kv_ss, lengths,
+            lengths_dtype, None, mask, mask_dtype, out, workspace, nbytes, dtype, batch, q_heads, kv_heads, nodes,
+            head_dim, mask_len, *strides, kv_ss, head_dim, 0, 0, 0, 0, 0, *strides, *tail)
+    return lib.slc_hip_tree_attention(
+        query, key, value, lengths, lengths_dtype, None, mask, mask_dtype, out, workspace, nbytes, dtype, batch,
+        q_heads, kv_heads, nodes, head_dim, rows, mask_len, *strides, rows * kv_ss, kv_ss, head_dim, 0, 0, 0, 0, 0,
+        *strides, *tail)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_tree_attention_entry_points_refuse(paged):
+    for bad in ({"dtype": I32}, {"dtype": 99}, {"lengths_dtype": F32}, {"batch": -1}, {"batch": 65536},
+                {"nodes": -1}, {"nodes": 4097}, {"q_heads": 3}, {"q_heads": 0}, {"kv_heads": 0}, {"head_dim": 0},
+                {"head_dim": 257}, {"query": None}, {"key": None}, {"value": None}, {"lengths": None}, {"out": None},
+                {"scale": 0.0}, {"scale": -1.0}, {"scale": float("nan")}, {"scale": float("inf")},
+                {"mask": P, "mask_dtype": I32}, {"mask": P, "mask_len": 65}, {"mask": P, "mask_len": -1}):
+        assert tree(paged, **bad) == -1, bad
+    assert tree(paged, batch=0) == 0 and tree(paged, nodes=0) == 0  # nothing to do, nothing launched
+    assert tree(paged, batch=0, query=None) == 0
+
+
+def test_tree_attention_entry_points_refuse_their_own_operands():
+    assert tree(rows=0) == -1 and tree(rows=2**30 + 1) == -1
+    for bad in ({"page_tokens": 8}, {"page_tokens": 48}, {"page_tokens": 0}, {"num_pages": -1}, {"rows": 0},
+                {"table": None}):
+        assert tree(True, **bad) == -1, bad
+
+
+def verify(tokens=P, parents=None, target=P, draft=None, uniforms=P, path=P, emitted=P, counts=P, workspace=P,
+           nbytes=1 << 20, counters=P, num_counters=64, dtype=F32, batch=2, nodes=3, vocab=100):
+    return _native.library().slc_hip_verify_tokens(
+        tokens, parents, target, draft, uniforms, path, emitted, counts, workspace, nbytes, counters, num_counters,
+        dtype, batch, nodes, vocab, nodes, nodes, nodes, nodes * vocab, vocab, nodes * vocab, vocab, None)
+
+
+def test_verify_entry_point_refuses():
+    for bad in ({"dtype": I64}, {"dtype": 99}, {"batch": -1}, {"batch": 65536}, {"nodes": 0}, {"nodes": 1025},
+                {"vocab": 0}, {"vocab": 2**31}, {"num_counters": 1}, {"nbytes": 15}, {"workspace": P + 4},
+                {"tokens": None}, {"target": None}, {"uniforms": None}, {"path": None}, {"emitted": None},
+                {"counts": None}, {"workspace": None}, {"counters": None}):
+        assert verify(**bad) == -1, bad
+    assert verify(batch=0) == 0 and verify(batch=0, tokens=None) == 0
+    size = _native.library().slc_hip_verify_tokens_workspace_size
+    assert size(2, 1024) == 16 and size(2, 1025) == 32 and size(0, 5) == 0
+
+
+def commit(key=(P, 2 * P), value=(3 * P, 4 * P), lengths=(5 * P, 6 * P), out=(7 * P, 8 * P), table=None, page_tokens=0,
+           pages=0, num_pages=0, path=P, counts=P, dtype=BF16, layers=2, batch=2, nodes=3, heads=2, head_dim=64,
+           capacity=64):
+    def pointers(values):
+        return None if values is None else (ctypes.c_void_p * len(values))(*values)
+
+    return _native.library().slc_hip_kv_commit(
+        pointers(key), pointers(value), pointers(lengths), pointers(out), table, pages, pages, page_tokens, num_pages,
+        path, counts, None, dtype, layers, batch, nodes, heads, head_dim, capacity, capacity * heads * head_dim,
+        heads * head_dim, head_dim, None)
+
+
+def test_commit_entry_point_refuses():
+    for bad in ({"dtype": I64}, {"layers": -1}, {"batch": -1}, {"batch": 65536}, {"nodes": 0}, {"nodes": 1025},
+                {"heads": 0}, {"head_dim": 0}, {"capacity": 0}, {"key": None}, {"value": None}, {"lengths": None},
+                {"out": None}, {"path": None}, {"counts": None}, {"key": (P, None)}, {"lengths": (None, P)},
+                {"key": (P, P + 1)}, {"table": P, "page_tokens": 8, "pages": 8, "num_pages": 16},
+                {"table": P, "page_tokens": 16, "pages": 3, "num_pages": 16},
+                {"table": P, "page_tokens": 16, "pages": 4, "num_pages": -1}):
+        assert commit(**bad) == -1, bad
+    assert commit(layers=0) == 0 and commit(batch=0) == 0 and commit(batch=0, key=None) == 0
+
+
+def test_state_refuses_what_does_not_fit_its_buffers():
+    state = PreallocatedKVCacheState.empty_from_key_template(torch.zeros(2, 2, 1, 64), num_layers=2, capacity=32)
+    query = torch.zeros(2, 4, 3, 64)
+    for bad in (
+        lambda: state.tree_attention(5, query, None, groups=2, scale=1.0),
+        lambda: state.tree_attention(0, query[:1], None, groups=2, scale=1.0),
+        lambda: state.tree_attention(0, query[..., :32], None, groups=2, scale=1.0),
+        lambda: state.tree_attention(0, query[0], None, groups=2, scale=1.0),
+        lambda: state.tree_attention(0, query, None, groups=4, scale=1.0),
+        lambda: state.tree_attention(0, query, None, torch.zeros(2, 1, 1, 33), groups=2, scale=1.0),
+        lambda: state.commit(torch.zeros(1, 3, dtype=torch.int64), torch.zeros(2, dtype=torch.int64)),
+        lambda: state.commit(torch.zeros(2, 3, dtype=torch.int64), torch.zeros(3, dtype=torch.int64)),
+    ):
+        with pytest.raises(ExecutionError):
+            bad()

@@ -1,0 +1,962 @@
+"""GPU tests of the operators on drafted tokens against plain 64-bit implementations."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from helpers import announce, assert_bitwise_equal, generator
+from stateful_llm_compiler_hip import _native, backends
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+NAN = float("nan")
+
+
+# ---- tree attention -----------------------------------------------------------------
+
+
+def random_tree(nodes, g, batch=None):
+    """Masks of ancestors and selves of random trees."""
+
+    masks = []
+    for _ in range(batch or 1):
+        mask = torch.eye(nodes, dtype=torch.bool)
+        for c in range(1, nodes):
+            mask[c] |= mask[int(torch.randint(max(0, c - 5), c, (1,), generator=g))]
+        masks.append(mask)
+    return torch.stack(masks) if batch else masks[0]
+
+
+def tree_reference(query, key, value, lengths, tree, mask, scale):
+    """fp64 output of tree attention over [B, Cap, KVH, D] buffers, and bounds of its
+    parts per output: the weighted magnitudes of V, the largest score and the largest
+    sum of a score's products' magnitudes of the row."""
+
+    batch, q_heads, nodes, head_dim = query.shape
+    capacity, kv_heads = key.shape[1:3]
+    groups = q_heads // kv_heads
+    out = torch.full(query.shape, NAN, dtype=torch.float64)
+    weighted, top, products = (torch.zeros(query.shape, dtype=torch.float64) for _ in range(3))
+    rows = capacity if mask is None else mask.shape[-1]
+    if tree is None:
+        tree = torch.ones(nodes, nodes, dtype=torch.bool).tril_()
+    tree = tree.expand(batch, nodes, nodes)
+    for b in range(batch):
+        length = min(max(int(lengths[b]), 0), capacity)
+        end = min(length + nodes, rows)
+        for i in range(nodes):
+            seen = torch.arange(end) < length
+            behind = torch.arange(length, max(end, length))
+            seen[length:end] = tree[b, i, behind - length]
+            if mask is not None:
+                seen &= mask[b, 0, 0, :end] != -INF
+            at = seen.nonzero().view(-1)
+            if not len(at):
+                continue
+            for h in range(q_heads):
+                q = query[b, h, i].double()
+                k, v = key[b, at, h // groups].double(), value[b, at, h // groups].double()
+                t = k @ q * scale
+                size = (k.abs() @ q.abs() * scale).max()
+                if mask is not None:
+                    t = t + mask[b, 0, 0, at].double()
+                w = torch.softmax(t, 0)
+                out[b, h, i] = w @ v
+                weighted[b, h, i] = w @ v.abs()
+                top[b, h, i], products[b, h, i] = (t - t.max()).abs().clamp_max(200).max(), size
+    return out, weighted, top, products
+
+
+def assert_tree_close(actual, reference, keys):
+    """|actual - exact| within what the formula's steps may be off.
+
+    With h half the type's spacing (bf16 2^-8, fp16 2^-11 relative) the 16-bit forms
+    round each weight (h of the weighted |V|, and h again through their sum) and the
+    output (h of it); fp16 weights under 2^-14 of the row's largest are off by up to
+    2^-25 each, of at most `keys` values of size |V|.  In fp32 (u = 2^-24): a score's
+    products and their sum are off by (D + 2) u of the products' magnitudes, the score
+    times log2 e by 3 u of its distance from the maximum, exp2 by 2 u (a unit in the
+    last place): each moves a weight by as much, and again through the sum; the sums
+    of `keys` weights and weighted values, in any order, by keys u each, and the
+    division by 2 u."""
+
+    exact, weighted, top, products = reference
+    actual = actual.cpu()
+    dtype = actual.dtype
+    actual = actual.double()
+    empty = torch.isnan(exact)
+    assert torch.equal(torch.isnan(actual), empty)
+    u = 2.0**-24
+    weights = 2 * ((exact.shape[-1] + 2) * u * products + 3 * u * top + 2 * u) + 2 * keys * u + 2 * u
+    bound = weighted * weights
+    if dtype == torch.float32:
+        bound = bound + u * exact.abs()
+    else:
+        h = torch.finfo(dtype).eps / 2
+        bound = bound + 2 * h * weighted + h * exact.abs() + h * bound
+        if dtype == torch.float16:
+            bound = bound + keys * 2.0**-25 * 2 * weighted.abs().amax() + 2.0**-25
+    bound, error = bound[~empty], (actual - exact)[~empty].abs()
+    assert (error <= bound).all(), float((error / bound).max())
+
+
+def paged(buffer, page_tokens, g, extra=3):
+    """Pool and table whose gather is ``buffer`` (capacity padded to whole pages with
+    NaN); the pages that no sequence owns hold NaN."""
+
+    batch, capacity = buffer[0].shape[:2]
+    pages = -(-capacity // page_tokens)
+    order = torch.randperm(batch * pages + extra, generator=g)[: batch * pages].view(batch, pages)
+    pools = []
+    for side in buffer:
+        pool = torch.full((batch * pages + extra, page_tokens, *side.shape[2:]), NAN, dtype=side.dtype)
+        whole = torch.full((batch, pages * page_tokens, *side.shape[2:]), NAN, dtype=side.dtype)
+        whole[:, :capacity] = side
+        pool[order.view(-1)] = whole.view(batch * pages, page_tokens, *side.shape[2:])
+        pools.append(pool)
+    return *pools, order.to(torch.int32)
+
+
+def tree_inputs(g, batch, q_heads, kv_heads, head_dim, nodes, capacity, dtype, lengths):
+    """Queries and caches; NaN and infinities in the rows behind the nodes."""
+
+    query = torch.randn(batch, q_heads, nodes, head_dim, generator=g).to(dtype)
+    key, value = (torch.randn(batch, capacity, kv_heads, head_dim, generator=g).to(dtype) for _ in range(2))
+    for b, length in enumerate(lengths):
+        end = max(0, length) + nodes
+        key[b, end:], value[b, end:] = NAN, INF
+        value[b, end + 1 :: 2] = NAN
+    return query, key, value, torch.tensor(lengths)
+
+
+TREE_CASES = [
+    # q_heads, kv_heads, head_dim, nodes, capacity, lengths
+    (14, 2, 64, 8, 700, [600, 13]),
+    (14, 2, 64, 16, 1100, [0, 1, 63, 1000]),
+    (14, 2, 64, 1, 300, [299, 0]),
+    (14, 2, 64, 33, 200, [130, 64]),
+    (14, 2, 64, 64, 420, [350, 17]),
+    (4, 2, 128, 5, 300, [255, 100, 40]),
+    (32, 8, 128, 7, 200, [129, 0]),
+    (8, 8, 64, 16, 128, [112]),
+    (2, 1, 64, 130, 400, [200, 64]),
+    (20, 1, 64, 3, 200, [100]),
+    (40, 1, 128, 9, 150, [100]),
+    (6, 2, 80, 11, 150, [90, 20]),
+    (5, 1, 72, 4, 150, [65]),
+    (12, 1, 256, 6, 150, [77]),
+    (6, 3, 256, 40, 150, [77]),
+    (9, 3, 33, 10, 150, [70, 3]),
+    (3, 1, 1, 4, 50, [20]),
+    (4, 4, 200, 17, 90, [64]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("case", TREE_CASES)
+def test_tree_attention(gpu, case, dtype):
+    q_heads, kv_heads, head_dim, nodes, capacity, lengths = case
+    announce(f"tree attention {case} {dtype}")
+    g = generator(1000 * q_heads + 10 * nodes + head_dim)
+    query, key, value, lengths = tree_inputs(g, len(lengths), q_heads, kv_heads, head_dim, nodes, capacity, dtype,
+                                             lengths)
+    tree = random_tree(nodes, g, len(lengths))
+    scale = head_dim**-0.5
+    reference = tree_reference(query, key, value, lengths, tree, None, scale)
+    out = backends.hip_tree_attention(query.to(gpu), key.to(gpu), value.to(gpu), lengths.to(gpu), tree.to(gpu),
+                                      scale=scale)
+    assert out.shape == query.shape and out.dtype == dtype
+    assert_tree_close(out, reference, int(lengths.max()) + nodes)
+    for page_tokens in (16, 64):
+        key_pool, value_pool, table = paged((key, value), page_tokens, g)
+        again = backends.hip_paged_tree_attention(query.to(gpu), key_pool.to(gpu), value_pool.to(gpu), table.to(gpu),
+                                                  lengths.int().to(gpu), tree.to(gpu), scale=scale)
+        assert_tree_close(again, reference, int(lengths.max()) + nodes)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kind", ["-inf", "lowest", "random", "all -inf", "all lowest", "short"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (4, 1, 80)])
+def test_tree_attention_with_a_mask(gpu, kind, dtype, heads):
+    q_heads, kv_heads, head_dim = heads
+    announce(f"tree attention mask {kind} {dtype} {heads}")
+    g = generator(5)
+    nodes, capacity = 9, 330
+    query, key, value, lengths = tree_inputs(g, 3, q_heads, kv_heads, head_dim, nodes, capacity, dtype, [310, 64, 0])
+    low = -INF if "-inf" in kind else torch.finfo(dtype).min
+    rows = 200 if kind == "short" else capacity
+    mask = torch.zeros(3, 1, 1, rows, dtype=dtype)
+    if kind == "random":
+        mask = (torch.randn(3, 1, 1, rows, generator=g) * 3).to(dtype)
+        mask[:, :, :, ::7] = -INF
+    elif kind.startswith("all"):
+        mask[0] = low
+        mask[1, :, :, :60] = low
+    elif kind == "short":
+        mask[0, :, :, 70:90] = low
+    else:
+        mask[0, :, :, :133] = low
+        mask[1, :, :, :64] = low  # nothing of the sequence is left
+    hidden = mask == -INF
+    for b in range(3):  # what a masked row holds is not seen
+        key[b, :rows][hidden[b, 0, 0]] = NAN
+        value[b, :rows][hidden[b, 0, 0]] = INF
+    tree = random_tree(nodes, g)
+    scale = head_dim**-0.5
+    reference = tree_reference(query, key, value, lengths, tree, mask, scale)
+    args = [t.to(gpu) for t in (query, key, value, lengths, tree, mask)]
+    assert_tree_close(backends.hip_tree_attention(*args, scale=scale), reference, capacity)
+    # The same from an fp32 mask that is a strided view.
+    wide = torch.zeros(3, 1, 1, 2 * rows)
+    wide[..., ::2] = mask.float()
+    args[5] = wide.to(gpu)[..., ::2]
+    assert_tree_close(backends.hip_tree_attention(*args, scale=scale), reference, capacity)
+    key_pool, value_pool, table = paged((key, value), 32, g)
+    out = backends.hip_paged_tree_attention(args[0], key_pool.to(gpu), value_pool.to(gpu), table.to(gpu), args[3],
+                                            args[4], mask.to(gpu), scale=scale)
+    assert_tree_close(out, reference, capacity)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("head_dim", [64, 128, 40])
+@pytest.mark.parametrize("nodes,length", [(12, 61), (70, 100), (3, 0)])
+def test_tree_attention_keeps_what_a_node_does_not_see_from_it(gpu, nodes, length, head_dim, dtype):
+    announce(f"tree attention unseen NaN {nodes} {length} {head_dim} {dtype}")
+    g = generator(17)
+    query, key, value, lengths = tree_inputs(g, 1, 6, 2, head_dim, nodes, length + nodes + 5, dtype, [length])
+    tree = random_tree(nodes, g)
+    tree[0, 0] = False  # node 0 sees the sequence only: nothing where that is empty
+    bad = nodes // 2
+    args = [query.to(gpu), key.to(gpu), value.to(gpu), lengths.to(gpu), tree.to(gpu)]
+    clean = backends.hip_tree_attention(*args, scale=0.1).cpu()
+    for fill in (NAN, INF, -INF):
+        for side in (1, 2):
+            dirty = list(args)
+            dirty[side] = args[side].clone()
+            dirty[side][0, length + bad, 0] = fill
+            out = backends.hip_tree_attention(*dirty, scale=0.1).cpu()
+            sees = tree[:, bad].clone()
+            assert torch.isfinite(out[:, 3:][:, :, 1:]).all()  # the other KV head's queries
+            assert torch.equal(out[:, 3:, 1:], clean[:, 3:, 1:])
+            assert torch.equal(out[:, :3, ~sees].nan_to_num(7.0), clean[:, :3, ~sees].nan_to_num(7.0))
+            if side == 2:
+                expected = torch.full_like(out[:, :3, sees], fill)
+                assert torch.equal(torch.isnan(out[:, :3, sees]), torch.isnan(expected))
+                if fill == fill:
+                    assert torch.equal(out[:, :3, sees], expected)
+
+
+def test_tree_attention_layouts(gpu):
+    announce("tree attention layouts")
+    g = generator(3)
+    batch, q_heads, kv_heads, head_dim, nodes, capacity = 3, 14, 2, 64, 10, 200
+    for dtype in (torch.bfloat16, torch.float32):
+        query, key, value, lengths = tree_inputs(g, batch, q_heads, kv_heads, head_dim, nodes, capacity, dtype,
+                                                 [100, 7, 150])
+        tree = random_tree(nodes, g, batch)
+        reference = tree_reference(query, key, value, lengths, tree, None, 0.125)
+        base = [t.to(gpu) for t in (query, key, value, lengths, tree)]
+        want = backends.hip_tree_attention(*base, scale=0.125)
+        assert_tree_close(want, reference, 200)
+
+        def same(query=base[0], key=base[1], value=base[2], lengths=base[3], tree=base[4]):
+            out = backends.hip_tree_attention(query, key, value, lengths, tree, scale=0.125)
+            assert out.shape == want.shape
+            assert_bitwise_equal(out, want)
+
+        def unaligned(query=base[0], key=base[1], value=base[2]):
+            out = backends.hip_tree_attention(query, key, value, base[3], base[4], scale=0.125)
+            assert_tree_close(out, reference, 200)
+
+        same(query=base[0].transpose(1, 2).contiguous().transpose(1, 2))  # [B, T, H, D]
+        same(lengths=base[3].int())
+        same(tree=base[4].transpose(1, 2).contiguous().transpose(1, 2))
+        # [B, KVH, Cap, D] caches, and rows with room between them.
+        same(key=base[1].permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3),
+             value=base[2].permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3))
+        roomy = [torch.full((batch, capacity + 3, kv_heads, 2 * head_dim), NAN, dtype=dtype, device=gpu)
+                 for _ in range(2)]
+        for room, side in zip(roomy, base[1:3]):
+            room[:, :capacity, :, :head_dim] = side
+        same(key=roomy[0][:, :capacity, :, :head_dim], value=roomy[1][:, :capacity, :, :head_dim])
+        # Rows that start on any element.
+        odd = [torch.full((batch, capacity, kv_heads, head_dim + 3), NAN, dtype=dtype, device=gpu) for _ in range(2)]
+        for room, side in zip(odd, base[1:3]):
+            room[..., 1 : head_dim + 1] = side
+        unaligned(key=odd[0][..., 1 : head_dim + 1], value=odd[1][..., 1 : head_dim + 1])
+        odd_query = torch.full((batch, q_heads, nodes, head_dim + 1), NAN, dtype=dtype, device=gpu)
+        odd_query[..., 1:] = base[0]
+        unaligned(query=odd_query[..., 1:])
+        # One query for all sequences, as an expanded view.
+        one = base[0][:1].expand(batch, -1, -1, -1)
+        out = backends.hip_tree_attention(one, *base[1:], scale=0.125)
+        assert_tree_close(out, tree_reference(query[:1].expand(batch, -1, -1, -1), key, value, lengths, tree, None, 0.125),
+                          200)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tree_attention_lengths_at_and_past_the_ends(gpu, dtype):
+    # Nodes past the capacity were not stored; a negative length is none.
+    announce(f"tree attention lengths {dtype}")
+    g = generator(8)
+    capacity, nodes, lengths = 100, 6, [97, 100, 105, -4, 94, 2**31 + 5]
+    query, key, value, _ = tree_inputs(g, len(lengths), 4, 2, 64, nodes, capacity, dtype, [capacity] * len(lengths))
+    tree = random_tree(nodes, g)
+    lengths = torch.tensor(lengths)
+    reference = tree_reference(query, key, value, lengths, tree, None, 0.125)
+    args = [t.to(gpu) for t in (query, key, value, lengths, tree)]
+    assert_tree_close(backends.hip_tree_attention(*args, scale=0.125), reference, capacity)
+
+
+def test_tree_attention_chain_and_single_tokens(gpu):
+    announce("tree attention chain")
+    g = generator(9)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        query, key, value, lengths = tree_inputs(g, 5, 14, 2, 64, 21, 400, dtype, [300, 5, 0, 64, 377])
+        args = [t.to(gpu) for t in (query, key, value, lengths)]
+        out = backends.hip_tree_attention(*args, None, scale=0.125)
+        assert_tree_close(out, tree_reference(query, key, value, lengths, None, None, 0.125), 400)
+        # One node is decode attention over a length that counts it.
+        one = backends.hip_tree_attention(args[0][:, :, :1], *args[1:], None, scale=0.125)
+        assert_tree_close(one, tree_reference(query[:, :, :1], key, value, lengths, None, None, 0.125), 400)
+        decode = backends.hip_decode_attention(args[0][:, :, :1], args[1], args[2], args[3] + 1, None, scale=0.125)
+        assert (one.float() - decode.float()).abs().max() <= 2e-2
+
+
+def test_tree_attention_of_many_sequences(gpu):
+    announce("tree attention 150 sequences")
+    g = generator(10)
+    lengths = torch.randint(0, 40, (150,), generator=g).tolist()
+    lengths[77] = 300
+    for dtype in (torch.bfloat16, torch.float32):
+        query, key, value, lengths_t = tree_inputs(g, 150, 4, 2, 64, 3, 310, dtype, lengths)
+        tree = random_tree(3, g, 150)
+        args = [t.to(gpu) for t in (query, key, value, lengths_t, tree)]
+        out = backends.hip_tree_attention(*args, scale=0.125)
+        assert_tree_close(out, tree_reference(query, key, value, lengths_t, tree, None, 0.125), 303)
+
+
+def test_tree_attention_of_large_and_far_scores(gpu):
+    # The running maximum moves over many tiles, by more than exp's range.
+    announce("tree attention large scores")
+    g = generator(11)
+    for dtype in (torch.bfloat16, torch.float32):
+        query, key, value, lengths = tree_inputs(g, 2, 4, 2, 64, 8, 900, dtype, [880, 880])
+        ramp = torch.linspace(0, 1, 900).view(1, -1, 1, 1)
+        key[0] = (query[0, 0, 0].float() * ramp[0] * 2).to(dtype)
+        key[1] = (query[1, 0, 0].float() * (1 - ramp[0]) * 2).to(dtype)
+        tree = random_tree(8, g)
+        args = [t.to(gpu) for t in (query, key, value, lengths, tree)]
+        out = backends.hip_tree_attention(*args, scale=1.0)
+        assert_tree_close(out, tree_reference(query, key, value, lengths, tree, None, 1.0), 900)
+
+
+def test_tree_attention_repeats_bit_for_bit_on_streams_and_in_graphs(gpu):
+    announce("tree attention streams and graphs")
+    g = generator(12)
+    query, key, value, lengths = tree_inputs(g, 4, 14, 2, 64, 16, 2100, torch.bfloat16, [2000, 1500, 3, 700])
+    tree = random_tree(16, g, 4).to(gpu)
+    args = [t.to(gpu) for t in (query, key, value, lengths)]
+    want = backends.hip_tree_attention(*args, tree, scale=0.125)
+    for _ in range(3):
+        assert_bitwise_equal(backends.hip_tree_attention(*args, tree, scale=0.125), want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for stream in streams * 2:
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            outs.append(backends.hip_tree_attention(*args, tree, scale=0.125))
+    torch.cuda.synchronize()
+    for out in outs:
+        assert_bitwise_equal(out, want)
+    static = [t.clone() for t in args]
+    workspace = _native.DeviceWorkspace(gpu)
+    backends.hip_tree_attention(*static, tree, scale=0.125, workspace=workspace)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = backends.hip_tree_attention(*static, tree, scale=0.125, workspace=workspace)
+    for turn in range(4):
+        static[0].copy_(args[0].roll(turn, 1))
+        static[3].copy_((args[3] + 5 * turn).clamp_max(2000))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_bitwise_equal(out, backends.hip_tree_attention(static[0], *args[1:3], static[3], tree, scale=0.125))
+
+
+def test_tree_attention_refuses(gpu):
+    q = torch.zeros(2, 4, 3, 64, device=gpu, dtype=torch.bfloat16)
+    kv = torch.zeros(2, 32, 2, 64, device=gpu, dtype=torch.bfloat16)
+    n = torch.zeros(2, device=gpu, dtype=torch.int64)
+    tree = torch.ones(3, 3, device=gpu, dtype=torch.bool)
+    mask = torch.zeros(2, 1, 1, 32, device=gpu)
+    run = backends.hip_tree_attention
+    for bad in (
+        lambda: run(q[0], kv, kv, n, tree, scale=1.0),
+        lambda: run(q, kv[0], kv[0], n, tree, scale=1.0),
+        lambda: run(q, kv, kv[:, :16], n, tree, scale=1.0),
+        lambda: run(q, kv[:1], kv[:1], n, tree, scale=1.0),
+        lambda: run(q[:, :3], kv, kv, n, tree, scale=1.0),
+        lambda: run(q[..., :32], kv, kv, n, tree, scale=1.0),
+        lambda: run(q.half(), kv, kv, n, tree, scale=1.0),
+        lambda: run(q.double(), kv.double(), kv.double(), n, tree, scale=1.0),
+        lambda: run(q, kv, kv, n.float(), tree, scale=1.0),
+        lambda: run(q, kv, kv, n[:1], tree, scale=1.0),
+        lambda: run(q, kv, kv, n, tree.float(), scale=1.0),
+        lambda: run(q, kv, kv, n, tree[:2], scale=1.0),
+        lambda: run(q, kv, kv, n, tree.expand(3, 3, 3), scale=1.0),
+        lambda: run(q, kv, kv, n, tree.cpu(), scale=1.0),
+        lambda: run(q, kv, kv, n, tree, mask.long(), scale=1.0),
+        lambda: run(q, kv, kv, n, tree, mask[:1], scale=1.0),
+        lambda: run(q, kv, kv, n, tree, torch.zeros(2, 1, 1, 33, device=gpu), scale=1.0),
+        lambda: run(q, kv, kv, n, tree, scale=0.0),
+        lambda: run(q, kv, kv, n, tree, scale=NAN),
+        lambda: run(q.transpose(2, 3), kv[..., :3], kv[..., :3], n, None, scale=1.0),
+        lambda: run(q, kv, kv.transpose(1, 2).contiguous().transpose(1, 2), n, tree, scale=1.0),
+        lambda: backends.hip_paged_tree_attention(q, kv, kv, torch.zeros(2, 2, device=gpu), n, tree, scale=1.0),
+        lambda: backends.hip_paged_tree_attention(q, kv, kv, torch.zeros(2, 0, device=gpu, dtype=torch.int32), n, tree,
+                                                  scale=1.0),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+    assert run(q[:0], kv[:0], kv[:0], n[:0], tree, scale=1.0).shape == (0, 4, 3, 64)
+    assert run(q[:, :, :0], kv, kv, n, None, scale=1.0).shape == (2, 4, 0, 64)
+
+
+# ---- verification -------------------------------------------------------------------
+
+
+def verify_reference(tokens, target, uniforms, parents=None, draft=None):
+    """The documented walk, a node at a time in 64 bits; also how near the closest
+    comparison came to its border, relative to its sides."""
+
+    batch, nodes, vocab = target.shape
+    paths, emitted, counts = [], [], []
+    for b in range(batch):
+        up = list(range(-1, nodes - 1)) if parents is None else parents[b].tolist()
+        path = [0]
+        while True:
+            node = path[-1]
+            p = target[b, node].double().nan_to_num(0.0).clamp_min(0)
+            w, m, mass, follows = p.clone(), 1.0, 0.0, None
+            for c in (c for c in range(node + 1, nodes) if up[c] == node):
+                x, u = int(tokens[b, c]), float(uniforms[b, c])
+                chance = float(w[x]) if 0 <= x < vocab else 0.0
+                if draft is None:
+                    accepted = u * m < chance and chance > 0
+                else:
+                    accepted = u * m * (float(draft[b, node, x]) if 0 <= x < vocab else 0.0) < chance
+                if accepted:
+                    follows = c
+                    break
+                if draft is None:
+                    m -= chance
+                    if 0 <= x < vocab:
+                        w[x] = 0.0
+                else:
+                    mass += m
+                    w = (p - mass * draft[b, node].double()).clamp_min(0)
+                    m = float(w.sum())
+            if follows is None:
+                break
+            path.append(follows)
+        if not float(w.sum()) > 0:
+            w = p
+        sums = w.cumsum(0)
+        drawn = int((sums <= float(uniforms[b, 0]) * sums[-1]).sum()) if float(sums[-1]) > 0 else -1
+        fill = [-1] * (nodes - len(path))
+        paths.append(path + fill)
+        emitted.append([int(tokens[b, c]) for c in path[1:]] + [drawn] + fill)
+        counts.append(len(path))
+    return tuple(torch.tensor(v) for v in (paths, emitted, counts))
+
+
+def check_verify(gpu, tokens, target, uniforms, parents=None, draft=None):
+    want = verify_reference(tokens, target, uniforms, parents, draft)
+    got = backends.hip_verify_tokens(tokens.to(gpu), target.to(gpu), uniforms.to(gpu),
+                                     parents=None if parents is None else parents.to(gpu),
+                                     draft_probs=None if draft is None else draft.to(gpu))
+    for a, b in zip(got, want):
+        assert a.dtype == torch.int64
+        assert torch.equal(a.cpu(), b)
+    return want
+
+
+def random_parents(batch, nodes, g, back=4):
+    parents = torch.full((batch, nodes), -1)
+    for c in range(1, nodes):
+        parents[:, c] = torch.randint(max(0, c - back), c, (batch,), generator=g)
+    return parents
+
+
+def probabilities(g, *shape, dtype=torch.float32, sharp=3.0):
+    return torch.softmax(torch.randn(*shape, generator=g) * sharp, -1).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("batch,nodes,vocab", [(1, 5, 151936), (3, 1, 1000), (2, 9, 1024), (7, 4, 1025), (4, 17, 33),
+                                               (2, 3, 1), (5, 2, 4099), (40, 6, 2048), (2, 70, 300)])
+def test_verify_chains(gpu, batch, nodes, vocab, dtype):
+    announce(f"verify chains {batch} {nodes} {vocab} {dtype}")
+    g = generator(vocab + nodes)
+    for turn in range(3):
+        logits = torch.randn(batch, nodes, vocab, generator=g) * 3
+        target = torch.softmax(logits, -1).to(dtype)
+        draft = torch.softmax(logits + 0.7 * torch.randn(batch, nodes, vocab, generator=g), -1).to(dtype)[:, : nodes - 1]
+        tokens = torch.zeros(batch, nodes, dtype=torch.int64)
+        if nodes > 1:
+            tokens[:, 1:] = torch.multinomial(draft.float().reshape(-1, vocab), 1, generator=g).view(batch, -1)
+        check_verify(gpu, tokens, target, torch.rand(batch, nodes, generator=g), draft=draft)
+        check_verify(gpu, tokens, target, torch.rand(batch, nodes, generator=g))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("with_draft", [False, True])
+@pytest.mark.parametrize("batch,nodes,vocab", [(4, 12, 50), (3, 64, 2000), (2, 65, 1100), (2, 200, 40), (1, 30, 151936)])
+def test_verify_trees(gpu, batch, nodes, vocab, with_draft, dtype):
+    announce(f"verify trees {batch} {nodes} {vocab} {with_draft} {dtype}")
+    g = generator(nodes)
+    for back in (2, 8, nodes):
+        parents = random_parents(batch, nodes, g, back)
+        target, draft = (probabilities(g, batch, nodes, vocab, dtype=dtype) for _ in range(2))
+        draft = ((draft.float() + target.float()) / 2).to(dtype)[:, : nodes - 1]
+        at = parents.clamp_min(0).clamp_max(nodes - 2)
+        rows = draft.float()[torch.arange(batch).unsqueeze(1), at]
+        tokens = torch.multinomial(rows.view(-1, vocab), 1, generator=g).view(batch, nodes)
+        check_verify(gpu, tokens, target, torch.rand(batch, nodes, generator=g), parents, draft if with_draft else None)
+
+
+def test_verify_at_borders(gpu):
+    announce("verify borders")
+    # Whole multiples of powers of two: every sum and product is exact, ties are real.
+    vocab, nodes = 4096, 3
+    target = torch.full((6, nodes, vocab), 1 / vocab)
+    draft = torch.full((6, nodes - 1, vocab), 1 / vocab)
+    draft[:, :, :2] = torch.tensor([2 / vocab, 0.0])
+    tokens = torch.tensor([[9, 0, 5]] * 6)
+    uniforms = torch.tensor([[0.0, 0.5, 0.0], [0.5, 0.499, 0.99], [0.25, 0.0, 0.0], [0.999, 0.5, 0.5],
+                             [1 - 2**-24, 0.0, 0.5], [0.75, 0.75, 0.75]])
+    want = check_verify(gpu, tokens, target, uniforms, draft=draft)
+    assert want[2].tolist() == [1, 3, 3, 1, 3, 1]  # u q < p, not <=
+    assert want[1][0, 0] == 1  # only token 1 is left
+    assert want[1][1].tolist() == [0, 5, vocab // 2]  # the first sum past one half
+    # Without a draft: u < p.
+    want = check_verify(gpu, tokens, target, torch.tensor([[0.5, 1 / vocab, 0.0], [0.0, 0.0, 1 / vocab]] * 3))
+    assert want[2].tolist() == [1, 2] * 3
+    assert want[1][0, 0] == vocab // 2  # of the 4095 that are left
+
+
+def test_verify_odd_probabilities(gpu):
+    announce("verify odd probabilities")
+    g = generator(2)
+    batch, nodes, vocab = 8, 4, 1500
+    target = probabilities(g, batch, nodes, vocab)
+    draft = probabilities(g, batch, nodes - 1, vocab)
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=g)
+    uniforms = torch.rand(batch, nodes, generator=g)
+    # Tokens outside the vocabulary are refused, NaN has no weight, a draft that is the target leaves none.
+    tokens[0, 1], tokens[1, 1], tokens[2, 2], tokens[3, 1] = -1, vocab, 2**40, -(2**40)
+    target[4, 0, 3:7] = NAN
+    tokens[4, 1] = 4
+    draft[5] = target[5, : nodes - 1]
+    draft[5, :, 17] = target[5, : nodes - 1, 17] = 0.0
+    tokens[5, 1:] = 17  # never accepted, and then nothing is left: the target is drawn from
+    target[6] = 0.0  # no probability at all: -1
+    target[7, :, : vocab - 1] = 0.0
+    target[7, :, vocab - 1] = 1.0
+    for d in (None, draft):
+        want = check_verify(gpu, tokens, target, uniforms, draft=d)
+        assert want[1][6, 0] == -1
+        assert want[2][:4].tolist()[:2] == [1, 1]
+
+
+def test_verify_padding_and_duplicates(gpu):
+    announce("verify padding and duplicates")
+    g = generator(4)
+    batch, nodes, vocab = 6, 7, 20
+    target = probabilities(g, batch, nodes, vocab, sharp=1.0)
+    # A node that is no earlier one's child is never reached: -1, itself, a later one, far ones.
+    parents = torch.tensor([[-1, 0, 0, 0, 0, 0, 0], [5, -1, 0, 2, -1, 2, 2], [0, 1, 2, 3, 4, 5, 6],
+                            [0, 0, 1, 2, 6, 6, 5], [-1, -1, -1, -1, -1, -1, -1], [-1, 2**40, 0, -(2**40), 2, 4, 7]])
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=g)
+    tokens[0] = torch.tensor([1, 3, 3, 3, 5, 5, 3])  # one token three times among the children
+    target[0, 0] = 0.0
+    target[0, 0, 3], target[0, 0, 5], target[0, 0, 11] = 0.25, 0.25, 0.5
+    draft = probabilities(g, batch, nodes - 1, vocab, sharp=1.0)
+    for turn in range(8):
+        uniforms = torch.rand(batch, nodes, generator=g)
+        check_verify(gpu, tokens, target, uniforms, parents)
+        check_verify(gpu, tokens, target, uniforms, parents, draft)
+
+
+def test_verify_widest_trees(gpu):
+    announce("verify 1024 nodes")
+    g = generator(6)
+    target = probabilities(g, 1, 1024, 700, sharp=1.0)
+    uniforms = torch.rand(1, 1024, generator=g)
+    star = torch.zeros(1, 1024, dtype=torch.int64)
+    star[0, 0] = -1
+    tokens = torch.randint(0, 700, (1, 1024), generator=g)
+    check_verify(gpu, tokens, target, uniforms, star)
+    # A chain of all of them, accepted throughout.
+    sure = torch.zeros(1, 1024, 700)
+    sure[0, torch.arange(1023), tokens[0, 1:]] = 1.0
+    sure[0, 1023, 699] = 1.0
+    want = check_verify(gpu, tokens, sure, uniforms)
+    assert want[2].item() == 1024 and want[1][0, -1] == 699
+
+
+def test_verify_layouts_streams_and_graphs(gpu):
+    announce("verify layouts")
+    g = generator(7)
+    batch, nodes, vocab = 5, 6, 5003
+    target, draft = probabilities(g, batch, nodes, vocab), probabilities(g, batch, nodes - 1, vocab)
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=g)
+    uniforms = torch.rand(batch, nodes, generator=g)
+    want = check_verify(gpu, tokens, target, uniforms, draft=draft)
+    wide = torch.full((batch, nodes + 1, vocab + 9), NAN, device=gpu)
+    wide[:, :nodes, 3 : vocab + 3] = target.to(gpu)
+    views = (tokens.to(gpu).t().contiguous().t(), wide[:, :nodes, 3 : vocab + 3], uniforms.to(gpu).t().contiguous().t())
+    workspace = _native.DeviceWorkspace(gpu)
+    for _ in range(3):
+        got = backends.hip_verify_tokens(*views, draft_probs=draft.to(gpu), workspace=workspace)
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    draft_gpu, results = draft.to(gpu), []
+    for stream in streams * 2:
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            results.append(backends.hip_verify_tokens(*views, draft_probs=draft_gpu))
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+    static = [tokens.to(gpu), target.to(gpu), uniforms.to(gpu)]
+    backends.hip_verify_tokens(*static, draft_probs=draft_gpu, workspace=workspace)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = backends.hip_verify_tokens(*static, draft_probs=draft_gpu, workspace=workspace)
+    for turn in range(4):
+        static[2].copy_(torch.rand(batch, nodes, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        expected = verify_reference(tokens, target, static[2].cpu(), None, draft)
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, expected))
+
+
+def test_verify_gives_the_targets_distribution(gpu):
+    """The first emitted token of 2^18 independent steps, with children drawn from the draft.
+
+    For a token of probability p the count is binomial; 6 standard deviations, plus 2^-12 of
+    the steps for fp32 probabilities that do not sum to 1 exactly, are passed by chance about
+    once in 10^8 tokens."""
+
+    announce("verify distribution")
+    g = generator(21)
+    steps, vocab, children = 2**18, 12, 3
+    p, q = (torch.softmax(torch.randn(vocab, generator=g), -1) for _ in range(2))
+    nodes = 1 + children
+    tokens = torch.zeros(steps, nodes, dtype=torch.int64)
+    tokens[:, 1:] = torch.multinomial(q, steps * children, replacement=True, generator=g).view(steps, children)
+    parents = torch.tensor([-1] + [0] * children).expand(steps, -1)
+    uniforms = torch.rand(steps, nodes, generator=g)
+    target = p.expand(steps, nodes, vocab).to(gpu)
+    draft = q.expand(steps, nodes - 1, vocab).to(gpu)
+    for d in (None, draft):
+        counts = torch.zeros(vocab, dtype=torch.int64)
+        for first in range(0, steps, 2**15):
+            part = slice(first, first + 2**15)
+            emitted = backends.hip_verify_tokens(tokens[part].to(gpu), target[part], uniforms[part].to(gpu),
+                                                 parents=parents[part].to(gpu),
+                                                 draft_probs=None if d is None else d[part])[1]
+            counts += torch.bincount(emitted[:, 0].cpu(), minlength=vocab)
+        deviation = (steps * p.double() * (1 - p.double())).sqrt()
+        assert ((counts - steps * p.double()).abs() <= 6 * deviation + steps * 2.0**-12).all()
+
+
+def test_verify_refuses(gpu):
+    tokens = torch.zeros(2, 3, device=gpu, dtype=torch.int64)
+    target, uniforms = torch.ones(2, 3, 5, device=gpu), torch.zeros(2, 3, device=gpu)
+    run = backends.hip_verify_tokens
+    for bad in (
+        lambda: run(tokens.int(), target, uniforms),
+        lambda: run(tokens[0], target, uniforms),
+        lambda: run(tokens[:, :0], target[:, :0], uniforms[:, :0]),
+        lambda: run(tokens, target[:, :2], uniforms),
+        lambda: run(tokens, target[..., :0], uniforms),
+        lambda: run(tokens, target.double(), uniforms),
+        lambda: run(tokens, target, uniforms.double()),
+        lambda: run(tokens, target, uniforms[:1]),
+        lambda: run(tokens, target, uniforms, parents=tokens.int()),
+        lambda: run(tokens, target, uniforms, parents=tokens[:, :2]),
+        lambda: run(tokens, target, uniforms, draft_probs=target),
+        lambda: run(tokens, target, uniforms, draft_probs=target[:, :2].half()),
+        lambda: run(tokens, target, uniforms.cpu()),
+        lambda: run(torch.zeros(1, 1025, device=gpu, dtype=torch.int64), torch.ones(1, 1025, 1, device=gpu),
+                    torch.zeros(1, 1025, device=gpu)),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+    assert [t.shape for t in run(tokens[:0], target[:0], uniforms[:0])] == [(0, 3), (0, 3), (0,)]
+
+
+# ---- commit -------------------------------------------------------------------------
+
+
+def commit_reference(buffers, lengths, path, counts):
+    """Buffers [B, Cap, H, D] of one layer after the moves."""
+
+    moved = [buffer.clone() for buffer in buffers]
+    capacity = buffers[0].shape[1]
+    for b in range(path.shape[0]):
+        n = int(lengths[b])
+        for j in range(int(counts[b])):
+            if j < int(path[b, j]) and n + int(path[b, j]) < capacity:
+                for old, new in zip(buffers, moved):
+                    new[b, n + j] = old[b, n + int(path[b, j])]
+    return moved
+
+
+def random_paths(g, batch, nodes):
+    path, counts = torch.full((batch, nodes), -1), torch.randint(1, nodes + 1, (batch,), generator=g)
+    for b in range(batch):
+        rest = torch.randperm(nodes - 1, generator=g)[: int(counts[b]) - 1] + 1
+        path[b, : int(counts[b])] = torch.cat([torch.zeros(1, dtype=torch.int64), rest.sort().values])
+    return path, counts
+
+
+def bits(tensor):
+    return tensor.view({2: torch.int16, 4: torch.int32}[tensor.element_size()])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("layers,batch,nodes,heads,head_dim,capacity,page_tokens", [
+    (24, 3, 8, 2, 64, 100, 0), (2, 5, 64, 2, 64, 256, 64), (3, 2, 5, 3, 33, 64, 16), (1, 1, 1, 1, 1, 4, 0),
+    (100, 2, 6, 1, 8, 40, 0), (2, 2, 200, 16, 128, 512, 32), (1, 70, 3, 2, 80, 32, 16), (2, 1, 1024, 2, 6, 1100, 0)])
+def test_commit(gpu, layers, batch, nodes, heads, head_dim, capacity, page_tokens, dtype):
+    announce(f"commit {layers} {batch} {nodes} {heads} {head_dim} {page_tokens} {dtype}")
+    g = generator(layers + nodes)
+    whole = -(-capacity // max(1, page_tokens)) * max(1, page_tokens)
+    keys, values = ([torch.randn(batch, whole, heads, head_dim, generator=g).to(dtype) for _ in range(layers)]
+                    for _ in range(2))
+    lengths = torch.randint(0, capacity - nodes + 1, (layers, batch), generator=g)
+    path, counts = random_paths(g, batch, nodes)
+    table = None
+    if page_tokens:
+        order = torch.randperm(batch * whole // page_tokens, generator=g).view(batch, -1)
+        table = order.to(torch.int32).to(gpu)
+
+        def place(buffer):
+            pool = torch.empty(order.numel(), page_tokens, heads, head_dim, dtype=dtype)
+            pool[order.view(-1)] = buffer.view(order.numel(), page_tokens, heads, head_dim)
+            return pool.to(gpu)
+
+        def back(pool):
+            return pool.cpu()[order].reshape(batch, whole, heads, head_dim)
+    else:
+        def place(buffer):
+            return buffer.to(gpu)
+
+        def back(buffer):
+            return buffer.cpu()
+
+    on_gpu = [place(buffer) for buffer in keys + values]
+    handle = backends.KVLayers(on_gpu[:layers], on_gpu[layers:], block_table=table)
+    out = backends.hip_kv_commit(handle, lengths.to(gpu), path.to(gpu), counts.to(gpu))
+    assert torch.equal(out.cpu(), lengths + counts)
+    for layer in range(layers):
+        want = commit_reference([keys[layer], values[layer]], lengths[layer], path, counts)
+        for got, expected in zip((on_gpu[layer], on_gpu[layers + layer]), want):
+            assert torch.equal(bits(back(got)), bits(expected))
+
+
+def test_commit_forms_of_lengths(gpu):
+    announce("commit lengths")
+    g = generator(1)
+    buffers = [torch.randn(2, 20, 2, 8, generator=g).to(gpu) for _ in range(6)]
+    handle = backends.KVLayers(buffers[:3], buffers[3:])
+    path, counts = torch.tensor([[0, 1, 2], [0, 1, -1]], device=gpu), torch.tensor([3, 2], device=gpu)
+    one = torch.tensor([4, 17], device=gpu)
+    run = backends.hip_kv_commit
+    assert run(handle, one, path, counts).tolist() == [7, 19] and one.tolist() == [4, 17]
+    each = [one.clone() for _ in range(3)]
+    assert [t.tolist() for t in run(handle, each, path, counts)] == [[7, 19]] * 3
+    assert run(handle, [one] * 3, path, counts, out=each) is each
+    assert [t.tolist() for t in each] == [[7, 19]] * 3
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    assert run(handle, each, path, counts, out=each, overflow=flag) is each
+    assert [t.tolist() for t in each] == [[10, 21]] * 3 and flag.item() == 1  # past the capacity of 20
+    stacked = one.repeat(3, 1)
+    flag.zero_()
+    run(handle, stacked, path, counts, out=stacked, overflow=flag)
+    assert stacked.tolist() == [[7, 19]] * 3 and flag.item() == 0
+    # Counts outside the path, and none at all.
+    assert run(handle, one, path, torch.tensor([-3, 99], device=gpu)).tolist() == [4, 20]
+    before = [t.clone() for t in buffers]
+    assert run(handle, one, path, torch.zeros_like(counts)).tolist() == [4, 17]
+    assert all(torch.equal(a, b) for a, b in zip(before, buffers))
+    for bad in (
+        lambda: run(handle, one, path, counts, out=one),  # three layers read it
+        lambda: run(handle, [one] * 3, path, counts, out=[one, each[1], each[2]]),
+        lambda: run(handle, each, path, counts, out=[each[1], each[0], each[2]]),
+        lambda: run(handle, each, path, counts, out=[each[0], each[0], each[2]]),
+        lambda: run(handle, each[:2], path, counts),
+        lambda: run(handle, one.int(), path, counts),
+        lambda: run(handle, one[:1], path, counts),
+        lambda: run(handle, one, path.int(), counts),
+        lambda: run(handle, one, path[:1], counts),
+        lambda: run(handle, one, path[:, :0], counts),
+        lambda: run(handle, one, path, counts.int()),
+        lambda: run(handle, one, path, counts.cpu()),
+        lambda: run(handle, one, path, counts, overflow=torch.zeros(1, device=gpu)),
+        lambda: run(handle, one, path, counts, out=torch.zeros(5, dtype=torch.int64, device=gpu)[1:3:1].int()),
+        lambda: backends.KVLayers(buffers[:3], buffers[:3]),
+        lambda: backends.KVLayers(buffers[:3], buffers[3:5]),
+        lambda: backends.KVLayers([], []),
+        lambda: backends.KVLayers(buffers[:1], [buffers[1].half()]),
+        lambda: backends.KVLayers(buffers[:1], [buffers[1][:, :10]]),
+        lambda: backends.KVLayers([buffers[0].cpu()], [buffers[1].cpu()]),
+        lambda: backends.KVLayers(buffers[:1], buffers[1:2], block_table=torch.zeros(1, 1, device=gpu)),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+    lap = torch.zeros(7, dtype=torch.int64, device=gpu)
+    with pytest.raises(ValueError):  # views that overlap in part
+        run(handle, each, path, counts, out=[lap[0:2], lap[1:3], lap[4:6]])
+
+
+def test_commit_does_not_leave_the_cache(gpu):
+    announce("commit bounds")
+    # Entries that are no node, sources past the capacity, pages that are none of the pool's.
+    buffers = [torch.arange(2 * 16.0, device=gpu).view(2, 16, 1, 1).clone() for _ in range(2)]
+    handle = backends.KVLayers(buffers[:1], buffers[1:])
+    path = torch.tensor([[0, 3, 2**40, -(2**40)], [1, 2, 3, 3]], device=gpu)
+    lengths = torch.tensor([13, 2], device=gpu)
+    out = backends.hip_kv_commit(handle, lengths, path, torch.tensor([4, 3], device=gpu))
+    assert out.tolist() == [17, 5]
+    want = torch.arange(2 * 16.0).view(2, 16)
+    want[1, 2:5] = torch.tensor([19.0, 20.0, 21.0])
+    assert all(torch.equal(b.cpu().view(2, 16), want) for b in buffers)
+    for start in (-1, -(2**40), 16, 2**40):
+        backends.hip_kv_commit(handle, torch.tensor([start, start], device=gpu), path,
+                               torch.tensor([4, 3], device=gpu))
+        assert all(torch.equal(b.cpu().view(2, 16), want) for b in buffers)
+    pools = [torch.arange(3 * 16.0, device=gpu).view(3, 16, 1, 1).clone() for _ in range(2)]
+    table = torch.tensor([[1, 7], [-1, 2]], dtype=torch.int32, device=gpu)
+    handle = backends.KVLayers(pools[:1], pools[1:], block_table=table)
+    path = torch.tensor([[0, 2, 3, -1], [0, 2, 3, -1]], device=gpu)
+    backends.hip_kv_commit(handle, torch.tensor([13, 14], device=gpu), path, torch.tensor([3, 3], device=gpu))
+    want = torch.arange(3 * 16.0).view(3, 16)
+    want[1, 14] = want[1, 15]  # row 15 to 14 of the first sequence; its row 16 has no page
+    want[2, 0] = want[2, 1]  # row 17 to 16 of the second; row 15 has no page
+    assert all(torch.equal(p.cpu().view(3, 16), want) for p in pools)
+    out = backends.hip_paged_tree_attention(
+        torch.ones(2, 1, 4, 1, device=gpu), *pools, table, torch.tensor([10, 20], device=gpu), None, scale=1.0)
+    assert out.shape == (2, 1, 4, 1)
+
+
+# ---- together -----------------------------------------------------------------------
+
+
+def model_step(config, weights, state, tokens, depths, tree):
+    """Logits behind every node: the decoder's operators over ``state``, nodes stored
+    behind the sequences."""
+
+    from stateful_llm_compiler_hip.qwen2 import inverse_frequency
+
+    b = backends
+    batch, nodes = tokens.shape
+    h = b.hip_embedding(tokens, weights["embed_tokens.weight"])
+    start = state.positions(0)
+    cosine, sine = b.hip_rope_table(start.unsqueeze(1) + depths, inverse_frequency(config, tokens.device), h.dtype)
+
+    def heads(x, count):
+        return x.view(batch, nodes, count, config.head_dim).transpose(1, 2)
+
+    for layer in range(config.num_layers):
+        p = f"layers.{layer}."
+        x = b.hip_rms_norm(h, weights[p + "input_layernorm.weight"], epsilon=config.rms_norm_eps)
+        q, k, v = (b.hip_linear(x, weights[f"{p}self_attn.{n}_proj.weight"], weights[f"{p}self_attn.{n}_proj.bias"])
+                   for n in "qkv")
+        q, state = state.rope_store(layer, heads(q, config.num_heads), heads(k, config.num_kv_heads),
+                                    heads(v, config.num_kv_heads), cosine, sine, state.positions(layer))
+        a = state.tree_attention(layer, q, tree, groups=config.groups, scale=config.head_dim**-0.5)
+        a = a.transpose(1, 2).reshape(batch, nodes, config.hidden_size)
+        h = b.hip_add(h, b.hip_linear(a, weights[p + "self_attn.o_proj.weight"], None))
+        x = b.hip_rms_norm(h, weights[p + "post_attention_layernorm.weight"], epsilon=config.rms_norm_eps)
+        m = b.hip_swiglu(b.hip_linear(x, weights[p + "mlp.gate_proj.weight"], None),
+                         b.hip_linear(x, weights[p + "mlp.up_proj.weight"], None))
+        h = b.hip_add(h, b.hip_linear(m, weights[p + "mlp.down_proj.weight"], None))
+    h = b.hip_rms_norm(h, weights["norm.weight"], epsilon=config.rms_norm_eps)
+    return b.hip_linear(h, weights["embed_tokens.weight"], None)
+
+
+@pytest.mark.parametrize("page_tokens", [None, 16])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_drafted_steps_give_the_tokens_of_single_steps(gpu, page_tokens, in_place):
+    """Greedy decoding in steps on trees, some of whose nodes are right, gives what the
+    runtime gives one token at a time, in fp32."""
+
+    from dataclasses import replace
+
+    from stateful_llm_compiler_hip.qwen2 import Qwen2Config, causal_prefill_mask, init_weights
+    from stateful_llm_compiler_hip.runtime import Qwen2Runtime
+
+    announce(f"drafted steps {page_tokens} {in_place}")
+    config = Qwen2Config(hidden_size=128, intermediate_size=256, num_layers=3, num_heads=4, num_kv_heads=2,
+                         vocab_size=503)
+    weights = init_weights(config, seed=3, dtype=torch.float32, device=str(gpu), std=0.3)
+    batch, prompt, steps, capacity = 3, 11, 24, 64
+    rt = Qwen2Runtime(config, weights, capacity=capacity, dtype=torch.float32, device=str(gpu))
+    g = generator(5)
+    ids = torch.randint(0, config.vocab_size, (batch, prompt), generator=g).to(gpu)
+    mask = causal_prefill_mask(batch, prompt, device=gpu)
+    positions = torch.arange(prompt, device=gpu).expand(batch, -1).contiguous()
+    logits, state = rt.prefill(ids, mask, positions)
+    token = logits[:, -1].argmax(-1, keepdim=True)
+    single = [token]
+    for step in range(steps + 8):
+        zero = torch.zeros(batch, 1, 1, prompt + step + 1, device=gpu)
+        logits, state = rt.decode(token, zero, state)
+        token = logits[:, -1].argmax(-1, keepdim=True)
+        single.append(token)
+    single = torch.cat(single, 1).cpu()
+
+    if page_tokens:
+        rt = Qwen2Runtime(config, weights, capacity=capacity, dtype=torch.float32, device=str(gpu),
+                          page_tokens=page_tokens)
+    logits, state = rt.prefill(ids, mask, positions)
+    state = replace(state, in_place_lengths=in_place)
+    done = [[int(t)] for t in logits[:, -1].argmax(-1)]
+    parents = torch.tensor([-1, 0, 0, 1, 2, 2, 5, 6])
+    nodes = len(parents)
+    tree = torch.eye(nodes, dtype=torch.bool)
+    for c in range(1, nodes):
+        tree[c] |= tree[parents[c]]
+    depths = tree.sum(-1) - 1
+    taken = []
+    while min(len(d) for d in done) < steps:
+        # The branch 0, 2, 5, 6, 7 gets the right tokens up to each depth in turn, the rest wrong ones.
+        tokens = torch.randint(0, config.vocab_size, (batch, nodes), generator=g)
+        for b in range(batch):
+            right = (len(taken) + b) % 5
+            tokens[b, 0] = done[b][-1]
+            for depth, c in enumerate((2, 5, 6, 7), 1):
+                if depth <= right:
+                    tokens[b, c] = single[b, min(len(done[b]) - 1 + depth, single.shape[1] - 1)]
+        logits = model_step(config, weights, state, tokens.to(gpu), depths.to(gpu), tree.to(gpu))
+        sure = torch.nn.functional.one_hot(logits.argmax(-1), config.vocab_size).float()
+        path, emitted, counts = backends.hip_verify_tokens(
+            tokens.to(gpu), sure, torch.full((batch, nodes), 0.5, device=gpu),
+            parents=parents.expand(batch, -1).contiguous().to(gpu))
+        state = state.commit(path, counts)
+        for b in range(batch):
+            done[b] += emitted[b, : counts[b]].tolist()
+        taken += counts.tolist()
+    state.check_capacity()
+    for b in range(batch):
+        assert done[b][:steps] == single[b, :steps].tolist()
+        assert int(state.lengths[2][b]) == prompt + len(done[b]) - 1
+    assert max(taken) == 5 and min(taken) == 1  # paths of all lengths were taken
