@@ -1,0 +1,43 @@
+// Arguments of the tree attention kernels, between the entry points (tree_attention.hip)
+// and the kernels' translation units.
+#pragma once
+#include "common.hpp"
+
+namespace slc_tree {
+
+struct TreeArgs {
+  const void* query;
+  const void* key;
+  const void* value;
+  const int32_t* table;  // null: contiguous buffers
+  const void* lengths;
+  const uint8_t* tree;  // null: node i sees nodes 0 .. i
+  const void* mask;
+  void* output;
+  int64_t table_sb, num_pages, tree_sb, tree_si, tree_sj, mask_sb, mask_ss;
+  int64_t q_sb, q_sh, q_st, kv_sb, kv_ss, kv_sh, o_sb, o_sh, o_st;
+  int64_t rows;  // rows that may be seen: the capacity, or the mask's length
+  int page_shift, lengths_dtype, mask_dtype;
+  int batch, q_heads, kv_heads, nodes, head_dim;
+  float scale;
+  bool vector_kv, vector_q, vector_o;  // rows that 16-byte loads (8- or 16-byte stores) take
+  // The split: `slots` pieces per KV head and row block at most.
+  int slots, row_blocks;
+  float* partial;  // [slot, KV head, row block][rows][DP], then their (max, sum) pairs
+  float2* stats;
+  int2* pieces;  // per sequence: its first slot and how many
+};
+
+// The kernel for `rows` query rows per KV head, and its launch; one pair per type, in
+// a translation unit each.
+struct Plan {
+  int rows_per_block, padded_dim;
+};
+Plan plan_bf16(int rows, int head_dim);
+Plan plan_f16(int rows, int head_dim);
+Plan plan_f32(int rows, int head_dim);
+int launch_bf16(const TreeArgs& a, const Plan& plan, hipStream_t stream);
+int launch_f16(const TreeArgs& a, const Plan& plan, hipStream_t stream);
+int launch_f32(const TreeArgs& a, const Plan& plan, hipStream_t stream);
+
+}  // namespace slc_tree

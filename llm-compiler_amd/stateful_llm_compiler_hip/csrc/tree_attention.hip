@@ -1,102 +1,37 @@
-// tree_attention: attention of a tree of drafted tokens over a KV cache.
-//
-//   out[b, h, i] = sum_s softmax_s(t)[s] value[s],  t[s] = scale q[b, h, i].key[s] (+ mask[b, s])
-//
-// over the rows s that node i sees: the sequence's, s < lengths[b], and of the
-// nodes' own rows lengths[b] + j those with tree[i, j].  fp32 throughout, one
-// rounding of the output; no row seen: NaN.
-//
-// One workgroup per (node, query head, sequence): a thread per key for the scores of
-// 256 keys, then a thread per dim for their weighted values.
+// tree_attention: attention of a tree of drafted tokens over a KV cache, contiguous or
+// paged: the entry points (argument checks, the split, the workspace).  The kernels are
+// in tree_kernel.hpp.
 #include <algorithm>
 #include <cmath>
 
-#include "common.hpp"
+#include "tree_args.hpp"
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kThreads = 256;
+using slc_tree::Plan;
+using slc_tree::TreeArgs;
 
-struct TreeArgs {
-  const void* query;
-  const void* key;
-  const void* value;
-  const int32_t* table;  // null: contiguous buffers
-  const void* lengths;
-  const uint8_t* tree;  // null: node i sees nodes 0 .. i
-  const void* mask;
-  void* output;
-  int64_t table_sb, num_pages, tree_sb, tree_si, tree_sj, mask_sb, mask_ss;
-  int64_t q_sb, q_sh, q_st, kv_sb, kv_ss, kv_sh, o_sb, o_sh, o_st;
-  int64_t rows;  // rows that may be seen: the capacity, or the mask's length
-  int page_shift, lengths_dtype, mask_dtype;
-  int q_heads, kv_heads, nodes, head_dim;
-  float scale;
+Plan plan_for(int dtype, int rows, int head_dim) {
+  if (dtype == SLC_BF16) return slc_tree::plan_bf16(rows, head_dim);
+  if (dtype == SLC_F16) return slc_tree::plan_f16(rows, head_dim);
+  return slc_tree::plan_f32(rows, head_dim);
+}
+
+// The split of a call: row blocks, pieces (a workgroup per CU, but room for each sequence
+// and some more) and the workspace for their partial results.
+struct Split {
+  int64_t row_blocks, slots, partial_bytes, stats_bytes, pieces_bytes;
+  int64_t bytes() const { return partial_bytes + stats_bytes + pieces_bytes; }
 };
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeArgs a) {
-  __shared__ float q[256], p[kThreads], part[kThreads / 64];
-  __shared__ int64_t at[kThreads];
-  const int i = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const int64_t b = blockIdx.z;
-  const int kvh = h / (a.q_heads / a.kv_heads);
-  int64_t length = slc::load_length(a.lengths, b, a.lengths_dtype);
-  length = length < 0 ? 0 : (length > a.rows ? a.rows : length);
-  const int64_t end = length + a.nodes < a.rows ? length + a.nodes : a.rows;
-  const T* key = static_cast<const T*>(a.key) + kvh * a.kv_sh;
-  const T* value = static_cast<const T*>(a.value) + kvh * a.kv_sh;
-  if (tid < a.head_dim)
-    q[tid] = slc::to_f32(static_cast<const T*>(a.query)[b * a.q_sb + h * a.q_sh + i * a.q_st + tid]) * a.scale;
-  float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-  for (int64_t base = 0; base < end; base += kThreads) {
-    __syncthreads();
-    const int64_t s = base + tid;
-    int64_t row = -1;
-    if (s < end) {
-      const int64_t j = s - length;
-      const bool seen = j < 0 || (a.tree == nullptr ? j <= i : a.tree[b * a.tree_sb + i * a.tree_si + j * a.tree_sj] != 0);
-      if (seen && a.table != nullptr) {
-        const int64_t page = a.table[b * a.table_sb + (s >> a.page_shift)];
-        if (page >= 0 && page < a.num_pages)
-          row = page * a.kv_sb + (s & ((int64_t{1} << a.page_shift) - 1)) * a.kv_ss;
-      } else if (seen) {
-        row = b * a.kv_sb + s * a.kv_ss;
-      }
-    }
-    float t = -INFINITY;
-    if (row >= 0) {
-      const float m = a.mask == nullptr ? 0.0f : slc::load_as_f32(a.mask, b * a.mask_sb + s * a.mask_ss, a.mask_dtype);
-      if (m == -INFINITY) {
-        row = -1;
-      } else {
-        t = 0.0f;
-        for (int d = 0; d < a.head_dim; ++d) t = fmaf(q[d], slc::to_f32(key[row + d]), t);
-        t += m;
-      }
-    }
-    at[tid] = row;
-    float most = slc::wave_max(t);
-    if ((tid & 63) == 0) part[tid >> 6] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    most = fmaxf(most, top);
-    const float shift = most == -INFINITY ? 0.0f : most;
-    const float alpha = exp2f((top - shift) * kLog2e);
-    p[tid] = row >= 0 ? exp2f((t - shift) * kLog2e) : 0.0f;
-    top = most;
-    __syncthreads();
-    sum *= alpha;
-    acc *= alpha;
-    const int keys = static_cast<int>(end - base < kThreads ? end - base : kThreads);
-    for (int k = 0; k < keys; ++k) {
-      sum += p[k];
-      if (tid < a.head_dim && at[k] >= 0) acc = fmaf(p[k], slc::to_f32(value[at[k] + tid]), acc);
-    }
-  }
-  if (tid < a.head_dim)
-    static_cast<T*>(a.output)[b * a.o_sb + h * a.o_sh + i * a.o_st + tid] = slc::from_f32<T>(acc / sum);
+Split split_for(const Plan& plan, int64_t batch, int64_t kv_heads, int64_t rows) {
+  Split s;
+  s.row_blocks = slc_host::ceil_div(rows, plan.rows_per_block);
+  s.slots = std::max<int64_t>(slc_host::device_cu_count() / (kv_heads * s.row_blocks), batch + batch / 4);
+  const int64_t places = s.slots * kv_heads * s.row_blocks * plan.rows_per_block;
+  s.partial_bytes = places * plan.padded_dim * 4;
+  s.stats_bytes = places * 8;
+  s.pieces_bytes = batch * 8;
+  return s;
 }
 
 int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, int dtype, int64_t batch,
@@ -118,33 +53,49 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
     SLC_REQUIRE(mask_len >= 0 && mask_len <= capacity, "%s: the mask is longer than the cache", what);
     a.rows = mask_len;
   }
-  (void)workspace;
-  (void)workspace_bytes;
+  a.batch = static_cast<int>(batch);
   a.q_heads = static_cast<int>(q_heads);
   a.kv_heads = static_cast<int>(kv_heads);
   a.nodes = static_cast<int>(nodes);
   a.head_dim = static_cast<int>(head_dim);
-  const dim3 grid(a.nodes, a.q_heads, static_cast<unsigned>(batch));
+  const int64_t rows = q_heads / kv_heads * nodes;
+  const Plan plan = plan_for(dtype, static_cast<int>(rows), a.head_dim);
+  const Split split = split_for(plan, batch, kv_heads, rows);
+  SLC_REQUIRE(split.slots * kv_heads * split.row_blocks <= 0x7fffff00, "%s: too many query rows", what);
+  SLC_REQUIRE(workspace != nullptr && workspace_bytes >= split.bytes() &&
+                  (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+              "%s: workspace too small or not on 16 bytes", what);
+  a.row_blocks = static_cast<int>(split.row_blocks);
+  a.slots = static_cast<int>(split.slots);
+  char* place = static_cast<char*>(workspace);
+  a.partial = reinterpret_cast<float*>(place);
+  a.stats = reinterpret_cast<float2*>(place + split.partial_bytes);
+  a.pieces = reinterpret_cast<int2*>(place + split.partial_bytes + split.stats_bytes);
+  const int es = slc_host::dtype_size(dtype);
+  const auto on = [es](int64_t bytes, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> sizes) {
+    uint64_t bits = 0;
+    for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+    for (int64_t n : sizes) bits |= static_cast<uint64_t>(n * es);
+    return bits % static_cast<uint64_t>(bytes) == 0;
+  };
+  // (A load's eight rows at most lie within 32-bit offsets.)
+  a.vector_kv = on(16, {a.key, a.value}, {a.kv_sb, a.kv_ss, a.kv_sh, head_dim}) && a.kv_ss * es <= (1 << 27);
+  a.vector_q = on(16, {a.query}, {a.q_sb, a.q_sh, a.q_st, head_dim});
+  a.vector_o = on(4 * es, {a.output}, {a.o_sb, a.o_sh, a.o_st, head_dim});
   hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case SLC_BF16:
-      hipLaunchKernelGGL(tree_attention_kernel<slc::bf16_t>, grid, dim3(kThreads), 0, s, a);
-      break;
-    case SLC_F16:
-      hipLaunchKernelGGL(tree_attention_kernel<slc::f16_t>, grid, dim3(kThreads), 0, s, a);
-      break;
-    default:
-      hipLaunchKernelGGL(tree_attention_kernel<float>, grid, dim3(kThreads), 0, s, a);
-  }
-  return slc_host::check_launch(what);
+  if (dtype == SLC_BF16) return slc_tree::launch_bf16(a, plan, s);
+  if (dtype == SLC_F16) return slc_tree::launch_f16(a, plan, s);
+  return slc_tree::launch_f32(a, plan, s);
 }
 
 }  // namespace
 
 extern "C" int64_t slc_hip_tree_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                          int64_t nodes, int64_t head_dim, int dtype) {
-  (void)batch, (void)q_heads, (void)kv_heads, (void)nodes, (void)head_dim, (void)dtype;
-  return 0;
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || nodes <= 0 || head_dim <= 0 || !slc_host::is_float_dtype(dtype))
+    return 0;
+  const int64_t rows = q_heads / kv_heads * nodes;
+  return split_for(plan_for(dtype, static_cast<int>(rows), static_cast<int>(head_dim)), batch, kv_heads, rows).bytes();
 }
 
 extern "C" int slc_hip_tree_attention(
