@@ -78,8 +78,8 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
     for (int64_t n : sizes) bits |= static_cast<uint64_t>(n * es);
     return bits % static_cast<uint64_t>(bytes) == 0;
   };
-  // (A load's eight rows at most lie within 32-bit offsets.)
-  a.vector_kv = on(16, {a.key, a.value}, {a.kv_sb, a.kv_ss, a.kv_sh, head_dim}) && a.kv_ss * es <= (1 << 27);
+  // (The 256 rows of a step lie within 2^30 bytes.)
+  a.vector_kv = on(16, {a.key, a.value}, {a.kv_sb, a.kv_ss, a.kv_sh, head_dim}) && a.kv_ss * es <= (1 << 22);
   a.vector_q = on(16, {a.query}, {a.q_sb, a.q_sh, a.q_st, head_dim});
   a.vector_o = on(4 * es, {a.output}, {a.o_sb, a.o_sh, a.o_st, head_dim});
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -54,12 +54,14 @@ __device__ __forceinline__ uint2 lds_read_tr(const unsigned char* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                        (__attribute__((address_space(3))) v4s_t*)(p)));
 }
-__device__ __forceinline__ void lds_dma16(const void* base, int bytes, unsigned char* lds, int voffset) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, int bytes) {
   const uint64_t address = reinterpret_cast<uint64_t>(base);
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(address));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(address >> 32));
-  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-      reinterpret_cast<void*>(static_cast<uint64_t>(hi) << 32 | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(static_cast<uint64_t>(hi) << 32 | lo), 0,
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+__device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, int voffset) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, voffset, 0, 0, 0);
 }
 
@@ -243,69 +245,90 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 
   if (wave == S::kConsumers) {
     // ---- producer -------------------------------------------------------------
+    constexpr int kTileOps = kTileBytes / 1024;
     const T* kbase = static_cast<const T*>(a.key) + kvh * a.kv_sh;
     const T* vbase = static_cast<const T*>(a.value) + kvh * a.kv_sh;
-    typedef const __attribute__((address_space(4))) int32_t* ConstInts;
-    const ConstInts table = (ConstInts)(a.table);
-    // Offset of cache row s, or -1 where its page is none of the pool's.
-    auto offset = [&](int s) -> int64_t {
-      if (a.table == nullptr) return b * a.kv_sb + static_cast<int64_t>(s) * a.kv_ss;
-      const int page = table[b * a.table_sb + (s >> a.page_shift)];
-      if (page < 0 || page >= a.num_pages) return -1;
-      return page * a.kv_sb + static_cast<int64_t>(s & ((1 << a.page_shift) - 1)) * a.kv_ss;
-    };
     const int row_in_op = lane / kChunks;
-    auto issue = [&](int step, int stage) {
-      unsigned char* dst = lds + stage * S::kStageBytes;
+    const bool paged = a.table != nullptr;
+    const int page_rows = paged ? 1 << a.page_shift : S::kStep;
+    const int segment = page_rows < S::kStep ? page_rows : S::kStep;  // rows of a step with one base
+    const int row_bytes = static_cast<int>(a.kv_ss) * ES;
+    // Lane L of load n fills row kOpRows n + L / kChunks of the step, chunk L % kChunks, with
+    // that row's chunk (L % kChunks) ^ (row & 7); columns past the head dim lie past every range.
+    // Rows kOpRows apart have another swizzle unless kOpRows is a multiple of 8.
+    constexpr int kSwizzles = kOpRows >= 8 ? 1 : 8 / kOpRows;
+    int voffset[kSwizzles];
+#pragma unroll
+    for (int i = 0; i < kSwizzles; ++i) {
+      const int row = i * kOpRows + row_in_op;
+      const int chunk = (lane % kChunks) ^ (row & 7);
+      voffset[i] = chunk * (16 / ES) < a.head_dim ? row * row_bytes + chunk * 16 : 0x40000000;
+    }
+    for (int t = 1 - S::kStages; t < nsteps; ++t) {
+      if (t >= 0) {
+        // Step t has landed: the kStages - 2 later ones (kOps each) may still fly.
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"((S::kStages - 2) * S::kOps) : "memory");
+        __syncthreads();
+      }
+      const int step = t + S::kStages - 1;
+      unsigned char* dst = lds + step % S::kStages * S::kStageBytes;
       const int s0 = (step0 + step) * S::kStep;
       const int end = step < nsteps ? piece.end : 0;
       if (a.vector_kv) {
-#pragma unroll 4
-        for (int n = 0; n < S::kOps / 2; ++n) {
-          // Rows kOpRows n .. of the step: tile n / (ops of a tile), whose K lies before its V.
-          constexpr int kTileOps = kTileBytes / 1024;
-          const int row = n * kOpRows;
-          const int rows = __builtin_amdgcn_readfirstlane(min(kOpRows, end - s0 - row));
-          const int64_t at = rows > 0 ? offset(__builtin_amdgcn_readfirstlane(s0 + row)) : 0;
-          const int bytes = rows > 0 && at >= 0 ? static_cast<int>(((rows - 1) * a.kv_ss + a.head_dim) * ES) : 0;
-          const int chunk = (lane % kChunks) ^ ((row + row_in_op) & 7);
-          // Columns past the head dim lie past every range.
-          const int voffset = chunk * (16 / ES) < a.head_dim ? static_cast<int>(row_in_op * a.kv_ss * ES) + chunk * 16
-                                                             : 0x7ffffff0;
-          unsigned char* place = dst + n / kTileOps * 2 * kTileBytes + n % kTileOps * 1024;
-          lds_dma16(kbase + at, bytes, place, voffset);
-          lds_dma16(vbase + at, bytes, place + kTileBytes, voffset);
+        for (int first = 0; first < S::kStep; first += segment) {
+          int rows = end - s0 - first;  // rows past the last one read as zero
+          rows = rows < segment ? rows : segment;
+          int64_t at = b * a.kv_sb + static_cast<int64_t>(s0 + first) * a.kv_ss;
+          if (paged && rows > 0) {
+            typedef const __attribute__((address_space(4))) int32_t* ConstInts;
+            const int page = ((ConstInts)(a.table))[b * a.table_sb + ((s0 + first) >> a.page_shift)];
+            at = page * a.kv_sb + ((s0 + first) & (page_rows - 1)) * a.kv_ss;
+            if (page < 0 || page >= a.num_pages) rows = 0;
+          }
+          const int bytes = rows > 0 ? (rows - 1) * row_bytes + a.head_dim * ES : 0;
+          const __amdgpu_buffer_rsrc_t rk = make_rsrc(kbase + (rows > 0 ? at : 0), bytes);
+          const __amdgpu_buffer_rsrc_t rv = make_rsrc(vbase + (rows > 0 ? at : 0), bytes);
+          const int first_op = first / kOpRows;
+          auto load = [&](int n, int i) {  // load n of the segment, n % kSwizzles == i
+            const int op = first_op + n;
+            unsigned char* place = dst + op / kTileOps * 2 * kTileBytes + op % kTileOps * 1024;
+            const int offset = voffset[i] + (n - i) * kOpRows * row_bytes;
+            lds_dma16(rk, place, offset);
+            lds_dma16(rv, place + kTileBytes, offset);
+          };
+          constexpr int kGroup = 16 / kOpRows;  // loads of 16 rows, the smallest page
+          for (int n = 0; n < segment / kOpRows; n += kGroup) {
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i) load(n + i, i % kSwizzles);
+          }
         }
       } else {
         // Any alignment: elements, a chunk of LDS per lane at a time.
         constexpr int kPer = 16 / ES;
+#pragma unroll 1
         for (int n = 0; n < S::kOps / 2; ++n) {
-          constexpr int kTileOps = kTileBytes / 1024;
           const int row = n * kOpRows + row_in_op;
           const int chunk = (lane % kChunks) ^ (row & 7);
           const int s = s0 + row;
           int64_t at = -1;
-          if (s < end) at = offset(s);
-          T k[kPer] = {}, v[kPer] = {};
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            if (at < 0 || chunk * kPer + e >= a.head_dim) continue;
-            k[e] = kbase[at + chunk * kPer + e];
-            v[e] = vbase[at + chunk * kPer + e];
+          if (s < end) {
+            at = b * a.kv_sb + s * a.kv_ss;
+            if (paged) {
+              const int page = a.table[b * a.table_sb + (s >> a.page_shift)];
+              at = page >= 0 && page < a.num_pages ? page * a.kv_sb + (s & (page_rows - 1)) * a.kv_ss : -1;
+            }
           }
           unsigned char* place = dst + n / kTileOps * 2 * kTileBytes + n % kTileOps * 1024 + lane * 16;
-          *reinterpret_cast<uint4*>(place) = __builtin_bit_cast(uint4, k);
-          *reinterpret_cast<uint4*>(place + kTileBytes) = __builtin_bit_cast(uint4, v);
+#pragma unroll 1
+          for (int side = 0; side < 2; ++side) {
+            const T* from = (side == 0 ? kbase : vbase) + (at < 0 ? 0 : at) + chunk * kPer;
+            T v[kPer];
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[e] = at >= 0 && chunk * kPer + e < a.head_dim ? from[e] : T{};
+            *reinterpret_cast<uint4*>(place + side * kTileBytes) = __builtin_bit_cast(uint4, v);
+          }
         }
       }
-    };
-#pragma unroll
-    for (int t = 0; t < S::kStages - 1; ++t) issue(t, t);
-    for (int t = 0; t < nsteps; ++t) {
-      // Step t has landed: the kStages - 2 later ones (kOps each) may still fly.
-      asm volatile("s_waitcnt vmcnt(%0)" ::"i"((S::kStages - 2) * S::kOps) : "memory");
-      __syncthreads();
-      issue(t + S::kStages - 1, (t + S::kStages - 1) % S::kStages);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if constexpr (WK > 1) {
@@ -428,16 +451,26 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       factor = kLog2e;
       bool hidden = false;
       float add[KB][4];
+      auto masks = [&](auto load) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int s = s0 + 16 * kb + 4 * g + r;
-          add[kb][r] = s >= piece.end ? -INFINITY
-                       : a.mask == nullptr ? 0.0f
-                                           : slc::load_as_f32(a.mask, b * a.mask_sb + s * a.mask_ss, a.mask_dtype);
-          hidden |= add[kb][r] == -INFINITY;
-        }
+          for (int r = 0; r < 4; ++r) {
+            const int s = s0 + 16 * kb + 4 * g + r;
+            add[kb][r] = s < piece.end ? load(s) : -INFINITY;
+            hidden |= add[kb][r] == -INFINITY;
+          }
+      };
+      const int64_t mask_at = b * a.mask_sb;
+      if (a.mask == nullptr) {
+        masks([](int) { return 0.0f; });
+      } else if (a.mask_dtype == SLC_F32) {
+        masks([&](int s) { return static_cast<const float*>(a.mask)[mask_at + s * a.mask_ss]; });
+      } else if (a.mask_dtype == SLC_BF16) {
+        masks([&](int s) { return slc::to_f32(static_cast<const slc::bf16_t*>(a.mask)[mask_at + s * a.mask_ss]); });
+      } else {
+        masks([&](int s) { return slc::to_f32(static_cast<const slc::f16_t*>(a.mask)[mask_at + s * a.mask_ss]); });
+      }
       const bool tail = s0 + KT > piece.length;
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
