@@ -697,13 +697,15 @@ SLC_API int slc_hip_linear_q8(const int8_t* input, const float* in_scales, const
  *   [B, capacity, kv_heads, D] (pages [num_pages, page_tokens, kv_heads, D]
  *   and block_table int32 [B, pages_per_seq], unit stride) with one set of strides;
  *   lengths int32 or int64; tree bytes; mask fp32, fp16 or bf16; scale > 0.
- *   nodes <= SLC_TREE_MAX_NODES, capacity <= 2^30.
+ *   batch <= 32768; nodes <= SLC_TREE_MAX_NODES, of a chain SLC_CHAIN_MAX_NODES;
+ *   capacity <= 2^30, batch * capacity <= 2^34.
  * The workspace (slc_hip_tree_attention_workspace_size bytes, 16-byte aligned; the
  * paged form needs the same) holds the partial results of a split over the rows;
  * calls that may overlap in time need their own.  Table entries that name no page of
  * the pool are not followed; a node that sees rows of such a page has no meaning.
  */
-#define SLC_TREE_MAX_NODES 4096
+#define SLC_TREE_MAX_NODES 1024
+#define SLC_CHAIN_MAX_NODES 4096
 SLC_API int64_t slc_hip_tree_attention_workspace_size(int64_t batch, int64_t q_heads,
                                                       int64_t kv_heads, int64_t nodes,
                                                       int64_t head_dim, int dtype);

@@ -29,8 +29,8 @@ from .hip_ops import _FLOATS, check_flag
 from .hip_paged import _check_pools
 from .hip_q8 import _call
 
-MAX_TREE_NODES = 4096  # SLC_TREE_MAX_NODES
-MAX_NODES = 1024  # SLC_VERIFY_MAX_NODES: nodes of a tree that is verified and committed
+MAX_NODES = 1024  # SLC_TREE_MAX_NODES, SLC_VERIFY_MAX_NODES
+MAX_CHAIN = 4096  # SLC_CHAIN_MAX_NODES: nodes of tree attention without a tree mask
 
 
 def _tree_operands(what, query, key, value, lengths, tree_mask, attention_mask, rows, kv_heads, scale):
@@ -54,8 +54,8 @@ def _tree_operands(what, query, key, value, lengths, tree_mask, attention_mask, 
         raise ValueError(f"{what}: GQA or head shapes do not match")
     if not 1 <= head_dim <= 256:
         raise ValueError(f"{what}: head_dim must be 1 to 256")
-    if nodes > MAX_TREE_NODES:
-        raise ValueError(f"{what}: at most {MAX_TREE_NODES} nodes")
+    if nodes > (MAX_CHAIN if tree_mask is None else MAX_NODES):
+        raise ValueError(f"{what}: a tree has at most {MAX_NODES} nodes, a chain {MAX_CHAIN}")
     if lengths.shape != (batch,) or lengths.dtype not in (torch.int64, torch.int32) or not lengths.is_contiguous():
         raise ValueError(f"{what}: lengths must be a contiguous int64 (or int32) [batch] tensor")
     if not 0.0 < scale <= torch.finfo(torch.float32).max:
@@ -102,7 +102,8 @@ def hip_tree_attention(
 
     Node i of sequence b sees the rows ``s < lengths[b]`` and those of its nodes j,
     ``lengths[b] + j``, with ``tree_mask[b, i, j]`` (bool, [T, T] or [B, T, T]; None: a
-    chain, j <= i); ``lengths`` are those before the nodes.  ``attention_mask`` is as in
+    chain, j <= i); ``lengths`` are those before the nodes.  A tree has at most 1024
+    nodes, a chain 4096.  ``attention_mask`` is as in
     ``hip_decode_attention``: additive [B, 1, 1, S] over the buffers' rows, the nodes'
     own included; rows from S on, and those whose mask is -inf, are not seen.  Rows
     past the capacity were not stored and are not seen either.  Nothing that a row

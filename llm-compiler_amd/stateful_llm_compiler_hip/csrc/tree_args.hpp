@@ -23,6 +23,7 @@ struct TreeArgs {
   bool vector_kv, vector_q, vector_o;  // rows that 16-byte loads (8- or 16-byte stores) take
   // The split: `slots` pieces per KV head and row block at most.
   int slots, row_blocks;
+  float inverse_slots;
   float* partial;  // [slot, KV head, row block][rows][DP], then their (max, sum) pairs
   float2* stats;
   int2* pieces;  // per sequence: its first slot and how many

@@ -27,6 +27,9 @@ Split split_for(const Plan& plan, int64_t batch, int64_t kv_heads, int64_t rows)
   Split s;
   s.row_blocks = slc_host::ceil_div(rows, plan.rows_per_block);
   s.slots = std::max<int64_t>(slc_host::device_cu_count() / (kv_heads * s.row_blocks), batch + batch / 4);
+  // Row blocks of one piece share its K and V rows: workgroup numbers that differ by a
+  // multiple of 8 run on one XCD, whose L2 then holds them.
+  if (s.row_blocks > 1) s.slots = (s.slots + 7) / 8 * 8;
   const int64_t places = s.slots * kv_heads * s.row_blocks * plan.rows_per_block;
   s.partial_bytes = places * plan.padded_dim * 4;
   s.stats_bytes = places * 8;
@@ -39,11 +42,13 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
         void* stream) {
   SLC_REQUIRE(slc_host::is_float_dtype(dtype), "%s: bad dtype %d", what, dtype);
   SLC_REQUIRE(a.lengths_dtype == SLC_I64 || a.lengths_dtype == SLC_I32, "%s: lengths must be int32 or int64", what);
-  SLC_REQUIRE(batch >= 0 && batch <= 65535 && nodes >= 0 && nodes <= SLC_TREE_MAX_NODES, "%s: bad batch or node count",
-              what);
+  SLC_REQUIRE(batch >= 0 && batch <= 32768, "%s: batch must be 0 to 32768", what);
+  SLC_REQUIRE(nodes >= 0 && nodes <= (a.tree == nullptr ? SLC_CHAIN_MAX_NODES : SLC_TREE_MAX_NODES),
+              "%s: a tree has at most %d nodes, a chain %d", what, SLC_TREE_MAX_NODES, SLC_CHAIN_MAX_NODES);
   SLC_REQUIRE(kv_heads > 0 && q_heads > 0 && q_heads % kv_heads == 0 && q_heads <= 65535, "%s: bad head counts", what);
   SLC_REQUIRE(head_dim >= 1 && head_dim <= 256, "%s: head_dim must be 1 to 256", what);
   SLC_REQUIRE(capacity >= 1 && capacity <= (int64_t{1} << 30), "%s: capacity must be 1 to 2^30", what);
+  SLC_REQUIRE(batch * capacity <= (int64_t{1} << 34), "%s: batch times capacity above 2^34", what);
   SLC_REQUIRE(a.scale > 0.0f && std::isfinite(a.scale), "%s: scale must be positive and finite", what);
   if (batch == 0 || nodes == 0) return SLC_OK;
   SLC_REQUIRE(a.query && a.key && a.value && a.lengths && a.output, "%s: null pointer", what);
@@ -61,12 +66,13 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
   const int64_t rows = q_heads / kv_heads * nodes;
   const Plan plan = plan_for(dtype, static_cast<int>(rows), a.head_dim);
   const Split split = split_for(plan, batch, kv_heads, rows);
-  SLC_REQUIRE(split.slots * kv_heads * split.row_blocks <= 0x7fffff00, "%s: too many query rows", what);
+  SLC_REQUIRE(rows < (1 << 24) && split.slots <= 65535 && split.row_blocks <= 65535, "%s: too many query rows", what);
   SLC_REQUIRE(workspace != nullptr && workspace_bytes >= split.bytes() &&
                   (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
               "%s: workspace too small or not on 16 bytes", what);
   a.row_blocks = static_cast<int>(split.row_blocks);
   a.slots = static_cast<int>(split.slots);
+  a.inverse_slots = 1.0f / static_cast<float>(split.slots);
   char* place = static_cast<char*>(workspace);
   a.partial = reinterpret_cast<float*>(place);
   a.stats = reinterpret_cast<float2*>(place + split.partial_bytes);

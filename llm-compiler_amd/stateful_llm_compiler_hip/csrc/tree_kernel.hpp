@@ -49,6 +49,10 @@ __device__ __forceinline__ f32x4_t mfma(slc::f16_t, uint4 a, uint4 b, f32x4_t c)
                                                 0, 0);
 }
 
+__device__ __forceinline__ f32x4_t mfma(uint32_t a, uint32_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b), c, 0, 0, 0);
+}
+
 __device__ __forceinline__ uint4 lds_read(const unsigned char* p) { return *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ uint2 lds_read_tr(const unsigned char* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -92,20 +96,18 @@ __device__ __forceinline__ uint4 without_special(uint4 v) {
   return make_uint4(without_special<T>(v.x), without_special<T>(v.y), without_special<T>(v.z), without_special<T>(v.w));
 }
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, 64);
-  return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int wave_scan(int v) {  // sums up to and with this lane
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int offset = 1; offset < 64; offset <<= 1) {
-    const int below = __shfl_up(v, offset, 64);
-    if (lane >= offset) v += below;
-  }
+// Sums up to and with this lane, in the VALU: rows of 16 lanes by shifts, then the rows
+// below by broadcasts of their last lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
 }
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
 // Four neighbouring dims of an output row.
 template <typename T>
@@ -130,61 +132,68 @@ __device__ __forceinline__ float4 divided(float4 v, float sum) {
   return make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
 }
 
+// n / d from d's rounded inverse, n < 2^24.
+__device__ __forceinline__ int quotient(int n, int d, float inverse) {
+  const int q = static_cast<int>(static_cast<float>(n) * inverse);
+  const int rest = n - q * d;
+  return q + (rest >= d) - (rest < 0);
+}
+
 struct Piece {
   int sequence;  // -1: none
   int index, count, first;
   int length, end;  // rows of the sequence, and with its nodes'
 };
 
-// The piece of slot x.  Sequences are cut into pieces of at most q steps, q the smallest
-// tried for which all pieces fit the slots; every wave finds its own for itself.
+// The piece of slot x.  Sequences are cut into pieces of about q steps, q the smallest
+// tried for which all pieces fit the slots; every wave finds its own for itself, by the
+// same arithmetic (fp32: what counts is that all agree and that no sequence has none).
 template <int STEP>
-__device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, int min_steps) {
+__device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_steps) {
   const int lane = threadIdx.x & 63;
-  auto bounds = [&](int b, int& length, int& end) {
-    const int64_t n = slc::load_length(a.lengths, b, a.lengths_dtype);
-    const int64_t rows = a.rows;
-    length = static_cast<int>(n < 0 ? 0 : (n > rows ? rows : n));
-    end = static_cast<int>(length + a.nodes < rows ? length + a.nodes : rows);
+  const int rows = static_cast<int>(a.rows);
+  auto length_of = [&](int b) {
+    const int64_t n = b < a.batch ? slc::load_length(a.lengths, b, a.lengths_dtype) : 0;
+    return static_cast<int>(n < 0 ? 0 : (n > rows ? rows : n));
   };
-  auto steps_of = [&](int b) {
-    if (b >= a.batch) return 0;
-    int length, end;
-    bounds(b, length, end);
-    return end > STEP ? (end + STEP - 1) / STEP : 1;
+  auto end_of = [&](int length) { return length + a.nodes < rows ? length + a.nodes : rows; };
+  auto steps_of = [&](int b, int length) {
+    const int n = (end_of(length) + STEP - 1) / STEP;
+    return b < a.batch ? (n > 1 ? n : 1) : 0;
   };
-  const int own = steps_of(lane);  // of the first 64 sequences
-  int64_t total = 0;
-  for (int base = 0; base < a.batch; base += 64) total += wave_sum(base == 0 ? own : steps_of(base + lane));
-  int q = static_cast<int>((total + a.slots - 1) / a.slots);
-  q = q < min_steps ? min_steps : q;
-  auto pieces_of = [&](int n) { return n == 0 ? 0 : (n + q - 1) / q; };
-  for (;;) {
-    int64_t pieces = 0;
-    for (int base = 0; base < a.batch; base += 64)
-      pieces += wave_sum(pieces_of(base == 0 ? own : steps_of(base + lane)));
-    if (pieces <= a.slots) break;
-    q += (q + 7) / 8;
-  }
+  // Of the first 64 sequences; more are read again in every pass.
+  const int own_length = length_of(lane), own = steps_of(lane, own_length);
+  int total = wave_sum(own);
+  for (int base = 64; base < a.batch; base += 64) total += wave_sum(steps_of(base + lane, length_of(base + lane)));
+  float q = fmaxf(static_cast<float>(total) * a.inverse_slots, min_steps);
   Piece p{-1, 0, 0, 0, 0, 0};
-  int before = 0;
-  for (int base = 0; base < a.batch; base += 64) {
-    const int n = pieces_of(base == 0 ? own : steps_of(base + lane));
-    const int upto = before + wave_scan(n);
-    const uint64_t hits = __ballot(upto > x);
-    if (hits != 0) {
-      const int at = __builtin_ctzll(hits);
-      p.sequence = base + at;
-      p.count = __builtin_amdgcn_readlane(n, at);
-      p.first = __builtin_amdgcn_readlane(upto, at) - p.count;
-      p.index = x - p.first;
-      bounds(p.sequence, p.length, p.end);
-      p.length = __builtin_amdgcn_readfirstlane(p.length);
-      p.end = __builtin_amdgcn_readfirstlane(p.end);
-      break;
+  for (;;) {
+    // Pieces up to and with each sequence; found on the way: the sequence of slot x.
+    const float inverse = __builtin_amdgcn_rcpf(q);
+    int before = 0;
+    p.sequence = -1;
+    for (int base = 0; base < a.batch; base += 64) {
+      const int length = base == 0 ? own_length : length_of(base + lane);
+      const int steps = base == 0 ? own : steps_of(base + lane, length);
+      // Rounded up, past rounding errors; at least one, and no more than steps (q >= 1).
+      int n = static_cast<int>(static_cast<float>(steps) * inverse + 0.9999f);
+      n = n < 1 ? (steps > 0 ? 1 : 0) : (n < steps ? n : steps);
+      const int upto = before + wave_scan(n);
+      const uint64_t hits = __ballot(upto > x);
+      if (hits != 0 && p.sequence < 0) {
+        const int at = __builtin_ctzll(hits);
+        p.sequence = base + at;
+        p.count = __builtin_amdgcn_readlane(n, at);
+        p.first = __builtin_amdgcn_readlane(upto, at) - p.count;
+        p.length = __builtin_amdgcn_readlane(length, at);
+      }
+      before = __builtin_amdgcn_readlane(upto, 63);
     }
-    before = __builtin_amdgcn_readlane(upto, 63);
+    if (before <= a.slots) break;
+    q *= 1.125f;
   }
+  p.index = x - p.first;
+  p.end = end_of(p.length);
   return p;
 }
 
@@ -201,57 +210,61 @@ struct Shape {
   static constexpr int kFit = 65536 / (2 * kTileBytes);
   static constexpr int WK = kWaves / WR < kFit ? kWaves / WR : kFit;
   static constexpr int kConsumers = WR * WK;
-  static constexpr int kThreads = (kConsumers + 1) * 64;
   static constexpr int kStep = WK * KT;
+  // Producers, each of a part of a step's rows that no page is smaller than.  One wave
+  // issues a load in 90 to 140 cycles, 8 bytes a cycle; four keep up with the memory.
+  static constexpr int kProducers = kStep >= 64 ? 4 : kStep / 16;
+  static constexpr int kThreads = (kConsumers + kProducers) * 64;
   static constexpr int kStageBytes = WK * 2 * kTileBytes;
   static constexpr int kStages = kStageBytes <= 16384 ? 4 : (kStageBytes <= 32768 ? 3 : 2);
-  static constexpr int kOps = kStageBytes / 1024;  // loads of a step
+  static constexpr int kOps = kStageBytes / 1024 / kProducers;  // a producer's loads of a step
   static constexpr int kRows = 16 * QB * WR;
   static constexpr int kQuads = DP / 16;           // float4 of a lane's outputs per query block
-  static constexpr int kMergeBytes = WK > 1 ? (WK - 1) * WR * QB * (kQuads * 4 + 2) * 256 : 0;
+  static constexpr int kMergeBytes = WK > 1 ? WK * WR * QB * (kQuads * 4 + 2) * 256 : 0;
   static constexpr int kLds = kStages * kStageBytes > kMergeBytes ? kStages * kStageBytes : kMergeBytes;
   static_assert((kStages - 2) * kOps < 64, "the wait counts at most 63 loads");
-  static_assert(kLds <= 160 * 1024, "LDS");
+  static_assert(kConsumers * 64 >= kStep, "a step's mask is loaded by a thread per row");
 };
 
 template <typename T, int DP, int QB, int WR, int KT>
-__global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_attention_kernel(TreeArgs a, int min_steps) {
+__global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_attention_kernel(TreeArgs a, float min_steps) {
   using S = Shape<T, DP, QB, WR, KT>;
   constexpr bool kWide = S::kWide;
-  constexpr int WK = S::WK, KB = KT / 16;
+  constexpr int WK = S::WK;
+  constexpr int SUB = KT < 32 ? KT : 32, KB = SUB / 16, kSubs = KT / SUB;  // keys at a time
   constexpr int kRowBytes = S::kRowBytes, kTileBytes = S::kTileBytes;
   constexpr int kChunks = kRowBytes / 16, kOpRows = 1024 / kRowBytes;
   constexpr int ES = sizeof(T);
   __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
+  constexpr int kMaxWords = SLC_TREE_MAX_NODES / 32 + 2;
+  __shared__ uint32_t tree_bits[(S::kRows + 1) * kMaxWords];
+  __shared__ __attribute__((aligned(16))) float mask_room[2][S::kStep];
 
-  // Row blocks of one piece run on one XCD (workgroup ids that differ by 8), whose L2
-  // then holds the K and V rows that they share.
-  const int id = blockIdx.x;
-  const int across = 8 * a.row_blocks;
-  const int unit = id / across * 8 + id % across % 8;
-  const int block = id % across / 8;
-  const int kvh = unit % a.kv_heads;
-  const int slot = unit / a.kv_heads;
-  if (slot >= a.slots) return;
+  const int kvh = blockIdx.x, slot = blockIdx.y, block = blockIdx.z;
   const Piece piece = find_piece<S::kStep>(a, slot, min_steps);
   if (piece.sequence < 0) return;
   const int64_t b = piece.sequence;
+  // Its steps: the sequence's, shared out as evenly as whole steps go.
   const int steps = piece.end > S::kStep ? (piece.end + S::kStep - 1) / S::kStep : 1;
-  const int step0 = static_cast<int>(static_cast<int64_t>(steps) * piece.index / piece.count);
-  const int nsteps = static_cast<int>(static_cast<int64_t>(steps) * (piece.index + 1) / piece.count) - step0;
+  const int share = static_cast<int>(static_cast<unsigned>(steps) / static_cast<unsigned>(piece.count));
+  const int spare = steps - share * piece.count;
+  const int step0 = piece.index * share + (piece.index < spare ? piece.index : spare);
+  const int nsteps = share + (piece.index < spare ? 1 : 0);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (tid == 0 && piece.index == 0 && kvh == 0 && block == 0) a.pieces[b] = make_int2(piece.first, piece.count);
 
-  if (wave == S::kConsumers) {
-    // ---- producer -------------------------------------------------------------
+  if (wave >= S::kConsumers) {
+    // ---- producers ------------------------------------------------------------
     constexpr int kTileOps = kTileBytes / 1024;
     const T* kbase = static_cast<const T*>(a.key) + kvh * a.kv_sh;
     const T* vbase = static_cast<const T*>(a.value) + kvh * a.kv_sh;
+    constexpr int kPart = S::kStep / S::kProducers;  // rows of a step that this producer loads
+    const int part0 = (wave - S::kConsumers) * kPart;
     const int row_in_op = lane / kChunks;
     const bool paged = a.table != nullptr;
-    const int page_rows = paged ? 1 << a.page_shift : S::kStep;
-    const int segment = page_rows < S::kStep ? page_rows : S::kStep;  // rows of a step with one base
+    const int page_rows = paged ? 1 << a.page_shift : kPart;
+    const int segment = page_rows < kPart ? page_rows : kPart;  // rows with one base
     const int row_bytes = static_cast<int>(a.kv_ss) * ES;
     // Lane L of load n fills row kOpRows n + L / kChunks of the step, chunk L % kChunks, with
     // that row's chunk (L % kChunks) ^ (row & 7); columns past the head dim lie past every range.
@@ -275,7 +288,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       const int s0 = (step0 + step) * S::kStep;
       const int end = step < nsteps ? piece.end : 0;
       if (a.vector_kv) {
-        for (int first = 0; first < S::kStep; first += segment) {
+        for (int first = part0; first < part0 + kPart; first += segment) {
           int rows = end - s0 - first;  // rows past the last one read as zero
           rows = rows < segment ? rows : segment;
           int64_t at = b * a.kv_sb + static_cast<int64_t>(s0 + first) * a.kv_ss;
@@ -306,7 +319,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
         // Any alignment: elements, a chunk of LDS per lane at a time.
         constexpr int kPer = 16 / ES;
 #pragma unroll 1
-        for (int n = 0; n < S::kOps / 2; ++n) {
+        for (int n = part0 / kOpRows; n < (part0 + kPart) / kOpRows; ++n) {
           const int row = n * kOpRows + row_in_op;
           const int chunk = (lane % kChunks) ^ (row & 7);
           const int s = s0 + row;
@@ -343,6 +356,8 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   const int g = lane >> 4, c = lane & 15;
   const int group = a.q_heads / a.kv_heads;
   const int rows = group * a.nodes;
+  const float inverse_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
+  const int node0 = quotient(block * S::kRows, group, inverse_group);  // the block's first
   int node[QB], head[QB];
   bool real[QB];
   // Q^T: 16-bit types hold 8 dims 32 kk + 8 g of a block, fp32 4 dims 16 kk + 4 g.
@@ -352,8 +367,8 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   for (int qb = 0; qb < QB; ++qb) {
     const int row = block * S::kRows + wr * 16 * QB + 16 * qb + c;
     real[qb] = row < rows;
-    node[qb] = real[qb] ? row / group : 0;
-    head[qb] = kvh * group + (real[qb] ? row % group : 0);
+    node[qb] = real[qb] ? quotient(row, group, inverse_group) : node0;
+    head[qb] = kvh * group + (real[qb] ? row - node[qb] * group : 0);
     const T* qp = static_cast<const T*>(a.query) + b * a.q_sb + head[qb] * a.q_sh + node[qb] * a.q_st;
 #pragma unroll
     for (int kk = 0; kk < kParts; ++kk) {
@@ -390,14 +405,8 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   const uint4 ones = make_uint4(one2, one2, one2, one2);
   const float scale_log2 = a.scale * kLog2e;
 
-  for (int step = 0; step < nsteps; ++step) {
-    __syncthreads();  // this step's tiles are in the ring
-    const int s0 = (step0 + step) * S::kStep + wk * KT;
-    if (s0 >= piece.end) continue;
-    const unsigned char* kt = lds + step % S::kStages * S::kStageBytes + wk * 2 * kTileBytes;
-    const unsigned char* vt = kt + kTileBytes;
-
-    f32x4_t st[KB][QB];
+  // S^T of SUB keys at kt.
+  auto scores = [&](const unsigned char* kt, f32x4_t (&st)[KB][QB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -410,22 +419,136 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
           if constexpr (kWide) {
-            st[kb][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka.x), __uint_as_float(qv[qb][kk].x), st[kb][qb], 0, 0, 0);
-            st[kb][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka.y), __uint_as_float(qv[qb][kk].y), st[kb][qb], 0, 0, 0);
-            st[kb][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka.z), __uint_as_float(qv[qb][kk].z), st[kb][qb], 0, 0, 0);
-            st[kb][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka.w), __uint_as_float(qv[qb][kk].w), st[kb][qb], 0, 0, 0);
+            st[kb][qb] = mfma(ka.x, qv[qb][kk].x, st[kb][qb]);
+            st[kb][qb] = mfma(ka.y, qv[qb][kk].y, st[kb][qb]);
+            st[kb][qb] = mfma(ka.z, qv[qb][kk].z, st[kb][qb]);
+            st[kb][qb] = mfma(ka.w, qv[qb][kk].w, st[kb][qb]);
           } else {
             st[kb][qb] = mfma(T{}, ka, qv[qb][kk], st[kb][qb]);
           }
         }
       }
+  };
+  // The running maximum after scores of at most mx in this lane.  It spans the 4 lane
+  // groups, but matters only when some lane passes the threshold.
+  auto raise = [&](int qb, float mx) {
+    if (!__any(mx > m_run[qb] + kThreshold)) return;
+    mx = slc::max_xor32(slc::max_xor16(mx));
+    const float m_new = fmaxf(m_run[qb], mx);
+    const float alpha = __builtin_amdgcn_exp2f((m_run[qb] - (m_new == -INFINITY ? 0.0f : m_new)) * kLog2e);
+#pragma unroll
+    for (int i = 0; i < kAcc; ++i) acc[i][qb] = acc[i][qb] * alpha;
+    l_part[qb] *= alpha;
+    m_run[qb] = m_new;
+  };
+  // O^T += V^T . P^T with weights exp2(score * factor - shift); DIRTY: without V's NaNs
+  // and infinities.
+  auto weigh = [&](auto dirty_tag, const unsigned char* vt, const f32x4_t (&st)[KB][QB], float factor,
+                   const float (&shift)[QB]) {
+    constexpr bool kDirty = decltype(dirty_tag)::value;
+    if constexpr (kWide) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float p[QB];
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) {
+            p[qb] = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][r], factor, -shift[qb]));
+            l_part[qb] += p[qb];
+          }
+          const int row = 16 * kb + 4 * g + r;
+#pragma unroll
+          for (int d = 0; d < DP / 64; ++d) {
+            uint4 va = lds_read(vt + row * kRowBytes + (((16 * d + c) ^ (row & 7)) << 4));
+            if constexpr (kDirty) va = without_special<T>(va);
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+              const uint32_t pb = __float_as_uint(p[qb]);
+              acc[4 * d][qb] = mfma(va.x, pb, acc[4 * d][qb]);
+              acc[4 * d + 1][qb] = mfma(va.y, pb, acc[4 * d + 1][qb]);
+              acc[4 * d + 2][qb] = mfma(va.z, pb, acc[4 * d + 2][qb]);
+              acc[4 * d + 3][qb] = mfma(va.w, pb, acc[4 * d + 3][qb]);
+            }
+          }
+        }
+    } else {
+      uint4 pv[QB];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(st[i / 4][qb][i % 4], factor, -shift[qb]));
+        pv[qb] = make_uint4(slc::pack2<T>(p[0], p[1]), slc::pack2<T>(p[2], p[3]), slc::pack2<T>(p[4], p[5]),
+                            slc::pack2<T>(p[6], p[7]));
+      }
+      // Lane c of group g addresses 4 dims of key 4 g + c / 4 and gets dim c of the
+      // group's 4 keys; the second read's keys lie 16 further.
+      const int row = 4 * g + (c >> 2);
+#pragma unroll
+      for (int i = 0; i < S::kQuads; ++i) {
+        const int dim = 16 * i + 4 * (c & 3);
+        const unsigned char* at = vt + row * kRowBytes + (((dim >> 3) ^ (row & 7)) << 4) + (dim & 7) * 2;
+        const uint2 lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * kRowBytes);
+        uint4 va = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        if constexpr (kDirty) va = without_special<T>(va);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) acc[i][qb] = mfma(T{}, va, pv[qb], acc[i][qb]);
+      }
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) acc[S::kQuads][qb] = mfma(T{}, ones, pv[qb], acc[S::kQuads][qb]);
+    }
+  };
 
-    // A weight is exp2(score * factor - shift).
-    float factor = scale_log2, shift[QB];
-    int seen_bits[QB];
-    bool dirty = false;
-    const bool plain = a.mask == nullptr && s0 + KT <= piece.length;
-    if (plain) {
+  // The steps whose rows all nodes see and that have no mask.
+  int plain_steps = a.mask != nullptr ? 0 : piece.length / S::kStep - step0;
+  plain_steps = plain_steps < 0 ? 0 : (plain_steps < nsteps ? plain_steps : nsteps);
+
+  // What the others need: the block's nodes' rows of the tree as bits (a word of ones in
+  // front, for the sequence's rows, a word of zeros behind), and a step's mask, loaded a
+  // step ahead.
+  const int words = (a.nodes + 31) / 32 + 2;
+  if (plain_steps < nsteps && a.tree != nullptr) {
+    int count = quotient(block * S::kRows + S::kRows - 1, group, inverse_group);
+    count = (count < a.nodes ? count : a.nodes - 1) - node0 + 1;
+    const int parts = (a.nodes + 63) / 64;
+#pragma unroll 2
+    for (int item = wave; item < count * parts; item += S::kConsumers) {
+      const int i = item / parts, part = item % parts;
+      const int j = part * 64 + lane;
+      const bool seen = j < a.nodes && a.tree[b * a.tree_sb + (node0 + i) * a.tree_si + j * a.tree_sj] != 0;
+      const uint64_t bits = __ballot(seen);
+      uint32_t* row = tree_bits + i * kMaxWords;
+      if (lane == 0) {
+        row[1 + 2 * part] = static_cast<uint32_t>(bits);
+        row[2 + 2 * part] = static_cast<uint32_t>(bits >> 32);
+        if (part == 0) row[0] = ~0u;
+        if (part == parts - 1) row[words - 1 + (words & 1)] = 0;
+      }
+    }
+  }
+  const bool stages_mask = a.mask != nullptr && tid < S::kStep;
+  auto mask_of = [&](int step) {
+    const int s = (step0 + step) * S::kStep + tid;
+    return step < nsteps && s < piece.end ? slc::load_as_f32(a.mask, b * a.mask_sb + s * a.mask_ss, a.mask_dtype)
+                                          : -INFINITY;
+  };
+  float mask_next = 0.0f;
+  if (stages_mask) {
+    mask_room[0][tid] = mask_of(0);
+    mask_next = mask_of(1);
+  }
+
+  int stage = 0;
+  for (int step = 0; step < plain_steps; ++step) {
+    __syncthreads();  // this step's tiles are in the ring
+    const unsigned char* kt = lds + stage * S::kStageBytes + wk * 2 * kTileBytes;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u) {
+      f32x4_t st[KB][QB];
+      float shift[QB];
+      scores(kt + u * SUB * kRowBytes, st);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         float mx = -INFINITY;
@@ -433,74 +556,64 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[kb][qb][r]);
-        mx *= a.scale;
-        if (__any(mx > m_run[qb] + kThreshold)) {
-          mx = slc::max_xor32(slc::max_xor16(mx));
-          const float m_new = fmaxf(m_run[qb], mx);
-          const float alpha = __builtin_amdgcn_exp2f((m_run[qb] - (m_new == -INFINITY ? 0.0f : m_new)) * kLog2e);
-#pragma unroll
-          for (int i = 0; i < kAcc; ++i) acc[i][qb] = acc[i][qb] * alpha;
-          l_part[qb] *= alpha;
-          m_run[qb] = m_new;
-        }
+        raise(qb, mx * a.scale);
         shift[qb] = m_run[qb] == -INFINITY ? 0.0f : m_run[qb] * kLog2e;
       }
-    } else {
-      // The tail of a sequence, or a mask: scores t = score * scale + mask, -inf where
-      // the row is not seen, then t - max.
-      factor = kLog2e;
+      weigh(std::false_type{}, kt + kTileBytes + u * SUB * kRowBytes, st, scale_log2, shift);
+    }
+  }
+
+  for (int step = plain_steps; step < nsteps; ++step) {
+    __syncthreads();
+    const unsigned char* kt = lds + stage * S::kStageBytes + wk * 2 * kTileBytes;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    if (stages_mask) {
+      mask_room[(step + 1) & 1][tid] = mask_next;
+      mask_next = mask_of(step + 2);
+    }
+#pragma unroll 1
+    for (int u = 0; u < kSubs; ++u) {
+      const int s0 = (step0 + step) * S::kStep + wk * KT + u * SUB;
+      if (s0 >= piece.end) break;
+      f32x4_t st[KB][QB];
+      scores(kt + u * SUB * kRowBytes, st);
+      // Scores t = score * scale + mask, -inf where the row is not seen, less the maximum.
+      const float* mask = a.mask != nullptr ? &mask_room[step & 1][wk * KT + u * SUB] : nullptr;
+      f32x4_t add[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+        add[kb] = mask != nullptr ? *reinterpret_cast<const f32x4_t*>(mask + 16 * kb + 4 * g) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+      const int j0 = s0 - piece.length;  // of the first key, as a node
+      const uint32_t inside = piece.end - s0 >= 32 ? ~0u : (1u << (piece.end - s0)) - 1;
+      uint32_t seen[QB];
       bool hidden = false;
-      float add[KB][4];
-      auto masks = [&](auto load) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int s = s0 + 16 * kb + 4 * g + r;
-            add[kb][r] = s < piece.end ? load(s) : -INFINITY;
-            hidden |= add[kb][r] == -INFINITY;
-          }
-      };
-      const int64_t mask_at = b * a.mask_sb;
-      if (a.mask == nullptr) {
-        masks([](int) { return 0.0f; });
-      } else if (a.mask_dtype == SLC_F32) {
-        masks([&](int s) { return static_cast<const float*>(a.mask)[mask_at + s * a.mask_ss]; });
-      } else if (a.mask_dtype == SLC_BF16) {
-        masks([&](int s) { return slc::to_f32(static_cast<const slc::bf16_t*>(a.mask)[mask_at + s * a.mask_ss]); });
-      } else {
-        masks([&](int s) { return slc::to_f32(static_cast<const slc::f16_t*>(a.mask)[mask_at + s * a.mask_ss]); });
-      }
-      const bool tail = s0 + KT > piece.length;
+      float shift[QB];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
+        seen[qb] = inside;
+        if (j0 > -32) {
+          if (a.tree == nullptr) {
+            const int n = node[qb] - j0 + 1;
+            seen[qb] &= n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1);
+          } else {
+            const uint32_t* row = tree_bits + (node[qb] - node0) * kMaxWords + ((j0 + 32) >> 5);
+            seen[qb] &= __builtin_amdgcn_alignbit(row[1], row[0], (j0 + 32) & 31);
+          }
+        }
+        hidden |= (~seen[qb] & (SUB == 32 ? ~0u : (1u << SUB) - 1)) != 0;
+        const uint32_t mine = seen[qb] >> (4 * g);
         float mx = -INFINITY;
-        seen_bits[qb] = 0;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            bool seen = add[kb][r] != -INFINITY;
-            const int j = s0 + 16 * kb + 4 * g + r - piece.length;
-            if (tail && seen && j >= 0) {
-              seen = a.tree == nullptr ? j <= node[qb]
-                                       : a.tree[b * a.tree_sb + node[qb] * a.tree_si + j * a.tree_sj] != 0;
-              hidden |= !seen;
-            }
-            seen_bits[qb] |= static_cast<int>(seen) << (4 * kb + r);
-            const float t = seen ? fmaf(st[kb][qb][r], a.scale, add[kb][r]) : -INFINITY;
+            hidden |= add[kb][r] == -INFINITY;
+            const bool sees = (mine >> (16 * kb + r) & 1) != 0 && add[kb][r] != -INFINITY;
+            const float t = sees ? fmaf(st[kb][qb][r], a.scale, add[kb][r]) : -INFINITY;
             st[kb][qb][r] = t;
             mx = fmaxf(mx, t);
           }
-        if (__any(mx > m_run[qb] + kThreshold)) {
-          mx = slc::max_xor32(slc::max_xor16(mx));
-          const float m_new = fmaxf(m_run[qb], mx);
-          const float alpha = __builtin_amdgcn_exp2f((m_run[qb] - (m_new == -INFINITY ? 0.0f : m_new)) * kLog2e);
-#pragma unroll
-          for (int i = 0; i < kAcc; ++i) acc[i][qb] = acc[i][qb] * alpha;
-          l_part[qb] *= alpha;
-          m_run[qb] = m_new;
-        }
+        raise(qb, mx);
         const float m_use = m_run[qb] == -INFINITY ? 0.0f : m_run[qb];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -508,89 +621,30 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
           for (int r = 0; r < 4; ++r) st[kb][qb][r] -= m_use;
         shift[qb] = 0.0f;
       }
+      const unsigned char* vt = kt + kTileBytes + u * SUB * kRowBytes;
+      bool dirty = false;
       if (__any(hidden)) {
-        // A weight of zero times NaN or infinity is NaN: where some row of the tile is
-        // hidden from some query, V is searched for them.
+        // A weight of zero times NaN or infinity is NaN: where a row is hidden from a
+        // query, V is searched for them.
         bool special = false;
-        for (int at = lane * 16; at < kTileBytes; at += 1024) {
+        for (int at = lane * 16; at < SUB * kRowBytes; at += 1024) {
           const uint4 v = lds_read(vt + at);
           special |= has_special<T>(v.x) || has_special<T>(v.y) || has_special<T>(v.z) || has_special<T>(v.w);
         }
         dirty = __any(special);
       }
-    }
-
-    // O^T += V^T . P^T; DIRTY: without V's NaNs and infinities.
-    auto weigh = [&](auto dirty_tag) {
-      constexpr bool kDirty = decltype(dirty_tag)::value;
-      if constexpr (kWide) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float p[QB];
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-              p[qb] = __builtin_amdgcn_exp2f(fmaf(st[kb][qb][r], factor, -shift[qb]));
-              l_part[qb] += p[qb];
-            }
-            const int row = 16 * kb + 4 * g + r;
-#pragma unroll
-            for (int d = 0; d < DP / 64; ++d) {
-              uint4 va = lds_read(vt + row * kRowBytes + (((16 * d + c) ^ (row & 7)) << 4));
-              if constexpr (kDirty) va = without_special<T>(va);
-#pragma unroll
-              for (int qb = 0; qb < QB; ++qb) {
-                acc[4 * d][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va.x), p[qb], acc[4 * d][qb], 0, 0, 0);
-                acc[4 * d + 1][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va.y), p[qb], acc[4 * d + 1][qb], 0, 0, 0);
-                acc[4 * d + 2][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va.z), p[qb], acc[4 * d + 2][qb], 0, 0, 0);
-                acc[4 * d + 3][qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(va.w), p[qb], acc[4 * d + 3][qb], 0, 0, 0);
-              }
-            }
-          }
-      } else {
-#pragma unroll
-        for (int half = 0; half < KB / 2; ++half) {
-          uint4 pv[QB];
-#pragma unroll
-          for (int qb = 0; qb < QB; ++qb) {
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              p[i] = __builtin_amdgcn_exp2f(fmaf(st[2 * half + i / 4][qb][i % 4], factor, -shift[qb]));
-            pv[qb] = make_uint4(slc::pack2<T>(p[0], p[1]), slc::pack2<T>(p[2], p[3]), slc::pack2<T>(p[4], p[5]),
-                                slc::pack2<T>(p[6], p[7]));
-          }
-          // Lane c of group g addresses 4 dims of key 4 g + c / 4 and gets dim c of the
-          // group's 4 keys; the second read's keys lie 16 further.
-          const int row = 32 * half + 4 * g + (c >> 2);
-#pragma unroll
-          for (int i = 0; i < S::kQuads; ++i) {
-            const int dim = 16 * i + 4 * (c & 3);
-            const unsigned char* at = vt + row * kRowBytes + (((dim >> 3) ^ (row & 7)) << 4) + (dim & 7) * 2;
-            const uint2 lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * kRowBytes);
-            uint4 va = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            if constexpr (kDirty) va = without_special<T>(va);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) acc[i][qb] = mfma(T{}, va, pv[qb], acc[i][qb]);
-          }
-#pragma unroll
-          for (int qb = 0; qb < QB; ++qb) acc[S::kQuads][qb] = mfma(T{}, ones, pv[qb], acc[S::kQuads][qb]);
-        }
+      if (!dirty) {
+        weigh(std::false_type{}, vt, st, kLog2e, shift);
+        continue;
       }
-    };
-    if (!dirty) {
-      weigh(std::false_type{});
-    } else {
-      weigh(std::true_type{});
+      weigh(std::true_type{}, vt, st, kLog2e, shift);
       // V's NaNs and infinities, for the queries that see their rows.
 #pragma unroll 1
-      for (int row = 0; row < KT; ++row) {
-        // Row 16 kb + 4 from + r: bit 4 kb + r of the lanes of group `from`.
-        const int from = (row & 15) >> 2, bit = (row >> 4) * 4 + (row & 3);
+      for (int row = 0; row < SUB; ++row) {
+        const bool open = mask == nullptr || mask[row] != -INFINITY;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-          const bool seen = (__shfl(seen_bits[qb], 16 * from + c, 64) >> bit & 1) != 0;
+          const bool sees = open && (seen[qb] >> row & 1) != 0;
 #pragma unroll
           for (int i = 0; i < S::kQuads; ++i) {
             const int dim = quad_dim(i);
@@ -604,7 +658,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float f = slc::to_f32(v[e]);
-              const float extra = seen && !(fabsf(f) < INFINITY) ? f : 0.0f;
+              const float extra = sees && !(fabsf(f) < INFINITY) ? f : 0.0f;
               if constexpr (kWide) {
                 acc[4 * (i / 4) + e][qb][i % 4] += extra;
               } else {
@@ -630,83 +684,70 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       return make_float4(acc[i][qb][0], acc[i][qb][1], acc[i][qb][2], acc[i][qb][3]);
     }
   };
-  float4 out[S::kQuads][QB];
-#pragma unroll
-  for (int i = 0; i < S::kQuads; ++i)
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) out[i][qb] = quad(i, qb);
-
-  if constexpr (WK > 1) {
-    // The first tile's waves take in the others' results.
-    constexpr int kFloats = S::kQuads * 4 + 2;
-    __syncthreads();  // the ring is free
-    float* room = reinterpret_cast<float*>(lds);
-    if (wk > 0) {
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        float* mine = room + (((wk - 1) * WR + wr) * QB + qb) * kFloats * 64;
-#pragma unroll
-        for (int i = 0; i < S::kQuads; ++i) reinterpret_cast<float4*>(mine)[i * 64 + lane] = out[i][qb];
-        mine[S::kQuads * 256 + lane] = m_run[qb];
-        mine[S::kQuads * 256 + 64 + lane] = l_run[qb];
-      }
+  const int64_t place = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * a.row_blocks + block;
+  auto store = [&](int i, int qb, float4 v, float top, float sum) {
+    if (!real[qb]) return;
+    const int dim = quad_dim(i);
+    if (piece.count > 1) {
+      const int64_t at = place * S::kRows + wr * 16 * QB + 16 * qb + c;
+      if (dim < a.head_dim) *reinterpret_cast<float4*>(a.partial + at * DP + dim) = v;
+      if (g == 0 && i == 0) a.stats[at] = make_float2(top, sum);
+    } else {
+      T* row = static_cast<T*>(a.output) + b * a.o_sb + head[qb] * a.o_sh + node[qb] * a.o_st;
+      store_quad<T>(row, dim, a.head_dim, a.vector_o, divided(v, sum));
     }
-    __syncthreads();
-    if (wk > 0) return;
+  };
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int i = 0; i < S::kQuads; ++i) store(i, qb, quad(i, qb), m_run[qb], l_run[qb]);
+  } else {
+    // The tiles' results meet in LDS, where each wave takes a share of the outputs.
+    constexpr int kFloats = S::kQuads * 256 + 128;  // of a wave's query block
+    __syncthreads();  // the ring is free
+    float* room = reinterpret_cast<float*>(lds) + wr * QB * kFloats;
+    constexpr int kTile = WR * QB * kFloats;  // from one tile's results to the next's
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      float top = m_run[qb];
+      float* mine = room + wk * kTile + qb * kFloats;
 #pragma unroll
-      for (int k = 1; k < WK; ++k)
-        top = fmaxf(top, room[(((k - 1) * WR + wr) * QB + qb) * kFloats * 64 + S::kQuads * 256 + lane]);
+      for (int i = 0; i < S::kQuads; ++i) reinterpret_cast<float4*>(mine)[i * 64 + lane] = quad(i, qb);
+      mine[S::kQuads * 256 + lane] = m_run[qb];
+      mine[S::kQuads * 256 + 64 + lane] = l_run[qb];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const float* from = room + qb * kFloats;
+      float top = -INFINITY, sum = 0.0f, w[WK];
+#pragma unroll
+      for (int k = 0; k < WK; ++k) {
+        w[k] = from[k * kTile + S::kQuads * 256 + lane];
+        top = fmaxf(top, w[k]);
+      }
       const float use = top == -INFINITY ? 0.0f : top;
-      const float own = __builtin_amdgcn_exp2f((m_run[qb] - use) * kLog2e);
-      l_run[qb] *= own;
 #pragma unroll
-      for (int i = 0; i < S::kQuads; ++i) {
-        out[i][qb].x *= own;
-        out[i][qb].y *= own;
-        out[i][qb].z *= own;
-        out[i][qb].w *= own;
+      for (int k = 0; k < WK; ++k) {
+        w[k] = __builtin_amdgcn_exp2f((w[k] - use) * kLog2e);
+        sum = fmaf(w[k], from[k * kTile + S::kQuads * 256 + 64 + lane], sum);
       }
-#pragma unroll 1
-      for (int k = 1; k < WK; ++k) {
-        const float* other = room + (((k - 1) * WR + wr) * QB + qb) * kFloats * 64;
-        const float w = __builtin_amdgcn_exp2f((other[S::kQuads * 256 + lane] - use) * kLog2e);
-        l_run[qb] = fmaf(w, other[S::kQuads * 256 + 64 + lane], l_run[qb]);
 #pragma unroll
-        for (int i = 0; i < S::kQuads; ++i) {
-          const float4 o = reinterpret_cast<const float4*>(other)[i * 64 + lane];
-          out[i][qb].x = fmaf(w, o.x, out[i][qb].x);
-          out[i][qb].y = fmaf(w, o.y, out[i][qb].y);
-          out[i][qb].z = fmaf(w, o.z, out[i][qb].z);
-          out[i][qb].w = fmaf(w, o.w, out[i][qb].w);
+      for (int n = 0; n < (S::kQuads + WK - 1) / WK; ++n) {
+        // One of wave wk's, a quad number known only at run time.
+        const int i = n * WK + wk;
+        if (i >= S::kQuads) break;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+          const float4 o = reinterpret_cast<const float4*>(from + k * kTile)[i * 64 + lane];
+          v.x = fmaf(w[k], o.x, v.x);
+          v.y = fmaf(w[k], o.y, v.y);
+          v.z = fmaf(w[k], o.z, v.z);
+          v.w = fmaf(w[k], o.w, v.w);
         }
+        store(i, qb, v, top, sum);
       }
-      m_run[qb] = top;
-    }
-  }
-
-  const int64_t place = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * a.row_blocks + block;
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int row = wr * 16 * QB + 16 * qb + c;
-    if (!real[qb]) continue;
-    if (piece.count > 1) {
-      float* partial = a.partial + (place * S::kRows + row) * DP;
-#pragma unroll
-      for (int i = 0; i < S::kQuads; ++i) {
-        const int dim = quad_dim(i);
-        if (dim < a.head_dim) *reinterpret_cast<float4*>(partial + dim) = out[i][qb];
-      }
-      if (g == 0) a.stats[place * S::kRows + row] = make_float2(m_run[qb], l_run[qb]);
-      continue;
-    }
-    T* op = static_cast<T*>(a.output) + b * a.o_sb + head[qb] * a.o_sh + node[qb] * a.o_st;
-#pragma unroll
-    for (int i = 0; i < S::kQuads; ++i) {
-      const int dim = quad_dim(i);
-      store_quad<T>(op, dim, a.head_dim, a.vector_o, divided(out[i][qb], l_run[qb]));
     }
   }
 }
@@ -767,10 +808,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 template <typename T, int DP, int QB, int WR, int KT>
 int launch_shape(const TreeArgs& a, hipStream_t stream) {
   using S = Shape<T, DP, QB, WR, KT>;
-  // Groups of 8 units (a piece of a KV head), each with its row blocks.
-  const int units = a.slots * a.kv_heads;
-  const int min_steps = (kMinPieceRows + S::kStep - 1) / S::kStep;
-  hipLaunchKernelGGL((tree_attention_kernel<T, DP, QB, WR, KT>), dim3((units + 7) / 8 * 8 * a.row_blocks),
+  const float min_steps = static_cast<float>((kMinPieceRows + S::kStep - 1) / S::kStep);
+  hipLaunchKernelGGL((tree_attention_kernel<T, DP, QB, WR, KT>), dim3(a.kv_heads, a.slots, a.row_blocks),
                      dim3(S::kThreads), 0, stream, a, min_steps);
   int status = slc_host::check_launch("tree attention");
   if (status != SLC_OK || a.slots <= a.batch || (a.rows + S::kStep - 1) / S::kStep <= min_steps) return status;
