@@ -699,9 +699,10 @@ SLC_API int slc_hip_linear_q8(const int8_t* input, const float* in_scales, const
  *   lengths int32 or int64; tree bytes; mask fp32, fp16 or bf16; scale > 0.
  *   batch <= 32768; nodes <= SLC_TREE_MAX_NODES, of a chain SLC_CHAIN_MAX_NODES;
  *   capacity <= 2^30, batch * capacity <= 2^34.
- * The workspace (slc_hip_tree_attention_workspace_size bytes, 16-byte aligned; the
- * paged form needs the same) holds the partial results of a split over the rows;
- * calls that may overlap in time need their own.  Table entries that name no page of
+ * The workspace (slc_hip_tree_attention_workspace_size bytes, 16-byte aligned) holds the
+ * partial results of a split over the rows, the counters
+ * (slc_hip_tree_attention_counter_count ints, zero between calls) the arrivals; the paged
+ * form needs the same; calls that may overlap in time need their own.  Table entries that name no page of
  * the pool are not followed; a node that sees rows of such a page has no meaning.
  */
 #define SLC_TREE_MAX_NODES 1024
@@ -709,11 +710,15 @@ SLC_API int slc_hip_linear_q8(const int8_t* input, const float* in_scales, const
 SLC_API int64_t slc_hip_tree_attention_workspace_size(int64_t batch, int64_t q_heads,
                                                       int64_t kv_heads, int64_t nodes,
                                                       int64_t head_dim, int dtype);
+SLC_API int64_t slc_hip_tree_attention_counter_count(int64_t batch, int64_t q_heads,
+                                                     int64_t kv_heads, int64_t nodes,
+                                                     int64_t head_dim, int dtype);
 SLC_API int slc_hip_tree_attention(
     const void* query, const void* key_buffer, const void* value_buffer, const void* lengths,
     int lengths_dtype, const uint8_t* tree, const void* mask, int mask_dtype, void* output,
-    void* workspace, int64_t workspace_bytes, int dtype, int64_t batch, int64_t q_heads,
-    int64_t kv_heads, int64_t nodes, int64_t head_dim, int64_t capacity, int64_t mask_len,
+    void* workspace, int64_t workspace_bytes, int* counters, int64_t num_counters, int dtype,
+    int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t head_dim,
+    int64_t capacity, int64_t mask_len,
     int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, int64_t kv_stride_b,
     int64_t kv_stride_s, int64_t kv_stride_h, int64_t tree_stride_b, int64_t tree_stride_i,
     int64_t tree_stride_j, int64_t mask_stride_b, int64_t mask_stride_s, int64_t out_stride_b,
@@ -723,7 +728,8 @@ SLC_API int slc_hip_paged_tree_attention(
     int64_t table_stride_b, int64_t pages_per_seq, int64_t page_tokens, int64_t num_pages,
     int64_t page_stride, const void* lengths, int lengths_dtype, const uint8_t* tree,
     const void* mask, int mask_dtype, void* output, void* workspace, int64_t workspace_bytes,
-    int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t head_dim,
+    int* counters, int64_t num_counters, int dtype, int64_t batch, int64_t q_heads,
+    int64_t kv_heads, int64_t nodes, int64_t head_dim,
     int64_t mask_len, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
     int64_t kv_stride_s, int64_t kv_stride_h, int64_t tree_stride_b, int64_t tree_stride_i,
     int64_t tree_stride_j, int64_t mask_stride_b, int64_t mask_stride_s, int64_t out_stride_b,

@@ -143,10 +143,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "slc_hip_swiglu_q8": (_I, [_P] * 4 + [_I, _L, _L, _L, _L, _P]),
     "slc_hip_linear_q8": (_I, [_P] * 6 + [_I, _L, _L, _L, _L, _L, _P]),
     "slc_hip_tree_attention_workspace_size": (_L, [_L] * 5 + [_I]),
+    "slc_hip_tree_attention_counter_count": (_L, [_L] * 5 + [_I]),
     "slc_hip_tree_attention": (
-        _I, [_P] * 4 + [_I, _P, _P, _I, _P, _P, _L, _I] + [_L] * 21 + [_F, _P]),
+        _I, [_P] * 4 + [_I, _P, _P, _I, _P, _P, _L, _P, _L, _I] + [_L] * 21 + [_F, _P]),
     "slc_hip_paged_tree_attention": (
-        _I, [_P] * 4 + [_L] * 5 + [_P, _I, _P, _P, _I, _P, _P, _L, _I] + [_L] * 19 + [_F, _P]),
+        _I, [_P] * 4 + [_L] * 5 + [_P, _I, _P, _P, _I, _P, _P, _L, _P, _L, _I] + [_L] * 19 + [_F, _P]),
     "slc_hip_verify_tokens_workspace_size": (_L, [_L, _L]),
     "slc_hip_verify_tokens": (_I, [_P] * 9 + [_L, _P, _L, _I] + [_L] * 10 + [_P]),
     "slc_hip_kv_commit": (_I, [_P] * 5 + [_L] * 4 + [_P] * 3 + [_I] + [_L] * 9 + [_P]),

@@ -20,6 +20,7 @@ The operators are for inference: their outputs carry no gradient.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Sequence
 
 import torch
@@ -80,11 +81,21 @@ def _tree_operands(what, query, key, value, lengths, tree_mask, attention_mask, 
         *tree_strides, *mask_strides)
 
 
-def _workspace(device, index, workspace, batch, q_heads, kv_heads, nodes, head_dim, dtype):
-    nbytes = _native.library().slc_hip_tree_attention_workspace_size(batch, q_heads, kv_heads, nodes, head_dim, dtype)
+@functools.lru_cache(maxsize=1024)
+def _tree_scratch(index, batch, q_heads, kv_heads, nodes, head_dim, dtype):
+    """Workspace bytes and counters of a call, by its sizes."""
+
+    lib = _native.library()
+    sizes = (batch, q_heads, kv_heads, nodes, head_dim, dtype)
+    with torch.cuda.device(index):
+        return (lib.slc_hip_tree_attention_workspace_size(*sizes), lib.slc_hip_tree_attention_counter_count(*sizes))
+
+
+def _tree_workspace(device, index, workspace, *sizes):
+    nbytes, count = _tree_scratch(index, *sizes)
     owner = workspace if workspace is not None else _native.stream_workspace(device)
-    buffer = owner.scratch("tree_attention", nbytes)
-    return (None if buffer is None else buffer.data_ptr()), nbytes
+    counters = owner.counters(count)
+    return owner.scratch("tree_attention", nbytes).data_ptr(), nbytes, counters.data_ptr(), counters.numel()
 
 
 def hip_tree_attention(
@@ -130,9 +141,9 @@ def hip_tree_attention(
         return output
     _, q_heads, nodes, head_dim = query.shape
     dtype = _native.dtype_tag(query.dtype)
-    buffer, nbytes = _workspace(query.device, index, workspace, batch, q_heads, kv_heads, nodes, head_dim, dtype)
+    scratch = _tree_workspace(query.device, index, workspace, batch, q_heads, kv_heads, nodes, head_dim, dtype)
     _call("slc_hip_tree_attention", index, query.data_ptr(), key_buffer.data_ptr(), value_buffer.data_ptr(), *operands,
-          output.data_ptr(), buffer, nbytes, dtype, batch, q_heads, kv_heads, nodes, head_dim, capacity, mask_len,
+          output.data_ptr(), *scratch, dtype, batch, q_heads, kv_heads, nodes, head_dim, capacity, mask_len,
           *query.stride()[:3], *key_buffer.stride()[:3], *strides, *output.stride()[:3], scale)
     return output
 
@@ -170,11 +181,12 @@ def hip_paged_tree_attention(
     if query.numel() == 0:
         return output
     dtype = _native.dtype_tag(query.dtype)
-    buffer, nbytes = _workspace(query.device, index, workspace, batch, q_heads, key_pool.shape[2], nodes, head_dim, dtype)
+    kv_heads = key_pool.shape[2]
+    scratch = _tree_workspace(query.device, index, workspace, batch, q_heads, kv_heads, nodes, head_dim, dtype)
     _call("slc_hip_paged_tree_attention", index, query.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
           block_table.data_ptr(), block_table.stride(0), pages, page_tokens, key_pool.shape[0], key_pool.stride(0),
-          *operands, output.data_ptr(), buffer, nbytes, dtype, batch, q_heads, key_pool.shape[2], nodes, head_dim,
-          mask_len, *query.stride()[:3], *key_pool.stride()[1:3], *strides, *output.stride()[:3], scale)
+          *operands, output.data_ptr(), *scratch, dtype, batch, q_heads, kv_heads, nodes, head_dim, mask_len,
+          *query.stride()[:3], *key_pool.stride()[1:3], *strides, *output.stride()[:3], scale)
     return output
 
 

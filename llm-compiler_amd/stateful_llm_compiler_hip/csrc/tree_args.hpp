@@ -5,6 +5,9 @@
 
 namespace slc_tree {
 
+// Rows that a piece has at least: shorter ones cost more in their results than they save.
+constexpr int kMinPieceRows = 256;
+
 struct TreeArgs {
   const void* query;
   const void* key;
@@ -26,7 +29,8 @@ struct TreeArgs {
   float inverse_slots;
   float* partial;  // [slot, KV head, row block][rows][DP], then their (max, sum) pairs
   float2* stats;
-  int2* pieces;  // per sequence: its first slot and how many
+  int* counters;  // [sequence, KV head, row block], zero between calls; null: a merge kernel
+  int2* pieces;   // for that: per sequence its first slot and how many
 };
 
 // The kernel for `rows` query rows per KV head, and its launch; one pair per type, in

@@ -37,7 +37,7 @@ Split split_for(const Plan& plan, int64_t batch, int64_t kv_heads, int64_t rows)
   return s;
 }
 
-int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, int dtype, int64_t batch,
+int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, int64_t num_counters, int dtype, int64_t batch,
         int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t head_dim, int64_t capacity, int64_t mask_len,
         void* stream) {
   SLC_REQUIRE(slc_host::is_float_dtype(dtype), "%s: bad dtype %d", what, dtype);
@@ -70,6 +70,7 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
   SLC_REQUIRE(workspace != nullptr && workspace_bytes >= split.bytes() &&
                   (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
               "%s: workspace too small or not on 16 bytes", what);
+  SLC_REQUIRE(a.counters != nullptr && num_counters >= batch * kv_heads * split.row_blocks, "%s: too few counters", what);
   a.row_blocks = static_cast<int>(split.row_blocks);
   a.slots = static_cast<int>(split.slots);
   a.inverse_slots = 1.0f / static_cast<float>(split.slots);
@@ -77,6 +78,10 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
   a.partial = reinterpret_cast<float*>(place);
   a.stats = reinterpret_cast<float2*>(place + split.partial_bytes);
   a.pieces = reinterpret_cast<int2*>(place + split.partial_bytes + split.stats_bytes);
+  // What the last piece of a sequence would put together at most; from 64 KB on a merge
+  // kernel does it (see tree_merge_kernel).
+  const int64_t most_pieces = std::min(split.slots - batch + 1, slc_host::ceil_div(a.rows, slc_tree::kMinPieceRows));
+  if (most_pieces * std::min<int64_t>(rows, plan.rows_per_block) * plan.padded_dim * 4 > 65536) a.counters = nullptr;
   const int es = slc_host::dtype_size(dtype);
   const auto on = [es](int64_t bytes, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> sizes) {
     uint64_t bits = 0;
@@ -104,10 +109,19 @@ extern "C" int64_t slc_hip_tree_attention_workspace_size(int64_t batch, int64_t 
   return split_for(plan_for(dtype, static_cast<int>(rows), static_cast<int>(head_dim)), batch, kv_heads, rows).bytes();
 }
 
+extern "C" int64_t slc_hip_tree_attention_counter_count(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes,
+                                                        int64_t head_dim, int dtype) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || nodes <= 0 || head_dim <= 0 || !slc_host::is_float_dtype(dtype))
+    return 0;
+  const int64_t rows = q_heads / kv_heads * nodes;
+  const Plan plan = plan_for(dtype, static_cast<int>(rows), static_cast<int>(head_dim));
+  return batch * kv_heads * slc_host::ceil_div(rows, plan.rows_per_block);
+}
+
 extern "C" int slc_hip_tree_attention(
     const void* query, const void* key_buffer, const void* value_buffer, const void* lengths, int lengths_dtype,
     const uint8_t* tree, const void* mask, int mask_dtype, void* output, void* workspace, int64_t workspace_bytes,
-    int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t head_dim, int64_t capacity,
+    int* counters, int64_t num_counters, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t head_dim, int64_t capacity,
     int64_t mask_len, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, int64_t kv_stride_b,
     int64_t kv_stride_s, int64_t kv_stride_h, int64_t tree_stride_b, int64_t tree_stride_i, int64_t tree_stride_j,
     int64_t mask_stride_b, int64_t mask_stride_s, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t,
@@ -127,8 +141,9 @@ extern "C" int slc_hip_tree_attention(
   a.tree_sb = tree_stride_b, a.tree_si = tree_stride_i, a.tree_sj = tree_stride_j;
   a.mask_sb = mask_stride_b, a.mask_ss = mask_stride_s;
   a.o_sb = out_stride_b, a.o_sh = out_stride_h, a.o_st = out_stride_t;
+  a.counters = counters;
   a.scale = scale;
-  return run("slc_hip_tree_attention", a, workspace, workspace_bytes, dtype, batch, q_heads, kv_heads, nodes, head_dim,
+  return run("slc_hip_tree_attention", a, workspace, workspace_bytes, num_counters, dtype, batch, q_heads, kv_heads, nodes, head_dim,
              capacity, mask_len, stream);
 }
 
@@ -136,8 +151,8 @@ extern "C" int slc_hip_paged_tree_attention(
     const void* query, const void* key_pool, const void* value_pool, const int32_t* block_table,
     int64_t table_stride_b, int64_t pages_per_seq, int64_t page_tokens, int64_t num_pages, int64_t page_stride,
     const void* lengths, int lengths_dtype, const uint8_t* tree, const void* mask, int mask_dtype, void* output,
-    void* workspace, int64_t workspace_bytes, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
-    int64_t nodes, int64_t head_dim, int64_t mask_len, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+    void* workspace, int64_t workspace_bytes, int* counters, int64_t num_counters, int dtype, int64_t batch,
+    int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t head_dim, int64_t mask_len, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
     int64_t kv_stride_s, int64_t kv_stride_h, int64_t tree_stride_b, int64_t tree_stride_i, int64_t tree_stride_j,
     int64_t mask_stride_b, int64_t mask_stride_s, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t,
     float scale, void* stream) {
@@ -166,7 +181,8 @@ extern "C" int slc_hip_paged_tree_attention(
   a.tree_sb = tree_stride_b, a.tree_si = tree_stride_i, a.tree_sj = tree_stride_j;
   a.mask_sb = mask_stride_b, a.mask_ss = mask_stride_s;
   a.o_sb = out_stride_b, a.o_sh = out_stride_h, a.o_st = out_stride_t;
+  a.counters = counters;
   a.scale = scale;
-  return run(what, a, workspace, workspace_bytes, dtype, batch, q_heads, kv_heads, nodes, head_dim,
+  return run(what, a, workspace, workspace_bytes, num_counters, dtype, batch, q_heads, kv_heads, nodes, head_dim,
              pages_per_seq * page_tokens, mask_len, stream);
 }

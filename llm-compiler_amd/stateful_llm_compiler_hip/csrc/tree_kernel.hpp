@@ -20,7 +20,7 @@
 //  * O^T[dim, query] += V^T . P^T: the score tile's C layout is the product's B layout
 //    once V's rows are taken in the same order.
 // The WK partial results meet in LDS; the pieces' partial results, where a sequence
-// has several, in tree_merge_kernel.
+// has several, in the last of them to end.
 #pragma once
 #include <cmath>
 #include <type_traits>
@@ -31,7 +31,6 @@ namespace slc_tree {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kThreshold = 5.5f;  // weights stay under e^5.5 = 245, fp16's range is 65504
-constexpr int kMinPieceRows = 256;
 
 namespace {
 
@@ -126,6 +125,11 @@ __device__ __forceinline__ void store_quad(T* row, int dim, int head_dim, bool v
   for (int i = 0; i < 4; ++i)
     if (dim + i < head_dim) row[dim + i] = slc::from_f32<T>(e[i]);
 }
+// First dim of the i-th four neighbouring outputs that a lane of group g holds.
+template <typename T>
+__device__ __forceinline__ int quad_dim(int i, int g) {
+  return sizeof(T) == 4 ? 64 * (i / 4) + 16 * g + 4 * (i % 4) : 16 * i + 4 * g;
+}
 // A sum of weights of zero: a node that sees no row, NaN.
 __device__ __forceinline__ float4 divided(float4 v, float sum) {
   const float by = sum == 0.0f ? __builtin_nanf("") : 1.0f / sum;
@@ -138,6 +142,9 @@ __device__ __forceinline__ int quotient(int n, int d, float inverse) {
   const int rest = n - q * d;
   return q + (rest >= d) - (rest < 0);
 }
+
+// The tail, whose rows only some nodes see, takes as long as so many steps more.
+constexpr int kTailSteps = 2;
 
 struct Piece {
   int sequence;  // -1: none
@@ -158,8 +165,8 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
   };
   auto end_of = [&](int length) { return length + a.nodes < rows ? length + a.nodes : rows; };
   auto steps_of = [&](int b, int length) {
-    const int n = (end_of(length) + STEP - 1) / STEP;
-    return b < a.batch ? (n > 1 ? n : 1) : 0;
+    const int n = (end_of(length) + STEP - 1) / STEP + kTailSteps;
+    return b < a.batch ? n : 0;
   };
   // Of the first 64 sequences; more are read again in every pass.
   const int own_length = length_of(lane), own = steps_of(lane, own_length);
@@ -197,6 +204,95 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
   return p;
 }
 
+// The pieces [first, first + count) of a sequence's row block put together by `threads`
+// threads: each takes kItems times four dims of a row, over a batch of pieces at a time.
+template <typename T, int DP, int ROWS, int kItems>
+__device__ __forceinline__ void merge_pieces(const TreeArgs& a, int64_t b, int kvh, int block, int first, int count,
+                                             int thread, int threads) {
+  constexpr int kBatch = 4, kQuads = DP / 16;
+  const int group = a.q_heads / a.kv_heads;
+  const float inverse_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
+  const int rows = group * a.nodes - block * ROWS < ROWS ? group * a.nodes - block * ROWS : ROWS;
+  const int items = (rows + 15) / 16 * kQuads * 64;  // a block of 16 rows, its quads, a wave's lanes
+  const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.row_blocks * ROWS;  // between pieces
+  const int64_t place = ((static_cast<int64_t>(first) * a.kv_heads + kvh) * a.row_blocks + block) * ROWS;
+  auto row_of = [](int item) { return item / (64 * kQuads) * 16 + (item & 15); };
+#pragma unroll 1
+  for (int base = thread; base < items; base += kItems * threads) {
+    float top[kItems], sum[kItems];
+    float4 v[kItems];
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      top[j] = -INFINITY;
+      sum[j] = 0.0f;
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll 1
+    for (int at = 0; at < count; at += kBatch) {
+      float2 s[kItems][kBatch];
+      float4 o[kItems][kBatch];
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        const int item = base + j * threads < items ? base + j * threads : base;
+        const float2* stats = a.stats + place + row_of(item);
+        const float* partial = a.partial + place * DP + item * 4;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const bool is = at + i < count;
+          const int64_t k = (is ? at + i : at) * stride;
+          s[j][i] = stats[k];
+          o[j][i] = *reinterpret_cast<const float4*>(partial + k * DP);
+          if (!is) {
+            s[j][i] = make_float2(-INFINITY, 0.0f);
+            o[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        float most = top[j];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) most = fmaxf(most, s[j][i].x);
+        const float use = most == -INFINITY ? 0.0f : most;
+        const float own = __builtin_amdgcn_exp2f((top[j] - use) * kLog2e);
+        top[j] = most;
+        sum[j] *= own;
+        v[j] = make_float4(v[j].x * own, v[j].y * own, v[j].z * own, v[j].w * own);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const float w = __builtin_amdgcn_exp2f((s[j][i].x - use) * kLog2e);
+          sum[j] = fmaf(w, s[j][i].y, sum[j]);
+          v[j].x = fmaf(w, o[j][i].x, v[j].x);
+          v[j].y = fmaf(w, o[j][i].y, v[j].y);
+          v[j].z = fmaf(w, o[j][i].z, v[j].z);
+          v[j].w = fmaf(w, o[j][i].w, v[j].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const int item = base + j * threads;
+      const int row = block * ROWS + row_of(item);
+      const int dim = quad_dim<T>(item / 64 % kQuads, item >> 4 & 3);
+      if (item >= items || row >= group * a.nodes) continue;
+      const int n = quotient(row, group, inverse_group);
+      const int h = kvh * group + row - n * group;
+      store_quad<T>(static_cast<T*>(a.output) + b * a.o_sb + h * a.o_sh + n * a.o_st, dim, a.head_dim, a.vector_o,
+                    divided(v[j], sum[j]));
+    }
+  }
+}
+// The same for large blocks, by workgroups of their own: one CU takes in about 10 bytes
+// a cycle, so that one workgroup is slow from some 64 KB on.
+template <typename T, int DP, int ROWS>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+  const int64_t b = blockIdx.z;
+  const int2 pieces = a.pieces[b];
+  if (pieces.y <= 1) return;
+  const int kvh = blockIdx.y / a.row_blocks, block = blockIdx.y % a.row_blocks;
+  merge_pieces<T, DP, ROWS, 1>(a, b, kvh, block, pieces.x, pieces.y, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+}
+
 // Sizes of a kernel: DP the padded head dim, QB blocks of 16 query rows a wave, WR waves
 // along the rows, KT keys a tile.
 template <typename T, int DP, int QB, int WR, int KT>
@@ -216,8 +312,10 @@ struct Shape {
   static constexpr int kProducers = kStep >= 64 ? 4 : kStep / 16;
   static constexpr int kThreads = (kConsumers + kProducers) * 64;
   static constexpr int kStageBytes = WK * 2 * kTileBytes;
-  static constexpr int kStages = kStageBytes <= 16384 ? 4 : (kStageBytes <= 32768 ? 3 : 2);
   static constexpr int kOps = kStageBytes / 1024 / kProducers;  // a producer's loads of a step
+  // Up to eight stages in 128 KB, and no more loads in flight than the wait can count.
+  static constexpr int kFill = 131072 / kStageBytes < 8 ? 131072 / kStageBytes : 8;
+  static constexpr int kStages = (kFill - 2) * kOps < 64 ? kFill : 63 / kOps + 2;
   static constexpr int kRows = 16 * QB * WR;
   static constexpr int kQuads = DP / 16;           // float4 of a lane's outputs per query block
   static constexpr int kMergeBytes = WK > 1 ? WK * WR * QB * (kQuads * 4 + 2) * 256 : 0;
@@ -239,20 +337,23 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   constexpr int kMaxWords = SLC_TREE_MAX_NODES / 32 + 2;
   __shared__ uint32_t tree_bits[(S::kRows + 1) * kMaxWords];
   __shared__ __attribute__((aligned(16))) float mask_room[2][S::kStep];
+  __shared__ int arrived;
 
   const int kvh = blockIdx.x, slot = blockIdx.y, block = blockIdx.z;
   const Piece piece = find_piece<S::kStep>(a, slot, min_steps);
   if (piece.sequence < 0) return;
   const int64_t b = piece.sequence;
-  // Its steps: the sequence's, shared out as evenly as whole steps go.
-  const int steps = piece.end > S::kStep ? (piece.end + S::kStep - 1) / S::kStep : 1;
-  const int share = static_cast<int>(static_cast<unsigned>(steps) / static_cast<unsigned>(piece.count));
-  const int spare = steps - share * piece.count;
-  const int step0 = piece.index * share + (piece.index < spare ? piece.index : spare);
-  const int nsteps = share + (piece.index < spare ? 1 : 0);
+  // Its steps: the sequence's and its tail's, shared out as evenly as whole steps go.
+  const int steps = (piece.end + S::kStep - 1) / S::kStep;
+  const int shared = steps + kTailSteps;
+  const int share = static_cast<int>(static_cast<unsigned>(shared) / static_cast<unsigned>(piece.count));
+  const int spare = shared - share * piece.count;
+  const int step0 = min(steps, piece.index * share + min(piece.index, spare));
+  const int nsteps = min(steps, step0 + share + (piece.index < spare ? 1 : 0)) - step0;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (tid == 0 && piece.index == 0 && kvh == 0 && block == 0) a.pieces[b] = make_int2(piece.first, piece.count);
+  if (a.counters == nullptr && tid == 0 && piece.index == 0 && kvh == 0 && block == 0)
+    a.pieces[b] = make_int2(piece.first, piece.count);
 
   if (wave >= S::kConsumers) {
     // ---- producers ------------------------------------------------------------
@@ -287,7 +388,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       unsigned char* dst = lds + step % S::kStages * S::kStageBytes;
       const int s0 = (step0 + step) * S::kStep;
       const int end = step < nsteps ? piece.end : 0;
-      if (a.vector_kv) {
+      if (__builtin_expect(a.vector_kv, 1)) {
         for (int first = part0; first < part0 + kPart; first += segment) {
           int rows = end - s0 - first;  // rows past the last one read as zero
           rows = rows < segment ? rows : segment;
@@ -374,7 +475,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
     for (int kk = 0; kk < kParts; ++kk) {
       constexpr int kPer = 16 / ES;
       const int dim = kk * kDims + kPer * g;
-      if (a.vector_q) {
+      if (__builtin_expect(a.vector_q, 1)) {
         qv[qb][kk] = dim < a.head_dim ? *reinterpret_cast<const uint4*>(qp + dim) : make_uint4(0, 0, 0, 0);
       } else {
         T e[kPer] = {};
@@ -399,8 +500,6 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 #pragma unroll
     for (int i = 0; i < kAcc; ++i) acc[i][qb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  // First dim of a lane's i-th four neighbouring outputs.
-  auto quad_dim = [&](int i) { return kWide ? 64 * (i / 4) + 16 * g + 4 * (i % 4) : 16 * i + 4 * g; };
   const uint32_t one2 = std::is_same_v<T, slc::bf16_t> ? 0x3f803f80u : 0x3c003c00u;
   const uint4 ones = make_uint4(one2, one2, one2, one2);
   const float scale_log2 = a.scale * kLog2e;
@@ -633,7 +732,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
         }
         dirty = __any(special);
       }
-      if (!dirty) {
+      if (__builtin_expect(!dirty, 1)) {
         weigh(std::false_type{}, vt, st, kLog2e, shift);
         continue;
       }
@@ -647,7 +746,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
           const bool sees = open && (seen[qb] >> row & 1) != 0;
 #pragma unroll
           for (int i = 0; i < S::kQuads; ++i) {
-            const int dim = quad_dim(i);
+            const int dim = quad_dim<T>(i, g);
             const unsigned char* at = vt + row * kRowBytes + (((dim * ES >> 4) ^ (row & 7)) << 4) + (dim * ES & 15);
             T v[4];
             if constexpr (kWide) {
@@ -687,11 +786,11 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   const int64_t place = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * a.row_blocks + block;
   auto store = [&](int i, int qb, float4 v, float top, float sum) {
     if (!real[qb]) return;
-    const int dim = quad_dim(i);
+    const int dim = quad_dim<T>(i, g);
     if (piece.count > 1) {
-      const int64_t at = place * S::kRows + wr * 16 * QB + 16 * qb + c;
-      if (dim < a.head_dim) *reinterpret_cast<float4*>(a.partial + at * DP + dim) = v;
-      if (g == 0 && i == 0) a.stats[at] = make_float2(top, sum);
+      // As the lanes hold them, so that a wave writes whole lines.
+      reinterpret_cast<float4*>(a.partial + place * S::kRows * DP)[((wr * QB + qb) * S::kQuads + i) * 64 + lane] = v;
+      if (g == 0 && i == 0) a.stats[place * S::kRows + wr * 16 * QB + 16 * qb + c] = make_float2(top, sum);
     } else {
       T* row = static_cast<T*>(a.output) + b * a.o_sb + head[qb] * a.o_sh + node[qb] * a.o_st;
       store_quad<T>(row, dim, a.head_dim, a.vector_o, divided(v, sum));
@@ -750,59 +849,20 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       }
     }
   }
-}
+  if (piece.count == 1 || a.counters == nullptr) return;
 
-// The pieces of a sequence together: a thread per four dims of a row.
-template <typename T, int DP, int ROWS>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
-  const int64_t b = blockIdx.z;
-  const int kvh = blockIdx.y;
-  const int2 pieces = a.pieces[b];
-  if (pieces.y <= 1) return;
-  const int quads = (a.head_dim + 3) / 4;
-  const int item = blockIdx.x * 256 + threadIdx.x;
-  const int row = item / quads, dim = item % quads * 4;
-  const int group = a.q_heads / a.kv_heads;
-  if (row >= group * a.nodes) return;
-  const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.row_blocks;
-  const int64_t place = pieces.x * stride + static_cast<int64_t>(kvh) * a.row_blocks + row / ROWS;
-  const float2* stats = a.stats + place * ROWS + row % ROWS;
-  const float* partial = a.partial + (place * ROWS + row % ROWS) * DP + dim;
-  float top = -INFINITY, sum = 0.0f;
-  float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int kBatch = 8;
-  for (int first = 0; first < pieces.y; first += kBatch) {
-    float2 s[kBatch];
-    float4 o[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int64_t at = (first + i < pieces.y ? first + i : first) * stride * ROWS;
-      s[i] = stats[at];
-      o[i] = *reinterpret_cast<const float4*>(partial + at * DP);
-      if (first + i >= pieces.y) s[i] = make_float2(-INFINITY, 0.0f);
-    }
-    float most = top;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) most = fmaxf(most, s[i].x);
-    const float use = most == -INFINITY ? 0.0f : most;
-    const float own = __builtin_amdgcn_exp2f((top - use) * kLog2e);
-    top = most;
-    sum *= own;
-    out = make_float4(out.x * own, out.y * own, out.z * own, out.w * own);
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (first + i >= pieces.y) continue;
-      const float w = __builtin_amdgcn_exp2f((s[i].x - use) * kLog2e);
-      sum = fmaf(w, s[i].y, sum);
-      out.x = fmaf(w, o[i].x, out.x);
-      out.y = fmaf(w, o[i].y, out.y);
-      out.z = fmaf(w, o[i].z, out.z);
-      out.w = fmaf(w, o[i].w, out.w);
-    }
+  // The last of a sequence's pieces to arrive puts all of them together: every wave's
+  // results come before the barrier, the count is an agent-scope acquire-release add.
+  const int mine = (piece.sequence * a.kv_heads + kvh) * a.row_blocks + block;
+  __syncthreads();
+  if (tid == 0) {
+    arrived = __hip_atomic_fetch_add(&a.counters[mine], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    if (arrived == piece.count - 1) __hip_atomic_store(&a.counters[mine], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  const int node = row / group, head = kvh * group + row % group;
-  store_quad<T>(static_cast<T*>(a.output) + b * a.o_sb + head * a.o_sh + node * a.o_st, dim, a.head_dim, a.vector_o,
-                divided(out, sum));
+  __syncthreads();
+  if (__builtin_amdgcn_readfirstlane(arrived) != piece.count - 1) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  merge_pieces<T, DP, S::kRows, 2>(a, piece.sequence, kvh, block, piece.first, piece.count, tid, S::kConsumers * 64);
 }
 
 template <typename T, int DP, int QB, int WR, int KT>
@@ -811,11 +871,13 @@ int launch_shape(const TreeArgs& a, hipStream_t stream) {
   const float min_steps = static_cast<float>((kMinPieceRows + S::kStep - 1) / S::kStep);
   hipLaunchKernelGGL((tree_attention_kernel<T, DP, QB, WR, KT>), dim3(a.kv_heads, a.slots, a.row_blocks),
                      dim3(S::kThreads), 0, stream, a, min_steps);
-  int status = slc_host::check_launch("tree attention");
-  if (status != SLC_OK || a.slots <= a.batch || (a.rows + S::kStep - 1) / S::kStep <= min_steps) return status;
-  const int items = a.q_heads / a.kv_heads * a.nodes * ((a.head_dim + 3) / 4);
-  hipLaunchKernelGGL((tree_merge_kernel<T, DP, S::kRows>), dim3((items + 255) / 256, a.kv_heads, a.batch), dim3(256), 0,
-                     stream, a);
+  const int status = slc_host::check_launch("tree attention");
+  // Its pieces are put together by the last of them, or by another kernel; there are none
+  // where every sequence is one.
+  if (status != SLC_OK || a.counters != nullptr || a.slots <= a.batch || a.rows <= kMinPieceRows) return status;
+  const int items = S::kRows * DP / 4;
+  hipLaunchKernelGGL((tree_merge_kernel<T, DP, S::kRows>), dim3((items + 255) / 256, a.kv_heads * a.row_blocks, a.batch),
+                     dim3(256), 0, stream, a);
   return slc_host::check_launch("tree attention merge");
 }
 

@@ -30,7 +30,7 @@ def test_wrappers_refuse_host_tensors():
 
 
 def tree(paged=False, query=P, key=P, value=P, lengths=P, lengths_dtype=I64, mask=None, mask_dtype=F32, out=P,
-         workspace=P, nbytes=1 << 40, dtype=BF16, batch=2, q_heads=4, kv_heads=2, nodes=3, head_dim=64, rows=64,
+         workspace=P, nbytes=1 << 40, counters=P, num_counters=1 << 20, dtype=BF16, batch=2, q_heads=4, kv_heads=2, nodes=3, head_dim=64, rows=64,
          mask_len=64, scale=0.125, tree_mask=None, table=P, page_tokens=16, num_pages=9, kv_ss=128):
     lib = _native.library()
     tail = (scale, None)
@@ -38,10 +38,10 @@ def tree(paged=False, query=P, key=P, value=P, lengths=P, lengths_dtype=I64, mas
     if paged:
         return lib.slc_hip_paged_tree_attention(
             query, key, value, table, rows // 16, rows // 16, page_tokens, num_pages, 16 * kv_ss, lengths,
-            lengths_dtype, tree_mask, mask, mask_dtype, out, workspace, nbytes, dtype, batch, q_heads, kv_heads, nodes,
+            lengths_dtype, tree_mask, mask, mask_dtype, out, workspace, nbytes, counters, num_counters, dtype, batch, q_heads, kv_heads, nodes,
             head_dim, mask_len, *strides, kv_ss, head_dim, 0, 0, 0, 0, 0, *strides, *tail)
     return lib.slc_hip_tree_attention(
-        query, key, value, lengths, lengths_dtype, tree_mask, mask, mask_dtype, out, workspace, nbytes, dtype, batch,
+        query, key, value, lengths, lengths_dtype, tree_mask, mask, mask_dtype, out, workspace, nbytes, counters, num_counters, dtype, batch,
         q_heads, kv_heads, nodes, head_dim, rows, mask_len, *strides, rows * kv_ss, kv_ss, head_dim, 0, 0, 0, 0, 0,
         *strides, *tail)
 
@@ -51,6 +51,7 @@ def test_tree_attention_entry_points_refuse(paged):
     for bad in ({"dtype": I32}, {"dtype": 99}, {"lengths_dtype": F32}, {"batch": -1}, {"batch": 32769},
                 {"nodes": -1}, {"nodes": 4097}, {"nodes": 1025, "tree_mask": P}, {"rows": 2**30, "batch": 17}, {"q_heads": 3}, {"q_heads": 0}, {"kv_heads": 0}, {"head_dim": 0},
                 {"head_dim": 257}, {"query": None}, {"key": None}, {"value": None}, {"lengths": None}, {"out": None},
+                {"workspace": None}, {"workspace": P + 8}, {"nbytes": 1000}, {"counters": None}, {"num_counters": 3},
                 {"scale": 0.0}, {"scale": -1.0}, {"scale": float("nan")}, {"scale": float("inf")},
                 {"mask": P, "mask_dtype": I32}, {"mask": P, "mask_len": 65}, {"mask": P, "mask_len": -1}):
         assert tree(paged, **bad) == -1, bad
