@@ -301,9 +301,9 @@ struct Shape {
   static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
   static constexpr int kTileBytes = KT * kRowBytes;  // of K or of V
   // Tiles side by side: eight waves (four of wide rows, whose registers no more than
-  // two a SIMD have), 64 KB a step at most.
+  // two a SIMD have), 32 KB a step at most.
   static constexpr int kWaves = kRowBytes <= 256 ? 8 : 4;
-  static constexpr int kFit = 65536 / (2 * kTileBytes);
+  static constexpr int kFit = 32768 / (2 * kTileBytes);
   static constexpr int WK = kWaves / WR < kFit ? kWaves / WR : kFit;
   static constexpr int kConsumers = WR * WK;
   static constexpr int kStep = WK * KT;
@@ -313,10 +313,13 @@ struct Shape {
   static constexpr int kThreads = (kConsumers + kProducers) * 64;
   static constexpr int kStageBytes = WK * 2 * kTileBytes;
   static constexpr int kOps = kStageBytes / 1024 / kProducers;  // a producer's loads of a step
-  // Up to eight stages in 128 KB, and no more loads in flight than the wait can count.
-  static constexpr int kFill = 131072 / kStageBytes < 8 ? 131072 / kStageBytes : 8;
-  static constexpr int kStages = (kFill - 2) * kOps < 64 ? kFill : 63 / kOps + 2;
   static constexpr int kRows = 16 * QB * WR;
+  static constexpr int kWords = SLC_TREE_MAX_NODES / 32 + 2;  // of a node's row of the tree, as bits
+  // Up to eight stages in what the rest leaves of 160 KB, and no more loads in flight than
+  // the wait can count.
+  static constexpr int kFree = 160 * 1024 - (kRows + 1) * kWords * 4 - 2 * kStep * 4 - 64;
+  static constexpr int kFill = kFree / kStageBytes < 8 ? kFree / kStageBytes : 8;
+  static constexpr int kStages = (kFill - 2) * kOps < 64 ? kFill : 63 / kOps + 2;
   static constexpr int kQuads = DP / 16;           // float4 of a lane's outputs per query block
   static constexpr int kMergeBytes = WK > 1 ? WK * WR * QB * (kQuads * 4 + 2) * 256 : 0;
   static constexpr int kLds = kStages * kStageBytes > kMergeBytes ? kStages * kStageBytes : kMergeBytes;
@@ -334,7 +337,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   constexpr int kChunks = kRowBytes / 16, kOpRows = 1024 / kRowBytes;
   constexpr int ES = sizeof(T);
   __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
-  constexpr int kMaxWords = SLC_TREE_MAX_NODES / 32 + 2;
+  constexpr int kMaxWords = S::kWords;
   __shared__ uint32_t tree_bits[(S::kRows + 1) * kMaxWords];
   __shared__ __attribute__((aligned(16))) float mask_room[2][S::kStep];
   __shared__ int arrived;
@@ -643,23 +646,25 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
     __syncthreads();  // this step's tiles are in the ring
     const unsigned char* kt = lds + stage * S::kStageBytes + wk * 2 * kTileBytes;
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    f32x4_t st[kSubs][KB][QB];
+    float shift[QB];
 #pragma unroll
-    for (int u = 0; u < kSubs; ++u) {
-      f32x4_t st[KB][QB];
-      float shift[QB];
-      scores(kt + u * SUB * kRowBytes, st);
+    for (int u = 0; u < kSubs; ++u) scores(kt + u * SUB * kRowBytes, st[u]);
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        float mx = -INFINITY;
+    for (int qb = 0; qb < QB; ++qb) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[kb][qb][r]);
-        raise(qb, mx * a.scale);
-        shift[qb] = m_run[qb] == -INFINITY ? 0.0f : m_run[qb] * kLog2e;
-      }
-      weigh(std::false_type{}, kt + kTileBytes + u * SUB * kRowBytes, st, scale_log2, shift);
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[u][kb][qb][r]);
+      raise(qb, mx * a.scale);
+      shift[qb] = m_run[qb] == -INFINITY ? 0.0f : m_run[qb] * kLog2e;
     }
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u)
+      weigh(std::false_type{}, kt + kTileBytes + u * SUB * kRowBytes, st[u], scale_log2, shift);
   }
 
   for (int step = plain_steps; step < nsteps; ++step) {
@@ -905,13 +910,14 @@ int launch_dim(const TreeArgs& a, int rows, hipStream_t stream) {
   constexpr int kBytes = DP * static_cast<int>(sizeof(T));
   constexpr int kQb = query_blocks<kBytes>(), kRows = 16 * kQb;
   constexpr int kKeys = kBytes == 1024 ? 16 : 32;
+  constexpr int kMore = kBytes == 128 ? 64 : kKeys;
   if constexpr (kQb > 1)
     if (rows == 16) return launch_shape<T, DP, 1, 1, kKeys>(a, stream);
   if (rows == kRows) return launch_shape<T, DP, kQb, 1, kKeys>(a, stream);
   if (rows == 2 * kRows) return launch_shape<T, DP, kQb, 2, kKeys>(a, stream);
   if constexpr (most_waves<kBytes>() > 4)
-    if (rows == 8 * kRows) return launch_shape<T, DP, kQb, 8, kKeys>(a, stream);
-  return launch_shape<T, DP, kQb, 4, kKeys>(a, stream);
+    if (rows == 8 * kRows) return launch_shape<T, DP, kQb, 8, kMore>(a, stream);
+  return launch_shape<T, DP, kQb, 4, kMore>(a, stream);
 }
 
 template <typename T>

@@ -25,6 +25,7 @@
 // passes over its row (the mass decides the next test); the last workgroup makes
 // them alone.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -34,6 +35,7 @@ constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBlock = 1024;  // weights per sum, 16 a lane
 constexpr int kPerLane = kBlock / 64;
+constexpr int kGroup = 4;  // neighbouring sums that a lane takes
 constexpr int kMaxNodes = SLC_VERIFY_MAX_NODES;
 
 struct VerifyArgs {
@@ -52,48 +54,195 @@ struct VerifyArgs {
   bool vector_ok;  // rows start on 16 bytes
 };
 
-// The weights of a row: max(p - mass * q, 0), or p without the listed tokens.
-template <typename P>
-struct Row {
-  const P* p;
-  const P* q;  // null: no draft row
-  double mass;
-  const int* skip;
-  int skips;
+// A value that all lanes share, in scalar registers: the walk's branches are the wave's.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits), lane));
+  const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits >> 32), lane));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+__device__ __forceinline__ double uniform(double v) { return lane_value(v, 0); }
 
-  __device__ __forceinline__ double value(float pv, float qv) const {
-    const double w = static_cast<double>(pv) - mass * static_cast<double>(qv);
-    return w > 0.0 ? w : 0.0;  // NaN has no weight
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), CTRL, ROWS, 0xf, false));
+  const uint64_t hi = static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), CTRL, ROWS, 0xf, false));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+// Sums up to and with this lane: rows of 16 lanes by shifts, then the rows below by
+// broadcasts of their last lanes.
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp<0x111, 0xf>(v);  // row_shr:1
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // row_bcast:15
+  v += dpp<0x143, 0xc>(v);  // row_bcast:31
+  return v;
+}
+
+// The nodes of a sequence.  Up to 64: one a lane, in registers of every wave.
+struct LaneNodes {
+  int above, token;  // parent and token, -1: none
+  double prob;       // target's probability of the token behind the parent
+  int place;         // lane j: the path's j-th node
+
+  __device__ __forceinline__ int token_of(int c) const { return __builtin_amdgcn_readlane(token, c); }
+  __device__ __forceinline__ double prob_of(int c) const { return lane_value(prob, c); }
+  __device__ __forceinline__ int next_child(int node, int after) const {
+    const uint64_t later = after >= 63 ? 0 : ~uint64_t{0} << (after + 1);
+    const uint64_t hits = __ballot(above == node) & later;
+    return hits != 0 ? __builtin_ctzll(hits) : -1;
   }
+  // Whether an elder sibling of node c has its token.
+  __device__ __forceinline__ bool again(int node, int c) const {
+    return (__ballot(above == node && token == token_of(c)) & ((uint64_t{1} << c) - 1)) != 0;
+  }
+  __device__ __forceinline__ void put(int at, int node) { place = (threadIdx.x & 63) == static_cast<unsigned>(at) ? node : place; }
+};
+// More: in LDS, which the workgroup's waves fill together.
+struct SharedNodes {
+  int* above;
+  int* token;
+  double* prob;
+  int* path;
+  int nodes;
 
-  // Column of the lane's i-th weight of the block at `base`.  DENSE: 16 neighbours a
-  // lane, for a scan in order; else as coalesced loads (16 bytes a lane, or one
-  // element) have them.
-  template <bool DENSE>
-  static __device__ __forceinline__ int64_t index(int64_t base, int i, bool vector) {
-    constexpr int kVec = 16 / sizeof(P);
+  __device__ __forceinline__ int token_of(int c) const { return uniform(token[c]); }
+  __device__ __forceinline__ double prob_of(int c) const { return uniform(prob[c]); }
+  __device__ __forceinline__ int next_child(int node, int after) const {
     const int lane = threadIdx.x & 63;
-    if constexpr (DENSE) return base + lane * kPerLane + i;
-    return vector ? base + (i / kVec) * (64 * kVec) + lane * kVec + i % kVec : base + i * 64 + lane;
+    for (int base = (after + 1) & ~63; base < nodes; base += 64) {
+      const int c = base + lane;
+      const uint64_t hits = __ballot(c > after && c < nodes && above[c] == node);
+      if (hits != 0) return base + __builtin_ctzll(hits);
+    }
+    return -1;
   }
+  __device__ __forceinline__ bool again(int node, int c) const {
+    const int lane = threadIdx.x & 63, t = token_of(c);
+    for (int base = node & ~63; base < c; base += 64) {
+      const int s = base + lane;
+      if (__ballot(s < c && above[s] == node && token[s] == t) != 0) return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ void put(int at, int node) { path[at] = node; }  // by every thread, one value
+};
 
-  template <bool DENSE>
-  __device__ __forceinline__ void load(int64_t base, int vocab, bool vector_ok, double (&w)[kPerLane]) const {
+template <typename P, bool SMALL>
+__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
+// A mass times q is rounded before it is subtracted, as the formulas' plain form does.
+#pragma clang fp contract(off)
+  __shared__ int arrived;
+  const int64_t b = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const P* target = static_cast<const P*>(a.target) + b * a.t_sb;
+  const P* draft = a.draft == nullptr ? nullptr : static_cast<const P*>(a.draft) + b * a.d_sb;
+  const float* uniforms = a.uniforms + b * a.uni_sb;
+  auto load_node = [&](int c, int& above, int& token, double& prob) {
+    const int64_t up = a.parents == nullptr ? c - 1 : a.parents[b * a.par_sb + c];
+    const int64_t t = a.tokens[b * a.tok_sb + c];
+    above = c > 0 && up >= 0 && up < c ? static_cast<int>(up) : -1;
+    const bool real = above >= 0 && t >= 0 && t < a.vocab;
+    token = real ? static_cast<int>(t) : -1;
+    prob = real ? static_cast<double>(slc::to_f32(target[above * a.t_st + t])) : 0.0;
+  };
+  using Nodes = std::conditional_t<SMALL, LaneNodes, SharedNodes>;
+  Nodes nodes;
+  float u_lane = 0.0f;    // SMALL: the lane's random number,
+  double q_lane = 0.0;    // and the draft's probability of its token
+  if constexpr (SMALL) {
+    nodes.above = nodes.token = nodes.place = -1;
+    nodes.prob = 0.0;
+    if (lane < a.nodes) {
+      u_lane = uniforms[lane];
+      load_node(lane, nodes.above, nodes.token, nodes.prob);
+      if (draft != nullptr && nodes.token >= 0)
+        q_lane = static_cast<double>(slc::to_f32(draft[nodes.above * a.d_st + nodes.token]));
+    }
+  } else {
+    __shared__ double prob[kMaxNodes];
+    __shared__ int above[kMaxNodes], token[kMaxNodes], path[kMaxNodes];
+    nodes = {above, token, prob, path, a.nodes};
+    for (int c = tid; c < a.nodes; c += kThreads) load_node(c, above[c], token[c], prob[c]);
+    __syncthreads();
+  }
+  auto random_of = [&](int c) {
+    if constexpr (SMALL) return lane_value(static_cast<double>(u_lane), c);
+    return uniform(static_cast<double>(uniforms[c]));
+  };
+  auto draft_of = [&](int node, int c) {
+    if constexpr (SMALL) return lane_value(q_lane, c);
+    const int t = nodes.token_of(c);
+    return t < 0 ? 0.0 : uniform(static_cast<double>(slc::to_f32(draft[node * a.d_st + t])));
+  };
+
+  // Down the tree from `node` to the first node without an accepted child; with draft
+  // rows only to the first whose first child is refused, as the next test needs a mass.
+  // Without, `excluded` says whether that node's children's tokens have no weight.
+  int count = 0, node = 0, tried = -1;
+  double mass = 0.0;
+  auto walk = [&](int from) {
+    node = from;
+    nodes.put(count++, node);
+    for (;;) {
+      int next = -1;
+      if (draft != nullptr) {
+        tried = nodes.next_child(node, node);
+        if (tried < 0) break;
+        if (uniform(static_cast<int>(random_of(tried) * draft_of(node, tried) < nodes.prob_of(tried))) != 0) next = tried;
+      } else {
+        double left = 1.0;
+        for (int c = nodes.next_child(node, node); c >= 0; c = nodes.next_child(node, c)) {
+          const double w = nodes.again(node, c) ? 0.0 : nodes.prob_of(c);
+          if (uniform(static_cast<int>(w > 0.0 && random_of(c) * left < w)) != 0) {
+            next = c;
+            break;
+          }
+          left -= w;
+        }
+      }
+      if (next < 0) break;
+      node = next;
+      nodes.put(count++, node);
+    }
+    mass = draft != nullptr && tried >= 0 ? 1.0 : 0.0;
+  };
+  walk(0);
+  bool excluded = draft == nullptr;
+
+  // The weights: max(p - mass * q, 0), or p without the children's tokens.  NaN has none.
+  // The lane's 16 of a block at `base`: DENSE: neighbours, for a scan in order; else as
+  // coalesced loads (16 bytes a lane, or one element) have them.
+  auto column = [&](bool dense, bool vector, int i) {
     constexpr int kVec = 16 / sizeof(P);
-    const bool vector = vector_ok && base + kBlock <= vocab;
+    if (dense) return lane * kPerLane + i;
+    return vector ? i / kVec * (64 * kVec) + lane * kVec + i % kVec : i * 64 + lane;
+  };
+  auto load = [&](auto dense_tag, int block, double (&w)[kPerLane]) {
+    constexpr bool kDense = decltype(dense_tag)::value;
+    constexpr int kVec = 16 / sizeof(P);
+    const int64_t base = static_cast<int64_t>(block) * kBlock;
+    const bool vector = a.vector_ok && base + kBlock <= a.vocab;
+    const P* p = target + node * a.t_st + base;
+    const P* q = mass > 0.0 ? draft + node * a.d_st + base : nullptr;
     float pv[kPerLane], qv[kPerLane];
     if (vector) {
       uint4 rp[kPerLane / kVec], rq[kPerLane / kVec];
 #pragma unroll
-      for (int j = 0; j < kPerLane / kVec; ++j)
-        rp[j] = *reinterpret_cast<const uint4*>(p + index<DENSE>(base, j * kVec, true));
+      for (int j = 0; j < kPerLane / kVec; ++j) {
+        rp[j] = *reinterpret_cast<const uint4*>(p + column(kDense, true, j * kVec));
+        rq[j] = make_uint4(0, 0, 0, 0);
+      }
       if (q != nullptr) {
 #pragma unroll
         for (int j = 0; j < kPerLane / kVec; ++j)
-          rq[j] = *reinterpret_cast<const uint4*>(q + index<DENSE>(base, j * kVec, true));
-      } else {
-#pragma unroll
-        for (int j = 0; j < kPerLane / kVec; ++j) rq[j] = make_uint4(0, 0, 0, 0);
+          rq[j] = *reinterpret_cast<const uint4*>(q + column(kDense, true, j * kVec));
       }
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) {
@@ -103,172 +252,74 @@ struct Row {
     } else {
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) {
-        const int64_t at = index<DENSE>(base, i, false);
-        pv[i] = at < vocab ? slc::to_f32(p[at]) : 0.0f;
-        qv[i] = at < vocab && q != nullptr ? slc::to_f32(q[at]) : 0.0f;
+        const int at = column(kDense, false, i);
+        pv[i] = base + at < a.vocab ? slc::to_f32(p[at]) : 0.0f;
+        qv[i] = base + at < a.vocab && q != nullptr ? slc::to_f32(q[at]) : 0.0f;
       }
     }
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) w[i] = value(pv[i], qv[i]);
-    for (int s = 0; s < skips; ++s) {
-      const int64_t token = skip[s];
-      if (token < base || token >= base + kBlock) continue;
+    for (int i = 0; i < kPerLane; ++i) {
+      const double v = static_cast<double>(pv[i]) - mass * static_cast<double>(qv[i]);
+      w[i] = v > 0.0 ? v : 0.0;
+    }
+    if (!excluded) return;
+    for (int c = nodes.next_child(node, node); c >= 0; c = nodes.next_child(node, c)) {
+      const int64_t at = nodes.token_of(c) - base;
+      if (at < 0 || at >= kBlock) continue;
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i)
-        if (index<DENSE>(base, i, vector) == token) w[i] = 0.0;
+        if (column(kDense, vector, i) == at) w[i] = 0.0;
     }
-  }
-};
-
-// A value that all lanes share, in scalar registers: the walk's branches are the wave's.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ double uniform(double v) {
-  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bits)));
-  const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bits >> 32)));
-  return __builtin_bit_cast(double, hi << 32 | lo);
-}
-
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, 64);
-  return v;
-}
-// Sums over this lane and those below it.
-__device__ __forceinline__ double wave_scan(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int offset = 1; offset < 64; offset <<= 1) {
-    const double below = __shfl_up(v, offset, 64);
-    if (lane >= offset) v += below;
-  }
-  return v;
-}
-
-template <typename P>
-__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
-// A mass times q is rounded before it is subtracted, as the formulas' plain form does.
-#pragma clang fp contract(off)
-  __shared__ double prob[kMaxNodes];
-  __shared__ int parent[kMaxNodes], token[kMaxNodes], path[kMaxNodes], skip[kMaxNodes];
-  __shared__ unsigned char accept[kMaxNodes];
-  __shared__ int arrived;
-  const int64_t b = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int nodes = a.nodes;
-  const P* target = static_cast<const P*>(a.target) + b * a.t_sb;
-  const P* draft = a.draft == nullptr ? nullptr : static_cast<const P*>(a.draft) + b * a.d_sb;
-  const float* uniforms = a.uniforms + b * a.uni_sb;
-
-  for (int c = tid; c < nodes; c += kThreads) {
-    const int64_t up = a.parents == nullptr ? c - 1 : a.parents[b * a.par_sb + c];
-    const int64_t t = a.tokens[b * a.tok_sb + c];
-    const int above = c > 0 && up >= 0 && up < c ? static_cast<int>(up) : -1;
-    const bool real = above >= 0 && t >= 0 && t < a.vocab;
-    parent[c] = above;
-    token[c] = real ? static_cast<int>(t) : -1;
-    prob[c] = real ? static_cast<double>(slc::to_f32(target[above * a.t_st + t])) : 0.0;
-    accept[c] = 0;
-  }
-  __syncthreads();
-  // Each node's test, as if its parent was reached and every elder sibling refused.
-  // Without draft rows a token that an elder sibling had too has no weight any more.
-  if (draft == nullptr) {
-    for (int c = tid; c < nodes; c += kThreads) {
-      bool twice = false;
-#pragma unroll 4
-      for (int s = 1; s < c; ++s) twice |= parent[s] == parent[c] && token[s] == token[c];
-      if (twice) prob[c] = 0.0;
-    }
-    __syncthreads();
-  }
-  for (int c = 1 + tid; c < nodes; c += kThreads) {
-    const int above = parent[c], t = token[c];
-    if (above < 0 || t < 0) continue;
-    const double u = static_cast<double>(uniforms[c]);
-    if (draft == nullptr) {
-      double left = 1.0;
-#pragma unroll 4
-      for (int s = 1; s < c; ++s) left -= parent[s] == above ? prob[s] : 0.0;
-      accept[c] = prob[c] > 0.0 && u * left < prob[c];
-    } else {
-      bool elder = false;
-#pragma unroll 4
-      for (int s = 1; s < c; ++s) elder |= parent[s] == above;
-      accept[c] = !elder && u * static_cast<double>(slc::to_f32(draft[above * a.d_st + t])) < prob[c];
-    }
-  }
-  __syncthreads();
-
-  // The next child of `node` behind `after` (an accepted one), or -1; every wave
-  // finds it for itself.
-  auto next_child = [&](int node, int after, bool accepted) {
-    for (int base = (after + 1) & ~63; base < nodes; base += 64) {
-      const int c = base + lane;
-      const bool hit = c > after && c < nodes && parent[c] == node && (!accepted || accept[c]);
-      const uint64_t hits = __ballot(hit);
-      if (hits != 0) return base + __builtin_ctzll(hits);
-    }
-    return -1;
   };
-  int count = 0, node = 0, tried = -1;
-  Row<P> row{nullptr, nullptr, 0.0, skip, 0};
-  // Down the tree from `from` to the first node without an accepted child.
-  auto walk = [&](int from) {
-    node = from;
-    path[count++] = node;  // by every thread, one value
-    for (;;) {
-      tried = next_child(node, node, draft == nullptr);
-      if (tried < 0 || uniform(static_cast<int>(accept[tried])) == 0) break;
-      node = tried;
-      path[count++] = node;
-    }
-    row.p = target + node * a.t_st;
-    row.q = draft != nullptr && tried >= 0 ? draft + node * a.d_st : nullptr;
-    row.mass = row.q != nullptr ? 1.0 : 0.0;
-  };
-  walk(0);
-  if (draft == nullptr) {
-    // The refused candidates: all children of the last node.
-    for (int c = next_child(node, node, false); c >= 0; c = next_child(node, c, false)) {
-      skip[row.skips++] = token[c];
-    }
-    __syncthreads();
-  }
 
   double* sums = a.sums + b * a.blocks;
   auto sum_blocks = [&](int first, int step) {
     for (int block = first; block < a.blocks; block += step) {
       double w[kPerLane], sum = 0.0;
-      row.template load<false>(static_cast<int64_t>(block) * kBlock, a.vocab, a.vector_ok, w);
+      load(std::false_type{}, block, w);
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) sum += w[i];
-      sum = wave_sum(sum);
-      if (lane == 0) __hip_atomic_store(&sums[block], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sum = wave_scan(sum);
+      if (lane == 63) __hip_atomic_store(&sums[block], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   };
   sum_blocks(blockIdx.x * kWaves + wave, a.segments * kWaves);
 
   // The last workgroup of the sequence goes on: every wave's sums come before the
-  // barrier, and the count is an agent-scope acquire-release add behind it.
+  // barrier, the count is an agent-scope release add behind it.
   __syncthreads();
   if (tid == 0)
-    arrived = __hip_atomic_fetch_add(&a.counters[b], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    arrived = __hip_atomic_fetch_add(&a.counters[b], 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (uniform(arrived) != a.segments - 1) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   if (tid == 0) __hip_atomic_store(&a.counters[b], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 
-  // Sums up to and with each of 64 blocks, on the `base` of those before.
-  auto scan_blocks = [&](int first, double base) {
-    const double v = first + lane < a.blocks
-                         ? __hip_atomic_load(&sums[first + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                         : 0.0;
-    return base + wave_scan(v);
+  // 256 blocks' sums, kGroup neighbours a lane, and the sums up to and with this lane's.
+  auto load_group = [&](int first, double (&s)[kGroup]) {
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const int block = first + lane * kGroup + i;
+      s[i] = block < a.blocks ? __hip_atomic_load(&sums[block], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    }
   };
+  auto scan_group = [&](const double (&s)[kGroup]) {
+    double own = s[0];
+#pragma unroll
+    for (int i = 1; i < kGroup; ++i) own += s[i];
+    return wave_scan(own);
+  };
+  double lead[kGroup], lead_scan;  // the first 256
   auto total_of = [&]() {
-    double total = 0.0;
-    for (int first = 0; first < a.blocks; first += 64) total = __shfl(scan_blocks(first, total), 63, 64);
-    return uniform(total);
+    load_group(0, lead);
+    lead_scan = scan_group(lead);
+    double total = lane_value(lead_scan, 63);
+    for (int first = 64 * kGroup; first < a.blocks; first += 64 * kGroup) {
+      double s[kGroup];
+      load_group(first, s);
+      total += lane_value(scan_group(s), 63);
+    }
+    return total;
   };
   auto sum_again = [&]() {
     __syncthreads();  // every wave has read the old sums
@@ -277,82 +328,107 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     return total_of();
   };
   double total = total_of();
-  while (row.q != nullptr) {
-    const int c = next_child(node, tried, false);
+  while (draft != nullptr && tried >= 0) {
+    const int c = nodes.next_child(node, tried);
     if (c < 0) break;
-    const int t = uniform(token[c]);
-    const double q = t < 0 ? 0.0 : uniform(static_cast<double>(slc::to_f32(row.q[t])));
-    const double rest = uniform(prob[c]) - row.mass * q;
-    const bool follows = static_cast<double>(uniforms[c]) * total * q < (rest > 0.0 ? rest : 0.0);
-    if (uniform(static_cast<int>(follows)) != 0) {
+    const double q = draft_of(node, c);
+    const double rest = nodes.prob_of(c) - mass * q;
+    if (uniform(static_cast<int>(random_of(c) * total * q < (rest > 0.0 ? rest : 0.0))) != 0) {
       walk(c);
     } else {
-      row.mass += total;
+      mass += total;
       tried = c;
     }
     total = sum_again();
   }
   if (!(total > 0.0)) {
-    row.mass = 0.0;
-    row.q = nullptr;
-    row.skips = 0;
+    mass = 0.0;
+    excluded = false;
     total = sum_again();
   }
-  __syncthreads();  // the path is written
+  if (wave != 0) return;
 
-  if (wave == 0) {
-    const double goal = static_cast<double>(uniforms[0]) * total;
-    // The first block whose sum passes the goal; a random number outside [0, 1) or an
-    // infinite sum may find none: the last block with any weight then.
-    int block = -1, spare = -1;
-    double before = 0.0, base = 0.0;
-    for (int first = 0; first < a.blocks && block < 0; first += 64) {
-      const double upto = scan_blocks(first, base);
-      double prior = __shfl_up(upto, 1, 64);
-      if (lane == 0) prior = base;
-      const uint64_t hits = __ballot(upto > goal);
-      const uint64_t any = __ballot(upto > prior);
-      if (hits != 0) {
-        const int hit = __builtin_ctzll(hits);
-        block = first + hit;
-        before = __shfl(prior, hit, 64);
-      } else if (any != 0) {
-        spare = first + 63 - __builtin_clzll(any);
-      }
-      base = __shfl(upto, 63, 64);
-    }
-    int64_t drawn = -1;
-    if (block < 0) block = spare;
-    if (block >= 0) {
-      double w[kPerLane], own = 0.0;
-      row.template load<true>(static_cast<int64_t>(block) * kBlock, a.vocab, a.vector_ok, w);
+  // The first block whose sum passes the goal; a random number outside [0, 1) or an
+  // infinite sum may find none: the last block with any weight then.
+  const double goal = random_of(0) * total;
+  int block = -1, spare = -1;
+  double before = 0.0, base = 0.0;
+  for (int first = 0; first < a.blocks && block < 0; first += 64 * kGroup) {
+    double s[kGroup], upto;
+    if (first == 0) {
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) own += w[i];
-      const double upto = before + wave_scan(own);
-      double run = __shfl_up(upto, 1, 64);
-      if (lane == 0) run = before;
-      int hit = -1, last = -1;
+      for (int i = 0; i < kGroup; ++i) s[i] = lead[i];
+      upto = lead_scan;
+    } else {
+      load_group(first, s);
+      upto = scan_group(s);
+    }
+    upto += base;
+    double run = dpp<0x138, 0xf>(upto);  // wave_shr:1
+    if (lane == 0) run = base;
+    int hit = -1, some = -1;
+    double start = run;
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        run += w[i];
-        if (w[i] > 0.0) last = i;
-        if (hit < 0 && w[i] > 0.0 && run > goal) hit = i;
+    for (int i = 0; i < kGroup; ++i) {
+      const double next = run + s[i];
+      if (s[i] > 0.0) some = i;
+      if (hit < 0 && next > goal) {
+        hit = i;
+        start = run;
       }
-      // Sums of another order than the block's may end a rounding before the goal:
-      // the block's last weight then.
-      const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
-      if (lasts != 0) {
-        const int from = hits != 0 ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts);
-        const int at = __shfl(hits != 0 ? hit : last, from, 64);
-        drawn = static_cast<int64_t>(block) * kBlock + from * kPerLane + at;
-      }
+      run = next;
     }
-    for (int j = lane; j < nodes; j += 64) {
-      a.path[b * nodes + j] = j < count ? path[j] : -1;
-      a.emitted[b * nodes + j] = j + 1 < count ? token[path[j + 1]] : (j + 1 == count ? drawn : -1);
+    const uint64_t hits = __ballot(hit >= 0), any = __ballot(some >= 0);
+    if (hits != 0) {
+      const int from = __builtin_ctzll(hits);
+      block = first + from * kGroup + __builtin_amdgcn_readlane(hit, from);
+      before = lane_value(start, from);
+    } else if (any != 0) {
+      const int from = 63 - __builtin_clzll(any);
+      spare = first + from * kGroup + __builtin_amdgcn_readlane(some, from);
     }
-    if (lane == 0) a.counts[b] = count;
+    base = lane_value(upto, 63);
   }
+  int64_t drawn = -1;
+  if (block < 0) block = spare;
+  if (block >= 0) {
+    double w[kPerLane], own = 0.0;
+    load(std::true_type{}, block, w);
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) own += w[i];
+    const double upto = before + wave_scan(own);
+    double run = dpp<0x138, 0xf>(upto);
+    if (lane == 0) run = before;
+    int hit = -1, last = -1;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      run += w[i];
+      if (w[i] > 0.0) last = i;
+      if (hit < 0 && w[i] > 0.0 && run > goal) hit = i;
+    }
+    // Sums of another order than the block's may end a rounding before the goal: the
+    // block's last weight then.
+    const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
+    if (lasts != 0) {
+      const int from = hits != 0 ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts);
+      drawn = static_cast<int64_t>(block) * kBlock + from * kPerLane +
+              __builtin_amdgcn_readlane(hits != 0 ? hit : last, from);
+    }
+  }
+  for (int j = lane; j < a.nodes; j += 64) {
+    int at, follow;
+    if constexpr (SMALL) {
+      at = nodes.place;
+      const int next = __shfl(nodes.place, lane + 1 < 64 ? lane + 1 : 63, 64);
+      follow = __shfl(nodes.token, next < 0 ? 0 : next, 64);
+    } else {
+      at = j < count ? nodes.path[j] : -1;
+      follow = j + 1 < count ? nodes.token[nodes.path[j + 1]] : -1;
+    }
+    a.path[b * a.nodes + j] = j < count ? at : -1;
+    a.emitted[b * a.nodes + j] = j + 1 < count ? follow : (j + 1 == count ? drawn : -1);
+  }
+  if (lane == 0) a.counts[b] = count;
 }
 
 template <typename P>
@@ -361,8 +437,8 @@ int launch(VerifyArgs a, int64_t batch, hipStream_t stream) {
     return (reinterpret_cast<uintptr_t>(p) % 16 | sb * sizeof(P) % 16 | st * sizeof(P) % 16) == 0;
   };
   a.vector_ok = aligned(a.target, a.t_sb, a.t_st) && aligned(a.draft, a.d_sb, a.d_st);
-  hipLaunchKernelGGL(verify_kernel<P>, dim3(a.segments, static_cast<unsigned>(batch)), dim3(kThreads), 0,
-                     stream, a);
+  auto kernel = a.nodes <= 64 ? verify_kernel<P, true> : verify_kernel<P, false>;
+  hipLaunchKernelGGL(kernel, dim3(a.segments, static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, a);
   return slc_host::check_launch("slc_hip_verify_tokens");
 }
 
