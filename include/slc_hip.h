@@ -755,18 +755,18 @@ SLC_API int slc_hip_paged_tree_attention(
  *   counts[b]     : accepted nodes, node 0 among them, and so emitted tokens
  * tokens, parents [B, nodes]; uniforms [B, nodes]; target [B, nodes, vocab] and draft
  * [B, nodes - 1, vocab] of one dtype, rows contiguous; path and emitted [B, nodes]
- * contiguous.  The workspace is slc_hip_verify_tokens_workspace_size bytes on 8 bytes,
- * the counters `batch` ints, zero between calls; calls that may overlap need their own.
+ * contiguous.  The counters are slc_hip_verify_tokens_counter_count ints on 8 bytes, zero
+ * between calls; calls that may overlap in time need their own.
  */
 #define SLC_VERIFY_MAX_NODES 1024
-SLC_API int64_t slc_hip_verify_tokens_workspace_size(int64_t batch, int64_t vocab);
+SLC_API int64_t slc_hip_verify_tokens_counter_count(int64_t batch, int64_t vocab);
 SLC_API int slc_hip_verify_tokens(
     const int64_t* tokens, const int64_t* parents, const void* target, const void* draft,
-    const float* uniforms, int64_t* path, int64_t* emitted, int64_t* counts, void* workspace,
-    int64_t workspace_bytes, int* counters, int64_t num_counters, int dtype, int64_t batch,
-    int64_t nodes, int64_t vocab, int64_t tok_stride_b, int64_t parent_stride_b,
-    int64_t uniform_stride_b, int64_t target_stride_b, int64_t target_stride_t,
-    int64_t draft_stride_b, int64_t draft_stride_t, void* stream);
+    const float* uniforms, int64_t* path, int64_t* emitted, int64_t* counts, int* counters,
+    int64_t num_counters, int dtype, int64_t batch, int64_t nodes, int64_t vocab,
+    int64_t tok_stride_b, int64_t parent_stride_b, int64_t uniform_stride_b,
+    int64_t target_stride_b, int64_t target_stride_t, int64_t draft_stride_b,
+    int64_t draft_stride_t, void* stream);
 
 /*
  * kv_commit: in every layer l, K and V row lengths[l][b] + path[b, j] moves to row

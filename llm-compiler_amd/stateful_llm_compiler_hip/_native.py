@@ -148,8 +148,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I, [_P] * 4 + [_I, _P, _P, _I, _P, _P, _L, _P, _L, _I] + [_L] * 21 + [_F, _P]),
     "slc_hip_paged_tree_attention": (
         _I, [_P] * 4 + [_L] * 5 + [_P, _I, _P, _P, _I, _P, _P, _L, _P, _L, _I] + [_L] * 19 + [_F, _P]),
-    "slc_hip_verify_tokens_workspace_size": (_L, [_L, _L]),
-    "slc_hip_verify_tokens": (_I, [_P] * 9 + [_L, _P, _L, _I] + [_L] * 10 + [_P]),
+    "slc_hip_verify_tokens_counter_count": (_L, [_L, _L]),
+    "slc_hip_verify_tokens": (_I, [_P] * 9 + [_L, _I] + [_L] * 10 + [_P]),
     "slc_hip_kv_commit": (_I, [_P] * 5 + [_L] * 4 + [_P] * 3 + [_I] + [_L] * 9 + [_P]),
     "slc_hip_rope": (
         _I,

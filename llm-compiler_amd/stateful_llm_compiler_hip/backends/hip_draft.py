@@ -190,6 +190,11 @@ def hip_paged_tree_attention(
     return output
 
 
+@functools.lru_cache(maxsize=1024)
+def _verify_counters(batch, vocab):
+    return _native.library().slc_hip_verify_tokens_counter_count(batch, vocab)
+
+
 def hip_verify_tokens(
     tokens: torch.Tensor,
     target_probs: torch.Tensor,
@@ -257,15 +262,13 @@ def hip_verify_tokens(
     counts = tokens.new_empty((batch,))
     if batch == 0:
         return path, emitted, counts
-    lib = _native.library()
-    nbytes = lib.slc_hip_verify_tokens_workspace_size(batch, vocab)
     owner = workspace if workspace is not None else _native.stream_workspace(tokens.device)
-    buffer, counters = owner.scratch("verify_tokens", nbytes), owner.counters(batch)
+    counters = owner.counters(_verify_counters(batch, vocab))
     draft, draft_strides = (None, (0, 0)) if draft_probs is None else (draft_probs.data_ptr(),
                                                                        draft_probs.stride()[:2])
     _call("slc_hip_verify_tokens", index, tokens.data_ptr(), None if parents is None else parents.data_ptr(),
           target_probs.data_ptr(), draft, uniforms.data_ptr(), path.data_ptr(), emitted.data_ptr(), counts.data_ptr(),
-          buffer.data_ptr(), nbytes, counters.data_ptr(), counters.numel(), _native.dtype_tag(target_probs.dtype),
+          counters.data_ptr(), counters.numel(), _native.dtype_tag(target_probs.dtype),
           batch, nodes, vocab, tokens.stride(0), 0 if parents is None else parents.stride(0), uniforms.stride(0),
           *target_probs.stride()[:2], *draft_strides)
     return path, emitted, counts

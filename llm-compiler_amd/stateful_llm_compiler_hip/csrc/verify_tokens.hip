@@ -31,6 +31,9 @@
 
 namespace {
 
+// The kernel's lambdas: one that is called would keep what it captures in memory.
+#define SLC_INLINE __attribute__((always_inline))
+
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBlock = 1024;  // weights per sum, 16 a lane
@@ -47,8 +50,8 @@ struct VerifyArgs {
   int64_t* path;           // [B, T]
   int64_t* emitted;        // [B, T]
   int64_t* counts;         // [B]
-  double* sums;            // [B, blocks]
-  int* counters;           // [B]
+  uint64_t* sums;          // [B, blocks], zero between calls
+  int* counters;           // [B], zero between calls
   int64_t tok_sb, par_sb, uni_sb, t_sb, t_st, d_sb, d_st;
   int nodes, vocab, blocks, segments;
   bool vector_ok;  // rows start on 16 bytes
@@ -85,7 +88,8 @@ __device__ __forceinline__ double wave_scan(double v) {
   return v;
 }
 
-// The nodes of a sequence.  Up to 64: one a lane, in registers of every wave.
+// The nodes of a sequence.  Up to 64: one a lane, in registers of every wave (the first
+// wave loads them and hands them on).
 struct LaneNodes {
   int above, token;  // parent and token, -1: none
   double prob;       // target's probability of the token behind the parent
@@ -134,17 +138,15 @@ struct SharedNodes {
   __device__ __forceinline__ void put(int at, int node) { path[at] = node; }  // by every thread, one value
 };
 
-template <typename P, bool SMALL>
+template <typename P, bool SMALL, bool DRAFT>
 __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
-// A mass times q is rounded before it is subtracted, as the formulas' plain form does.
-#pragma clang fp contract(off)
   __shared__ int arrived;
   const int64_t b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const P* target = static_cast<const P*>(a.target) + b * a.t_sb;
-  const P* draft = a.draft == nullptr ? nullptr : static_cast<const P*>(a.draft) + b * a.d_sb;
+  const P* draft = DRAFT ? static_cast<const P*>(a.draft) + b * a.d_sb : nullptr;
   const float* uniforms = a.uniforms + b * a.uni_sb;
-  auto load_node = [&](int c, int& above, int& token, double& prob) {
+  auto load_node = [&](int c, int& above, int& token, double& prob) SLC_INLINE {
     const int64_t up = a.parents == nullptr ? c - 1 : a.parents[b * a.par_sb + c];
     const int64_t t = a.tokens[b * a.tok_sb + c];
     above = c > 0 && up >= 0 && up < c ? static_cast<int>(up) : -1;
@@ -159,10 +161,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   if constexpr (SMALL) {
     nodes.above = nodes.token = nodes.place = -1;
     nodes.prob = 0.0;
-    if (lane < a.nodes) {
+    if (wave == 0 && lane < a.nodes) {
       u_lane = uniforms[lane];
       load_node(lane, nodes.above, nodes.token, nodes.prob);
-      if (draft != nullptr && nodes.token >= 0)
+      if (DRAFT && nodes.token >= 0)
         q_lane = static_cast<double>(slc::to_f32(draft[nodes.above * a.d_st + nodes.token]));
     }
   } else {
@@ -172,11 +174,11 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     for (int c = tid; c < a.nodes; c += kThreads) load_node(c, above[c], token[c], prob[c]);
     __syncthreads();
   }
-  auto random_of = [&](int c) {
+  auto random_of = [&](int c) SLC_INLINE {
     if constexpr (SMALL) return lane_value(static_cast<double>(u_lane), c);
     return uniform(static_cast<double>(uniforms[c]));
   };
-  auto draft_of = [&](int node, int c) {
+  auto draft_of = [&](int node, int c) SLC_INLINE {
     if constexpr (SMALL) return lane_value(q_lane, c);
     const int t = nodes.token_of(c);
     return t < 0 ? 0.0 : uniform(static_cast<double>(slc::to_f32(draft[node * a.d_st + t])));
@@ -187,12 +189,12 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   // Without, `excluded` says whether that node's children's tokens have no weight.
   int count = 0, node = 0, tried = -1;
   double mass = 0.0;
-  auto walk = [&](int from) {
+  auto walk = [&](int from) SLC_INLINE {
     node = from;
     nodes.put(count++, node);
     for (;;) {
       int next = -1;
-      if (draft != nullptr) {
+      if constexpr (DRAFT) {
         tried = nodes.next_child(node, node);
         if (tried < 0) break;
         if (uniform(static_cast<int>(random_of(tried) * draft_of(node, tried) < nodes.prob_of(tried))) != 0) next = tried;
@@ -211,60 +213,105 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
       node = next;
       nodes.put(count++, node);
     }
-    mass = draft != nullptr && tried >= 0 ? 1.0 : 0.0;
+    mass = DRAFT && tried >= 0 ? 1.0 : 0.0;
   };
-  walk(0);
-  bool excluded = draft == nullptr;
+  bool excluded = !DRAFT;
+  if constexpr (SMALL) {
+    // The first wave walks for all of the workgroup: every load of it is one of a cache
+    // line of its own, and those of eight waves cost 32 sequences 31 us instead of NN.
+    __shared__ LaneNodes shared_nodes[64];
+    __shared__ float shared_u[64];
+    __shared__ double shared_q[64];
+    __shared__ int shared_walk[3];
+    if (wave == 0) {
+      walk(0);
+      shared_nodes[lane] = nodes;
+      shared_u[lane] = u_lane;
+      shared_q[lane] = q_lane;
+      if (lane < 3) shared_walk[lane] = lane == 0 ? count : (lane == 1 ? node : tried);
+    }
+    __syncthreads();
+    if (wave != 0) {
+      nodes = shared_nodes[lane];
+      u_lane = shared_u[lane];
+      q_lane = shared_q[lane];
+      count = uniform(shared_walk[0]);
+      node = uniform(shared_walk[1]);
+      tried = uniform(shared_walk[2]);
+      mass = DRAFT && tried >= 0 ? 1.0 : 0.0;
+    }
+  } else {
+    walk(0);
+  }
 
   // The weights: max(p - mass * q, 0), or p without the children's tokens.  NaN has none.
   // The lane's 16 of a block at `base`: DENSE: neighbours, for a scan in order; else as
   // coalesced loads (16 bytes a lane, or one element) have them.
-  auto column = [&](bool dense, bool vector, int i) {
-    constexpr int kVec = 16 / sizeof(P);
+  auto column = [&](bool dense, bool vector, int i) SLC_INLINE {
+    constexpr int kVec = 16 / sizeof(P);  // elements of a load
     if (dense) return lane * kPerLane + i;
     return vector ? i / kVec * (64 * kVec) + lane * kVec + i % kVec : i * 64 + lane;
   };
-  auto load = [&](auto dense_tag, int block, double (&w)[kPerLane]) {
-    constexpr bool kDense = decltype(dense_tag)::value;
-    constexpr int kVec = 16 / sizeof(P);
-    const int64_t base = static_cast<int64_t>(block) * kBlock;
-    const bool vector = a.vector_ok && base + kBlock <= a.vocab;
-    const P* p = target + node * a.t_st + base;
-    const P* q = mass > 0.0 ? draft + node * a.d_st + base : nullptr;
-    float pv[kPerLane], qv[kPerLane];
-    if (vector) {
-      uint4 rp[kPerLane / kVec], rq[kPerLane / kVec];
+  constexpr int kVec = 16 / sizeof(P), kLoads = kPerLane / kVec, kWords = 4 * kLoads;
+  struct Raw {
+    uint32_t p[kWords], q[kWords];
+  };
+  auto is_vector = [&](int block) SLC_INLINE { return a.vector_ok && (block + 1) * static_cast<int64_t>(kBlock) <= a.vocab; };
+  auto load_vector = [&](auto dense_tag, const P* row, int block, uint32_t (&words)[kWords]) SLC_INLINE {
 #pragma unroll
-      for (int j = 0; j < kPerLane / kVec; ++j) {
-        rp[j] = *reinterpret_cast<const uint4*>(p + column(kDense, true, j * kVec));
-        rq[j] = make_uint4(0, 0, 0, 0);
-      }
-      if (q != nullptr) {
-#pragma unroll
-        for (int j = 0; j < kPerLane / kVec; ++j)
-          rq[j] = *reinterpret_cast<const uint4*>(q + column(kDense, true, j * kVec));
-      }
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        pv[i] = slc::to_f32(reinterpret_cast<const P*>(&rp[i / kVec])[i % kVec]);
-        qv[i] = slc::to_f32(reinterpret_cast<const P*>(&rq[i / kVec])[i % kVec]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        const int at = column(kDense, false, i);
-        pv[i] = base + at < a.vocab ? slc::to_f32(p[at]) : 0.0f;
-        qv[i] = base + at < a.vocab && q != nullptr ? slc::to_f32(q[at]) : 0.0f;
-      }
+    for (int j = 0; j < kLoads; ++j) {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(block) * kBlock +
+                                                      column(decltype(dense_tag)::value, true, j * kVec));
+      words[4 * j] = v.x;
+      words[4 * j + 1] = v.y;
+      words[4 * j + 2] = v.z;
+      words[4 * j + 3] = v.w;
     }
+  };
+  auto load_any = [&](auto dense_tag, const P* row, int block, uint32_t (&words)[kWords]) SLC_INLINE {
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-      const double v = static_cast<double>(pv[i]) - mass * static_cast<double>(qv[i]);
-      w[i] = v > 0.0 ? v : 0.0;
+      const int64_t at = static_cast<int64_t>(block) * kBlock + column(decltype(dense_tag)::value, false, i);
+      const P v = row[at < a.vocab ? at : 0];
+      if constexpr (sizeof(P) == 4) {
+        words[i] = at < a.vocab ? __float_as_uint(v) : 0;
+      } else {
+        const uint32_t bits = at < a.vocab ? v.bits : 0;
+        words[i / 2] = i % 2 == 0 ? bits : words[i / 2] | bits << 16;
+      }
+    }
+  };
+  // Where no mass is taken off, q's place is p's: loaded, not looked at.
+  auto load = [&](auto dense_tag, int block, Raw& raw) SLC_INLINE {
+    const P* p = target + node * a.t_st;
+    const P* q = mass > 0.0 ? draft + node * a.d_st : p;
+    if (is_vector(block)) {
+      load_vector(dense_tag, p, block, raw.p);
+      if constexpr (DRAFT) load_vector(dense_tag, q, block, raw.q);
+    } else {
+      load_any(dense_tag, p, block, raw.p);
+      if constexpr (DRAFT) load_any(dense_tag, q, block, raw.q);
+    }
+  };
+  auto element = [](const uint32_t (&words)[kWords], int i) SLC_INLINE {
+    if constexpr (sizeof(P) == 4) {
+      return __uint_as_float(words[i]);
+    } else {
+      return slc::to_f32(P{static_cast<uint16_t>(words[i / 2] >> (16 * (i % 2)))});
+    }
+  };
+  auto weights = [&](auto dense_tag, int block, const Raw& raw, double (&w)[kPerLane]) SLC_INLINE {
+    constexpr bool kDense = decltype(dense_tag)::value;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      double v = static_cast<double>(element(raw.p, i));
+      if constexpr (DRAFT) v = fma(-mass, mass > 0.0 ? static_cast<double>(element(raw.q, i)) : 0.0, v);
+      w[i] = fmax(v, 0.0);  // 0 for NaN
     }
     if (!excluded) return;
+    const bool vector = is_vector(block);
     for (int c = nodes.next_child(node, node); c >= 0; c = nodes.next_child(node, c)) {
-      const int64_t at = nodes.token_of(c) - base;
+      const int64_t at = nodes.token_of(c) - static_cast<int64_t>(block) * kBlock;
       if (at < 0 || at >= kBlock) continue;
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i)
@@ -272,45 +319,102 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     }
   };
 
-  double* sums = a.sums + b * a.blocks;
-  auto sum_blocks = [&](int first, int step) {
-    for (int block = first; block < a.blocks; block += step) {
-      double w[kPerLane], sum = 0.0;
-      load(std::false_type{}, block, w);
+  // A block's sum is published with its sign set: a word of zeros is none yet.
+  uint64_t* sums = a.sums + b * a.blocks;
+  auto sum_block = [&](int block, const Raw& raw) SLC_INLINE {
+    double w[kPerLane], sum = 0.0;
+    weights(std::false_type{}, block, raw, w);
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) sum += w[i];
-      sum = wave_scan(sum);
-      if (lane == 63) __hip_atomic_store(&sums[block], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = 0; i < kPerLane; ++i) sum += w[i];
+    sum = wave_scan(sum);
+    if (lane == 63)
+      __hip_atomic_store(&sums[block], __builtin_bit_cast(uint64_t, -sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  auto sum_blocks = [&](int first, int step) SLC_INLINE {
+    // Whole blocks of 16-byte loads: a block's are in flight while the one before is
+    // summed (the last one's twice, so that no branch makes the loop wait for them).
+    const int whole = a.vector_ok ? a.vocab / kBlock : 0;
+    const P* p = target + node * a.t_st;
+    const P* q = mass > 0.0 ? draft + node * a.d_st : p;
+    int block = first;
+    if (block < whole) {
+      Raw raw;
+      load_vector(std::false_type{}, p, block, raw.p);
+      if constexpr (DRAFT) load_vector(std::false_type{}, q, block, raw.q);
+#pragma unroll 2
+      for (; block < whole; block += step) {
+        const Raw now = raw;
+        const int next = block + step < whole ? block + step : block;
+        load_vector(std::false_type{}, p, next, raw.p);
+        if constexpr (DRAFT) load_vector(std::false_type{}, q, next, raw.q);
+        sum_block(block, now);
+      }
+    }
+#pragma unroll 1
+    for (; block < a.blocks; block += step) {
+      Raw raw;
+      load_any(std::false_type{}, p, block, raw.p);
+      if constexpr (DRAFT) load_any(std::false_type{}, q, block, raw.q);
+      sum_block(block, raw);
     }
   };
   sum_blocks(blockIdx.x * kWaves + wave, a.segments * kWaves);
 
-  // The last workgroup of the sequence goes on: every wave's sums come before the
-  // barrier, the count is an agent-scope release add behind it.
+  // The last workgroup of the sequence goes on.  Sums that are not there yet are waited
+  // for one by one, so nothing orders them and the count: a release and an acquire, whose
+  // cache write-backs and invalidations delay all other workgroups' loads, would cost
+  // 32 sequences 10 of 18 us.
   __syncthreads();
   if (tid == 0)
-    arrived = __hip_atomic_fetch_add(&a.counters[b], 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
+    arrived = __hip_atomic_fetch_add(&a.counters[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (uniform(arrived) != a.segments - 1) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   if (tid == 0) __hip_atomic_store(&a.counters[b], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 
+  // The first wave decides; the others sum blocks for it where it needs other weights.
+  __shared__ int order_node, order_excluded;
+  __shared__ double order_mass;
+  if (wave != 0) {
+    for (;;) {
+      __syncthreads();  // an order is there
+      node = uniform(order_node);
+      if (node < 0) return;
+      mass = uniform(order_mass);
+      excluded = uniform(order_excluded) != 0;
+      sum_blocks(wave, kWaves);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+      __syncthreads();
+    }
+  }
   // 256 blocks' sums, kGroup neighbours a lane, and the sums up to and with this lane's.
-  auto load_group = [&](int first, double (&s)[kGroup]) {
+  auto load_group = [&](int first, double (&s)[kGroup]) SLC_INLINE {
+    // The bound ends the wait whatever happens; a sum's store was issued long before.
+    for (int turn = 0; turn < (1 << 20); ++turn) {
+      uint64_t bits[kGroup];
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-      const int block = first + lane * kGroup + i;
-      s[i] = block < a.blocks ? __hip_atomic_load(&sums[block], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+      for (int i = 0; i < kGroup; ++i) {
+        // (A load that a branch guards would be waited for before the next.)
+        const int block = first + lane * kGroup + i;
+        bits[i] = __hip_atomic_load(&sums[block < a.blocks ? block : a.blocks - 1], __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT);
+      }
+      bool there = true;
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        there &= bits[i] != 0;
+        s[i] = first + lane * kGroup + i < a.blocks ? -__builtin_bit_cast(double, bits[i]) : 0.0;
+      }
+      if (__all(there)) return;
     }
   };
-  auto scan_group = [&](const double (&s)[kGroup]) {
+  auto scan_group = [&](const double (&s)[kGroup]) SLC_INLINE {
     double own = s[0];
 #pragma unroll
     for (int i = 1; i < kGroup; ++i) own += s[i];
     return wave_scan(own);
   };
   double lead[kGroup], lead_scan;  // the first 256
-  auto total_of = [&]() {
+  auto total_of = [&]() SLC_INLINE {
     load_group(0, lead);
     lead_scan = scan_group(lead);
     double total = lane_value(lead_scan, 63);
@@ -321,19 +425,25 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     }
     return total;
   };
-  auto sum_again = [&]() {
-    __syncthreads();  // every wave has read the old sums
-    sum_blocks(wave, kWaves);
+  auto sum_again = [&]() SLC_INLINE {
+    if (lane == 0) {
+      order_node = node;
+      order_mass = mass;
+      order_excluded = excluded;
+    }
     __syncthreads();
+    sum_blocks(0, kWaves);
+    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // none of the old sums
     return total_of();
   };
   double total = total_of();
-  while (draft != nullptr && tried >= 0) {
+  while (DRAFT && tried >= 0) {
     const int c = nodes.next_child(node, tried);
     if (c < 0) break;
     const double q = draft_of(node, c);
-    const double rest = nodes.prob_of(c) - mass * q;
-    if (uniform(static_cast<int>(random_of(c) * total * q < (rest > 0.0 ? rest : 0.0))) != 0) {
+    const double rest = fmax(fma(-mass, q, nodes.prob_of(c)), 0.0);
+    if (uniform(static_cast<int>(random_of(c) * total * q < rest)) != 0) {
       walk(c);
     } else {
       mass += total;
@@ -346,7 +456,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     excluded = false;
     total = sum_again();
   }
-  if (wave != 0) return;
+  if (lane == 0) order_node = -1;
+  __syncthreads();  // the other waves end
 
   // The first block whose sum passes the goal; a random number outside [0, 1) or an
   // infinite sum may find none: the last block with any weight then.
@@ -392,8 +503,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   int64_t drawn = -1;
   if (block < 0) block = spare;
   if (block >= 0) {
+    Raw raw;
     double w[kPerLane], own = 0.0;
-    load(std::true_type{}, block, w);
+    load(std::true_type{}, block, raw);
+    weights(std::true_type{}, block, raw, w);
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) own += w[i];
     const double upto = before + wave_scan(own);
@@ -415,6 +528,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
               __builtin_amdgcn_readlane(hits != 0 ? hit : last, from);
     }
   }
+  for (int first = lane; first < a.blocks; first += 64)
+    __hip_atomic_store(&sums[first], uint64_t{0}, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   for (int j = lane; j < a.nodes; j += 64) {
     int at, follow;
     if constexpr (SMALL) {
@@ -437,7 +552,8 @@ int launch(VerifyArgs a, int64_t batch, hipStream_t stream) {
     return (reinterpret_cast<uintptr_t>(p) % 16 | sb * sizeof(P) % 16 | st * sizeof(P) % 16) == 0;
   };
   a.vector_ok = aligned(a.target, a.t_sb, a.t_st) && aligned(a.draft, a.d_sb, a.d_st);
-  auto kernel = a.nodes <= 64 ? verify_kernel<P, true> : verify_kernel<P, false>;
+  auto kernel = a.draft != nullptr ? (a.nodes <= 64 ? verify_kernel<P, true, true> : verify_kernel<P, false, true>)
+                                   : (a.nodes <= 64 ? verify_kernel<P, true, false> : verify_kernel<P, false, false>);
   hipLaunchKernelGGL(kernel, dim3(a.segments, static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, a);
   return slc_host::check_launch("slc_hip_verify_tokens");
 }
@@ -446,29 +562,26 @@ int64_t block_count(int64_t vocab) { return slc_host::ceil_div(vocab, kBlock); }
 
 }  // namespace
 
-extern "C" int64_t slc_hip_verify_tokens_workspace_size(int64_t batch, int64_t vocab) {
-  return batch > 0 && vocab > 0 ? batch * block_count(vocab) * static_cast<int64_t>(sizeof(double)) : 0;
+extern "C" int64_t slc_hip_verify_tokens_counter_count(int64_t batch, int64_t vocab) {
+  return batch > 0 && vocab > 0 ? (batch + 1) / 2 * 2 + 2 * batch * block_count(vocab) : 0;
 }
 
 extern "C" int slc_hip_verify_tokens(
     const int64_t* tokens, const int64_t* parents, const void* target, const void* draft,
-    const float* uniforms, int64_t* path, int64_t* emitted, int64_t* counts, void* workspace,
-    int64_t workspace_bytes, int* counters, int64_t num_counters, int dtype, int64_t batch,
-    int64_t nodes, int64_t vocab, int64_t tok_stride_b, int64_t parent_stride_b,
-    int64_t uniform_stride_b, int64_t target_stride_b, int64_t target_stride_t,
-    int64_t draft_stride_b, int64_t draft_stride_t, void* stream) {
+    const float* uniforms, int64_t* path, int64_t* emitted, int64_t* counts, int* counters,
+    int64_t num_counters, int dtype, int64_t batch, int64_t nodes, int64_t vocab,
+    int64_t tok_stride_b, int64_t parent_stride_b, int64_t uniform_stride_b, int64_t target_stride_b,
+    int64_t target_stride_t, int64_t draft_stride_b, int64_t draft_stride_t, void* stream) {
   const char* what = "slc_hip_verify_tokens";
   SLC_REQUIRE(slc_host::is_float_dtype(dtype), "%s: bad dtype %d", what, dtype);
   SLC_REQUIRE(batch >= 0 && batch <= 65535, "%s: batch must be 0 to 65535", what);
   SLC_REQUIRE(nodes >= 1 && nodes <= kMaxNodes, "%s: 1 to %d nodes", what, kMaxNodes);
   SLC_REQUIRE(vocab >= 1 && vocab <= 0x7fffffff - kBlock, "%s: bad vocabulary size", what);
   if (batch == 0) return SLC_OK;
-  SLC_REQUIRE(tokens && target && uniforms && path && emitted && counts && counters && workspace,
-              "%s: null pointer", what);
-  SLC_REQUIRE(workspace_bytes >= slc_hip_verify_tokens_workspace_size(batch, vocab) &&
-                  (reinterpret_cast<uintptr_t>(workspace) & 7) == 0,
-              "%s: workspace too small or not on 8 bytes", what);
-  SLC_REQUIRE(num_counters >= batch, "%s: too few counters", what);
+  SLC_REQUIRE(tokens && target && uniforms && path && emitted && counts && counters, "%s: null pointer", what);
+  SLC_REQUIRE(num_counters >= slc_hip_verify_tokens_counter_count(batch, vocab) &&
+                  (reinterpret_cast<uintptr_t>(counters) & 7) == 0,
+              "%s: too few counters, or not on 8 bytes", what);
   VerifyArgs a{};
   a.tokens = tokens;
   a.parents = parents;
@@ -478,8 +591,8 @@ extern "C" int slc_hip_verify_tokens(
   a.path = path;
   a.emitted = emitted;
   a.counts = counts;
-  a.sums = static_cast<double*>(workspace);
   a.counters = counters;
+  a.sums = reinterpret_cast<uint64_t*>(counters + (batch + 1) / 2 * 2);
   a.tok_sb = tok_stride_b;
   a.par_sb = parent_stride_b;
   a.uni_sb = uniform_stride_b;
@@ -490,9 +603,10 @@ extern "C" int slc_hip_verify_tokens(
   a.nodes = static_cast<int>(nodes);
   a.vocab = static_cast<int>(vocab);
   a.blocks = static_cast<int>(block_count(vocab));
-  // One block a wave while the grid stays within what the card holds a few times.
+  // One block a wave, but no more workgroups than CUs: the kernel's registers leave room
+  // for one each (32 sequences 15 us, with twice or more as many 20).
   a.segments = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(slc_host::ceil_div(a.blocks, kWaves), 4096 / batch)));
+      1, std::min<int64_t>(slc_host::ceil_div(a.blocks, kWaves), slc_host::device_cu_count() / batch)));
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case SLC_BF16:

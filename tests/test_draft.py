@@ -66,22 +66,22 @@ def test_tree_attention_entry_points_refuse_their_own_operands():
         assert tree(True, **bad) == -1, bad
 
 
-def verify(tokens=P, parents=None, target=P, draft=None, uniforms=P, path=P, emitted=P, counts=P, workspace=P,
-           nbytes=1 << 20, counters=P, num_counters=64, dtype=F32, batch=2, nodes=3, vocab=100):
+def verify(tokens=P, parents=None, target=P, draft=None, uniforms=P, path=P, emitted=P, counts=P, counters=P,
+           num_counters=64, dtype=F32, batch=2, nodes=3, vocab=100):
     return _native.library().slc_hip_verify_tokens(
-        tokens, parents, target, draft, uniforms, path, emitted, counts, workspace, nbytes, counters, num_counters,
-        dtype, batch, nodes, vocab, nodes, nodes, nodes, nodes * vocab, vocab, nodes * vocab, vocab, None)
+        tokens, parents, target, draft, uniforms, path, emitted, counts, counters, num_counters, dtype,
+        batch, nodes, vocab, nodes, nodes, nodes, nodes * vocab, vocab, nodes * vocab, vocab, None)
 
 
 def test_verify_entry_point_refuses():
     for bad in ({"dtype": I64}, {"dtype": 99}, {"batch": -1}, {"batch": 65536}, {"nodes": 0}, {"nodes": 1025},
-                {"vocab": 0}, {"vocab": 2**31}, {"num_counters": 1}, {"nbytes": 15}, {"workspace": P + 4},
+                {"vocab": 0}, {"vocab": 2**31}, {"num_counters": 5}, {"counters": P + 4},
                 {"tokens": None}, {"target": None}, {"uniforms": None}, {"path": None}, {"emitted": None},
-                {"counts": None}, {"workspace": None}, {"counters": None}):
+                {"counts": None}, {"counters": None}):
         assert verify(**bad) == -1, bad
     assert verify(batch=0) == 0 and verify(batch=0, tokens=None) == 0
-    size = _native.library().slc_hip_verify_tokens_workspace_size
-    assert size(2, 1024) == 16 and size(2, 1025) == 32 and size(0, 5) == 0
+    count = _native.library().slc_hip_verify_tokens_counter_count
+    assert count(2, 1024) == 6 and count(3, 1025) == 16 and count(0, 5) == 0
 
 
 def commit(key=(P, 2 * P), value=(3 * P, 4 * P), lengths=(5 * P, 6 * P), out=(7 * P, 8 * P), table=None, page_tokens=0,
