@@ -19,8 +19,8 @@ The operators are for inference: their outputs carry no gradient.
 
 from __future__ import annotations
 
-import ctypes
 import functools
+from array import array
 from typing import Sequence
 
 import torch
@@ -28,7 +28,10 @@ import torch
 from .. import _native
 from .hip_ops import _FLOATS, check_flag
 from .hip_paged import _check_pools
-from .hip_q8 import _call
+from .hip_q8 import _CONTIGUOUS, _call
+
+_LENGTHS = (torch.int64, torch.int32)
+_MOST = torch.finfo(torch.float32).max
 
 MAX_NODES = 1024  # SLC_TREE_MAX_NODES, SLC_VERIFY_MAX_NODES
 MAX_CHAIN = 4096  # SLC_CHAIN_MAX_NODES: nodes of tree attention without a tree mask
@@ -38,18 +41,18 @@ def _tree_operands(what, query, key, value, lengths, tree_mask, attention_mask, 
     """Device index and the tree's, mask's and lengths' arguments, after the checks
     that both layouts share."""
 
-    index = query.get_device()
-    if index < 0 or any(
-        tensor is not None and tensor.get_device() != index
-        for tensor in (key, value, lengths, tree_mask, attention_mask)
+    index, dtype = query.get_device(), query.dtype
+    if index < 0 or key.get_device() != index or value.get_device() != index or lengths.get_device() != index or (
+        (tree_mask is not None and tree_mask.get_device() != index)
+        or (attention_mask is not None and attention_mask.get_device() != index)
     ):
         raise ValueError(f"{what}: all tensors must be on the GPU, and on one")
     batch, q_heads, nodes, head_dim = query.shape
     if query.stride(3) != 1 and head_dim > 1:
         raise ValueError(f"{what}: query head dim must be contiguous")
-    if query.dtype not in _FLOATS:
-        raise ValueError(f"{what}: unsupported dtype {query.dtype}")
-    if key.dtype != query.dtype or value.dtype != query.dtype:
+    if dtype not in _FLOATS:
+        raise ValueError(f"{what}: unsupported dtype {dtype}")
+    if key.dtype != dtype or value.dtype != dtype:
         raise ValueError(f"{what}: Q/K/V dtypes must match")
     if key.shape[3] != head_dim or kv_heads < 1 or q_heads < 1 or q_heads % kv_heads:
         raise ValueError(f"{what}: GQA or head shapes do not match")
@@ -57,16 +60,18 @@ def _tree_operands(what, query, key, value, lengths, tree_mask, attention_mask, 
         raise ValueError(f"{what}: head_dim must be 1 to 256")
     if nodes > (MAX_CHAIN if tree_mask is None else MAX_NODES):
         raise ValueError(f"{what}: a tree has at most {MAX_NODES} nodes, a chain {MAX_CHAIN}")
-    if lengths.shape != (batch,) or lengths.dtype not in (torch.int64, torch.int32) or not lengths.is_contiguous():
+    if lengths.shape != (batch,) or lengths.dtype not in _LENGTHS or not lengths.is_contiguous():
         raise ValueError(f"{what}: lengths must be a contiguous int64 (or int32) [batch] tensor")
-    if not 0.0 < scale <= torch.finfo(torch.float32).max:
+    if not 0.0 < scale <= _MOST:
         raise ValueError(f"{what}: scale must be positive and finite")
     tree, tree_strides = None, (0, 0, 0)
     if tree_mask is not None:
+        tree_strides = tree_mask.stride()
+        if len(tree_strides) == 2:
+            tree_strides = (0, *tree_strides)
         if tree_mask.dtype != torch.bool or tree_mask.shape not in ((nodes, nodes), (batch, nodes, nodes)):
             raise ValueError(f"{what}: tree_mask must be a bool [T, T] or [batch, T, T] tensor")
         tree = tree_mask.data_ptr()
-        tree_strides = tree_mask.stride() if tree_mask.ndim == 3 else (0, *tree_mask.stride())
     mask, mask_dtype, mask_strides, mask_len = None, 0, (0, 0), rows
     if attention_mask is not None:
         if (attention_mask.ndim != 4 or attention_mask.shape[:3] != (batch, 1, 1)
@@ -127,24 +132,26 @@ def hip_tree_attention(
     """
 
     what = "HIP tree attention"
-    if query.ndim != 4 or key_buffer.ndim != 4 or key_buffer.shape != value_buffer.shape:
+    shape, buffer_shape = query.shape, key_buffer.shape
+    if len(shape) != 4 or len(buffer_shape) != 4 or buffer_shape != value_buffer.shape:
         raise ValueError(f"{what}: illegal shapes")
-    if key_buffer.stride() != value_buffer.stride() or (key_buffer.stride(3) != 1 and key_buffer.shape[3] > 1):
+    strides = key_buffer.stride()
+    if strides != value_buffer.stride() or (strides[3] != 1 and buffer_shape[3] > 1):
         raise ValueError(f"{what}: K/V buffers need equal strides and a contiguous head dim")
-    batch, capacity, kv_heads, _ = key_buffer.shape
-    if query.shape[0] != batch or capacity < 1:
+    batch, capacity, kv_heads, _ = buffer_shape
+    if shape[0] != batch or capacity < 1:
         raise ValueError(f"{what}: query and buffers need one batch, and the buffers rows")
-    index, operands, mask_len, strides = _tree_operands(
+    index, operands, mask_len, mask_strides = _tree_operands(
         what, query, key_buffer, value_buffer, lengths, tree_mask, attention_mask, capacity, kv_heads, scale)
     output = torch.empty_like(query)
-    if query.numel() == 0:
+    _, q_heads, nodes, head_dim = shape
+    if batch == 0 or nodes == 0:
         return output
-    _, q_heads, nodes, head_dim = query.shape
     dtype = _native.dtype_tag(query.dtype)
     scratch = _tree_workspace(query.device, index, workspace, batch, q_heads, kv_heads, nodes, head_dim, dtype)
     _call("slc_hip_tree_attention", index, query.data_ptr(), key_buffer.data_ptr(), value_buffer.data_ptr(), *operands,
           output.data_ptr(), *scratch, dtype, batch, q_heads, kv_heads, nodes, head_dim, capacity, mask_len,
-          *query.stride()[:3], *key_buffer.stride()[:3], *strides, *output.stride()[:3], scale)
+          *query.stride()[:3], *strides[:3], *mask_strides, *output.stride()[:3], scale)
     return output
 
 
@@ -190,6 +197,12 @@ def hip_paged_tree_attention(
     return output
 
 
+def _rows(tensor):
+    """``tensor``, or a copy of it where its last axis is not contiguous."""
+
+    return tensor if tensor.stride(-1) == 1 or tensor.shape[-1] == 1 else tensor.contiguous()
+
+
 @functools.lru_cache(maxsize=1024)
 def _verify_counters(batch, vocab):
     return _native.library().slc_hip_verify_tokens_counter_count(batch, vocab)
@@ -231,45 +244,46 @@ def hip_verify_tokens(
 
     what = "HIP verify tokens"
     index = tokens.get_device()
-    if index < 0 or any(
-        tensor is not None and tensor.get_device() != index
-        for tensor in (target_probs, uniforms, parents, draft_probs)
+    if index < 0 or target_probs.get_device() != index or uniforms.get_device() != index or (
+        (parents is not None and parents.get_device() != index)
+        or (draft_probs is not None and draft_probs.get_device() != index)
     ):
         raise ValueError(f"{what}: all tensors must be on the GPU, and on one")
-    if tokens.dtype != torch.int64 or tokens.ndim != 2 or tokens.shape[1] < 1:
+    shape, target_shape = tokens.shape, target_probs.shape
+    if tokens.dtype != torch.int64 or len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{what}: tokens must be an int64 [batch, nodes] tensor")
-    batch, nodes = tokens.shape
+    batch, nodes = shape
     if nodes > MAX_NODES:
         raise ValueError(f"{what}: at most {MAX_NODES} nodes")
-    if parents is not None and (parents.dtype != torch.int64 or parents.shape != tokens.shape):
+    if parents is not None and (parents.dtype != torch.int64 or parents.shape != shape):
         raise ValueError(f"{what}: parents must be int64 and shaped like the tokens")
-    if uniforms.dtype != torch.float32 or uniforms.shape != tokens.shape:
+    if uniforms.dtype != torch.float32 or uniforms.shape != shape:
         raise ValueError(f"{what}: uniforms must be fp32 and shaped like the tokens")
-    if target_probs.ndim != 3 or target_probs.shape[:2] != tokens.shape or target_probs.shape[2] < 1:
+    if len(target_shape) != 3 or target_shape[:2] != shape or target_shape[2] < 1:
         raise ValueError(f"{what}: target_probs must be [batch, nodes, vocabulary]")
-    if target_probs.dtype not in _FLOATS:
-        raise ValueError(f"{what}: unsupported dtype {target_probs.dtype}")
-    vocab = target_probs.shape[2]
-    if draft_probs is not None and (
-        draft_probs.shape != (batch, nodes - 1, vocab) or draft_probs.dtype != target_probs.dtype
-    ):
+    dtype, vocab = target_probs.dtype, target_shape[2]
+    if dtype not in _FLOATS:
+        raise ValueError(f"{what}: unsupported dtype {dtype}")
+    if draft_probs is not None and (draft_probs.shape != (batch, nodes - 1, vocab) or draft_probs.dtype != dtype):
         raise ValueError(f"{what}: draft_probs must be [batch, nodes - 1, vocabulary] of the target's dtype")
-    tokens, parents, uniforms, target_probs, draft_probs = (
-        tensor if tensor is None or tensor.stride(-1) == 1 or tensor.shape[-1] == 1 else tensor.contiguous()
-        for tensor in (tokens, parents, uniforms, target_probs, draft_probs)
-    )
-    path, emitted = (tokens.new_empty((batch, nodes)) for _ in range(2))
-    counts = tokens.new_empty((batch,))
+    path = torch.empty_like(tokens, memory_format=_CONTIGUOUS)
+    emitted = torch.empty_like(path)
+    counts = path.new_empty(batch)
     if batch == 0:
         return path, emitted, counts
+    tokens, uniforms, target_probs = _rows(tokens), _rows(uniforms), _rows(target_probs)
+    up, up_stride, draft, draft_strides = None, 0, None, (0, 0)
+    if parents is not None:
+        parents = _rows(parents)
+        up, up_stride = parents.data_ptr(), parents.stride(0)
+    if draft_probs is not None:
+        draft_probs = _rows(draft_probs)
+        draft, draft_strides = draft_probs.data_ptr(), draft_probs.stride()[:2]
     owner = workspace if workspace is not None else _native.stream_workspace(tokens.device)
     counters = owner.counters(_verify_counters(batch, vocab))
-    draft, draft_strides = (None, (0, 0)) if draft_probs is None else (draft_probs.data_ptr(),
-                                                                       draft_probs.stride()[:2])
-    _call("slc_hip_verify_tokens", index, tokens.data_ptr(), None if parents is None else parents.data_ptr(),
-          target_probs.data_ptr(), draft, uniforms.data_ptr(), path.data_ptr(), emitted.data_ptr(), counts.data_ptr(),
-          counters.data_ptr(), counters.numel(), _native.dtype_tag(target_probs.dtype),
-          batch, nodes, vocab, tokens.stride(0), 0 if parents is None else parents.stride(0), uniforms.stride(0),
+    _call("slc_hip_verify_tokens", index, tokens.data_ptr(), up, target_probs.data_ptr(), draft, uniforms.data_ptr(),
+          path.data_ptr(), emitted.data_ptr(), counts.data_ptr(), counters.data_ptr(), counters.numel(),
+          _native.dtype_tag(dtype), batch, nodes, vocab, tokens.stride(0), up_stride, uniforms.stride(0),
           *target_probs.stride()[:2], *draft_strides)
     return path, emitted, counts
 
@@ -312,32 +326,34 @@ class KVLayers:
             self._pages = (block_table.data_ptr(), block_table.stride(0), pages, page_tokens, first.shape[0])
         if self.capacity < 1 or self.heads < 1 or self.head_dim < 1:
             raise ValueError(f"{what}: the buffers are empty")
-        pointers = [buffer.data_ptr() for buffer in buffers]
-        if len(set(pointers)) != len(pointers):
+        self._pointers = array("Q", [buffer.data_ptr() for buffer in buffers])
+        if len(set(self._pointers)) != len(buffers):
             raise ValueError(f"{what}: a buffer is there twice")
-        count = len(self.keys)
-        self._pointers = ctypes.c_void_p * count
-        self._keys, self._values = self._pointers(*pointers[:count]), self._pointers(*pointers[count:])
+        self._keys = self._pointers.buffer_info()[0]
+        self._values = self._keys + 8 * len(self.keys)
         self._dtype, self._strides = _native.dtype_tag(first.dtype), first.stride()[:3]
 
 
-def _layer_pointers(layers: KVLayers, lengths, what: str, name: str):
+def _layer_pointers(layers: KVLayers, lengths, what: str, name: str) -> array:
     """Device pointers of each layer's lengths: a tensor [B] (all layers'), [L, B], or
     a sequence of L tensors [B]."""
 
-    count, batch = len(layers.keys), layers.batch
+    count, batch, index = len(layers.keys), layers.batch, layers.index
     if isinstance(lengths, torch.Tensor):
-        if (lengths.dtype != torch.int64 or lengths.shape not in ((batch,), (count, batch))
-                or not lengths.is_contiguous() or lengths.get_device() != layers.index):
+        shape = lengths.shape
+        if (lengths.dtype != torch.int64 or shape not in ((batch,), (count, batch)) or not lengths.is_contiguous()
+                or lengths.get_device() != index):
             raise ValueError(f"{what}: {name} must be a contiguous int64 [B] or [layers, B] tensor on the caches' GPU")
-        start, step = lengths.data_ptr(), 8 * batch if lengths.ndim == 2 else 0
-        return [start + step * layer for layer in range(count)]
+        start, step = lengths.data_ptr(), 8 * batch
+        if len(shape) == 1 or batch == 0:
+            return array("Q", [start]) * count
+        return array("Q", range(start, start + step * count, step))
     if len(lengths) != count or any(
         length.dtype != torch.int64 or length.shape != (batch,) or not length.is_contiguous()
-        or length.get_device() != layers.index for length in lengths
+        or length.get_device() != index for length in lengths
     ):
         raise ValueError(f"{what}: {name} must be one contiguous int64 [B] tensor per layer, on the caches' GPU")
-    return [length.data_ptr() for length in lengths]
+    return array("Q", [length.data_ptr() for length in lengths])
 
 
 def hip_kv_commit(
@@ -368,9 +384,10 @@ def hip_kv_commit(
         overflow is not None and overflow.get_device() != index
     ):
         raise ValueError(f"{what}: all tensors must be on the GPU, and on one")
-    if path.dtype != torch.int64 or path.ndim != 2 or path.shape[0] != batch or not path.is_contiguous():
+    shape = path.shape
+    if path.dtype != torch.int64 or len(shape) != 2 or shape[0] != batch or not path.is_contiguous():
         raise ValueError(f"{what}: path must be a contiguous int64 [B, nodes] tensor")
-    if not 1 <= path.shape[1] <= MAX_NODES:
+    if not 1 <= shape[1] <= MAX_NODES:
         raise ValueError(f"{what}: 1 to {MAX_NODES} nodes")
     if counts.dtype != torch.int64 or counts.shape != (batch,) or not counts.is_contiguous():
         raise ValueError(f"{what}: counts must be a contiguous int64 [B] tensor")
@@ -383,19 +400,18 @@ def hip_kv_commit(
         targets = _layer_pointers(layers, out, what, "out")
         # A layer reads its length while another layer's is written.
         places = sorted({*sources, *targets})
-        if any(high - low < 8 * batch for low, high in zip(places, places[1:])) or any(
+        if batch and (any(high - low < 8 * batch for low, high in zip(places, places[1:])) or any(
             target in sources and (source != target or sources.count(target) > 1)
             for source, target in zip(sources, targets)
-        ):
+        )):
             raise ValueError(f"{what}: out may be a layer's own lengths, but overlap no other layer's")
-    if targets[0] == targets[-1]:  # one tensor for all layers: the first one's workgroups write it
-        targets = targets[:1] + [None] * (count - 1)
-    elif len(set(targets)) != count:
-        raise ValueError(f"{what}: every layer needs an output of its own")
+        if len(set(targets)) not in (1, count):
+            raise ValueError(f"{what}: every layer needs an output of its own")
     if batch == 0:
         return out
-    pointers = layers._pointers
-    _call("slc_hip_kv_commit", index, layers._keys, layers._values, pointers(*sources), pointers(*targets),
+    if targets[0] == targets[-1]:  # one tensor for all layers: the first one's workgroups write it
+        targets = targets[:1] + array("Q", [0]) * (count - 1)
+    _call("slc_hip_kv_commit", index, layers._keys, layers._values, sources.buffer_info()[0], targets.buffer_info()[0],
           *layers._pages, path.data_ptr(), counts.data_ptr(), None if overflow is None else overflow.data_ptr(),
-          layers._dtype, count, batch, path.shape[1], layers.heads, layers.head_dim, layers.capacity, *layers._strides)
+          layers._dtype, count, batch, shape[1], layers.heads, layers.head_dim, layers.capacity, *layers._strides)
     return out
