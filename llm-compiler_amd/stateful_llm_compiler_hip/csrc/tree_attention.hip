@@ -73,16 +73,18 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
   SLC_REQUIRE(a.counters != nullptr && num_counters >= batch * kv_heads * split.row_blocks, "%s: too few counters", what);
   a.row_blocks = static_cast<int>(split.row_blocks);
   a.slots = static_cast<int>(split.slots);
-  a.inverse_slots = 1.0f / static_cast<float>(split.slots);
+  // Pieces are rounded up to whole ones; the search for their size starts as if that took
+  // a third of a slot per sequence.
+  a.inverse_slots = 1.0f / (static_cast<float>(split.slots) - 0.3f * static_cast<float>(batch));
   char* place = static_cast<char*>(workspace);
   a.partial = reinterpret_cast<float*>(place);
   a.stats = reinterpret_cast<float2*>(place + split.partial_bytes);
   a.pieces = reinterpret_cast<int2*>(place + split.partial_bytes + split.stats_bytes);
+  const int es = slc_host::dtype_size(dtype);
   // What the last piece of a sequence would put together at most; from 64 KB on a merge
   // kernel does it (see tree_merge_kernel).
-  const int64_t most_pieces = std::min(split.slots - batch + 1, slc_host::ceil_div(a.rows, slc_tree::kMinPieceRows));
+  const int64_t most_pieces = std::min(split.slots - batch + 1, slc_host::ceil_div(a.rows, slc_tree::min_piece_rows(es)));
   if (most_pieces * std::min<int64_t>(rows, plan.rows_per_block) * plan.padded_dim * 4 > 65536) a.counters = nullptr;
-  const int es = slc_host::dtype_size(dtype);
   const auto on = [es](int64_t bytes, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> sizes) {
     uint64_t bits = 0;
     for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);

@@ -20,7 +20,7 @@
 //  * O^T[dim, query] += V^T . P^T: the score tile's C layout is the product's B layout
 //    once V's rows are taken in the same order.
 // The WK partial results meet in LDS; the pieces' partial results, where a sequence
-// has several, in the last of them to end.
+// has several, in the last of them to end or in a kernel of their own.
 #pragma once
 #include <cmath>
 #include <type_traits>
@@ -143,8 +143,11 @@ __device__ __forceinline__ int quotient(int n, int d, float inverse) {
   return q + (rest >= d) - (rest < 0);
 }
 
-// The tail, whose rows only some nodes see, takes as long as so many steps more.
-constexpr int kTailSteps = 2;
+// The tail, whose rows only some nodes see, takes as long as so many steps more: a step
+// with masks has twice the instructions, and wide trees span several short steps (64
+// nodes, batch of 16: 32.5 us with 2, 31.2 with 5 or 6).
+template <int STEP>
+constexpr int kTailSteps = STEP <= 64 ? 5 : 2;
 
 struct Piece {
   int sequence;  // -1: none
@@ -165,7 +168,7 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
   };
   auto end_of = [&](int length) { return length + a.nodes < rows ? length + a.nodes : rows; };
   auto steps_of = [&](int b, int length) {
-    const int n = (end_of(length) + STEP - 1) / STEP + kTailSteps;
+    const int n = (end_of(length) + STEP - 1) / STEP + kTailSteps<STEP>;
     return b < a.batch ? n : 0;
   };
   // Of the first 64 sequences; more are read again in every pass.
@@ -197,100 +200,116 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
       before = __builtin_amdgcn_readlane(upto, 63);
     }
     if (before <= a.slots) break;
-    q *= 1.125f;
+    q *= 1.05f;
   }
   p.index = x - p.first;
   p.end = end_of(p.length);
   return p;
 }
 
-// The pieces [first, first + count) of a sequence's row block put together by `threads`
-// threads: each takes kItems times four dims of a row, over a batch of pieces at a time.
-template <typename T, int DP, int ROWS, int kItems>
-__device__ __forceinline__ void merge_pieces(const TreeArgs& a, int64_t b, int kvh, int block, int first, int count,
-                                             int thread, int threads) {
-  constexpr int kBatch = 4, kQuads = DP / 16;
+// Results pass between workgroups, which may be on XCDs with L2s of their own, by loads
+// and stores of agent scope: they go past the L2, so that no cache has to be written back
+// or emptied for them as a release and an acquire would.
+__device__ __forceinline__ void put_pair(float2* place, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(place), __builtin_bit_cast(uint64_t, make_float2(x, y)), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_pair(const float2* place) {
+  return __builtin_bit_cast(
+      float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(place), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Units of 16 rows and 16 dims that a row block has.
+template <int DP, int ROWS>
+__device__ __forceinline__ int block_units(const TreeArgs& a, int block) {
+  const int rows = a.q_heads / a.kv_heads * a.nodes - block * ROWS;
+  return ((rows < ROWS ? rows : ROWS) + 15) / 16 * (DP / 16);
+}
+// Units unit, unit + step, .. (kUnits of them, those below `units`) of a sequence's row
+// block (each float4 of a wave's lanes, in two planes of pairs) put together from the
+// `count` pieces from slot `first` on, kBatch at a time.
+template <typename T, int DP, int ROWS, int kUnits, int kBatch>
+__device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kvh, int block, int first, int count,
+                                            int unit, int step, int units) {
+  constexpr int kQuads = DP / 16;
+  const int lane = threadIdx.x & 63;
   const int group = a.q_heads / a.kv_heads;
   const float inverse_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
-  const int rows = group * a.nodes - block * ROWS < ROWS ? group * a.nodes - block * ROWS : ROWS;
-  const int items = (rows + 15) / 16 * kQuads * 64;  // a block of 16 rows, its quads, a wave's lanes
   const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.row_blocks * ROWS;  // between pieces
   const int64_t place = ((static_cast<int64_t>(first) * a.kv_heads + kvh) * a.row_blocks + block) * ROWS;
-  auto row_of = [](int item) { return item / (64 * kQuads) * 16 + (item & 15); };
+  const float2* stats = a.stats + place + (lane & 15);
+  const float2* partial = reinterpret_cast<const float2*>(a.partial + place * DP) + lane;
+  float top[kUnits], sum[kUnits];
+  float4 v[kUnits];
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    top[j] = -INFINITY;
+    sum[j] = 0.0f;
+    v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
 #pragma unroll 1
-  for (int base = thread; base < items; base += kItems * threads) {
-    float top[kItems], sum[kItems];
-    float4 v[kItems];
+  for (int at = 0; at < count; at += kBatch) {
+    float2 s[kUnits][kBatch], lo[kUnits][kBatch], hi[kUnits][kBatch];
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      top[j] = -INFINITY;
-      sum[j] = 0.0f;
-      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll 1
-    for (int at = 0; at < count; at += kBatch) {
-      float2 s[kItems][kBatch];
-      float4 o[kItems][kBatch];
+    for (int j = 0; j < kUnits; ++j) {
+      const int u = unit + j * step < units ? unit + j * step : unit;
 #pragma unroll
-      for (int j = 0; j < kItems; ++j) {
-        const int item = base + j * threads < items ? base + j * threads : base;
-        const float2* stats = a.stats + place + row_of(item);
-        const float* partial = a.partial + place * DP + item * 4;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const bool is = at + i < count;
-          const int64_t k = (is ? at + i : at) * stride;
-          s[j][i] = stats[k];
-          o[j][i] = *reinterpret_cast<const float4*>(partial + k * DP);
-          if (!is) {
-            s[j][i] = make_float2(-INFINITY, 0.0f);
-            o[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kItems; ++j) {
-        float most = top[j];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) most = fmaxf(most, s[j][i].x);
-        const float use = most == -INFINITY ? 0.0f : most;
-        const float own = __builtin_amdgcn_exp2f((top[j] - use) * kLog2e);
-        top[j] = most;
-        sum[j] *= own;
-        v[j] = make_float4(v[j].x * own, v[j].y * own, v[j].z * own, v[j].w * own);
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const float w = __builtin_amdgcn_exp2f((s[j][i].x - use) * kLog2e);
-          sum[j] = fmaf(w, s[j][i].y, sum[j]);
-          v[j].x = fmaf(w, o[j][i].x, v[j].x);
-          v[j].y = fmaf(w, o[j][i].y, v[j].y);
-          v[j].z = fmaf(w, o[j][i].z, v[j].z);
-          v[j].w = fmaf(w, o[j][i].w, v[j].w);
-        }
+      for (int i = 0; i < kBatch; ++i) {
+        const int64_t k = (at + i < count ? at + i : at) * stride;
+        s[j][i] = get_pair(stats + k + u / kQuads * 16);
+        lo[j][i] = get_pair(partial + k * (DP / 2) + u * 128);
+        hi[j][i] = get_pair(partial + k * (DP / 2) + u * 128 + 64);
       }
     }
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const int item = base + j * threads;
-      const int row = block * ROWS + row_of(item);
-      const int dim = quad_dim<T>(item / 64 % kQuads, item >> 4 & 3);
-      if (item >= items || row >= group * a.nodes) continue;
-      const int n = quotient(row, group, inverse_group);
-      const int h = kvh * group + row - n * group;
-      store_quad<T>(static_cast<T*>(a.output) + b * a.o_sb + h * a.o_sh + n * a.o_st, dim, a.head_dim, a.vector_o,
-                    divided(v[j], sum[j]));
+    for (int j = 0; j < kUnits; ++j) {
+      float most = top[j];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (at + i >= count) {
+          s[j][i] = make_float2(-INFINITY, 0.0f);
+          lo[j][i] = hi[j][i] = make_float2(0.f, 0.f);
+        }
+        most = fmaxf(most, s[j][i].x);
+      }
+      const float use = most == -INFINITY ? 0.0f : most;
+      const float own = __builtin_amdgcn_exp2f((top[j] - use) * kLog2e);
+      top[j] = most;
+      sum[j] *= own;
+      v[j] = make_float4(v[j].x * own, v[j].y * own, v[j].z * own, v[j].w * own);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float w = __builtin_amdgcn_exp2f((s[j][i].x - use) * kLog2e);
+        sum[j] = fmaf(w, s[j][i].y, sum[j]);
+        v[j].x = fmaf(w, lo[j][i].x, v[j].x);
+        v[j].y = fmaf(w, lo[j][i].y, v[j].y);
+        v[j].z = fmaf(w, hi[j][i].x, v[j].z);
+        v[j].w = fmaf(w, hi[j][i].y, v[j].w);
+      }
     }
   }
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    const int u = unit + j * step;
+    const int row = block * ROWS + u / kQuads * 16 + (lane & 15);
+    if (u >= units || row >= group * a.nodes) continue;
+    const int n = quotient(row, group, inverse_group);
+    const int h = kvh * group + row - n * group;
+    store_quad<T>(static_cast<T*>(a.output) + b * a.o_sb + h * a.o_sh + n * a.o_st, quad_dim<T>(u % kQuads, lane >> 4),
+                  a.head_dim, a.vector_o, divided(v[j], sum[j]));
+  }
 }
-// The same for large blocks, by workgroups of their own: one CU takes in about 10 bytes
-// a cycle, so that one workgroup is slow from some 64 KB on.
+// The same for large results, by workgroups of their own: one CU takes in about 10 bytes
+// a cycle, so that the last piece alone is slow from some 64 KB on.
 template <typename T, int DP, int ROWS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const int64_t b = blockIdx.z;
   const int2 pieces = a.pieces[b];
-  if (pieces.y <= 1) return;
   const int kvh = blockIdx.y / a.row_blocks, block = blockIdx.y % a.row_blocks;
-  merge_pieces<T, DP, ROWS, 1>(a, b, kvh, block, pieces.x, pieces.y, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+  const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int units = block_units<DP, ROWS>(a, block);
+  if (pieces.y <= 1 || unit >= units) return;
+  merge_units<T, DP, ROWS, 1, 8>(a, b, kvh, block, pieces.x, pieces.y, unit, 1, unit + 1);
 }
 
 // Sizes of a kernel: DP the padded head dim, QB blocks of 16 query rows a wave, WR waves
@@ -346,17 +365,22 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   const Piece piece = find_piece<S::kStep>(a, slot, min_steps);
   if (piece.sequence < 0) return;
   const int64_t b = piece.sequence;
-  // Its steps: the sequence's and its tail's, shared out as evenly as whole steps go.
+  // Its steps: the sequence's and its tail's, shared out as evenly as whole steps go; the
+  // last pieces take the spare ones, the tail's count with the last step.
   const int steps = (piece.end + S::kStep - 1) / S::kStep;
-  const int shared = steps + kTailSteps;
+  const int shared = steps + kTailSteps<S::kStep>;
   const int share = static_cast<int>(static_cast<unsigned>(shared) / static_cast<unsigned>(piece.count));
-  const int spare = shared - share * piece.count;
-  const int step0 = min(steps, piece.index * share + min(piece.index, spare));
-  const int nsteps = min(steps, step0 + share + (piece.index < spare ? 1 : 0)) - step0;
+  const int shorter = piece.count - (shared - share * piece.count);  // pieces without a spare one
+  auto first_step = [&](int index) { return max(0, min(steps - 1, index * share + max(0, index - shorter))); };
+  int count = piece.count;
+  while (count > 1 && first_step(count - 1) == first_step(count - 2)) --count;
+  if (piece.index >= count) return;
+  const int step0 = first_step(piece.index);
+  const int nsteps = (piece.index + 1 < count ? first_step(piece.index + 1) : steps) - step0;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (a.counters == nullptr && tid == 0 && piece.index == 0 && kvh == 0 && block == 0)
-    a.pieces[b] = make_int2(piece.first, piece.count);
+    a.pieces[b] = make_int2(piece.first, count);
 
   if (wave >= S::kConsumers) {
     // ---- producers ------------------------------------------------------------
@@ -792,10 +816,12 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   auto store = [&](int i, int qb, float4 v, float top, float sum) {
     if (!real[qb]) return;
     const int dim = quad_dim<T>(i, g);
-    if (piece.count > 1) {
+    if (count > 1) {
       // As the lanes hold them, so that a wave writes whole lines.
-      reinterpret_cast<float4*>(a.partial + place * S::kRows * DP)[((wr * QB + qb) * S::kQuads + i) * 64 + lane] = v;
-      if (g == 0 && i == 0) a.stats[place * S::kRows + wr * 16 * QB + 16 * qb + c] = make_float2(top, sum);
+      float2* to = reinterpret_cast<float2*>(a.partial + place * S::kRows * DP) + ((wr * QB + qb) * S::kQuads + i) * 128 + lane;
+      put_pair(to, v.x, v.y);
+      put_pair(to + 64, v.z, v.w);
+      if (g == 0 && i == 0) put_pair(&a.stats[place * S::kRows + wr * 16 * QB + 16 * qb + c], top, sum);
     } else {
       T* row = static_cast<T*>(a.output) + b * a.o_sb + head[qb] * a.o_sh + node[qb] * a.o_st;
       store_quad<T>(row, dim, a.head_dim, a.vector_o, divided(v, sum));
@@ -854,35 +880,37 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       }
     }
   }
-  if (piece.count == 1 || a.counters == nullptr) return;
+  if (count == 1 || a.counters == nullptr) return;
 
-  // The last of a sequence's pieces to arrive puts all of them together: every wave's
-  // results come before the barrier, the count is an agent-scope acquire-release add.
-  const int mine = (piece.sequence * a.kv_heads + kvh) * a.row_blocks + block;
+  // The last of a sequence's pieces to arrive puts all of them together.  Each wave's
+  // results are in the memory before it counts itself in.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
-    arrived = __hip_atomic_fetch_add(&a.counters[mine], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    if (arrived == piece.count - 1) __hip_atomic_store(&a.counters[mine], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int* const counter = a.counters + (piece.sequence * a.kv_heads + kvh) * a.row_blocks + block;
+    arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (arrived == count - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (__builtin_amdgcn_readfirstlane(arrived) != piece.count - 1) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  merge_pieces<T, DP, S::kRows, 2>(a, piece.sequence, kvh, block, piece.first, piece.count, tid, S::kConsumers * 64);
+  if (__builtin_amdgcn_readfirstlane(arrived) != count - 1) return;
+  const int units = block_units<DP, S::kRows>(a, block);
+#pragma unroll 1
+  for (int unit = wave; unit < units; unit += 2 * S::kConsumers)
+    merge_units<T, DP, S::kRows, 2, 4>(a, b, kvh, block, piece.first, count, unit, S::kConsumers, units);
 }
 
 template <typename T, int DP, int QB, int WR, int KT>
 int launch_shape(const TreeArgs& a, hipStream_t stream) {
   using S = Shape<T, DP, QB, WR, KT>;
-  const float min_steps = static_cast<float>((kMinPieceRows + S::kStep - 1) / S::kStep);
+  const float min_steps = static_cast<float>((min_piece_rows(sizeof(T)) + S::kStep - 1) / S::kStep);
   hipLaunchKernelGGL((tree_attention_kernel<T, DP, QB, WR, KT>), dim3(a.kv_heads, a.slots, a.row_blocks),
                      dim3(S::kThreads), 0, stream, a, min_steps);
   const int status = slc_host::check_launch("tree attention");
   // Its pieces are put together by the last of them, or by another kernel; there are none
   // where every sequence is one.
-  if (status != SLC_OK || a.counters != nullptr || a.slots <= a.batch || a.rows <= kMinPieceRows) return status;
-  const int items = S::kRows * DP / 4;
-  hipLaunchKernelGGL((tree_merge_kernel<T, DP, S::kRows>), dim3((items + 255) / 256, a.kv_heads * a.row_blocks, a.batch),
-                     dim3(256), 0, stream, a);
+  if (status != SLC_OK || a.counters != nullptr || a.slots <= a.batch || a.rows <= min_piece_rows(sizeof(T))) return status;
+  hipLaunchKernelGGL((tree_merge_kernel<T, DP, S::kRows>),
+                     dim3((S::kRows * DP / 256 + 3) / 4, a.kv_heads * a.row_blocks, a.batch), dim3(256), 0, stream, a);
   return slc_host::check_launch("tree attention merge");
 }
 
