@@ -80,7 +80,9 @@ def _tree_operands(what, query, key, value, lengths, tree_mask, attention_mask, 
         mask_len = attention_mask.shape[3]
         if mask_len > rows:
             raise ValueError(f"{what}: mask is longer than the cache's capacity")
-        mask, mask_dtype = attention_mask.data_ptr(), _native.dtype_tag(attention_mask.dtype)
+        # (A mask of no rows hides all; its null pointer would stand for no mask.)
+        mask = attention_mask.data_ptr() if mask_len else lengths.data_ptr()
+        mask_dtype = _native.dtype_tag(attention_mask.dtype)
         mask_strides = (attention_mask.stride(0), attention_mask.stride(3))
     return index, (lengths.data_ptr(), _native.dtype_tag(lengths.dtype), tree, mask, mask_dtype), mask_len, (
         *tree_strides, *mask_strides)
@@ -314,6 +316,8 @@ class KVLayers:
             raise ValueError(f"{what}: buffers need one shape, dtype and set of strides")
         if first.stride(3) != 1 and first.shape[3] > 1:
             raise ValueError(f"{what}: the head dim must be contiguous")
+        if any(stride == 0 and size > 1 for stride, size in zip(first.stride(), first.shape)):
+            raise ValueError(f"{what}: expanded buffers cannot be written")
         if block_table is None:
             self.batch, self.capacity, self.heads, self.head_dim = first.shape
             self._pages = (None, 0, 0, 0, 0)
@@ -370,6 +374,7 @@ def hip_kv_commit(
 
     ``path`` [B, T] and ``counts`` [B], int64, as ``hip_verify_tokens`` gives them:
     a row's path ascends within its count (entries that are no node are not moved).
+    Pages that rows move in belong to one sequence.
     ``lengths``: int64 [B], the same for all layers, or [layers, B], or one [B] tensor
     per layer.  ``out`` receives the new ones, in any of these forms, and may be
     ``lengths`` itself where these are a tensor for each layer.  Rows behind the new
@@ -407,6 +412,10 @@ def hip_kv_commit(
             raise ValueError(f"{what}: out may be a layer's own lengths, but overlap no other layer's")
         if len(set(targets)) not in (1, count):
             raise ValueError(f"{what}: every layer needs an output of its own")
+        for tensor in (path, counts):
+            start, end = tensor.data_ptr(), tensor.data_ptr() + 8 * tensor.numel()
+            if any(start - 8 * batch < target < end for target in targets):
+                raise ValueError(f"{what}: out overlaps the path or the counts")
     if batch == 0:
         return out
     if targets[0] == targets[-1]:  # one tensor for all layers: the first one's workgroups write it

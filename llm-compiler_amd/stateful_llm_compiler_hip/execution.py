@@ -126,7 +126,7 @@ class PreallocatedKVCacheState:
     # current stream's workspace.
     workspace: _native.DeviceWorkspace | None = None
     # The checked layers of commit(), made by the first one and passed on to later
-    # versions; made anew for other buffers.
+    # versions; made anew for other buffers or another block table.
     layers: KVLayers | None = field(default=None, compare=False, repr=False)
 
     def __post_init__(self) -> None:
@@ -432,9 +432,10 @@ class PreallocatedKVCacheState:
 
         if path.ndim != 2 or path.shape[0] != self.lengths[0].shape[0] or counts.shape != (path.shape[0],):
             raise ExecutionError("KV commit takes a B x T path and B counts")
-        layers = self.layers
-        if layers is None or layers.keys is not self.keys or layers.values is not self.values:
-            layers = KVLayers(self.keys, self.values, block_table=self._block_table())
+        layers, table = self.layers, self._block_table()
+        if (layers is None or layers.keys is not self.keys or layers.values is not self.values
+                or layers.block_table is not table):
+            layers = KVLayers(self.keys, self.values, block_table=table)
         out = hip_kv_commit(layers, self.lengths, path, counts, out=self.lengths if self.in_place_lengths else None,
                             overflow=self.overflow)
         object.__setattr__(self, "layers", layers)

@@ -387,6 +387,114 @@ def test_tree_attention_repeats_bit_for_bit_on_streams_and_in_graphs(gpu):
         assert_bitwise_equal(out, backends.hip_tree_attention(static[0], *args[1:3], static[3], tree, scale=0.125))
 
 
+def dense_reference(query, key, value, lengths, tree, scale):
+    """``tree_reference`` without a mask, on the inputs' device a head at a time, for
+    lengths of at least one."""
+
+    batch, q_heads, nodes, head_dim = query.shape
+    capacity, kv_heads = key.shape[1:3]
+    parts = [torch.empty(query.shape, dtype=torch.float64) for _ in range(4)]
+    if tree is None:
+        tree = torch.ones(nodes, nodes, dtype=torch.bool, device=query.device).tril_()
+    for b in range(batch):
+        length = int(lengths[b])
+        end = length + nodes
+        seen = torch.cat([torch.ones(nodes, length, dtype=torch.bool, device=query.device), tree], 1)
+        for h in range(q_heads):
+            q = query[b, h].double()
+            k, v = (side[b, :end, h * kv_heads // q_heads].double() for side in (key, value))
+            t = (q @ k.T * scale).masked_fill(~seen, -INF)
+            w = torch.softmax(t, -1)
+            away = (t.amax(-1, keepdim=True) - t).clamp_max(200).masked_fill(~seen, 0).amax(-1, keepdim=True)
+            size = (q.abs() @ k.abs().T * scale).masked_fill(~seen, 0).amax(-1, keepdim=True)
+            for part, x in zip(parts, (w @ v, w @ v.abs(), away.expand(nodes, head_dim), size.expand(nodes, head_dim))):
+                part[b, h] = x.cpu()
+    return parts
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("case", [
+    # q_heads, kv_heads, head_dim, nodes, lengths, whether a tree
+    (2, 1, 64, 1024, [900], True),
+    (2, 1, 64, 4096, [301], False),
+    (14, 2, 64, 8, [69001], True),
+    (4, 2, 128, 5, [39990, 3], True),
+    (16, 1, 64, 100, [9000, 1], True),
+    (3, 1, 40, 30, [20000], True),
+])
+def test_tree_attention_of_wide_trees_and_long_caches(gpu, case, dtype):
+    q_heads, kv_heads, head_dim, nodes, lengths, is_tree = case
+    announce(f"tree attention {case} {dtype}")
+    g = generator(nodes)
+    capacity = max(lengths) + nodes + 7
+    tensors = tree_inputs(g, len(lengths), q_heads, kv_heads, head_dim, nodes, capacity, dtype, lengths)
+    query, key, value, lengths = (t.to(gpu) for t in tensors)
+    tree = random_tree(nodes, g).to(gpu) if is_tree else None
+    out = backends.hip_tree_attention(query, key, value, lengths, tree, scale=head_dim**-0.5)
+    assert_tree_close(out, dense_reference(query, key, value, lengths, tree, head_dim**-0.5), capacity)
+
+
+def test_tree_attention_with_a_mask_of_no_rows(gpu):
+    announce("tree attention empty mask")
+    for dtype in (torch.bfloat16, torch.float32):
+        query, cache = torch.ones(2, 4, 3, 64, device=gpu, dtype=dtype), torch.ones(2, 32, 2, 64, device=gpu, dtype=dtype)
+        lengths = torch.tensor([0, 20], device=gpu)
+        mask = torch.zeros(2, 1, 1, 0, device=gpu)
+        assert backends.hip_tree_attention(query, cache, cache, lengths, None, mask, scale=1.0).isnan().all()
+
+
+def test_offsets_past_32_bits(gpu):
+    """Caches and pools of more than 2^31 elements: attention and commit at their ends."""
+
+    g = generator(31)
+    dtype, nodes, length = torch.bfloat16, 6, 300
+    query, key, value, lengths = tree_inputs(g, 1, 4, 1, 64, nodes, 320, dtype, [length])
+    tree = random_tree(nodes, g)
+    reference = tree_reference(query, key, value, lengths, tree, None, 0.125)
+    path, counts = torch.tensor([[0, 2, 5, -1, -1, -1]], device=gpu), torch.tensor([3], device=gpu)
+    moved = commit_reference([key, value], lengths, path.cpu(), counts.cpu())
+    query, lengths, tree = query.to(gpu), lengths.to(gpu), tree.to(gpu)
+
+    announce("offsets past 32 bits: a sequence")
+    caches = [torch.zeros(2, 2**25 + 16, 1, 64, dtype=dtype, device=gpu) for _ in range(2)]
+    for cache, side in zip(caches, (key, value)):
+        cache[1, :320] = side[0].to(gpu)
+    both = torch.cat([lengths * 0, lengths])
+    out = backends.hip_tree_attention(query.expand(2, -1, -1, -1), *caches, both, tree, scale=0.125)
+    assert_tree_close(out[1:], reference, 320)
+    backends.hip_kv_commit(backends.KVLayers(caches[:1], caches[1:]), both, path.expand(2, -1).contiguous(),
+                           torch.cat([counts * 0, counts]))
+    for cache, side in zip(caches, moved):
+        assert torch.equal(bits(cache[1:, :320].cpu()), bits(side))
+        assert not cache[0].any()
+    del caches, cache
+
+    announce("offsets past 32 bits: pages")
+    pools = [torch.zeros(2**21 + 40, 16, 1, 64, dtype=dtype, device=gpu) for _ in range(2)]
+    table = (2**21 + 39 - torch.arange(20, dtype=torch.int32, device=gpu)).unsqueeze(0)
+    for pool, side in zip(pools, (key, value)):
+        pool[table[0].long()] = side.view(20, 16, 1, 64).to(gpu)
+    out = backends.hip_paged_tree_attention(query, *pools, table, lengths, tree, scale=0.125)
+    assert_tree_close(out, reference, 320)
+    backends.hip_kv_commit(backends.KVLayers(pools[:1], pools[1:], block_table=table), lengths, path, counts)
+    for pool, side in zip(pools, moved):
+        assert torch.equal(bits(pool[table[0].long()].cpu().view(1, 320, 1, 64)), bits(side))
+        assert not pool[: 2**21].any()
+    del pools, pool
+
+    # Rows 4 MB apart, and a little more, which are no longer on 16 bytes.
+    query, key, value, lengths = tree_inputs(g, 1, 4, 1, 64, nodes, 1060, dtype, [1050])
+    reference = tree_reference(query, key, value, lengths, tree.cpu(), None, 0.125)
+    rooms = [torch.empty(1060 * (2**21 + 1), dtype=dtype, device=gpu) for _ in range(2)]
+    for step in (2**21, 2**21 + 1):
+        announce(f"offsets past 32 bits: rows {step} elements apart")
+        caches = [room.as_strided((1, 1060, 1, 64), (2**21, step, 64, 1)) for room in rooms]
+        for cache, side in zip(caches, (key, value)):
+            cache.copy_(side)
+        out = backends.hip_tree_attention(query.to(gpu), *caches, lengths.to(gpu), tree, scale=0.125)
+        assert_tree_close(out, reference, 1060)
+
+
 def test_tree_attention_refuses(gpu):
     q = torch.zeros(2, 4, 3, 64, device=gpu, dtype=torch.bfloat16)
     kv = torch.zeros(2, 32, 2, 64, device=gpu, dtype=torch.bfloat16)
@@ -676,6 +784,29 @@ def test_verify_gives_the_targets_distribution(gpu):
         assert ((counts - steps * p.double()).abs() <= 6 * deviation + steps * 2.0**-12).all()
 
 
+def test_verify_offsets_past_32_bits(gpu):
+    """A vocabulary of 2^24 + 8 and 2^31 probabilities and more."""
+
+    announce("verify offsets past 32 bits")
+    nodes, vocab = 64, 2**24 + 8
+    target = torch.zeros(2, nodes, vocab, dtype=torch.float16, device=gpu)
+    tokens = torch.randint(0, vocab, (2, nodes), generator=generator(3))
+    target[0, 0, 7] = 1.0
+    target[1, torch.arange(nodes - 1), tokens[1, 1:]] = 1.0
+    target[1, -1, 5], target[1, -1, 2**24] = 0.25, 0.75
+    uniforms = torch.full((2, nodes), 0.5, device=gpu)
+    path, emitted, counts = backends.hip_verify_tokens(tokens.to(gpu), target, uniforms)
+    assert counts.tolist() == [1, nodes] and emitted[0, 0].item() == 7
+    assert emitted[1].tolist() == tokens[1, 1:].tolist() + [2**24]
+    # And with draft rows, those of another token: the leftover is the target's.
+    draft = torch.zeros_like(target[:, : nodes - 1])
+    draft[..., vocab - 1] = 1.0
+    tokens[:] = vocab - 1
+    path, emitted, counts = backends.hip_verify_tokens(tokens.to(gpu), target.flip(0), uniforms, draft_probs=draft)
+    assert counts.tolist() == [1, 1] and emitted[1, 0].item() == 7
+    assert path.tolist() == [[0] + [-1] * (nodes - 1)] * 2
+
+
 def test_verify_refuses(gpu):
     tokens = torch.zeros(2, 3, device=gpu, dtype=torch.int64)
     target, uniforms = torch.ones(2, 3, 5, device=gpu), torch.zeros(2, 3, device=gpu)
@@ -827,6 +958,21 @@ def test_commit_forms_of_lengths(gpu):
         run(handle, each, path, counts, out=[lap[0:2], lap[1:3], lap[4:6]])
 
 
+def test_commit_refuses_outputs_over_its_inputs(gpu):
+    announce("commit over its inputs")
+    buffers = [torch.zeros(2, 20, 2, 8, device=gpu) for _ in range(4)]
+    handle = backends.KVLayers(buffers[:2], buffers[2:])
+    path = torch.zeros(2, 3, dtype=torch.int64, device=gpu)
+    room = torch.zeros(5, dtype=torch.int64, device=gpu)
+    lengths, counts = torch.zeros(2, dtype=torch.int64, device=gpu), room[1:3]
+    for out in (counts, room[0:2], room[2:4], path[0, :2], path[1, 1:]):
+        with pytest.raises(ValueError):
+            backends.hip_kv_commit(handle, lengths, path, counts, out=out)
+    assert backends.hip_kv_commit(handle, lengths, path, counts, out=room[3:5]).tolist() == [0, 0]
+    with pytest.raises(ValueError):  # one sequence's rows for all
+        backends.KVLayers([buffers[0][:1].expand(2, -1, -1, -1)], [buffers[1][:1].expand(2, -1, -1, -1)])
+
+
 def test_commit_does_not_leave_the_cache(gpu):
     announce("commit bounds")
     # Entries that are no node, sources past the capacity, pages that are none of the pool's.
@@ -960,3 +1106,83 @@ def test_drafted_steps_give_the_tokens_of_single_steps(gpu, page_tokens, in_plac
         assert done[b][:steps] == single[b, :steps].tolist()
         assert int(state.lengths[2][b]) == prompt + len(done[b]) - 1
     assert max(taken) == 5 and min(taken) == 1  # paths of all lengths were taken
+
+
+def test_commit_follows_the_states_block_table(gpu):
+    from dataclasses import replace
+
+    from stateful_llm_compiler_hip.execution import PagedKVCacheState
+
+    announce("commit block table")
+    template = torch.zeros(1, 1, 1, 8, device=gpu, dtype=torch.bfloat16)
+    state = PagedKVCacheState.empty_from_key_template(template, num_layers=2, capacity=32, page_tokens=16)
+    path, counts = torch.tensor([[0, 2, -1]], device=gpu), torch.tensor([2], device=gpu)
+    state = state.commit(path, counts)
+    state = replace(state, block_table=state.block_table.flip(1).contiguous())
+    for buffer in state.keys + state.values:
+        buffer.copy_(torch.arange(32.0, device=gpu).view(2, 16, 1, 1).expand(2, 16, 1, 8))
+    state = state.commit(path, counts)
+    page = int(state.block_table[0, 0])
+    for buffer in state.keys + state.values:
+        want = torch.arange(32.0).view(2, 16)
+        want[page, 3] = want[page, 4]  # row 2 + 2 to row 2 + 1
+        assert torch.equal(buffer[:, :, 0, 0].float().cpu(), want)
+    assert state.lengths[1].item() == 4
+
+
+def test_a_captured_step_goes_on_at_every_replay(gpu):
+    """Attention, verification and the commit in place, captured on a workspace that is
+    new, and with another graph on the same one, replayed among eager steps."""
+
+    from dataclasses import replace
+
+    from stateful_llm_compiler_hip.execution import PreallocatedKVCacheState
+
+    announce("captured step")
+    g = generator(41)
+    batch, nodes, vocab, capacity, layers = 3, 7, 900, 400, 2
+    tree = random_tree(nodes, g)
+    parents = torch.tensor([-1] + [int(tree[c, :c].nonzero().max()) for c in range(1, nodes)])
+    tree, parents = tree.to(gpu), parents.expand(batch, -1).contiguous().to(gpu)
+    query = torch.randn(batch, 8, nodes, 64, generator=g).to(gpu, torch.bfloat16)
+    template = torch.zeros(batch, 2, 1, 64, device=gpu, dtype=torch.bfloat16)
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=g).to(gpu)
+    target = probabilities(g, batch, nodes, vocab).to(gpu)
+    target[torch.arange(batch).unsqueeze(1), parents.clamp_min(0), tokens] += 0.5
+    uniforms = torch.rand(batch, nodes, generator=g).to(gpu)
+
+    def state_of(workspace):
+        state = PreallocatedKVCacheState.empty_from_key_template(template, num_layers=layers, capacity=capacity)
+        start = torch.tensor([300, 0, 17], device=gpu)
+        state = replace(state, in_place_lengths=True, workspace=workspace, lengths=tuple(start.clone() for _ in range(layers)),
+                        zero_slots=frozenset())
+        for buffer, seed in zip(state.keys + state.values, range(2 * layers)):
+            buffer.copy_(torch.randn(buffer.shape, generator=generator(seed)))
+        return state
+
+    def step(state, workspace):
+        outs = [state.tree_attention(slot, query, tree, groups=4, scale=0.125) for slot in range(layers)]
+        path, emitted, counts = backends.hip_verify_tokens(tokens, target, uniforms, parents=parents, workspace=workspace)
+        state.commit(path, counts)
+        return outs + [path, emitted, counts]
+
+    eager_workspace, workspace = _native.DeviceWorkspace(gpu), _native.DeviceWorkspace(gpu)
+    eager, captured, other = state_of(eager_workspace), state_of(workspace), state_of(workspace)
+    graphs = []
+    for state in (captured, other):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(state, workspace)
+        graphs.append((graph, outs, state))
+    for turn in range(5):
+        uniforms.copy_(torch.rand(batch, nodes, generator=g))
+        want = step(eager, eager_workspace)
+        for graph, outs, state in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, outs, state in graphs:
+            for got, expected in zip(outs, want):
+                assert torch.equal(got, expected)
+            for got, expected in zip(state.lengths + state.keys + state.values, eager.lengths + eager.keys + eager.values):
+                assert torch.equal(got, expected)
+    assert eager.lengths[0].tolist() != [300, 0, 17]
