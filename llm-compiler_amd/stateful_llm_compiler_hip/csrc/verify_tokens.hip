@@ -17,13 +17,17 @@
 // between two tokens moves by 1e-16 of the sum with the order of additions.
 //
 // The bytes are one row (p) or two (p and q) of the vocabulary per sequence, and
-// a call is bound by the chain of memory round trips, not by them: the nodes' own
-// probabilities (all gathered at once), the row, its blocks' sums, one block again.
-// So several workgroups share a sequence: each walks the tree for itself, sums
-// blocks of 1024 weights, one a wave, and the last to arrive finds the block and
+// small batches are bound by the chain of memory round trips, not by them: the nodes'
+// tokens, their probabilities (all gathered at once), the row, its blocks' sums, one
+// block again.  So several workgroups share a sequence: each walks the tree for itself
+// and sums blocks of 1024 weights, one a wave, and the last to arrive finds the block and
 // the token.  Only a node whose second child is tried with a draft row needs more
 // passes over its row (the mass decides the next test); the last workgroup makes
 // them alone.
+//
+// In a graph, vocabulary 151936, fp32: a chain of 5 nodes 7.5 us, 8 trees of 64 without
+// draft rows 7.7 us; 32 chains of 9 15.5 us, 39 MB at 2.5 TB/s: of it some 7 us are the
+// round trips and the launch again, 8 us the rows at the rate of a large copy.
 #include <algorithm>
 #include <type_traits>
 
@@ -88,8 +92,7 @@ __device__ __forceinline__ double wave_scan(double v) {
   return v;
 }
 
-// The nodes of a sequence.  Up to 64: one a lane, in registers of every wave (the first
-// wave loads them and hands them on).
+// The nodes of a sequence.  Up to 64: one a lane, in registers of every wave.
 struct LaneNodes {
   int above, token;  // parent and token, -1: none
   double prob;       // target's probability of the token behind the parent
@@ -161,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   if constexpr (SMALL) {
     nodes.above = nodes.token = nodes.place = -1;
     nodes.prob = 0.0;
-    if (wave == 0 && lane < a.nodes) {
+    if (lane < a.nodes) {
       u_lane = uniforms[lane];
       load_node(lane, nodes.above, nodes.token, nodes.prob);
       if (DRAFT && nodes.token >= 0)
@@ -216,33 +219,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     mass = DRAFT && tried >= 0 ? 1.0 : 0.0;
   };
   bool excluded = !DRAFT;
-  if constexpr (SMALL) {
-    // The first wave walks for all of the workgroup: every load of it is one of a cache
-    // line of its own, and those of eight waves cost 32 sequences 31 us instead of NN.
-    __shared__ LaneNodes shared_nodes[64];
-    __shared__ float shared_u[64];
-    __shared__ double shared_q[64];
-    __shared__ int shared_walk[3];
-    if (wave == 0) {
-      walk(0);
-      shared_nodes[lane] = nodes;
-      shared_u[lane] = u_lane;
-      shared_q[lane] = q_lane;
-      if (lane < 3) shared_walk[lane] = lane == 0 ? count : (lane == 1 ? node : tried);
-    }
-    __syncthreads();
-    if (wave != 0) {
-      nodes = shared_nodes[lane];
-      u_lane = shared_u[lane];
-      q_lane = shared_q[lane];
-      count = uniform(shared_walk[0]);
-      node = uniform(shared_walk[1]);
-      tried = uniform(shared_walk[2]);
-      mass = DRAFT && tried >= 0 ? 1.0 : 0.0;
-    }
-  } else {
-    walk(0);
-  }
+  walk(0);
 
   // The weights: max(p - mass * q, 0), or p without the children's tokens.  NaN has none.
   // The lane's 16 of a block at `base`: DENSE: neighbours, for a scan in order; else as
@@ -362,8 +339,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
 
   // The last workgroup of the sequence goes on.  Sums that are not there yet are waited
   // for one by one, so nothing orders them and the count: a release and an acquire, whose
-  // cache write-backs and invalidations delay all other workgroups' loads, would cost
-  // 32 sequences 10 of 18 us.
+  // cache write-backs and invalidations delay all other workgroups' loads, make 30 us of
+  // 32 chains' 15.
   __syncthreads();
   if (tid == 0)
     arrived = __hip_atomic_fetch_add(&a.counters[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -604,7 +581,7 @@ extern "C" int slc_hip_verify_tokens(
   a.vocab = static_cast<int>(vocab);
   a.blocks = static_cast<int>(block_count(vocab));
   // One block a wave, but no more workgroups than CUs: the kernel's registers leave room
-  // for one each (32 sequences 15 us, with twice or more as many 20).
+  // for one each (32 chains 15 us, with twice as many 21).
   a.segments = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>(slc_host::ceil_div(a.blocks, kWaves), slc_host::device_cu_count() / batch)));
   hipStream_t s = static_cast<hipStream_t>(stream);
