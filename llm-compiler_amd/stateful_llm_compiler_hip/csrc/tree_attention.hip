@@ -27,9 +27,6 @@ Split split_for(const Plan& plan, int64_t batch, int64_t kv_heads, int64_t rows)
   Split s;
   s.row_blocks = slc_host::ceil_div(rows, plan.rows_per_block);
   s.slots = std::max<int64_t>(slc_host::device_cu_count() / (kv_heads * s.row_blocks), batch + batch / 4);
-  // Row blocks of one piece share its K and V rows: workgroup numbers that differ by a
-  // multiple of 8 run on one XCD, whose L2 then holds them.
-  if (s.row_blocks > 1) s.slots = (s.slots + 7) / 8 * 8;
   const int64_t places = s.slots * kv_heads * s.row_blocks * plan.rows_per_block;
   s.partial_bytes = places * plan.padded_dim * 4;
   s.stats_bytes = places * 8;

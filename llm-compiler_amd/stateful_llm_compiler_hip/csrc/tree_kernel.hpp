@@ -9,7 +9,7 @@
 //
 // A workgroup owns one KV head of one sequence, a block of query rows (all nodes of all
 // query heads of that KV head; row = node * group + head) and a piece of the cache rows,
-// so K and V are read once for all of them.  One producer wave streams steps of K and V
+// so K and V are read once for all of them.  Producer waves stream steps of K and V
 // into an LDS ring with direct-to-LDS loads (16-byte chunks, XOR-swizzled by row; rows
 // past the last one read as zero).  WR x WK consumer waves own 16 QB query rows and one
 // of the step's WK tiles of KT keys each, so few query rows still keep all waves busy:
@@ -21,6 +21,13 @@
 //    once V's rows are taken in the same order.
 // The WK partial results meet in LDS; the pieces' partial results, where a sequence
 // has several, in the last of them to end or in a kernel of their own.
+//
+// What bounds it, in a graph, 14 query heads on 2 of 64, bf16: 32 sequences of 4096 to
+// 8192 rows (101 MB) take 23.9 us with 2 nodes, 4.2 TB/s, and 32.6 with 16, whose 112
+// query rows keep the VALU (exponentials, maxima, packing) as busy as the memory; of 16
+// sequences with 64 nodes, 30.6 us, some 20 us are those steps.  Before the first tile
+// lies about 4 us (the pieces, the descriptors, the first loads), behind the last one 3 to
+// 6 us (results through LDS and memory): one sequence of 600 rows and 8 nodes takes 10.2.
 #pragma once
 #include <cmath>
 #include <type_traits>
@@ -209,7 +216,8 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
 
 // Results pass between workgroups, which may be on XCDs with L2s of their own, by loads
 // and stores of agent scope: they go past the L2, so that no cache has to be written back
-// or emptied for them as a release and an acquire would.
+// or emptied for them as a release and an acquire would (13 nodes on 4 sequences in fp32,
+// in a graph: 13.0 us, with those 14.5).
 __device__ __forceinline__ void put_pair(float2* place, float x, float y) {
   __hip_atomic_store(reinterpret_cast<uint64_t*>(place), __builtin_bit_cast(uint64_t, make_float2(x, y)), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
@@ -300,7 +308,8 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
   }
 }
 // The same for large results, by workgroups of their own: one CU takes in about 10 bytes
-// a cycle, so that the last piece alone is slow from some 64 KB on.
+// a cycle, so that the last piece alone is slow from some 64 KB on (5 pieces of 56 rows of
+// 64, 70 KB, in a graph: 13.0 us, with this kernel 11.1; 3 pieces, 42 KB: 10.9 us by the last).
 template <typename T, int DP, int ROWS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const int64_t b = blockIdx.z;
@@ -327,7 +336,8 @@ struct Shape {
   static constexpr int kConsumers = WR * WK;
   static constexpr int kStep = WK * KT;
   // Producers, each of a part of a step's rows that no page is smaller than.  One wave
-  // issues a load in 90 to 140 cycles, 8 bytes a cycle; four keep up with the memory.
+  // issues a load in 90 to 140 cycles, 8 bytes a cycle; four keep up with the memory (32
+  // sequences of 4096 to 8192 rows, 2 nodes, in a graph: 24.1 us, 25.5 with one).
   static constexpr int kProducers = kStep >= 64 ? 4 : kStep / 16;
   static constexpr int kThreads = (kConsumers + kProducers) * 64;
   static constexpr int kStageBytes = WK * 2 * kTileBytes;
@@ -914,38 +924,48 @@ int launch_shape(const TreeArgs& a, hipStream_t stream) {
   return slc_host::check_launch("tree attention merge");
 }
 
-// Query blocks of 16 rows a wave by the padded row's bytes: two of 128-byte rows (each
-// K and V fragment read from LDS serves both); wider rows leave no registers for that.
+// The waves along the rows and their query blocks, by the query rows and the padded
+// row's bytes.  Of 128-byte rows a wave takes two blocks of 16 query rows, each K and V
+// fragment from LDS serving both (in a graph, 14 query heads on 2, bf16: 32 sequences, 16
+// nodes, 112 rows 32.7 us, with one 35.8; 16 sequences, 64 nodes 30.6 us, with one 47.3),
+// but one of up to 16 rows (32 sequences, 2 nodes 24.1 us, with two 24.5) and from 33 to 64,
+// where four waves along the rows are as many as with two of 128 (one sequence, 8 nodes
+// 10.2 us, with two 10.9).  Wider rows leave no registers for two.
 template <int BYTES>
-constexpr int query_blocks() { return BYTES <= 128 ? 2 : 1; }
+constexpr bool kTwo = BYTES <= 128;
 template <int BYTES>
 constexpr int most_waves() { return BYTES <= 256 ? 8 : 4; }
 
 template <typename T, int DP>
 int rows_per_block(int rows) {
   constexpr int kBytes = DP * static_cast<int>(sizeof(T));
-  constexpr int kRows = 16 * query_blocks<kBytes>(), kMost = most_waves<kBytes>();
-  if (rows <= 16) return 16;
-  for (int wr = 1; wr < kMost; wr *= 2)
-    if (rows <= kRows * wr) return kRows * wr;
+  constexpr int kWhole = (kTwo<kBytes> ? 32 : 16) * most_waves<kBytes>();
+  for (int size = 16; size < kWhole; size *= 2)
+    if (rows <= size) return size;
   // Whole blocks where they need no more padding than halves.
-  const int whole = kRows * kMost, half = whole / 2;
-  return (rows + whole - 1) / whole * 2 == (rows + half - 1) / half ? whole : half;
+  return (rows + kWhole - 1) / kWhole * 2 == (rows + kWhole / 2 - 1) / (kWhole / 2) ? kWhole : kWhole / 2;
 }
 
+// Tiles are of 32 keys (16 of rows of 1024 bytes); of 64 where all eight waves lie along
+// 128-byte rows, a step of 32 keys being short (16 sequences, 64 nodes 30.6 us, with 32
+// keys 31.8; where two tiles are side by side 32 keys are better: 8 sequences, 16 nodes
+// 14.0 us, with 64 keys 15.1).
 template <typename T, int DP>
 int launch_dim(const TreeArgs& a, int rows, hipStream_t stream) {
   constexpr int kBytes = DP * static_cast<int>(sizeof(T));
-  constexpr int kQb = query_blocks<kBytes>(), kRows = 16 * kQb;
   constexpr int kKeys = kBytes == 1024 ? 16 : 32;
-  constexpr int kMore = kBytes == 128 ? 64 : kKeys;
-  if constexpr (kQb > 1)
-    if (rows == 16) return launch_shape<T, DP, 1, 1, kKeys>(a, stream);
-  if (rows == kRows) return launch_shape<T, DP, kQb, 1, kKeys>(a, stream);
-  if (rows == 2 * kRows) return launch_shape<T, DP, kQb, 2, kKeys>(a, stream);
-  if constexpr (most_waves<kBytes>() > 4)
-    if (rows == 8 * kRows) return launch_shape<T, DP, kQb, 8, kMore>(a, stream);
-  return launch_shape<T, DP, kQb, 4, kMore>(a, stream);
+  if (rows == 16) return launch_shape<T, DP, 1, 1, kKeys>(a, stream);
+  if constexpr (kTwo<kBytes>) {
+    if (rows == 32) return launch_shape<T, DP, 2, 1, kKeys>(a, stream);
+    if (rows == 64) return launch_shape<T, DP, 1, 4, kKeys>(a, stream);
+    if (rows == 128) return launch_shape<T, DP, 2, 4, kKeys>(a, stream);
+    return launch_shape<T, DP, 2, 8, 64>(a, stream);
+  } else {
+    if (rows == 32) return launch_shape<T, DP, 1, 2, kKeys>(a, stream);
+    if constexpr (most_waves<kBytes>() == 8)
+      if (rows == 128) return launch_shape<T, DP, 1, 8, kKeys>(a, stream);
+    return launch_shape<T, DP, 1, 4, kKeys>(a, stream);
+  }
 }
 
 template <typename T>
