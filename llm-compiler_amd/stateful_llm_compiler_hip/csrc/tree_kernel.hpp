@@ -352,6 +352,10 @@ struct Shape {
   static constexpr int kQuads = DP / 16;           // float4 of a lane's outputs per query block
   static constexpr int kMergeBytes = WK > 1 ? WK * WR * QB * (kQuads * 4 + 2) * 256 : 0;
   static constexpr int kLds = kStages * kStageBytes > kMergeBytes ? kStages * kStageBytes : kMergeBytes;
+  // The chunks of a row lie XORed with this.  A transposing read takes two neighbouring
+  // chunks of each of 8 rows, which in rows of 256 bytes and more must differ in more than
+  // the lowest bit to lie on banks of their own.
+  __device__ static int swizzle(int row) { return kRowBytes >= 256 ? (row & 7) * 2 : row & 7; }
   static_assert((kStages - 2) * kOps < 64, "the wait counts at most 63 loads");
   static_assert(kConsumers * 64 >= kStep, "a step's mask is loaded by a thread per row");
 };
@@ -405,14 +409,14 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
     const int segment = page_rows < kPart ? page_rows : kPart;  // rows with one base
     const int row_bytes = static_cast<int>(a.kv_ss) * ES;
     // Lane L of load n fills row kOpRows n + L / kChunks of the step, chunk L % kChunks, with
-    // that row's chunk (L % kChunks) ^ (row & 7); columns past the head dim lie past every range.
+    // that row's chunk (L % kChunks) ^ S::swizzle(row); columns past the head dim lie past every range.
     // Rows kOpRows apart have another swizzle unless kOpRows is a multiple of 8.
     constexpr int kSwizzles = kOpRows >= 8 ? 1 : 8 / kOpRows;
     int voffset[kSwizzles];
 #pragma unroll
     for (int i = 0; i < kSwizzles; ++i) {
       const int row = i * kOpRows + row_in_op;
-      const int chunk = (lane % kChunks) ^ (row & 7);
+      const int chunk = (lane % kChunks) ^ S::swizzle(row);
       voffset[i] = chunk * (16 / ES) < a.head_dim ? row * row_bytes + chunk * 16 : 0x40000000;
     }
     for (int t = 1 - S::kStages; t < nsteps; ++t) {
@@ -459,7 +463,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 #pragma unroll 1
         for (int n = part0 / kOpRows; n < (part0 + kPart) / kOpRows; ++n) {
           const int row = n * kOpRows + row_in_op;
-          const int chunk = (lane % kChunks) ^ (row & 7);
+          const int chunk = (lane % kChunks) ^ S::swizzle(row);
           const int s = s0 + row;
           int64_t at = -1;
           if (s < end) {
@@ -551,7 +555,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int kk = 0; kk < kParts; ++kk) {
-        const uint4 ka = lds_read(kt + (16 * kb + c) * kRowBytes + (((4 * kk + g) ^ (c & 7)) << 4));
+        const uint4 ka = lds_read(kt + (16 * kb + c) * kRowBytes + (((4 * kk + g) ^ S::swizzle(c)) << 4));
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
           if constexpr (kWide) {
@@ -596,7 +600,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
           const int row = 16 * kb + 4 * g + r;
 #pragma unroll
           for (int d = 0; d < DP / 64; ++d) {
-            uint4 va = lds_read(vt + row * kRowBytes + (((16 * d + c) ^ (row & 7)) << 4));
+            uint4 va = lds_read(vt + row * kRowBytes + (((16 * d + c) ^ S::swizzle(row)) << 4));
             if constexpr (kDirty) va = without_special<T>(va);
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
@@ -624,7 +628,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 #pragma unroll
       for (int i = 0; i < S::kQuads; ++i) {
         const int dim = 16 * i + 4 * (c & 3);
-        const unsigned char* at = vt + row * kRowBytes + (((dim >> 3) ^ (row & 7)) << 4) + (dim & 7) * 2;
+        const unsigned char* at = vt + row * kRowBytes + (((dim >> 3) ^ S::swizzle(row)) << 4) + (dim & 7) * 2;
         const uint2 lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * kRowBytes);
         uint4 va = make_uint4(lo.x, lo.y, hi.x, hi.y);
         if constexpr (kDirty) va = without_special<T>(va);
@@ -786,7 +790,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 #pragma unroll
           for (int i = 0; i < S::kQuads; ++i) {
             const int dim = quad_dim<T>(i, g);
-            const unsigned char* at = vt + row * kRowBytes + (((dim * ES >> 4) ^ (row & 7)) << 4) + (dim * ES & 15);
+            const unsigned char* at = vt + row * kRowBytes + (((dim * ES >> 4) ^ S::swizzle(row)) << 4) + (dim * ES & 15);
             T v[4];
             if constexpr (kWide) {
               *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(at);
