@@ -776,9 +776,10 @@ SLC_API int slc_hip_verify_tokens(
  * moved.  Rows behind the new lengths keep what they held.
  *   key, value, lengths, lengths_out: host arrays of `layers` device pointers; the
  *   caches all different; lengths_out[l] NULL (not written), lengths[l] itself or
- *   memory that no other layer reads or writes; caches as in slc_hip_tree_attention
- *   (block_table NULL: stride_b per sequence, else per page); path int64 [B, nodes]
- *   contiguous, counts int64 [B].
+ *   memory that no other layer reads or writes and that is not path or counts; caches
+ *   as in slc_hip_tree_attention (block_table NULL: stride_b per sequence, else per
+ *   page; pages that rows move in belong to one sequence), heads * head_dim at most
+ *   2^20; path int64 [B, nodes] contiguous, counts int64 [B].
  */
 #define SLC_KV_COMMIT_MAX_LAYERS 96 /* of one launch; more take several */
 SLC_API int slc_hip_kv_commit(

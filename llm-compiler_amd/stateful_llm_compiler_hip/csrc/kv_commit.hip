@@ -5,8 +5,8 @@
 // path[b, 0 .. counts[b]) in ascending order, belong at lengths[b] + 0 .. counts[b).
 // Pure data movement of the few rows whose place changes: the bytes are small
 // and a call is the latency of two dependent round trips, so one launch takes
-// all layers (24 layers of 2 KV heads of 64, bf16, in a graph: 2.9 us for 3 rows of one
-// sequence, 5.0 us for 11 rows of each of 32, in pages).  A workgroup owns one layer of one
+// all layers (24 layers of 2 KV heads of 64, bf16, in a graph: 2.7 us for 3 rows of one
+// sequence, 4.1 us for 11 rows of each of 32, in pages).  A workgroup owns one layer of one
 // sequence (it reads the length once and may write it in place) and moves chunks in path
 // order, a batch of loads, a barrier, their stores: a row's source lies behind its place,
 // so what a batch overwrites no later batch reads.
@@ -18,6 +18,7 @@ constexpr int kMaxLayers = SLC_KV_COMMIT_MAX_LAYERS;
 constexpr int kMaxNodes = SLC_VERIFY_MAX_NODES;
 constexpr int kThreads = 256;
 constexpr int kInFlight = 4;  // chunks a thread holds between load and store
+typedef uint32_t chunk16_t __attribute__((ext_vector_type(4)));
 
 struct CommitArgs {
   void* key[kMaxLayers];
@@ -70,19 +71,19 @@ __global__ __launch_bounds__(kThreads) void kv_commit_kernel(CommitArgs a) {
     return page * a.sb + (s & ((int64_t{1} << a.page_shift) - 1)) * a.ss;
   };
   const int row_units = 2 * a.heads * a.head_units;
-  const int64_t total = static_cast<int64_t>(moves) * row_units;
+  const int total = moves * row_units;  // under 2^31: 1023 rows of 2^21 elements
   U* key = static_cast<U*>(a.key[layer]);
   U* value = static_cast<U*>(a.value[layer]);
-  for (int64_t base = 0; base < total; base += kThreads * kInFlight) {
+  for (int base = 0; base < total; base += kThreads * kInFlight) {
     U chunk[kInFlight];
     U* place[kInFlight];
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
-      const int64_t item = base + i * kThreads + tid;
+      const int item = base + i * kThreads + tid;
       place[i] = nullptr;
       if (item >= total) continue;
-      const int move = static_cast<int>(item / row_units);
-      int unit = static_cast<int>(item % row_units);
+      const int move = item / row_units;
+      int unit = item - move * row_units;
       U* buffer = unit < row_units / 2 ? key : value;
       unit = unit < row_units / 2 ? unit : unit - row_units / 2;
       const int64_t source = offset(length + from[move]), target = offset(length + to[move]);
@@ -114,7 +115,7 @@ extern "C" int slc_hip_kv_commit(
   const char* what = "slc_hip_kv_commit";
   SLC_REQUIRE(slc_host::is_float_dtype(dtype), "%s: bad dtype %d", what, dtype);
   SLC_REQUIRE(layers >= 0 && batch >= 0 && batch <= 65535 && heads > 0 && head_dim > 0 && capacity > 0 &&
-                  heads * head_dim <= (int64_t{1} << 24),
+                  heads <= (1 << 20) && head_dim <= (1 << 20) && heads * head_dim <= (1 << 20),
               "%s: bad sizes", what);
   SLC_REQUIRE(nodes >= 1 && nodes <= kMaxNodes, "%s: 1 to %d nodes", what, kMaxNodes);
   if (block_table != nullptr)
@@ -160,7 +161,7 @@ extern "C" int slc_hip_kv_commit(
     a.head_units = static_cast<int>(head_dim * es / unit);
     const dim3 grid(n, static_cast<unsigned>(batch));
     if (unit == 16) {
-      hipLaunchKernelGGL(kv_commit_kernel<uint4>, grid, dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL(kv_commit_kernel<chunk16_t>, grid, dim3(kThreads), 0, s, a);
     } else if (unit == 4) {
       hipLaunchKernelGGL(kv_commit_kernel<uint32_t>, grid, dim3(kThreads), 0, s, a);
     } else {
