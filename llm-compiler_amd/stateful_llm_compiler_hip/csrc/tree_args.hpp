@@ -6,8 +6,9 @@
 namespace slc_tree {
 
 // Rows that a piece has at least: shorter ones cost more in their results than they save.
-// (fp32 products are slow.  In a graph, 8 nodes on a sequence of 600 rows, bf16: 256 rows
-// 10.9 us, 128 rows 11.1; 13 on 4 of up to 1001, fp32: 256 rows 15.1, 128 rows 13.0.)
+// (fp32 products are slow.  8 nodes on a sequence of 600 rows, bf16: 256 rows 11.1 us, 128
+// rows 13.0, most of them in more launches; 13 on 4 of up to 1001, fp32: 256 rows 15.3, 128
+// rows 13.2.)
 constexpr int min_piece_rows(int element_size) { return element_size == 4 ? 128 : 256; }
 
 struct TreeArgs {

@@ -23,11 +23,11 @@
 // has several, in the last of them to end or in a kernel of their own.
 //
 // What bounds it, in a graph, 14 query heads on 2 of 64, bf16: 32 sequences of 4096 to
-// 8192 rows (101 MB) take 23.9 us with 2 nodes, 4.2 TB/s, and 32.6 with 16, whose 112
+// 8192 rows (101 MB) take 24.0 us with 2 nodes, 4.2 TB/s, and 32.9 with 16, whose 112
 // query rows keep the VALU (exponentials, maxima, packing) as busy as the memory; of 16
 // sequences with 64 nodes, 30.6 us, some 20 us are those steps.  Before the first tile
 // lies about 4 us (the pieces, the descriptors, the first loads), behind the last one 3 to
-// 6 us (results through LDS and memory): one sequence of 600 rows and 8 nodes takes 10.2.
+// 6 us (results through LDS and memory): one sequence of 600 rows and 8 nodes takes 10.5.
 #pragma once
 #include <cmath>
 #include <type_traits>
@@ -214,19 +214,6 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
   return p;
 }
 
-// Results pass between workgroups, which may be on XCDs with L2s of their own, by loads
-// and stores of agent scope: they go past the L2, so that no cache has to be written back
-// or emptied for them as a release and an acquire would (13 nodes on 4 sequences in fp32,
-// in a graph: 13.0 us, with those 14.5).
-__device__ __forceinline__ void put_pair(float2* place, float x, float y) {
-  __hip_atomic_store(reinterpret_cast<uint64_t*>(place), __builtin_bit_cast(uint64_t, make_float2(x, y)), __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 get_pair(const float2* place) {
-  return __builtin_bit_cast(
-      float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(place), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-
 // Units of 16 rows and 16 dims that a row block has.
 template <int DP, int ROWS>
 __device__ __forceinline__ int block_units(const TreeArgs& a, int block) {
@@ -234,7 +221,7 @@ __device__ __forceinline__ int block_units(const TreeArgs& a, int block) {
   return ((rows < ROWS ? rows : ROWS) + 15) / 16 * (DP / 16);
 }
 // Units unit, unit + step, .. (kUnits of them, those below `units`) of a sequence's row
-// block (each float4 of a wave's lanes, in two planes of pairs) put together from the
+// block (each float4 of a wave's lanes) put together from the
 // `count` pieces from slot `first` on, kBatch at a time.
 template <typename T, int DP, int ROWS, int kUnits, int kBatch>
 __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kvh, int block, int first, int count,
@@ -246,7 +233,7 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
   const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.row_blocks * ROWS;  // between pieces
   const int64_t place = ((static_cast<int64_t>(first) * a.kv_heads + kvh) * a.row_blocks + block) * ROWS;
   const float2* stats = a.stats + place + (lane & 15);
-  const float2* partial = reinterpret_cast<const float2*>(a.partial + place * DP) + lane;
+  const float4* partial = reinterpret_cast<const float4*>(a.partial + place * DP) + lane;
   float top[kUnits], sum[kUnits];
   float4 v[kUnits];
 #pragma unroll
@@ -257,16 +244,16 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
   }
 #pragma unroll 1
   for (int at = 0; at < count; at += kBatch) {
-    float2 s[kUnits][kBatch], lo[kUnits][kBatch], hi[kUnits][kBatch];
+    float2 s[kUnits][kBatch];
+    float4 o[kUnits][kBatch];
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
       const int u = unit + j * step < units ? unit + j * step : unit;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int64_t k = (at + i < count ? at + i : at) * stride;
-        s[j][i] = get_pair(stats + k + u / kQuads * 16);
-        lo[j][i] = get_pair(partial + k * (DP / 2) + u * 128);
-        hi[j][i] = get_pair(partial + k * (DP / 2) + u * 128 + 64);
+        s[j][i] = stats[k + u / kQuads * 16];
+        o[j][i] = partial[k * (DP / 4) + u * 64];
       }
     }
 #pragma unroll
@@ -276,7 +263,7 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
       for (int i = 0; i < kBatch; ++i) {
         if (at + i >= count) {
           s[j][i] = make_float2(-INFINITY, 0.0f);
-          lo[j][i] = hi[j][i] = make_float2(0.f, 0.f);
+          o[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         most = fmaxf(most, s[j][i].x);
       }
@@ -289,10 +276,10 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
       for (int i = 0; i < kBatch; ++i) {
         const float w = __builtin_amdgcn_exp2f((s[j][i].x - use) * kLog2e);
         sum[j] = fmaf(w, s[j][i].y, sum[j]);
-        v[j].x = fmaf(w, lo[j][i].x, v[j].x);
-        v[j].y = fmaf(w, lo[j][i].y, v[j].y);
-        v[j].z = fmaf(w, hi[j][i].x, v[j].z);
-        v[j].w = fmaf(w, hi[j][i].y, v[j].w);
+        v[j].x = fmaf(w, o[j][i].x, v[j].x);
+        v[j].y = fmaf(w, o[j][i].y, v[j].y);
+        v[j].z = fmaf(w, o[j][i].z, v[j].z);
+        v[j].w = fmaf(w, o[j][i].w, v[j].w);
       }
     }
   }
@@ -308,8 +295,11 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
   }
 }
 // The same for large results, by workgroups of their own: one CU takes in about 10 bytes
-// a cycle, so that the last piece alone is slow from some 64 KB on (5 pieces of 56 rows of
-// 64, 70 KB, in a graph: 13.0 us, with this kernel 11.1; 3 pieces, 42 KB: 10.9 us by the last).
+// a cycle, so that the last piece alone is slow from some 64 KB on, and below that a second
+// launch costs the host more than it saves.  Up to 3 pieces of 56 rows of 64 (42 KB): a call
+// 10.7 us, 10.5 in a graph, with this kernel 12.8 and 10.0; 8 sequences of up to 8 pieces of
+// 112 rows (229 KB) 24.2 us, with this kernel 14.7; pages, 28 rows of 128 (up to 16 pieces,
+// 229 KB) 42, with it 35.
 template <typename T, int DP, int ROWS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const int64_t b = blockIdx.z;
@@ -832,10 +822,8 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
     const int dim = quad_dim<T>(i, g);
     if (count > 1) {
       // As the lanes hold them, so that a wave writes whole lines.
-      float2* to = reinterpret_cast<float2*>(a.partial + place * S::kRows * DP) + ((wr * QB + qb) * S::kQuads + i) * 128 + lane;
-      put_pair(to, v.x, v.y);
-      put_pair(to + 64, v.z, v.w);
-      if (g == 0 && i == 0) put_pair(&a.stats[place * S::kRows + wr * 16 * QB + 16 * qb + c], top, sum);
+      reinterpret_cast<float4*>(a.partial + place * S::kRows * DP)[((wr * QB + qb) * S::kQuads + i) * 64 + lane] = v;
+      if (g == 0 && i == 0) a.stats[place * S::kRows + wr * 16 * QB + 16 * qb + c] = make_float2(top, sum);
     } else {
       T* row = static_cast<T*>(a.output) + b * a.o_sb + head[qb] * a.o_sh + node[qb] * a.o_st;
       store_quad<T>(row, dim, a.head_dim, a.vector_o, divided(v, sum));
@@ -896,17 +884,18 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   }
   if (count == 1 || a.counters == nullptr) return;
 
-  // The last of a sequence's pieces to arrive puts all of them together.  Each wave's
-  // results are in the memory before it counts itself in.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // The last of a sequence's pieces to arrive puts all of them together: every wave's
+  // results come before the barrier, each piece's count releases them, and the last one
+  // acquires them all.
   __syncthreads();
   if (tid == 0) {
     int* const counter = a.counters + (piece.sequence * a.kv_heads + kvh) * a.row_blocks + block;
-    arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
     if (arrived == count - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (__builtin_amdgcn_readfirstlane(arrived) != count - 1) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   const int units = block_units<DP, S::kRows>(a, block);
 #pragma unroll 1
   for (int unit = wave; unit < units; unit += 2 * S::kConsumers)
