@@ -421,6 +421,8 @@ def dense_reference(query, key, value, lengths, tree, scale):
     (4, 2, 128, 5, [39990, 3], True),
     (16, 1, 64, 100, [9000, 1], True),
     (3, 1, 40, 30, [20000], True),
+    (6, 2, 256, 9, [5001, 700], True),
+    (8, 2, 200, 30, [3000], True),
 ])
 def test_tree_attention_of_wide_trees_and_long_caches(gpu, case, dtype):
     q_heads, kv_heads, head_dim, nodes, lengths, is_tree = case
@@ -431,7 +433,12 @@ def test_tree_attention_of_wide_trees_and_long_caches(gpu, case, dtype):
     query, key, value, lengths = (t.to(gpu) for t in tensors)
     tree = random_tree(nodes, g).to(gpu) if is_tree else None
     out = backends.hip_tree_attention(query, key, value, lengths, tree, scale=head_dim**-0.5)
-    assert_tree_close(out, dense_reference(query, key, value, lengths, tree, head_dim**-0.5), capacity)
+    reference = dense_reference(query, key, value, lengths, tree, head_dim**-0.5)
+    assert_tree_close(out, reference, capacity)
+    key_pool, value_pool, table = paged(tensors[1:3], 16, g)
+    out = backends.hip_paged_tree_attention(query, key_pool.to(gpu), value_pool.to(gpu), table.to(gpu), lengths, tree,
+                                            scale=head_dim**-0.5)
+    assert_tree_close(out, reference, capacity)
 
 
 def test_tree_attention_with_a_mask_of_no_rows(gpu):
