@@ -5,11 +5,10 @@
 
 namespace slc_tree {
 
-// Rows that a piece has at least: shorter ones cost more in their results than they save.
-// (fp32 products are slow.  8 nodes on a sequence of 600 rows, bf16: 256 rows 11.1 us, 128
-// rows 13.0, most of them in more launches; 13 on 4 of up to 1001, fp32: 256 rows 15.3, 128
-// rows 13.2.)
-constexpr int min_piece_rows(int element_size) { return element_size == 4 ? 128 : 256; }
+// Rows that a piece has at least, 32 KB of K: shorter ones cost more in their results than
+// they save (in a graph: 16 nodes on one sequence of 2000 rows of 128 bytes, 256 rows 12.4
+// us, 128 rows 13.5; one node on 9 of up to 392 of 512 bytes, 256 rows 20.8 us, 64 rows 13.0).
+constexpr int min_piece_rows(int padded_row_bytes) { return padded_row_bytes >= 512 ? 64 : 32768 / padded_row_bytes; }
 
 struct TreeArgs {
   const void* query;

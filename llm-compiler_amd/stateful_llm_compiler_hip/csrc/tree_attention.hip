@@ -80,7 +80,7 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
   const int es = slc_host::dtype_size(dtype);
   // What the last piece of a sequence would put together at most; from 64 KB on a merge
   // kernel does it (see tree_merge_kernel).
-  const int64_t most_pieces = std::min(split.slots - batch + 1, slc_host::ceil_div(a.rows, slc_tree::min_piece_rows(es)));
+  const int64_t most_pieces = std::min(split.slots - batch + 1, slc_host::ceil_div(a.rows, slc_tree::min_piece_rows(plan.padded_dim * es)));
   if (most_pieces * std::min<int64_t>(rows, plan.rows_per_block) * plan.padded_dim * 4 > 65536) a.counters = nullptr;
   const auto on = [es](int64_t bytes, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> sizes) {
     uint64_t bits = 0;

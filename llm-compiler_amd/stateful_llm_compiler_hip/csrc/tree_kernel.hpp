@@ -905,13 +905,13 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
 template <typename T, int DP, int QB, int WR, int KT>
 int launch_shape(const TreeArgs& a, hipStream_t stream) {
   using S = Shape<T, DP, QB, WR, KT>;
-  const float min_steps = static_cast<float>((min_piece_rows(sizeof(T)) + S::kStep - 1) / S::kStep);
+  const float min_steps = static_cast<float>((min_piece_rows(S::kRowBytes) + S::kStep - 1) / S::kStep);
   hipLaunchKernelGGL((tree_attention_kernel<T, DP, QB, WR, KT>), dim3(a.kv_heads, a.slots, a.row_blocks),
                      dim3(S::kThreads), 0, stream, a, min_steps);
   const int status = slc_host::check_launch("tree attention");
   // Its pieces are put together by the last of them, or by another kernel; there are none
   // where every sequence is one.
-  if (status != SLC_OK || a.counters != nullptr || a.slots <= a.batch || a.rows <= min_piece_rows(sizeof(T))) return status;
+  if (status != SLC_OK || a.counters != nullptr || a.slots <= a.batch || a.rows <= min_piece_rows(S::kRowBytes)) return status;
   hipLaunchKernelGGL((tree_merge_kernel<T, DP, S::kRows>),
                      dim3((S::kRows * DP / 256 + 3) / 4, a.kv_heads * a.row_blocks, a.batch), dim3(256), 0, stream, a);
   return slc_host::check_launch("tree attention merge");
