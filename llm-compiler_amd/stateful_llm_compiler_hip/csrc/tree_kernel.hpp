@@ -23,11 +23,11 @@
 // has several, in the last of them to end or in a kernel of their own.
 //
 // What bounds it, in a graph, 14 query heads on 2 of 64, bf16: 32 sequences of 4096 to
-// 8192 rows (101 MB) take 24.0 us with 2 nodes, 4.2 TB/s, and 32.9 with 16, whose 112
+// 8192 rows (101 MB) take 24.0 us with 2 nodes, 4.2 TB/s, and 32.0 with 16, whose 112
 // query rows keep the VALU (exponentials, maxima, packing) as busy as the memory; of 16
-// sequences with 64 nodes, 30.6 us, some 20 us are those steps.  Before the first tile
+// sequences with 64 nodes, 29.4 us, some 19 us are those steps.  Before the first tile
 // lies about 4 us (the pieces, the descriptors, the first loads), behind the last one 3 to
-// 6 us (results through LDS and memory): one sequence of 600 rows and 8 nodes takes 10.5.
+// 6 us (results through LDS and memory): one sequence of 600 rows and 8 nodes takes 10.1.
 #pragma once
 #include <cmath>
 #include <type_traits>
@@ -333,10 +333,11 @@ struct Shape {
   static constexpr int kStageBytes = WK * 2 * kTileBytes;
   static constexpr int kOps = kStageBytes / 1024 / kProducers;  // a producer's loads of a step
   static constexpr int kRows = 16 * QB * WR;
+  static constexpr int kMaskRows = kConsumers * 64;  // of the mask in LDS at a time, twice
   static constexpr int kWords = SLC_TREE_MAX_NODES / 32 + 2;  // of a node's row of the tree, as bits
   // Up to eight stages in what the rest leaves of 160 KB, and no more loads in flight than
   // the wait can count.
-  static constexpr int kFree = 160 * 1024 - (kRows + 1) * kWords * 4 - 2 * kStep * 4 - 64;
+  static constexpr int kFree = 160 * 1024 - (kRows + 1) * kWords * 4 - 2 * kMaskRows * 4 - 64;
   static constexpr int kFill = kFree / kStageBytes < 8 ? kFree / kStageBytes : 8;
   static constexpr int kStages = (kFill - 2) * kOps < 64 ? kFill : 63 / kOps + 2;
   static constexpr int kQuads = DP / 16;           // float4 of a lane's outputs per query block
@@ -347,10 +348,12 @@ struct Shape {
   // the lowest bit to lie on banks of their own.
   __device__ static int swizzle(int row) { return kRowBytes >= 256 ? (row & 7) * 2 : row & 7; }
   static_assert((kStages - 2) * kOps < 64, "the wait counts at most 63 loads");
-  static_assert(kConsumers * 64 >= kStep, "a step's mask is loaded by a thread per row");
+  static_assert(kMaskRows % kStep == 0, "whole steps of the mask are loaded by a thread per row");
 };
 
-template <typename T, int DP, int QB, int WR, int KT>
+// MASKED: with a mask; by itself the form without one has fewer registers and less code (16
+// sequences, 64 nodes 30.5 -> 29.4 us, one sequence 10.5 -> 10.1).
+template <typename T, int DP, int QB, int WR, int KT, bool MASKED>
 __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_attention_kernel(TreeArgs a, float min_steps) {
   using S = Shape<T, DP, QB, WR, KT>;
   constexpr bool kWide = S::kWide;
@@ -362,7 +365,8 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
   constexpr int kMaxWords = S::kWords;
   __shared__ uint32_t tree_bits[(S::kRows + 1) * kMaxWords];
-  __shared__ __attribute__((aligned(16))) float mask_room[2][S::kStep];
+  constexpr int kMaskRows = S::kMaskRows, kMaskSteps = kMaskRows / S::kStep;
+  __shared__ __attribute__((aligned(16))) float mask_room[2][MASKED ? kMaskRows : 4];
   __shared__ int arrived;
 
   const int kvh = blockIdx.x, slot = blockIdx.y, block = blockIdx.z;
@@ -631,12 +635,12 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   };
 
   // The steps whose rows all nodes see and that have no mask.
-  int plain_steps = a.mask != nullptr ? 0 : piece.length / S::kStep - step0;
+  int plain_steps = MASKED ? 0 : piece.length / S::kStep - step0;
   plain_steps = plain_steps < 0 ? 0 : (plain_steps < nsteps ? plain_steps : nsteps);
 
   // What the others need: the block's nodes' rows of the tree as bits (a word of ones in
-  // front, for the sequence's rows, a word of zeros behind), and a step's mask, loaded a
-  // step ahead.
+  // front, for the sequence's rows, a word of zeros behind), and the mask, a row a thread,
+  // loaded steps ahead (32 sequences, 8 nodes, a mask: 36.9 us, a step ahead 42.3).
   const int words = (a.nodes + 31) / 32 + 2;
   if (plain_steps < nsteps && a.tree != nullptr) {
     int count = quotient(block * S::kRows + S::kRows - 1, group, inverse_group);
@@ -657,14 +661,12 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       }
     }
   }
-  const bool stages_mask = a.mask != nullptr && tid < S::kStep;
-  auto mask_of = [&](int step) {
-    const int s = (step0 + step) * S::kStep + tid;
-    return step < nsteps && s < piece.end ? slc::load_as_f32(a.mask, b * a.mask_sb + s * a.mask_ss, a.mask_dtype)
-                                          : -INFINITY;
+  auto mask_of = [&](int part) {  // this thread's row of the steps from part * kMaskSteps on
+    const int s = step0 * S::kStep + part * kMaskRows + tid;
+    return s < piece.end ? slc::load_as_f32(a.mask, b * a.mask_sb + s * a.mask_ss, a.mask_dtype) : -INFINITY;
   };
   float mask_next = 0.0f;
-  if (stages_mask) {
+  if constexpr (MASKED) {
     mask_room[0][tid] = mask_of(0);
     mask_next = mask_of(1);
   }
@@ -699,9 +701,63 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
     __syncthreads();
     const unsigned char* kt = lds + stage * S::kStageBytes + wk * 2 * kTileBytes;
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
-    if (stages_mask) {
-      mask_room[(step + 1) & 1][tid] = mask_next;
-      mask_next = mask_of(step + 2);
+    const int part = step / kMaskSteps, in_part = step % kMaskSteps;
+    if (MASKED && in_part == kMaskSteps - 1) {
+      mask_room[(part + 1) & 1][tid] = mask_next;
+      mask_next = mask_of(part + 2);
+    }
+    const float* masks = MASKED ? &mask_room[part & 1][in_part * S::kStep + wk * KT] : nullptr;  // of the wave's keys
+    if constexpr (MASKED) {
+      bool open = false, masked = false;  // of this lane's keys: not all masked out, some
+      f32x4_t add[kSubs][KB];
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          add[u][kb] = *reinterpret_cast<const f32x4_t*>(masks + u * SUB + 16 * kb + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            open |= add[u][kb][r] != -INFINITY;
+            masked |= add[u][kb][r] == -INFINITY;
+          }
+        }
+      // (Of the padding itself: a mask of -inf in part of that batch 43.7 us, without this 66.)
+      if (!__any(open)) continue;
+      if ((step0 + step) * S::kStep + (wk + 1) * KT <= piece.length && !__any(masked)) {
+        // All nodes see all of them: of padded batches, most (16 sequences, 64 nodes, a mask:
+        // 43.6 us; by the selections below, 32 keys at a time, 50.4).
+        f32x4_t st[kSubs][KB][QB];
+        float shift[QB];
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) scores(kt + u * SUB * kRowBytes, st[u]);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                st[u][kb][qb][r] = fmaf(st[u][kb][qb][r], a.scale, add[u][kb][r]);
+                mx = fmaxf(mx, st[u][kb][qb][r]);
+              }
+          raise(qb, mx);
+          // The lowest value times log2 e has no place in fp32; less the maximum it has.
+          const float m_use = m_run[qb] == -INFINITY ? 0.0f : m_run[qb];
+#pragma unroll
+          for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) st[u][kb][qb][r] -= m_use;
+          shift[qb] = 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u)
+          weigh(std::false_type{}, kt + kTileBytes + u * SUB * kRowBytes, st[u], kLog2e, shift);
+        continue;
+      }
     }
 #pragma unroll 1
     for (int u = 0; u < kSubs; ++u) {
@@ -710,11 +766,11 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       f32x4_t st[KB][QB];
       scores(kt + u * SUB * kRowBytes, st);
       // Scores t = score * scale + mask, -inf where the row is not seen, less the maximum.
-      const float* mask = a.mask != nullptr ? &mask_room[step & 1][wk * KT + u * SUB] : nullptr;
+      const float* mask = MASKED ? masks + u * SUB : nullptr;
       f32x4_t add[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
-        add[kb] = mask != nullptr ? *reinterpret_cast<const f32x4_t*>(mask + 16 * kb + 4 * g) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+        add[kb] = MASKED ? *reinterpret_cast<const f32x4_t*>(mask + 16 * kb + 4 * g) : f32x4_t{0.f, 0.f, 0.f, 0.f};
       const int j0 = s0 - piece.length;  // of the first key, as a node
       const uint32_t inside = piece.end - s0 >= 32 ? ~0u : (1u << (piece.end - s0)) - 1;
       uint32_t seen[QB];
@@ -739,8 +795,8 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            hidden |= add[kb][r] == -INFINITY;
-            const bool sees = (mine >> (16 * kb + r) & 1) != 0 && add[kb][r] != -INFINITY;
+            hidden |= MASKED && add[kb][r] == -INFINITY;
+            const bool sees = (mine >> (16 * kb + r) & 1) != 0 && (!MASKED || add[kb][r] != -INFINITY);
             const float t = sees ? fmaf(st[kb][qb][r], a.scale, add[kb][r]) : -INFINITY;
             st[kb][qb][r] = t;
             mx = fmaxf(mx, t);
@@ -773,7 +829,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       // V's NaNs and infinities, for the queries that see their rows.
 #pragma unroll 1
       for (int row = 0; row < SUB; ++row) {
-        const bool open = mask == nullptr || mask[row] != -INFINITY;
+        const bool open = !MASKED || mask[row] != -INFINITY;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
           const bool sees = open && (seen[qb] >> row & 1) != 0;
@@ -906,8 +962,9 @@ template <typename T, int DP, int QB, int WR, int KT>
 int launch_shape(const TreeArgs& a, hipStream_t stream) {
   using S = Shape<T, DP, QB, WR, KT>;
   const float min_steps = static_cast<float>((min_piece_rows(S::kRowBytes) + S::kStep - 1) / S::kStep);
-  hipLaunchKernelGGL((tree_attention_kernel<T, DP, QB, WR, KT>), dim3(a.kv_heads, a.slots, a.row_blocks),
-                     dim3(S::kThreads), 0, stream, a, min_steps);
+  const auto kernel = a.mask != nullptr ? tree_attention_kernel<T, DP, QB, WR, KT, true>
+                                        : tree_attention_kernel<T, DP, QB, WR, KT, false>;
+  hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.slots, a.row_blocks), dim3(S::kThreads), 0, stream, a, min_steps);
   const int status = slc_host::check_launch("tree attention");
   // Its pieces are put together by the last of them, or by another kernel; there are none
   // where every sequence is one.
