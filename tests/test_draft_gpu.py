@@ -222,6 +222,53 @@ def test_tree_attention_with_a_mask(gpu, kind, dtype, heads):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kind", ["blocks", "padding", "lowest", "NaN", "short"])
+@pytest.mark.parametrize("q_heads,kv_heads,head_dim,nodes", [(14, 2, 64, 20), (14, 2, 64, 16), (6, 1, 64, 9), (2, 1, 64, 3),
+                                                             (4, 2, 128, 7), (2, 1, 256, 5)])
+def test_tree_attention_of_long_masked_caches(gpu, q_heads, kv_heads, head_dim, nodes, kind, dtype):
+    """Masks over thousands of rows: tiles of which all, some and no keys are masked out."""
+
+    announce(f"tree attention long mask {q_heads} {head_dim} {nodes} {kind} {dtype}")
+    g = generator(nodes)
+    lengths, capacity = [1900, 611], 1950
+    query, key, value, lengths = tree_inputs(g, 2, q_heads, kv_heads, head_dim, nodes, capacity, dtype, lengths)
+    rows = 1500 if kind == "short" else capacity
+    mask = (torch.randn(2, 1, 1, rows, generator=g) * 2).to(dtype)
+    if kind == "blocks":
+        for first in range(0, rows, 50):
+            if torch.rand(1, generator=g) < 0.6:
+                mask[0, ..., first : first + int(torch.randint(20, 140, (1,), generator=g))] = -INF
+        mask[1, ..., 200:456] = -INF
+    elif kind in ("padding", "short"):
+        mask[0, ..., :1111] = -INF
+        mask[1, ..., :512] = -INF
+    elif kind == "lowest":
+        mask[0, ..., :1111] = torch.finfo(dtype).min
+        mask[1, ..., :620] = torch.finfo(dtype).min  # and of some nodes
+    else:
+        mask[0, ..., 1203] = NAN
+        mask[1, ..., 700:] = NAN  # behind the nodes
+    hidden = mask == -INF
+    for b in range(2):
+        key[b, :rows][hidden[b, 0, 0]] = INF
+        value[b, :rows][hidden[b, 0, 0]] = NAN
+    tree = random_tree(nodes, g)
+    scale = head_dim**-0.5
+    reference = tree_reference(query, key, value, lengths, tree, mask, scale)
+    args = [t.to(gpu) for t in (query, key, value, lengths, tree, mask)]
+
+    def check(out):
+        for b in range(2):  # by itself: a sequence of NaN has no bounds for the other
+            assert_tree_close(out[b], [part[b] for part in reference], capacity)
+
+    check(backends.hip_tree_attention(*args, scale=scale))
+    key_pool, value_pool, table = paged((key, value), 16, g)
+    out = backends.hip_paged_tree_attention(args[0], key_pool.to(gpu), value_pool.to(gpu), table.to(gpu), *args[3:],
+                                            scale=scale)
+    check(out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("head_dim", [64, 128, 40])
 @pytest.mark.parametrize("nodes,length", [(12, 61), (70, 100), (3, 0)])
 def test_tree_attention_keeps_what_a_node_does_not_see_from_it(gpu, nodes, length, head_dim, dtype):
