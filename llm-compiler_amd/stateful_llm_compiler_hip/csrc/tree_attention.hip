@@ -78,10 +78,14 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
   a.stats = reinterpret_cast<float2*>(place + split.partial_bytes);
   a.pieces = reinterpret_cast<int2*>(place + split.partial_bytes + split.stats_bytes);
   const int es = slc_host::dtype_size(dtype);
-  // What the last piece of a sequence would put together at most; from 64 KB on a merge
+  // What the last piece of a sequence would put together at most, and how many pieces would
+  // release their results, each a write-back of its L2: from 64 KB or 32 pieces on a merge
   // kernel does it (see tree_merge_kernel).
-  const int64_t most_pieces = std::min(split.slots - batch + 1, slc_host::ceil_div(a.rows, slc_tree::min_piece_rows(plan.padded_dim * es)));
-  if (most_pieces * std::min<int64_t>(rows, plan.rows_per_block) * plan.padded_dim * 4 > 65536) a.counters = nullptr;
+  const int64_t whole = slc_host::ceil_div(a.rows, slc_tree::min_piece_rows(plan.padded_dim * es));
+  const int64_t most_pieces = std::min(split.slots - batch + 1, whole > 1 ? whole + 1 : 1);
+  const int64_t all_pieces = std::min(split.slots, batch * most_pieces) * kv_heads * split.row_blocks;
+  if (most_pieces * std::min<int64_t>(rows, plan.rows_per_block) * plan.padded_dim * 4 > 65536 || all_pieces > 32)
+    a.counters = nullptr;
   const auto on = [es](int64_t bytes, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> sizes) {
     uint64_t bits = 0;
     for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);

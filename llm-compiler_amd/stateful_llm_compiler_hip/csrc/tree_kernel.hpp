@@ -178,6 +178,12 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
     const int n = (end_of(length) + STEP - 1) / STEP + kTailSteps<STEP>;
     return b < a.batch ? n : 0;
   };
+  // Pieces of one: no more than whole smallest ones, and one for the tail where there are several.
+  const float inverse_min = 1.0f / min_steps;
+  auto most_of = [&](int steps) {
+    const int n = static_cast<int>(static_cast<float>(steps - kTailSteps<STEP>) * inverse_min + 0.9999f);
+    return n > 1 ? n + 1 : 1;
+  };
   // Of the first 64 sequences; more are read again in every pass.
   const int own_length = length_of(lane), own = steps_of(lane, own_length);
   int total = wave_sum(own);
@@ -192,8 +198,10 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
     for (int base = 0; base < a.batch; base += 64) {
       const int length = base == 0 ? own_length : length_of(base + lane);
       const int steps = base == 0 ? own : steps_of(base + lane, length);
-      // Rounded up, past rounding errors; at least one, and no more than steps (q >= 1).
+      // Rounded up, past rounding errors; at least one.
       int n = static_cast<int>(static_cast<float>(steps) * inverse + 0.9999f);
+      const int most = most_of(steps);
+      n = n < most ? n : most;
       n = n < 1 ? (steps > 0 ? 1 : 0) : (n < steps ? n : steps);
       const int upto = before + wave_scan(n);
       const uint64_t hits = __ballot(upto > x);

@@ -488,6 +488,33 @@ def test_tree_attention_of_wide_trees_and_long_caches(gpu, case, dtype):
     assert_tree_close(out, reference, capacity)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("case", [
+    # batch, q_heads, kv_heads, head_dim, nodes, low, high
+    (17, 14, 2, 64, 16, 211, 221),
+    (17, 14, 2, 64, 32, 211, 240),
+    (17, 14, 2, 64, 49, 211, 221),
+    (20, 32, 8, 128, 15, 91, 145),
+    (29, 12, 1, 256, 11, 50, 286),
+    (9, 14, 2, 64, 8, 1, 700),
+    (3, 4, 2, 64, 5, 100, 270),
+])
+def test_tree_attention_of_batches_of_short_caches(gpu, case, dtype):
+    """Around the fewest rows that a piece has, where one, two and more are cut."""
+
+    batch, q_heads, kv_heads, head_dim, nodes, low, high = case
+    announce(f"tree attention short {case} {dtype}")
+    g = generator(nodes + batch)
+    lengths = torch.randint(low, high + 1, (batch,), generator=g).tolist()
+    tensors = tree_inputs(g, batch, q_heads, kv_heads, head_dim, nodes, high + nodes, dtype, lengths)
+    query, key, value, lengths = (t.to(gpu) for t in tensors)
+    tree = random_tree(nodes, g).to(gpu)
+    reference = dense_reference(query, key, value, lengths, tree, head_dim**-0.5)
+    for _ in range(2):
+        out = backends.hip_tree_attention(query, key, value, lengths, tree, scale=head_dim**-0.5)
+        assert_tree_close(out, reference, high + nodes)
+
+
 def test_tree_attention_with_a_mask_of_no_rows(gpu):
     announce("tree attention empty mask")
     for dtype in (torch.bfloat16, torch.float32):
