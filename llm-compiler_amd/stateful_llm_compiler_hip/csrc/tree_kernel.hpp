@@ -302,12 +302,12 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
                   a.head_dim, a.vector_o, divided(v[j], sum[j]));
   }
 }
-// The same for large results, by workgroups of their own: one CU takes in about 10 bytes
-// a cycle, so that the last piece alone is slow from some 64 KB on, and below that a second
-// launch costs the host more than it saves.  Up to 3 pieces of 56 rows of 64 (42 KB): a call
-// 10.7 us, 10.5 in a graph, with this kernel 12.8 and 10.0; 8 sequences of up to 8 pieces of
-// 112 rows (229 KB) 24.2 us, with this kernel 14.7; pages, 28 rows of 128 (up to 16 pieces,
-// 229 KB) 42, with it 35.
+// The same by workgroups of their own, for large results and many pieces.  One CU takes in
+// about 10 bytes a cycle, so that the last piece alone is slow from some 64 KB on (8 sequences
+// of up to 8 pieces of 112 rows, 229 KB: 24.2 us, with this kernel 14.7), and each piece's
+// release is a write-back of its L2 (17 sequences of 2 pieces, 49 nodes: 31.5 us, with this
+// kernel 17.1; 4 of up to 8, 64 in all, in a graph: 13.7 and 12.3).  Below, a second launch
+// costs the host more than it saves: 3 pieces of 56 rows (42 KB) 10.5 us a call, 12.8 with it.
 template <typename T, int DP, int ROWS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const int64_t b = blockIdx.z;
