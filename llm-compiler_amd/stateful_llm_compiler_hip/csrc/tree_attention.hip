@@ -20,13 +20,19 @@ Plan plan_for(int dtype, int rows, int head_dim) {
 // The split of a call: row blocks, pieces (a workgroup per CU, but room for each sequence
 // and some more) and the workspace for their partial results.
 struct Split {
-  int64_t row_blocks, slots, partial_bytes, stats_bytes, pieces_bytes;
+  int64_t row_blocks, slots, extra, partial_bytes, stats_bytes, pieces_bytes;
   int64_t bytes() const { return partial_bytes + stats_bytes + pieces_bytes; }
 };
 Split split_for(const Plan& plan, int64_t batch, int64_t kv_heads, int64_t rows) {
   Split s;
   s.row_blocks = slc_host::ceil_div(rows, plan.rows_per_block);
-  s.slots = std::max<int64_t>(slc_host::device_cu_count() / (kv_heads * s.row_blocks), batch + batch / 4);
+  const int64_t cus = slc_host::device_cu_count(), each = kv_heads * s.row_blocks;
+  // Where whole sequences are enough for all CUs only those far longer than the others are
+  // cut: more workgroups than CUs are a second round (128 sequences of 500 to 2000 rows, 8
+  // nodes, 2 KV heads: 25 us, pieces of even length in 160 slots 39; 1024 of 100 to 600 rows, one
+  // node: 87 us, 239).
+  s.extra = batch * each >= cus ? batch / 4 : -1;
+  s.slots = s.extra >= 0 ? batch + s.extra : std::max<int64_t>(cus / each, batch + batch / 4);
   const int64_t places = s.slots * kv_heads * s.row_blocks * plan.rows_per_block;
   s.partial_bytes = places * plan.padded_dim * 4;
   s.stats_bytes = places * 8;
@@ -70,6 +76,7 @@ int run(const char* what, TreeArgs a, void* workspace, int64_t workspace_bytes, 
   SLC_REQUIRE(a.counters != nullptr && num_counters >= batch * kv_heads * split.row_blocks, "%s: too few counters", what);
   a.row_blocks = static_cast<int>(split.row_blocks);
   a.slots = static_cast<int>(split.slots);
+  a.extra = static_cast<int>(split.extra);
   // Pieces are rounded up to whole ones; the search for their size starts as if that took
   // a third of a slot per sequence.
   a.inverse_slots = 1.0f / (static_cast<float>(split.slots) - 0.3f * static_cast<float>(batch));

@@ -158,7 +158,8 @@ constexpr int kTailSteps = STEP <= 64 ? 5 : 2;
 
 struct Piece {
   int sequence;  // -1: none
-  int index, count, first;
+  int index, count;
+  int head, tail;      // slots of the first piece, and of the second
   int length, end;  // rows of the sequence, and with its nodes'
 };
 
@@ -184,12 +185,49 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
     const int n = static_cast<int>(static_cast<float>(steps - kTailSteps<STEP>) * inverse_min + 0.9999f);
     return n > 1 ? n + 1 : 1;
   };
+  Piece p{-1, 0, 0, 0, 0, 0, 0};
+  if (a.extra >= 0) {
+    // A large batch: n - 1 < steps / q further pieces of each sequence fit the extra slots
+    // for q = sum of steps / extra, so that nothing is searched for.
+    int sum = 0;
+#pragma unroll 4
+    for (int b = lane; b < a.batch; b += 64) sum += steps_of(b, length_of(b));
+    sum = wave_sum(sum);
+    const float inverse = 1.0f / fmaxf(static_cast<float>(sum) * 1.001f / static_cast<float>(a.extra), min_steps);
+    auto further = [&](int steps) {
+      const int n = static_cast<int>(static_cast<float>(steps) * inverse + 0.9999f), most = most_of(steps);
+      return a.extra > 0 && steps > 0 ? max(1, min(n, most)) - 1 : 0;
+    };
+    if (x >= a.extra) {
+      p.sequence = x - a.extra;
+      p.length = __builtin_amdgcn_readfirstlane(length_of(p.sequence));
+      p.count = 1 + __builtin_amdgcn_readfirstlane(further(steps_of(p.sequence, p.length)));
+    }
+    int before = 0;
+    for (int base = 0; base < a.batch && p.count != 1; base += 64) {
+      const int length = length_of(base + lane), n = further(steps_of(base + lane, length));
+      const int upto = before + wave_scan(n);
+      const uint64_t hits = x < a.extra ? __ballot(upto > x) : __ballot(base + lane == p.sequence);
+      if (hits != 0) {
+        const int at = __builtin_ctzll(hits);
+        p.sequence = base + at;
+        p.count = 1 + __builtin_amdgcn_readlane(n, at);
+        p.tail = __builtin_amdgcn_readlane(upto - n, at);
+        p.length = __builtin_amdgcn_readlane(length, at);
+        break;
+      }
+      before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    p.head = a.extra + p.sequence;
+    p.index = x < a.extra ? x - p.tail + 1 : 0;
+    p.end = end_of(p.length);
+    return p;
+  }
   // Of the first 64 sequences; more are read again in every pass.
   const int own_length = length_of(lane), own = steps_of(lane, own_length);
   int total = wave_sum(own);
   for (int base = 64; base < a.batch; base += 64) total += wave_sum(steps_of(base + lane, length_of(base + lane)));
   float q = fmaxf(static_cast<float>(total) * a.inverse_slots, min_steps);
-  Piece p{-1, 0, 0, 0, 0, 0};
   for (;;) {
     // Pieces up to and with each sequence; found on the way: the sequence of slot x.
     const float inverse = __builtin_amdgcn_rcpf(q);
@@ -209,7 +247,7 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
         const int at = __builtin_ctzll(hits);
         p.sequence = base + at;
         p.count = __builtin_amdgcn_readlane(n, at);
-        p.first = __builtin_amdgcn_readlane(upto, at) - p.count;
+        p.head = __builtin_amdgcn_readlane(upto, at) - p.count;
         p.length = __builtin_amdgcn_readlane(length, at);
       }
       before = __builtin_amdgcn_readlane(upto, 63);
@@ -217,7 +255,8 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
     if (before <= a.slots) break;
     q *= 1.05f;
   }
-  p.index = x - p.first;
+  p.index = x - p.head;
+  p.tail = p.head + 1;
   p.end = end_of(p.length);
   return p;
 }
@@ -230,16 +269,16 @@ __device__ __forceinline__ int block_units(const TreeArgs& a, int block) {
 }
 // Units unit, unit + step, .. (kUnits of them, those below `units`) of a sequence's row
 // block (each float4 of a wave's lanes) put together from the
-// `count` pieces from slot `first` on, kBatch at a time.
+// `count` pieces in slot `head` and from slot `tail` on, kBatch at a time.
 template <typename T, int DP, int ROWS, int kUnits, int kBatch>
-__device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kvh, int block, int first, int count,
+__device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kvh, int block, int head, int tail, int count,
                                             int unit, int step, int units) {
   constexpr int kQuads = DP / 16;
   const int lane = threadIdx.x & 63;
   const int group = a.q_heads / a.kv_heads;
   const float inverse_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
   const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.row_blocks * ROWS;  // between pieces
-  const int64_t place = ((static_cast<int64_t>(first) * a.kv_heads + kvh) * a.row_blocks + block) * ROWS;
+  const int64_t place = (static_cast<int64_t>(kvh) * a.row_blocks + block) * ROWS;
   const float2* stats = a.stats + place + (lane & 15);
   const float4* partial = reinterpret_cast<const float4*>(a.partial + place * DP) + lane;
   float top[kUnits], sum[kUnits];
@@ -259,7 +298,8 @@ __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kv
       const int u = unit + j * step < units ? unit + j * step : unit;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int64_t k = (at + i < count ? at + i : at) * stride;
+        const int piece = at + i < count ? at + i : at;
+        const int64_t k = (piece == 0 ? head : tail + piece - 1) * stride;
         s[j][i] = stats[k + u / kQuads * 16];
         o[j][i] = partial[k * (DP / 4) + u * 64];
       }
@@ -316,7 +356,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int units = block_units<DP, ROWS>(a, block);
   if (pieces.y <= 1 || unit >= units) return;
-  merge_units<T, DP, ROWS, 1, 8>(a, b, kvh, block, pieces.x, pieces.y, unit, 1, unit + 1);
+  const int head = a.extra >= 0 ? a.extra + static_cast<int>(b) : pieces.x - 1;
+  merge_units<T, DP, ROWS, 1, 8>(a, b, kvh, block, head, pieces.x, pieces.y, unit, 1, unit + 1);
 }
 
 // Sizes of a kernel: DP the padded head dim, QB blocks of 16 query rows a wave, WR waves
@@ -396,7 +437,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (a.counters == nullptr && tid == 0 && piece.index == 0 && kvh == 0 && block == 0)
-    a.pieces[b] = make_int2(piece.first, count);
+    a.pieces[b] = make_int2(piece.tail, count);
 
   if (wave >= S::kConsumers) {
     // ---- producers ------------------------------------------------------------
@@ -963,7 +1004,7 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
   const int units = block_units<DP, S::kRows>(a, block);
 #pragma unroll 1
   for (int unit = wave; unit < units; unit += 2 * S::kConsumers)
-    merge_units<T, DP, S::kRows, 2, 4>(a, b, kvh, block, piece.first, count, unit, S::kConsumers, units);
+    merge_units<T, DP, S::kRows, 2, 4>(a, b, kvh, block, piece.head, piece.tail, count, unit, S::kConsumers, units);
 }
 
 template <typename T, int DP, int QB, int WR, int KT>

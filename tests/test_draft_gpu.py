@@ -515,6 +515,28 @@ def test_tree_attention_of_batches_of_short_caches(gpu, case, dtype):
         assert_tree_close(out, reference, high + nodes)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("batch,q_heads,kv_heads,head_dim,nodes", [(140, 4, 2, 64, 3), (70, 32, 4, 64, 2), (301, 2, 1, 128, 1)])
+def test_tree_attention_of_large_batches_of_uneven_lengths(gpu, batch, q_heads, kv_heads, head_dim, nodes, dtype):
+    """Whole sequences for all CUs, but for a few that are far longer."""
+
+    announce(f"tree attention uneven {batch} {dtype}")
+    g = generator(batch)
+    capacity = 1800
+    lengths = torch.randint(1, 60, (batch,), generator=g).tolist()
+    for at, length in ((0, 1500), (batch // 2, 900), (batch // 2 + 1, 1790), (batch - 1, 1200)):
+        lengths[at] = length
+    query = torch.randn(batch, q_heads, nodes, head_dim, generator=g).to(dtype).to(gpu)
+    key, value = (torch.randn(batch, capacity, kv_heads, head_dim, device=gpu, generator=torch.Generator(gpu).manual_seed(n))
+                  .to(dtype) for n in (1, 2))
+    lengths = torch.tensor(lengths, device=gpu)
+    tree = random_tree(nodes, g).to(gpu)
+    reference = dense_reference(query, key, value, lengths, tree, head_dim**-0.5)
+    for _ in range(2):
+        out = backends.hip_tree_attention(query, key, value, lengths, tree, scale=head_dim**-0.5)
+        assert_tree_close(out, reference, capacity)
+
+
 def test_tree_attention_with_a_mask_of_no_rows(gpu):
     announce("tree attention empty mask")
     for dtype in (torch.bfloat16, torch.float32):
