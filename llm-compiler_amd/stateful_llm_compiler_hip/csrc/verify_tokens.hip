@@ -436,7 +436,9 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   if (lane == 0) order_node = -1;
   __syncthreads();  // the other waves end
 
-  // The first block whose sum passes the goal; a random number outside [0, 1) or an
+  // The first block with weight whose sum passes the goal.  A lane's start is a scan's sum, the
+  // end of the lane before it one of neighbours: a rounding apart, the goal may lie between
+  // them, and the blocks behind it weigh nothing.  A random number outside [0, 1) or an
   // infinite sum may find none: the last block with any weight then.
   const double goal = random_of(0) * total;
   int block = -1, spare = -1;
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     for (int i = 0; i < kGroup; ++i) {
       const double next = run + s[i];
       if (s[i] > 0.0) some = i;
-      if (hit < 0 && next > goal) {
+      if (hit < 0 && s[i] > 0.0 && next > goal) {
         hit = i;
         start = run;
       }

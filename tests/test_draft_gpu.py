@@ -820,6 +820,33 @@ def test_verify_widest_trees(gpu):
     assert want[2].item() == 1024 and want[1][0, -1] == 699
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("drafted", [False, True])
+def test_verify_draws_a_token_with_weight_at_a_border_between_sums(gpu, drafted, dtype):
+    """A goal of half the sum, next to which the order of additions decides on which side
+    of it a block's sum lies, with blocks of no weight behind: what is drawn has weight."""
+
+    announce(f"verify border between sums {drafted} {dtype}")
+    # Vocabularies of up to 256 blocks of 1024, and more than 256.
+    for blocks, small, last in ((13, (4, 5), 12), (64, (12, 13, 14), 63), (300, (255, 256, 257), 299), (300, (4, 5), 299)):
+        for few in range(1, len(small) + 1):
+            for power in (-53, -54, -55, -56):
+                target = torch.zeros(1, 2, blocks * 1024, dtype=torch.float64)
+                target[:, :, 7] = target[:, :, last * 1024 + 9] = 0.5
+                for block in small[:few]:
+                    target[:, :, block * 1024 + 3] = 2.0**power
+                target = target.to(dtype)
+                draft = torch.zeros(1, 1, blocks * 1024, dtype=dtype)
+                draft[:, :, 5] = 1.0  # a token that the target does not give: what it leaves is the target
+                tokens = torch.tensor([[0, 5]], device=gpu)
+                _, emitted, counts = backends.hip_verify_tokens(
+                    tokens, target.to(gpu), torch.tensor([[0.5, 0.5]], device=gpu),
+                    draft_probs=draft.to(gpu) if drafted else None)
+                assert counts.tolist() == [1]
+                token = int(emitted[0, 0])
+                assert token >= 0 and float(target[0, 0, token]) > 0, (blocks, few, power, token)
+
+
 def test_verify_layouts_streams_and_graphs(gpu):
     announce("verify layouts")
     g = generator(7)
