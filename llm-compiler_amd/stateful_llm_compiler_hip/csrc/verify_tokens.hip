@@ -71,6 +71,13 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
 }
 __device__ __forceinline__ double uniform(double v) { return lane_value(v, 0); }
 
+// A probability as a weight: none where it is NaN or negative (fmax gives its other operand
+// for NaN).
+template <typename P>
+__device__ __forceinline__ double weight_of(P v) {
+  return fmax(static_cast<double>(slc::to_f32(v)), 0.0);
+}
+
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp(double v) {
   const uint64_t bits = __builtin_bit_cast(uint64_t, v);
@@ -155,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     above = c > 0 && up >= 0 && up < c ? static_cast<int>(up) : -1;
     const bool real = above >= 0 && t >= 0 && t < a.vocab;
     token = real ? static_cast<int>(t) : -1;
-    prob = real ? static_cast<double>(slc::to_f32(target[above * a.t_st + t])) : 0.0;
+    prob = real ? weight_of(target[above * a.t_st + t]) : 0.0;
   };
   using Nodes = std::conditional_t<SMALL, LaneNodes, SharedNodes>;
   Nodes nodes;

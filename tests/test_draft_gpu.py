@@ -847,6 +847,33 @@ def test_verify_draws_a_token_with_weight_at_a_border_between_sums(gpu, drafted,
                 assert token >= 0 and float(target[0, 0, token]) > 0, (blocks, few, power, token)
 
 
+@pytest.mark.parametrize("nodes", [5, 64, 65, 130])
+def test_verify_siblings_without_a_probability(gpu, nodes):
+    """A refused sibling's NaN or negative probability takes nothing from the mass that
+    the younger ones are tried with."""
+
+    announce(f"verify siblings without a probability {nodes}")
+    g = generator(nodes)
+    vocab = 1100
+    rows = []
+    for odd in (NAN, -0.25, -INF, 0.0):
+        target = probabilities(g, 1, nodes, vocab, sharp=1.0)
+        target[0, 0] = 0.0
+        target[0, 0, 3], target[0, 0, 5], target[0, 0, 7], target[0, 0, 11] = odd, 0.25, 0.5, 0.25
+        rows.append(target)
+    target = torch.cat(rows)
+    parents = torch.zeros(4, nodes, dtype=torch.int64)
+    parents[:, 0] = -1
+    tokens = torch.full((4, nodes), 3)  # the first, and all between the tried ones and behind them
+    tokens[:, nodes // 2], tokens[:, nodes - 1] = 5, 7
+    # 0.5 of the 0.75 that the refusal of token 5 leaves is 2 / 3, of 1 one half.
+    for first, second, count in ((0.5, 0.66, 2), (0.5, 0.67, 1), (0.2, 0.9, 2), (0.25, 0.5, 2), (0.26, 0.999, 1)):
+        uniforms = torch.full((4, nodes), 0.5)
+        uniforms[:, nodes // 2], uniforms[:, nodes - 1] = first, second
+        want = check_verify(gpu, tokens, target, uniforms, parents)
+        assert want[2].tolist() == [count] * 4
+
+
 def test_verify_layouts_streams_and_graphs(gpu):
     announce("verify layouts")
     g = generator(7)
