@@ -748,8 +748,8 @@ SLC_API int slc_hip_paged_tree_attention(
  * An accepted child is the next node.  Where none is, the token that follows is the
  * first i with w(0) + .. + w(i) > uniforms[b, 0] * sum w, or, where no w is positive,
  * the same of p (-1 where no p is).  A node whose parent is not an earlier node, and
- * a token outside the vocabulary, is never accepted; a probability that is NaN or
- * negative has no weight.  Probabilities sum to 1.
+ * a token outside the vocabulary, is never accepted; a probability (p or q) that is NaN
+ * or negative counts as 0.  Probabilities sum to 1.
  *   path[b, :]    : the accepted nodes in ascending order, 0 first, then -1
  *   emitted[b, :] : their tokens without node 0's, the token that follows, then -1
  *   counts[b]     : accepted nodes, node 0 among them, and so emitted tokens

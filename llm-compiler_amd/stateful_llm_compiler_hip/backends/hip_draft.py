@@ -237,7 +237,8 @@ def hip_verify_tokens(
     refusal adds m to M.  Without draft rows w = p, a child is accepted where
     u m < w(x), and a refusal takes w(x) from m and sets it to 0.  Where no child is
     accepted the token that follows is the first i with w(0) + .. + w(i) > u_0 sum w
-    (p where no w is positive; -1 where no p is).  All in fp64.
+    (p where no w is positive; -1 where no p is).  All in fp64; a probability that is NaN
+    or negative counts as 0.
 
     ``path`` [B, T]: the accepted nodes in ascending order, then -1; ``emitted`` [B, T]:
     their tokens without node 0's, the token that follows, then -1; ``counts`` [B]: how

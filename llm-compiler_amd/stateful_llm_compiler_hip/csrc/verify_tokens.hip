@@ -175,7 +175,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
       u_lane = uniforms[lane];
       load_node(lane, nodes.above, nodes.token, nodes.prob);
       if (DRAFT && nodes.token >= 0)
-        q_lane = static_cast<double>(slc::to_f32(draft[nodes.above * a.d_st + nodes.token]));
+        q_lane = weight_of(draft[nodes.above * a.d_st + nodes.token]);
     }
   } else {
     __shared__ double prob[kMaxNodes];
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   auto draft_of = [&](int node, int c) SLC_INLINE {
     if constexpr (SMALL) return lane_value(q_lane, c);
     const int t = nodes.token_of(c);
-    return t < 0 ? 0.0 : uniform(static_cast<double>(slc::to_f32(draft[node * a.d_st + t])));
+    return t < 0 ? 0.0 : uniform(weight_of(draft[node * a.d_st + t]));
   };
 
   // Down the tree from `node` to the first node without an accepted child; with draft
@@ -228,7 +228,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   bool excluded = !DRAFT;
   walk(0);
 
-  // The weights: max(p - mass * q, 0), or p without the children's tokens.  NaN has none.
+  // The weights: max(p - mass * q, 0), or p without the children's tokens.  NaN and negative
+  // probabilities have none, p's and q's.
   // The lane's 16 of a block at `base`: DENSE: neighbours, for a scan in order; else as
   // coalesced loads (16 bytes a lane, or one element) have them.
   auto column = [&](bool dense, bool vector, int i) SLC_INLINE {
@@ -289,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       double v = static_cast<double>(element(raw.p, i));
-      if constexpr (DRAFT) v = fma(-mass, mass > 0.0 ? static_cast<double>(element(raw.q, i)) : 0.0, v);
+      if constexpr (DRAFT) v = fma(-mass, mass > 0.0 ? weight_of(element(raw.q, i)) : 0.0, v);
       w[i] = fmax(v, 0.0);  // 0 for NaN
     }
     if (!excluded) return;

@@ -874,6 +874,38 @@ def test_verify_siblings_without_a_probability(gpu, nodes):
         assert want[2].tolist() == [count] * 4
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("nodes", [6, 70])
+def test_verify_draft_probabilities_that_are_none(gpu, nodes, dtype):
+    """NaN and negative draft probabilities count as zero: a token without weight is not
+    accepted by them, and they take nothing from the target's and add nothing to it."""
+
+    announce(f"verify draft probabilities that are none {nodes} {dtype}")
+    g = generator(nodes)
+    vocab, batch = 1500, 6
+    target = probabilities(g, batch, nodes, vocab).to(dtype)
+    draft = probabilities(g, batch, nodes - 1, vocab).to(dtype)
+    odd = torch.rand(draft.shape, generator=g)
+    draft[odd < 0.2] = NAN
+    draft[(odd >= 0.2) & (odd < 0.4)] = -0.5
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=g)
+    # Tokens without weight whose draft probability is negative or NaN, first among the children.
+    target[:3, 0, 17], draft[:2, 0, 17], draft[2, 0, 17] = 0.0, -0.25, NAN
+    tokens[:3, 1] = 17
+    clean = draft.float().nan_to_num(0.0).clamp_min(0.0).to(dtype)
+    for parents in (None, random_parents(batch, nodes, g)):
+        for turn in range(4):
+            uniforms = torch.rand(batch, nodes, generator=g).clamp_min(2.0**-20)
+            want = verify_reference(tokens, target, uniforms, parents, clean)
+            got = backends.hip_verify_tokens(tokens.to(gpu), target.to(gpu), uniforms.to(gpu),
+                                             parents=None if parents is None else parents.to(gpu),
+                                             draft_probs=draft.to(gpu))
+            for a, b in zip(got, want):
+                assert torch.equal(a.cpu(), b)
+            if parents is None:
+                assert want[2][:3].tolist() == [1] * 3
+
+
 def test_verify_layouts_streams_and_graphs(gpu):
     announce("verify layouts")
     g = generator(7)
