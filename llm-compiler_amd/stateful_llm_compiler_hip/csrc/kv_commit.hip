@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kThreads) void kv_commit_kernel(CommitArgs a) {
     for (int base = 0; base < count; base += 64) {
       const int j = base + lane;
       const int64_t n = j < count ? a.path[b * a.nodes + j] : -1;
-      const bool move = n > j && n < a.nodes && length >= 0 && length + n < a.capacity;
+      const bool move = n > j && n < a.nodes && length >= 0 && length < a.capacity - n;
       const uint64_t hits = __ballot(move);
       if (move) {
         const int at = found + __popcll(hits & ((uint64_t{1} << lane) - 1));
@@ -98,9 +98,9 @@ __global__ __launch_bounds__(kThreads) void kv_commit_kernel(CommitArgs a) {
       if (place[i] != nullptr) *place[i] = chunk[i];
   }
   if (tid == 0) {
-    const int64_t next = length + count;
+    const int64_t next = static_cast<int64_t>(static_cast<uint64_t>(length) + static_cast<uint64_t>(count));
     if (a.lengths_out[layer] != nullptr) a.lengths_out[layer][b] = next;
-    if (a.overflow != nullptr && (next > a.capacity || next < 0)) *a.overflow = 1;
+    if (a.overflow != nullptr && (length > a.capacity - count || next < 0)) *a.overflow = 1;
   }
 }
 

@@ -1192,6 +1192,25 @@ def test_commit_does_not_leave_the_cache(gpu):
     assert out.shape == (2, 1, 4, 1)
 
 
+@pytest.mark.parametrize("page_tokens", [0, 16])
+def test_commit_of_lengths_next_to_the_largest_integer(gpu, page_tokens):
+    """A length whose sum with a node passes 64 bits moves nothing."""
+
+    announce(f"commit far lengths {page_tokens}")
+    shape = (2, 16, 1, 4) if page_tokens else (1, 32, 1, 4)
+    buffers = [torch.randn(shape, device=gpu) for _ in range(2)]
+    before = [buffer.clone() for buffer in buffers]
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device=gpu) if page_tokens else None
+    handle = backends.KVLayers(buffers[:1], buffers[1:], block_table=table)
+    path, counts = torch.tensor([[0, 2, 3]], device=gpu), torch.tensor([3], device=gpu)
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    for length in (2**63 - 1, 2**63 - 2, 2**63 - 3, 2**63 - 4, 2**62, -(2**63)):
+        flag.zero_()
+        backends.hip_kv_commit(handle, torch.tensor([length], device=gpu), path, counts, overflow=flag)
+        assert flag.item() == 1
+        assert all(torch.equal(a, b) for a, b in zip(buffers, before))
+
+
 # ---- together -----------------------------------------------------------------------
 
 
