@@ -771,9 +771,11 @@ SLC_API int slc_hip_verify_tokens(
 /*
  * kv_commit: in every layer l, K and V row lengths[l][b] + path[b, j] moves to row
  * lengths[l][b] + j for j < counts[b], and lengths_out[l][b] = lengths[l][b] +
- * counts[b] (in place allowed; *overflow set past the capacity).  path ascends
- * within a count; entries outside [0, nodes) and rows past the capacity are not
- * moved.  Rows behind the new lengths keep what they held.
+ * counts[b] (in place allowed).  path ascends within a count; entries outside
+ * [0, nodes) and rows past the capacity are not moved, counts are taken as within
+ * [0, nodes].  *overflow is set where the new length lies past the capacity or counts
+ * a row that is not there: by such an entry, row or count, or where a row to move lies
+ * in a page that is none of the pool's.  Rows behind the new lengths keep what they held.
  *   key, value, lengths, lengths_out: host arrays of `layers` device pointers; the
  *   caches all different; lengths_out[l] NULL (not written), lengths[l] itself or
  *   memory that no other layer reads or writes and that is not path or counts; caches

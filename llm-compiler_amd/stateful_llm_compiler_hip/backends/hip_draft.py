@@ -379,8 +379,10 @@ def hip_kv_commit(
     ``lengths``: int64 [B], the same for all layers, or [layers, B], or one [B] tensor
     per layer.  ``out`` receives the new ones, in any of these forms, and may be
     ``lengths`` itself where these are a tensor for each layer.  Rows behind the new
-    lengths keep what they held; lengths past the capacity set the optional int32
-    ``overflow`` flag.
+    lengths keep what they held.  The optional int32 ``overflow`` flag is set where a new
+    length lies past the capacity, and where it counts a row that is not there: an accepted
+    node whose row lies past the capacity (so that it was not stored) or in a page that is none of the
+    pool's, an entry that is no node, a count outside [0, T] (taken as the nearest within).
     """
 
     what = "HIP KV commit"

@@ -43,15 +43,19 @@ __global__ __launch_bounds__(kThreads) void kv_commit_kernel(CommitArgs a) {
   const int64_t b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t length = a.lengths[layer][b];
-  int64_t count = a.counts[b];
-  count = count < 0 ? 0 : (count > a.nodes ? a.nodes : count);
+  const int64_t asked = a.counts[b];
+  const int64_t count = asked < 0 ? 0 : (asked > a.nodes ? a.nodes : asked);
+  // What the new length counts without a row of its own sets the flag.
+  bool lost = asked != count;
   if (tid < 64) {
     // The rows that move: sources behind their places, inside the cache.
     int found = 0;
     for (int base = 0; base < count; base += 64) {
       const int j = base + lane;
       const int64_t n = j < count ? a.path[b * a.nodes + j] : -1;
-      const bool move = n > j && n < a.nodes && length >= 0 && length < a.capacity - n;
+      const bool there = n >= j && n < a.nodes && length >= 0 && length < a.capacity - n;
+      const bool move = there && n > j;
+      lost |= j < count && !there;
       const uint64_t hits = __ballot(move);
       if (move) {
         const int at = found + __popcll(hits & ((uint64_t{1} << lane) - 1));
@@ -87,7 +91,10 @@ __global__ __launch_bounds__(kThreads) void kv_commit_kernel(CommitArgs a) {
       U* buffer = unit < row_units / 2 ? key : value;
       unit = unit < row_units / 2 ? unit : unit - row_units / 2;
       const int64_t source = offset(length + from[move]), target = offset(length + to[move]);
-      if (source < 0 || target < 0) continue;
+      if (source < 0 || target < 0) {
+        lost = true;
+        continue;
+      }
       const int64_t column = unit / a.head_units * a.sh + unit % a.head_units;
       chunk[i] = buffer[source + column];
       place[i] = buffer + target + column;
@@ -100,8 +107,9 @@ __global__ __launch_bounds__(kThreads) void kv_commit_kernel(CommitArgs a) {
   if (tid == 0) {
     const int64_t next = static_cast<int64_t>(static_cast<uint64_t>(length) + static_cast<uint64_t>(count));
     if (a.lengths_out[layer] != nullptr) a.lengths_out[layer][b] = next;
-    if (a.overflow != nullptr && (length > a.capacity - count || next < 0)) *a.overflow = 1;
+    lost |= length > a.capacity - count || next < 0;
   }
+  if (lost && a.overflow != nullptr) *a.overflow = 1;
 }
 
 }  // namespace

@@ -1211,6 +1211,61 @@ def test_commit_of_lengths_next_to_the_largest_integer(gpu, page_tokens):
         assert all(torch.equal(a, b) for a, b in zip(buffers, before))
 
 
+def test_commit_flags_rows_that_are_not_moved(gpu):
+    """Accepted nodes whose rows were not stored, or whose places are none of the pool's,
+    and counts that no path has set the flag; all else leaves it."""
+
+    announce("commit flag")
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+
+    def flagged(handle, length, path, count):
+        flag.zero_()
+        batch = handle.batch
+        lengths = torch.full((batch,), 2, device=gpu)
+        lengths[-1] = length
+        paths = torch.tensor([[0] + [-1] * (len(path) - 1)] * (batch - 1) + [path], device=gpu)
+        counts = torch.ones(batch, dtype=torch.int64, device=gpu)
+        counts[-1] = count
+        out = backends.hip_kv_commit(handle, lengths, paths, counts, overflow=flag)
+        assert int(out[-1]) == length + max(0, min(count, len(path)))
+        return flag.item()
+
+    for batch, layers in ((1, 1), (3, 2)):
+        buffers = [torch.arange(batch * 100.0, device=gpu).view(batch, 100, 1, 1).clone() for _ in range(2 * layers)]
+        handle = backends.KVLayers(buffers[:layers], buffers[layers:])
+        before = buffers[0].clone()
+        # Row 97 + 5 was not stored: row 98 keeps what it held, the new length 99 counts it.
+        assert flagged(handle, 97, [0, 5, -1, -1, -1, -1], 2) == 1
+        assert torch.equal(buffers[0], before)
+        assert flagged(handle, 97, [0, 2, -1, -1, -1, -1], 2) == 0  # row 99, the last
+        assert flagged(handle, 97, [0, 1, 2, -1, -1, -1], 3) == 0  # as far as the capacity
+        assert flagged(handle, 97, [0, 5, 5, 5, 5, 5], 1) == 0  # what is not accepted does not count
+        assert flagged(handle, 97, [0, 1, 2, 3, -1, -1], 4) == 1
+        assert flagged(handle, 4, [0, 2, 4, -1, -1, -1], 3) == 0
+        assert flagged(handle, 4, [0, 2, 4, -1, -1, -1], 0) == 0
+        assert flagged(handle, 4, [0, 1, 2, 3, 4, 5], 6) == 0
+        assert flagged(handle, 4, [0, 1, 2, 3, 4, 5], 7) == 1  # cut to the path's six
+        assert flagged(handle, 4, [0, 1, 2, 3, 4, 5], -1) == 1
+        assert flagged(handle, 4, [0, 2, -1, -1, -1, -1], 3) == 1  # the third is no node
+        assert flagged(handle, 4, [0, 2, 6, -1, -1, -1], 3) == 1
+        assert flagged(handle, 4, [0, 2, 6, -1, -1, -1], 2) == 0
+    wide = [-1] * 200
+    buffers = [torch.zeros(1, 300, 1, 1, device=gpu) for _ in range(2)]
+    handle = backends.KVLayers(buffers[:1], buffers[1:])
+    wide[:151] = range(49, 200)
+    assert flagged(handle, 101, wide, 150) == 0  # past a wave's 64, to row 101 + 198
+    assert flagged(handle, 101, wide, 151) == 1
+    pools = [torch.arange(3 * 16.0, device=gpu).view(3, 16, 1, 1).clone() for _ in range(2)]
+    table = torch.tensor([[1, 7]], dtype=torch.int32, device=gpu)
+    handle = backends.KVLayers(pools[:1], pools[1:], block_table=table)
+    assert flagged(handle, 12, [0, 2, 3, -1, -1, -1], 3) == 0
+    assert flagged(handle, 12, [0, 2, 4, -1, -1, -1], 3) == 1  # row 16 has no page
+    table[0, 1] = -1
+    assert flagged(handle, 12, [0, 2, 4, -1, -1, -1], 3) == 1
+    table[0, 1] = 0
+    assert flagged(handle, 12, [0, 2, 4, -1, -1, -1], 3) == 0
+
+
 # ---- together -----------------------------------------------------------------------
 
 
