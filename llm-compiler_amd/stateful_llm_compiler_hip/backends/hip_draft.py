@@ -293,7 +293,9 @@ def hip_verify_tokens(
 
 class KVLayers:
     """The KV caches of a model's layers, checked once, for ``hip_kv_commit``: a program
-    makes it with its caches and keeps it as long as them.
+    makes it with its caches and keeps it as long as them (it holds their addresses: for
+    tensors that get other memory, by ``set_`` or ``.data``, it is made anew).  A copy and
+    an unpickled one are made and checked anew, of the copied buffers.
 
     ``keys`` and ``values``: one buffer per layer, B x Cap x KVH x D, or with
     ``block_table`` (int32 [B, pages]) one page pool per layer.
@@ -334,9 +336,14 @@ class KVLayers:
         self._pointers = array("Q", [buffer.data_ptr() for buffer in buffers])
         if len(set(self._pointers)) != len(buffers):
             raise ValueError(f"{what}: a buffer is there twice")
-        self._keys = self._pointers.buffer_info()[0]
-        self._values = self._keys + 8 * len(self.keys)
         self._dtype, self._strides = _native.dtype_tag(first.dtype), first.stride()[:3]
+
+    def __reduce__(self):
+        return _kv_layers, (type(self), self.keys, self.values, self.block_table)
+
+
+def _kv_layers(kind, keys, values, block_table):
+    return kind(keys, values, block_table=block_table)
 
 
 def _layer_pointers(layers: KVLayers, lengths, what: str, name: str) -> array:
@@ -423,7 +430,8 @@ def hip_kv_commit(
         return out
     if targets[0] == targets[-1]:  # one tensor for all layers: the first one's workgroups write it
         targets = targets[:1] + array("Q", [0]) * (count - 1)
-    _call("slc_hip_kv_commit", index, layers._keys, layers._values, sources.buffer_info()[0], targets.buffer_info()[0],
+    keys = layers._pointers.buffer_info()[0]
+    _call("slc_hip_kv_commit", index, keys, keys + 8 * count, sources.buffer_info()[0], targets.buffer_info()[0],
           *layers._pages, path.data_ptr(), counts.data_ptr(), None if overflow is None else overflow.data_ptr(),
           layers._dtype, count, batch, shape[1], layers.heads, layers.head_dim, layers.capacity, *layers._strides)
     return out

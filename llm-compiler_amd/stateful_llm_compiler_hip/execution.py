@@ -126,7 +126,7 @@ class PreallocatedKVCacheState:
     # current stream's workspace.
     workspace: _native.DeviceWorkspace | None = None
     # The checked layers of commit(), made by the first one and passed on to later
-    # versions; made anew for other buffers or another block table.
+    # versions; made anew for other buffers or another block table, and by copies.
     layers: KVLayers | None = field(default=None, compare=False, repr=False)
 
     def __post_init__(self) -> None:
@@ -444,6 +444,10 @@ class PreallocatedKVCacheState:
 
     def _block_table(self) -> torch.Tensor | None:
         return None
+
+    def __getstate__(self) -> dict[str, Any]:
+        # A copy has buffers of its own, and checks them at its first commit.
+        return {**self.__dict__, "layers": None}
 
     def check_capacity(self) -> None:
         """Synchronise and raise if any store or advance overflowed the capacity."""

@@ -3,13 +3,16 @@ entry points on arguments that are checked before any device call."""
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
+from dataclasses import replace
 
 import pytest
 import torch
 
 from stateful_llm_compiler_hip import _native, backends
-from stateful_llm_compiler_hip.execution import ExecutionError, PreallocatedKVCacheState
+from stateful_llm_compiler_hip.execution import ExecutionError, PagedKVCacheState, PreallocatedKVCacheState
 
 P = 0x1000  # 4 KiB-aligned, never dereferenced on these paths
 F32, F16, BF16, I32, I64 = 0, 1, 2, 3, 4
@@ -122,3 +125,78 @@ def test_state_refuses_what_does_not_fit_its_buffers():
     ):
         with pytest.raises(ExecutionError):
             bad()
+
+
+def committing(monkeypatch):
+    """States on host memory commit, the entry point left out: what it would get, the
+    device pointers of keys and values, is noted."""
+
+    from stateful_llm_compiler_hip.backends import hip_draft
+
+    calls = []
+
+    def entry_point(name, index, keys, values, lengths, out, *rest):
+        layers = rest[-9]
+        read = ctypes.c_uint64 * layers
+        calls.append([list(read.from_address(at)) for at in (keys, values)])
+
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    monkeypatch.setattr(hip_draft, "_call", entry_point)
+    return calls
+
+
+def pointers(state):
+    return [[t.data_ptr() for t in side] for side in (state.keys, state.values)]
+
+
+def state_to_commit(paged):
+    template = torch.zeros(2, 2, 1, 8)
+    make = PagedKVCacheState if paged else PreallocatedKVCacheState
+    state = make.empty_from_key_template(template, num_layers=3, capacity=32, **({"page_tokens": 16} if paged else {}))
+    return replace(state, overflow=None)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_copies_of_a_state_commit_their_own_buffers(monkeypatch, paged):
+    calls = committing(monkeypatch)
+    path, counts = torch.zeros(2, 3, dtype=torch.int64), torch.ones(2, dtype=torch.int64)
+    state = state_to_commit(paged).commit(path, counts)
+    assert calls[-1] == pointers(state)
+    for other in (copy.deepcopy(state), pickle.loads(pickle.dumps(state)), copy.deepcopy(copy.copy(state))):
+        assert other.keys[0].data_ptr() != state.keys[0].data_ptr()
+        for _ in range(2):
+            other = other.commit(path, counts)
+            assert calls[-1] == pointers(other)
+    copy.copy(state).commit(path, counts)
+    assert calls[-1] == pointers(state)
+    gone = copy.deepcopy(state)
+    kept = pointers(state)
+    del state
+    gone.commit(path, counts)
+    assert calls[-1] == pointers(gone) != kept
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_copies_of_checked_layers_hold_their_own_buffers(monkeypatch, paged):
+    calls = committing(monkeypatch)
+    state = state_to_commit(paged)
+    layers = backends.KVLayers(state.keys, state.values, block_table=state.block_table if paged else None)
+    path, counts = torch.zeros(2, 3, dtype=torch.int64), torch.ones(2, dtype=torch.int64)
+    for other in (copy.deepcopy(layers), pickle.loads(pickle.dumps(layers)), copy.copy(layers)):
+        backends.hip_kv_commit(other, state.lengths, path, counts)
+        assert calls[-1] == [[t.data_ptr() for t in side] for side in (other.keys, other.values)]
+        assert (other.keys[0] is layers.keys[0]) == (calls[-1] == pointers(state))
+        assert paged == (other.block_table is not None)
+        if paged:
+            assert other._pages[0] == other.block_table.data_ptr()
+
+
+def test_committed_states_load_where_there_is_no_gpu(monkeypatch):
+    with monkeypatch.context() as context:
+        committing(context)
+        state = state_to_commit(False).commit(torch.zeros(2, 3, dtype=torch.int64), torch.ones(2, dtype=torch.int64))
+        saved = pickle.dumps(state)
+    loaded = pickle.loads(saved)
+    assert torch.equal(loaded.keys[0], state.keys[0]) and loaded.generation == state.generation
+    assert torch.equal(copy.deepcopy(state).lengths[1], state.lengths[1])
