@@ -127,7 +127,7 @@ class PreallocatedKVCacheState:
     workspace: _native.DeviceWorkspace | None = None
     # The checked layers of commit(), made by the first one and passed on to later
     # versions; made anew for other buffers or another block table, and by copies.
-    layers: KVLayers | None = field(default=None, compare=False, repr=False)
+    layers: KVLayers | None = field(default=None, compare=False, repr=False, kw_only=True)
 
     def __post_init__(self) -> None:
         if self.capacity <= 0:

@@ -200,3 +200,15 @@ def test_committed_states_load_where_there_is_no_gpu(monkeypatch):
     loaded = pickle.loads(saved)
     assert torch.equal(loaded.keys[0], state.keys[0]) and loaded.generation == state.generation
     assert torch.equal(copy.deepcopy(state).lengths[1], state.lengths[1])
+
+
+def test_paged_states_take_their_table_as_the_tenth_argument():
+    """The fields keep their order in the constructor, where ``layers`` is by name only."""
+
+    state = PagedKVCacheState.empty_from_key_template(torch.zeros(2, 2, 1, 8), num_layers=2, capacity=32, page_tokens=16)
+    other = PagedKVCacheState(state.keys, state.values, state.lengths, 32, 4, None, True, None, None, state.block_table, 16)
+    assert other.block_table is state.block_table and other.page_tokens == 16 and other.generation == 4
+    assert other.layers is None and other.zero_slots is None and other.in_place_lengths
+    with pytest.raises(TypeError):
+        PreallocatedKVCacheState(state.keys, state.values, state.lengths, 16, 0, None, False, None, None, None)
+    assert replace(other, layers=None, generation=5).generation == 5
