@@ -439,7 +439,7 @@ class PreallocatedKVCacheState:
         out = hip_kv_commit(layers, self.lengths, path, counts, out=self.lengths if self.in_place_lengths else None,
                             overflow=self.overflow)
         object.__setattr__(self, "layers", layers)
-        zero = None if self.zero_slots is None else frozenset()
+        zero = None if self.zero_slots else self.zero_slots  # the counts are the device's
         return replace(self, lengths=tuple(out), generation=self.generation + 1, zero_slots=zero)
 
     def _block_table(self) -> torch.Tensor | None:

@@ -212,3 +212,26 @@ def test_paged_states_take_their_table_as_the_tenth_argument():
     with pytest.raises(TypeError):
         PreallocatedKVCacheState(state.keys, state.values, state.lengths, 16, 0, None, False, None, None, None)
     assert replace(other, layers=None, generation=5).generation == 5
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_what_a_commit_leaves_at_length_zero_takes_a_prefill(monkeypatch, paged):
+    """Which slots are at zero is unknown to the host after a commit, whose counts the
+    device has; slots that were past zero stay refused without a look."""
+
+    committing(monkeypatch)
+    stored = []
+    for kind in (PreallocatedKVCacheState, PagedKVCacheState):
+        monkeypatch.setattr(kind, "store", lambda self, slot, *args, **kwargs: stored.append(slot))
+        monkeypatch.setattr(kind, "advance", lambda self, slot, *, delta: self)
+    state = state_to_commit(paged)
+    path, counts = torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, dtype=torch.int64)
+    rows = torch.zeros(2, 2, 4, 8)
+    after = replace(state.commit(path, counts), lengths=state.lengths)  # as counts of zero leave them
+    after.prefill_store(1, rows, rows)
+    assert stored == [1]
+    full = replace(state, lengths=tuple(torch.full((2,), 4) for _ in range(3)), zero_slots=frozenset())
+    for later in (replace(state.commit(path, counts), lengths=full.lengths), full.commit(path, counts)):
+        with pytest.raises(ExecutionError, match="length to be 0"):
+            later.prefill_store(1, rows, rows)
+    assert full.commit(path, counts).zero_slots == frozenset() and stored == [1]
