@@ -537,6 +537,109 @@ def test_tree_attention_of_large_batches_of_uneven_lengths(gpu, batch, q_heads, 
         assert_tree_close(out, reference, capacity)
 
 
+def large_reference(query, key, value, lengths, tree, mask, scale):
+    """``tree_reference`` on the inputs' device, a KV head at a time; rows that the mask
+    hides take no part, whatever they hold."""
+
+    batch, q_heads, nodes, head_dim = query.shape
+    capacity, kv_heads = key.shape[1:3]
+    group = q_heads // kv_heads
+    if tree is None:
+        tree = torch.ones(nodes, nodes, dtype=torch.bool, device=query.device).tril_()
+    parts = [torch.empty(query.shape, dtype=torch.float64, device=query.device) for _ in range(4)]
+    for b, length in enumerate(lengths.tolist()):
+        end = min(length + nodes, capacity)
+        seen = torch.cat([torch.ones(nodes, length, dtype=torch.bool, device=query.device), tree], 1)[:, :end]
+        add = torch.zeros(end, dtype=torch.float64, device=query.device)
+        if mask is not None:
+            hidden = mask[b, 0, 0, :end] == -INF
+            add, seen = mask[b, 0, 0, :end].double().masked_fill(hidden, 0), seen & ~hidden
+        for h in range(kv_heads):
+            q = query[b, h * group : (h + 1) * group].double()
+            k, v = (side[b, :end, h].double() for side in (key, value))
+            if mask is not None:
+                k, v = (side.masked_fill(hidden.unsqueeze(1), 0) for side in (k, v))
+            products = (q.view(-1, head_dim) @ k.T).view(group, nodes, end) * scale + add
+            t = products.masked_fill(~seen, -INF)
+            w = torch.softmax(t, -1)
+            away = (t.amax(-1, keepdim=True) - t).clamp_max(200).masked_fill(~seen, 0).amax(-1, keepdim=True)
+            size = (q.abs().view(-1, head_dim) @ k.abs().T).view(group, nodes, end) * scale
+            size = size.masked_fill(~seen, 0).amax(-1, keepdim=True)
+            rows = w.view(-1, end)
+            bounds = (rows @ v.abs(), away.expand(-1, -1, head_dim), size.expand(-1, -1, head_dim))
+            for part, x in zip(parts, (rows @ v, *(bound.nan_to_num(0.0) for bound in bounds))):
+                part[b, h * group : (h + 1) * group] = x.reshape(group, nodes, head_dim)
+    return [part.cpu() for part in parts]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("batch,q_heads,kv_heads,head_dim,nodes", [
+    (140, 4, 2, 64, 3), (70, 32, 4, 64, 2), (301, 2, 1, 128, 1), (130, 14, 2, 40, 9), (9, 60, 30, 256, 2),
+    # Fewer than four sequences: none is cut.
+    (3, 180, 90, 64, 2), (1, 256, 256, 64, 1), (2, 8, 2, 64, 4096)])
+def test_tree_attention_of_large_batches_on_pages_with_masks_in_graphs(gpu, batch, q_heads, kv_heads, head_dim, nodes,
+                                                                       masked, dtype):
+    """Whole sequences for all CUs, of which the far longer ones are cut: others at every
+    replay of one graph, and none; masks that hide whole tiles within the cut pieces."""
+
+    announce(f"tree attention large {batch} {kv_heads} {nodes} {masked} {dtype}")
+    g = generator(batch + nodes)
+    chain = nodes > 1024
+    capacity = 1808 if not chain else 4608
+    query = torch.randn(batch, q_heads, nodes, head_dim, generator=g).to(dtype).to(gpu)
+    key, value = (torch.randn(batch, capacity, kv_heads, head_dim, device=gpu, generator=torch.Generator(gpu).manual_seed(n))
+                  .to(dtype) for n in (1, 2))
+    high = capacity - nodes
+    turns = []
+    for long in ((0, batch // 2, batch - 1), (batch // 3, batch // 3 + 1), ()):
+        lengths = torch.randint(0, 60, (batch,), generator=g)
+        for at, length in zip(long, (high, high * 2 // 3, high - 65)):
+            lengths[at % batch] = length
+        turns.append(lengths)
+    tree = None if chain else random_tree(nodes, g).to(gpu)
+    mask = None
+    if masked:
+        mask = torch.randn(batch, 1, 1, capacity, generator=g)
+        mask[0, ..., :700] = mask[1::3, ..., 200:900] = mask[::5, ..., 1000:1300] = -INF
+        mask[1::4, ..., :21] = -INF  # and some whole sequences
+        mask[torch.rand(mask.shape, generator=g) < 0.02] = -INF
+        mask = mask.to(gpu, dtype)
+        hidden = (mask[:, 0, 0] == -INF)[..., None, None]
+        key, value = key.masked_fill(hidden, INF), value.masked_fill(hidden, NAN)
+    pages = capacity // 16
+    order = torch.randperm(batch * pages + 2, generator=g)[: batch * pages].view(batch, pages).to(gpu)
+    pools = []
+    for side in (key, value):
+        pool = torch.full((batch * pages + 2, 16, kv_heads, head_dim), NAN, dtype=dtype, device=gpu)
+        pool[order.view(-1)] = side.view(batch * pages, 16, kv_heads, head_dim)
+        pools.append(pool)
+    table = order.to(torch.int32)
+    references = [large_reference(query, key, value, lengths.to(gpu), tree, mask, head_dim**-0.5) for lengths in turns]
+    for paged_form in (False, True):
+        workspace = _native.DeviceWorkspace(gpu)
+        lengths = turns[0].to(gpu)
+
+        def run(lengths, workspace=None):
+            if paged_form:
+                return backends.hip_paged_tree_attention(query, *pools, table, lengths, tree, mask, scale=head_dim**-0.5,
+                                                         workspace=workspace)
+            return backends.hip_tree_attention(query, key, value, lengths, tree, mask, scale=head_dim**-0.5,
+                                               workspace=workspace)
+
+        run(lengths, workspace)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(lengths, workspace)
+        for turn in (1, 0, 2, 1):
+            lengths.copy_(turns[turn])
+            out.fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert_tree_close(out, references[turn], capacity)
+            assert_bitwise_equal(out, run(lengths))
+
+
 def test_tree_attention_with_a_mask_of_no_rows(gpu):
     announce("tree attention empty mask")
     for dtype in (torch.bfloat16, torch.float32):
