@@ -30,10 +30,10 @@ struct TreeArgs {
   int slots, row_blocks;
   float inverse_slots;
   int extra;  // large batches: slots of further pieces, before one of each sequence's first; else -1
-  float* partial;  // [slot, KV head, row block][rows][DP], then their (max, sum) pairs
+  float* partial;  // [place, KV head, row block][rows][DP], then their (max, sum) pairs (see Piece)
   float2* stats;
   int* counters;  // [sequence, KV head, row block], zero between calls; null: a merge kernel
-  int2* pieces;   // for that: per sequence the slot of its second piece, and how many
+  int2* pieces;   // for that: per sequence the place of its second piece, and how many
 };
 
 // The kernel for `rows` query rows per KV head, and its launch; one pair per type, in

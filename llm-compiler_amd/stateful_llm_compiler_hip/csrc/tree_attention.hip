@@ -33,7 +33,10 @@ Split split_for(const Plan& plan, int64_t batch, int64_t kv_heads, int64_t rows)
   // node: 87 us, 239).
   s.extra = batch * each >= cus ? batch / 4 : -1;
   s.slots = s.extra >= 0 ? batch + s.extra : std::max<int64_t>(cus / each, batch + batch / 4);
-  const int64_t places = s.slots * kv_heads * s.row_blocks * plan.rows_per_block;
+  // Of these only the pieces of a sequence that is cut have partial results: the further
+  // ones, and as many first ones at most (1024 sequences of 64 nodes, 32 heads on 8 of 128: 545
+  // MB; places for all of them were 1.36 GB).
+  const int64_t places = (s.extra >= 0 ? 2 * s.extra : s.slots) * kv_heads * s.row_blocks * plan.rows_per_block;
   s.partial_bytes = places * plan.padded_dim * 4;
   s.stats_bytes = places * 8;
   s.pieces_bytes = batch * 8;

@@ -159,7 +159,10 @@ constexpr int kTailSteps = STEP <= 64 ? 5 : 2;
 struct Piece {
   int sequence;  // -1: none
   int index, count;
-  int head, tail;      // slots of the first piece, and of the second
+  // Places of the partial results of the first piece and of the second, which the others
+  // follow: the slots, but in large batches the first piece's lies behind all further ones', as
+  // far as the second's from the start.
+  int head, tail;
   int length, end;  // rows of the sequence, and with its nodes'
 };
 
@@ -218,7 +221,7 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs& a, int x, float min_
       }
       before = __builtin_amdgcn_readlane(upto, 63);
     }
-    p.head = a.extra + p.sequence;
+    p.head = a.extra + p.tail;
     p.index = x < a.extra ? x - p.tail + 1 : 0;
     p.end = end_of(p.length);
     return p;
@@ -269,7 +272,7 @@ __device__ __forceinline__ int block_units(const TreeArgs& a, int block) {
 }
 // Units unit, unit + step, .. (kUnits of them, those below `units`) of a sequence's row
 // block (each float4 of a wave's lanes) put together from the
-// `count` pieces in slot `head` and from slot `tail` on, kBatch at a time.
+// `count` pieces at place `head` and from place `tail` on, kBatch at a time.
 template <typename T, int DP, int ROWS, int kUnits, int kBatch>
 __device__ __forceinline__ void merge_units(const TreeArgs& a, int64_t b, int kvh, int block, int head, int tail, int count,
                                             int unit, int step, int units) {
@@ -356,7 +359,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int units = block_units<DP, ROWS>(a, block);
   if (pieces.y <= 1 || unit >= units) return;
-  const int head = a.extra >= 0 ? a.extra + static_cast<int>(b) : pieces.x - 1;
+  const int head = a.extra >= 0 ? a.extra + pieces.x : pieces.x - 1;
   merge_units<T, DP, ROWS, 1, 8>(a, b, kvh, block, head, pieces.x, pieces.y, unit, 1, unit + 1);
 }
 
@@ -921,7 +924,8 @@ __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_att
       return make_float4(acc[i][qb][0], acc[i][qb][1], acc[i][qb][2], acc[i][qb][3]);
     }
   };
-  const int64_t place = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * a.row_blocks + block;
+  const int own = piece.index == 0 ? piece.head : piece.tail + piece.index - 1;
+  const int64_t place = (static_cast<int64_t>(own) * a.kv_heads + kvh) * a.row_blocks + block;
   auto store = [&](int i, int qb, float4 v, float top, float sum) {
     if (!real[qb]) return;
     const int dim = quad_dim<T>(i, g);

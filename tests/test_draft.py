@@ -235,3 +235,17 @@ def test_what_a_commit_leaves_at_length_zero_takes_a_prefill(monkeypatch, paged)
         with pytest.raises(ExecutionError, match="length to be 0"):
             later.prefill_store(1, rows, rows)
     assert full.commit(path, counts).zero_slots == frozenset() and stored == [1]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_tree_workspace_of_large_batches_holds_what_is_cut_only(dtype):
+    """Where whole sequences are enough for all CUs, a quarter as many further pieces and
+    their sequences' first ones have partial results."""
+
+    size = _native.library().slc_hip_tree_attention_workspace_size
+    for batch, q_heads, kv_heads, nodes, head_dim in ((1024, 32, 8, 64, 128), (32, 32, 32, 1024, 128), (2048, 2, 1, 1, 64),
+                                                      (3, 512, 512, 1, 64), (1027, 14, 2, 5, 256)):
+        rows = q_heads // kv_heads * nodes
+        padded = max(16, min(256, 1 << (rows - 1).bit_length()))  # of a row block at most
+        places = 2 * (batch // 4) * kv_heads * (rows + padded - 1)
+        assert size(batch, q_heads, kv_heads, nodes, head_dim, dtype) <= places * (4 * head_dim + 8) + 8 * batch
