@@ -98,6 +98,9 @@ SLC_API int slc_hip_version(void);
 /* Message describing the last failure on the calling thread ("" if none). */
 SLC_API const char* slc_hip_last_error(void);
 
+/* The capture that `stream` is in, a number of its own for each; 0: none. */
+SLC_API uint64_t slc_hip_capture_id(void* stream);
+
 /*
  * BENCH-ONLY.  Not for serving code: while armed, the calling thread's
  * entry points change what they launch (see slc_hip_set_timing_repeats).

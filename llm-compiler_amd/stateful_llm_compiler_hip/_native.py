@@ -58,6 +58,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "slc_hip_last_error": (ctypes.c_char_p, []),
     "slc_hip_set_timing_events": (None, [_P, _P]),
     "slc_hip_set_timing_repeats": (None, [ctypes.c_int]),
+    "slc_hip_capture_id": (ctypes.c_uint64, [_P]),
     "slc_hip_kv_store": (
         _I,
         [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _P],
@@ -231,6 +232,12 @@ def softmax_order_tag(order: str) -> int:
         raise ValueError(f"softmax order must be one of {sorted(SOFTMAX_ORDERS)}, got {order!r}") from error
 
 
+def _capture_id(device: torch.device) -> int:
+    """The capture that PyTorch's current stream on ``device`` is in; 0: none."""
+
+    return library().slc_hip_capture_id(torch.cuda.current_stream(device).cuda_stream)
+
+
 class DeviceWorkspace:
     """Caller-owned device memory of the kernels that combine work across
     workgroups: one zero-filled int32 counter array, shared by every kernel
@@ -238,11 +245,16 @@ class DeviceWorkspace:
     per kernel kind for partial results.  Kernels that run in order (one
     stream, or one captured graph) can share a workspace; kernels that may run
     concurrently need separate ones.  Buffers that were outgrown stay alive (a
-    captured graph may still hold their address)."""
+    captured graph may still hold their address).
+
+    Counters that are made while a graph is captured are zeroed at its replays only, and
+    lie in its memory: they serve that capture, and other graphs and eager calls get
+    their own."""
 
     def __init__(self, device: torch.device | str) -> None:
         self.device = torch.device(device)
         self._counters: torch.Tensor | None = None
+        self._capture = 0  # that the counters were made in; 0: none
         self._scratch: dict[str, torch.Tensor] = {}
         self._retired: list[torch.Tensor] = []
 
@@ -250,11 +262,15 @@ class DeviceWorkspace:
         """Zeroed int32 counters, at least ``count`` (and at least 1) of them."""
 
         current = self._counters
-        if current is None or current.numel() < count:
-            if current is not None:
+        if current is not None and current.numel() >= count and self._capture == 0:
+            return current
+        capture, held = _capture_id(self.device), 0 if current is None else current.numel()
+        if held < count or capture != self._capture:
+            if current is not None and self._capture == 0:
                 self._retired.append(current)
-            size = max(int(count), 2 * (current.numel() if current is not None else 0), 64)
+            size = max(int(count), 64, 2 * held if held < count else held)
             self._counters = torch.zeros(size, dtype=torch.int32, device=self.device)
+            self._capture = capture
         return self._counters
 
     def scratch(self, name: str, nbytes: int) -> torch.Tensor | None:

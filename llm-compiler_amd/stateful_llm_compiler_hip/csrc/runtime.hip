@@ -58,6 +58,17 @@ extern "C" int slc_hip_version(void) { return 200; }
 
 extern "C" const char* slc_hip_last_error(void) { return g_last_error; }
 
+extern "C" uint64_t slc_hip_capture_id(void* stream) {
+  if (stream == nullptr) return 0;  // the default stream cannot be captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 extern "C" void slc_hip_set_timing_events(void* begin, void* end) {
   g_begin = static_cast<hipEvent_t>(begin);
   g_end = static_cast<hipEvent_t>(end);

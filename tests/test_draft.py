@@ -249,3 +249,30 @@ def test_tree_workspace_of_large_batches_holds_what_is_cut_only(dtype):
         padded = max(16, min(256, 1 << (rows - 1).bit_length()))  # of a row block at most
         places = 2 * (batch // 4) * kv_heads * (rows + padded - 1)
         assert size(batch, q_heads, kv_heads, nodes, head_dim, dtype) <= places * (4 * head_dim + 8) + 8 * batch
+
+
+def test_counters_made_in_a_capture_serve_that_capture_only(monkeypatch):
+    """They are zeroed where the graph is replayed, not where it is captured: an eager
+    call and another graph that came first would find what the memory held."""
+
+    now = [0]
+    monkeypatch.setattr(_native, "_capture_id", lambda device: now[0], raising=False)
+    workspace = _native.DeviceWorkspace("cpu")
+
+    def counters(capture, count):
+        now[0] = capture
+        return workspace.counters(count)
+
+    first = counters(7, 100)
+    assert counters(7, 30) is first and first.numel() == 100  # within the capture: one
+    second, eager = counters(8, 30), counters(0, 30)
+    assert len({t.data_ptr() for t in (first, second, eager)}) == 3 and second.numel() == eager.numel() == 100
+    # Those of an eager call were zeroed at once: all take them, while they are enough.
+    assert counters(9, 100) is eager and counters(0, 1) is eager and counters(10, 64) is eager
+    more = counters(11, 101)
+    assert more is not eager and more.numel() == 200 and counters(11, 150) is more
+    assert any(t is eager for t in workspace._retired)  # graph 9 holds them
+    other = counters(0, 5)
+    assert other is not more and other.numel() == 200 and counters(12, 200) is other
+    assert not any(t is more or t is first or t is second for t in workspace._retired)
+    assert all(int(t.abs().sum()) == 0 for t in (first, second, eager, more, other))

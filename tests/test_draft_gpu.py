@@ -1552,3 +1552,64 @@ def test_a_captured_step_goes_on_at_every_replay(gpu):
             for got, expected in zip(state.lengths + state.keys + state.values, eager.lengths + eager.keys + eager.values):
                 assert torch.equal(got, expected)
     assert eager.lengths[0].tolist() != [300, 0, 17]
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_graphs_captured_without_a_call_before_run_in_any_order(gpu, shared):
+    """On the capture stream's workspace and on one of their own: each graph, and eager
+    calls between, has counters that are zero, whatever the memory held."""
+
+    announce(f"graphs without a call before {shared}")
+    g = generator(77)
+    batch, nodes, vocab = 4, 5, 9000
+    target, draft = probabilities(g, batch, nodes, vocab).to(gpu), probabilities(g, batch, nodes - 1, vocab).to(gpu)
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=g).to(gpu)
+    uniforms = torch.rand(batch, nodes, generator=g).to(gpu)
+    query, key, value, lengths = (t.to(gpu) for t in tree_inputs(g, 2, 4, 2, 64, 6, 700, torch.bfloat16, [600, 3]))
+
+    def step(workspace):
+        return (*backends.hip_verify_tokens(tokens, target, uniforms, draft_probs=draft, workspace=workspace),
+                backends.hip_tree_attention(query, key, value, lengths, None, scale=0.125, workspace=workspace))
+
+    want = step(None)
+    workspace = _native.DeviceWorkspace(gpu) if shared else None
+    # Graphs of one pool; the first leaves ones in memory that the next ones' temporaries take.
+    filler = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(filler):
+        rooms = [torch.full((size,), -1, dtype=torch.int32, device=gpu) for size in (64, 80, 128, 512, 1024) for _ in range(8)]
+        del rooms
+    filler.replay()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(3):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=filler.pool()):
+            out = step(workspace)
+        graphs.append((graph, out))
+
+    def check(out):
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+    check(step(workspace))
+    for at in (2, 0, 1, 0, 2):
+        for tensor in graphs[at][1]:
+            tensor.fill_(3)
+        graphs[at][0].replay()
+        check(graphs[at][1])
+        check(step(workspace))
+
+
+def test_each_capture_has_a_number(gpu):
+    announce("capture numbers")
+    stream, seen = torch.cuda.Stream(), []
+    assert _native.library().slc_hip_capture_id(stream.cuda_stream) == 0
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            x = torch.zeros(4, device=gpu)
+            seen += [_native._capture_id(gpu), _native.library().slc_hip_capture_id(stream.cuda_stream)]
+        assert _native._capture_id(gpu) == 0 and _native.library().slc_hip_capture_id(stream.cuda_stream) == 0
+    assert seen[0] == seen[1] != 0 and seen[2] == seen[3] != 0 and seen[0] != seen[2]
+    assert _native.library().slc_hip_capture_id(None) == 0 and x.numel() == 4
