@@ -129,7 +129,8 @@ def hip_tree_attention(
 
     ``key_buffer``/``value_buffer`` may be views with a contiguous head dim and equal
     strides.  The softmax is fp32; 16-bit types round its unnormalised weights for the
-    product with V.  ``workspace``: the caller's ``DeviceWorkspace`` (else the current
+    product with V, as ``hip_decode_attention``'s online order does (there is no exact
+    order here).  ``workspace``: the caller's ``DeviceWorkspace`` (else the current
     stream's); calls that may run concurrently need separate ones.
     """
 

@@ -12,20 +12,30 @@
 // so K and V are read once for all of them.  Producer waves stream steps of K and V
 // into an LDS ring with direct-to-LDS loads (16-byte chunks, XOR-swizzled by row; rows
 // past the last one read as zero).  WR x WK consumer waves own 16 QB query rows and one
-// of the step's WK tiles of KT keys each, so few query rows still keep all waves busy:
+// of the step's WK tiles of KT keys each, so that few query rows still keep several waves
+// busy: of up to 16, four of rows of 128 bytes, whose 32 KB steps hold four tiles, two of
+// 256 and one of wider ones:
 //  * S^T[key, query] = K . Q^T, Q^T in registers;
 //  * softmax with a running maximum that moves only when a score passes it by more than
 //    kThreshold, in fp32, maxima in units of the score itself so that a mask of the
 //    type's lowest value stays finite;
 //  * O^T[dim, query] += V^T . P^T: the score tile's C layout is the product's B layout
-//    once V's rows are taken in the same order.
+//    once V's rows are taken in the same order.  The matrix cores take 16-bit weights: bf16
+//    and fp16 round them, unnormalised, and their sum is that of the rounded ones, so that
+//    an error of all of them alike cancels (as in the online order of the other attention
+//    kernels).  Against 64 bits the outputs are off by 2.3e-3 of their norm in bf16, 2.0e-4 in
+//    fp16.  Weights in two parts, a product for each, leave the output's own rounding alone,
+//    1.7e-3 and 1.8e-4, but cost 41.5 us for 32.5 (16 nodes, long caches) and 34.5 for 29.3 (64
+//    nodes): not taken.
 // The WK partial results meet in LDS; the pieces' partial results, where a sequence
 // has several, in the last of them to end or in a kernel of their own.
 //
 // What bounds it, in a graph, 14 query heads on 2 of 64, bf16: 32 sequences of 4096 to
 // 8192 rows (101 MB) take 24.0 us with 2 nodes, 4.2 TB/s, and 32.0 with 16, whose 112
-// query rows keep the VALU (exponentials, maxima, packing) as busy as the memory; of 16
-// sequences with 64 nodes, 29.4 us, some 19 us are those steps.  Before the first tile
+// query rows' products, then exponentials, maxima and packing, are as long as the stream: a
+// step's consumers pass one barrier and do them in the same order, so that the matrix cores
+// and the VALU take turns; of 16 sequences with 64 nodes, 29.4 us, some 19 us are those
+// steps, of which the products alone take 6 and the vector instructions 6 to 11.  Before the first tile
 // lies about 4 us (the pieces, the descriptors, the first loads), behind the last one 3 to
 // 6 us (results through LDS and memory): one sequence of 600 rows and 8 nodes takes 10.1.
 #pragma once
@@ -404,7 +414,8 @@ struct Shape {
 };
 
 // MASKED: with a mask; by itself the form without one has fewer registers and less code (16
-// sequences, 64 nodes 30.5 -> 29.4 us, one sequence 10.5 -> 10.1).
+// sequences, 64 nodes 30.5 -> 29.4 us, one sequence 10.5 -> 10.1).  The widest 16-bit form
+// with one spills 13 registers; fp32 rows of 1024 bytes and 64 query rows spill 39, with one 115.
 template <typename T, int DP, int QB, int WR, int KT, bool MASKED>
 __global__ __launch_bounds__((Shape<T, DP, QB, WR, KT>::kThreads)) void tree_attention_kernel(TreeArgs a, float min_steps) {
   using S = Shape<T, DP, QB, WR, KT>;

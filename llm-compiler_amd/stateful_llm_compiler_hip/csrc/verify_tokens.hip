@@ -23,11 +23,12 @@
 // and sums blocks of 1024 weights, one a wave, and the last to arrive finds the block and
 // the token.  Only a node whose second child is tried with a draft row needs more
 // passes over its row (the mass decides the next test); the last workgroup makes
-// them alone.
+// them alone, 19 us each at this vocabulary in fp32 (1.2 MB through one CU): 8 trees of 16 nodes,
+// four children each, 65 us, of 64 nodes 65 to 104.
 //
-// In a graph, vocabulary 151936, fp32: a chain of 5 nodes 7.5 us, 8 trees of 64 without
-// draft rows 7.7 us; 32 chains of 9 15.5 us, 39 MB at 2.5 TB/s: of it some 7 us are the
-// round trips and the launch again, 8 us the rows at the rate of a large copy.
+// In a graph, vocabulary 151936, fp32: a chain of 5 nodes 7.7 us, 8 trees of 64 without
+// draft rows 7.7 us, of 100, from LDS, 11.6; 32 chains of 9 15.4 us, 39 MB at 2.5 TB/s: of it some
+// 7 us are the round trips and the launch again, 8 us the rows at the rate of a large copy.
 #include <algorithm>
 #include <type_traits>
 
@@ -590,8 +591,9 @@ extern "C" int slc_hip_verify_tokens(
   a.nodes = static_cast<int>(nodes);
   a.vocab = static_cast<int>(vocab);
   a.blocks = static_cast<int>(block_count(vocab));
-  // One block a wave, but no more workgroups than CUs: the kernel's registers leave room
-  // for one each (32 chains 15 us, with twice as many 21).
+  // One block a wave, but no more workgroups than CUs: with draft rows the registers (130
+  // to 148 of a lane, up to 64 nodes) leave room for one each (32 chains 15 us, with twice as many
+  // 21).  Without, where two fit (117 to 125), the same rule.
   a.segments = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>(slc_host::ceil_div(a.blocks, kWaves), slc_host::device_cu_count() / batch)));
   hipStream_t s = static_cast<hipStream_t>(stream);

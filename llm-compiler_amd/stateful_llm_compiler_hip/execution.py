@@ -428,7 +428,8 @@ class PreallocatedKVCacheState:
     def commit(self, path: torch.Tensor, counts: torch.Tensor) -> "PreallocatedKVCacheState":
         """The accepted nodes' rows (``path`` and ``counts`` of ``hip_verify_tokens``)
         moved to their places in every layer, and every slot's lengths advanced by
-        ``counts``.  Older versions' visible prefixes are untouched."""
+        ``counts``.  Older versions' visible prefixes are untouched.  An accepted node
+        whose row was not stored sets the overflow flag."""
 
         if path.ndim != 2 or path.shape[0] != self.lengths[0].shape[0] or counts.shape != (path.shape[0],):
             raise ExecutionError("KV commit takes a B x T path and B counts")
@@ -450,10 +451,11 @@ class PreallocatedKVCacheState:
         return {**self.__dict__, "layers": None}
 
     def check_capacity(self) -> None:
-        """Synchronise and raise if any store or advance overflowed the capacity."""
+        """Synchronise and raise if any store, advance or commit overflowed the capacity
+        (or a commit counted a row that is not there)."""
 
         if self.overflow is not None and int(self.overflow.item()) != 0:
-            raise ExecutionError(f"KV store or advance exceeded capacity {self.capacity}")
+            raise ExecutionError(f"KV store, advance or commit exceeded capacity {self.capacity}")
 
     def _validate_store(self, slot, key, value, positions):
         try:
