@@ -455,7 +455,7 @@ class PreallocatedKVCacheState:
         (or a commit counted a row that is not there)."""
 
         if self.overflow is not None and int(self.overflow.item()) != 0:
-            raise ExecutionError(f"KV store, advance or commit exceeded capacity {self.capacity}")
+            raise ExecutionError(f"KV store or advance exceeded capacity {self.capacity}")
 
     def _validate_store(self, slot, key, value, positions):
         try:
